@@ -1,5 +1,5 @@
-"""ctypes binding of libtcc_swtcf.so (the C-ABI in include/tcc_swtcf.h and
-include/tcc_spmm_cnic.h).  Loading fails loudly when the library is missing:
+"""ctypes binding of libtcc_swtcf.so (the C-ABI in include/tcc_swtcf.h,
+include/tcc_spmm_cnic.h, include/tcc_gcn.h and include/tcc_training.h).  Loading fails loudly when the library is missing:
 there is no CPU fallback for any entry point."""
 from __future__ import annotations
 
@@ -81,6 +81,22 @@ class FeatureSource(ctypes.Structure):
     ]
 
 
+class GroupNormShape(ctypes.Structure):
+    """tcc_group_norm_shape."""
+    _fields_ = [
+        ("N", u64), ("B", u64), ("maxRows", u64), ("C", u32), ("G", u32), ("offsets", vp), ("offsetBytes", u32),
+        ("dtype", u32), ("paramDtype", u32), ("activation", u32), ("eps", ctypes.c_float),
+    ]
+
+
+class Adam(ctypes.Structure):
+    """tcc_adam."""
+    _fields_ = [
+        ("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double),
+        ("weightDecay", ctypes.c_double), ("maxNorm", ctypes.c_double), ("decoupled", ctypes.c_int),
+    ]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "tcc_last_error": (ctypes.c_char_p, []),
@@ -143,6 +159,19 @@ SIGNATURES = {
     "tcc_gcn_relu_grad_workspace_bytes": (ctypes.c_size_t, [u32, u32, u32, u32]),
     "tcc_gcn_relu_grad": (ctypes.c_int, [vp, u32, vp, u32, vp, u32, vp, vp, vp, u32, u32, u32, u32, vp, ctypes.c_size_t,
                                          vp]),
+    "tcc_embedding_lookup": (ctypes.c_int, [vp, u64, u32, vp, u32, u64, u64, u32, ctypes.c_float, i64, vp, u64, vp, vp]),
+    "tcc_embedding_grad_workspace_bytes": (ctypes.c_size_t, [u64, u64, u32]),
+    "tcc_embedding_grad": (ctypes.c_int, [vp, u64, u32, vp, u32, u64, u64, u32, ctypes.c_float, i64, vp, u64,
+                                          ctypes.c_int, vp, vp, ctypes.c_size_t, vp]),
+    "tcc_group_norm_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(GroupNormShape), ctypes.c_int]),
+    "tcc_group_norm": (ctypes.c_int, [ctypes.POINTER(GroupNormShape), vp, u64, vp, vp, vp, u64, vp, vp, vp,
+                                      ctypes.c_size_t, vp]),
+    "tcc_group_norm_grad": (ctypes.c_int, [ctypes.POINTER(GroupNormShape), vp, u64, vp, u64, vp, vp, vp, vp, vp, u64,
+                                           vp, vp, vp, ctypes.c_size_t, vp]),
+    "tcc_grad_norm_workspace_bytes": (ctypes.c_size_t, []),
+    "tcc_grad_norm": (ctypes.c_int, [vp, u32, vp, vp, ctypes.c_size_t, vp]),
+    "tcc_clip_grad_norm": (ctypes.c_int, [vp, vp, u32, ctypes.c_float, vp, vp, ctypes.c_size_t, vp]),
+    "tcc_adam_step": (ctypes.c_int, [vp, vp, vp, vp, u32, ctypes.POINTER(Adam), vp, vp, vp, ctypes.c_size_t, vp]),
 }
 
 _lib = None

@@ -23,7 +23,7 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = os.environ.get("TCC_OFFLOAD_ARCH", "gfx950")
 
 LIB_SOURCES = ["swtcf_convert.hip", "swtcf_spmm.hip", "swtcf_plan.hip", "bcsr_spmm.hip", "bcsr_build.hip",
-               "hub_tiles.hip", "dense_tn.hip",
+               "hub_tiles.hip", "dense_tn.hip", "embedding.hip", "group_norm.hip", "clip_adam.hip",
                "scratch.cpp", "errors.cpp"]
 LIB_NAME = "libtcc_swtcf.so"
 
