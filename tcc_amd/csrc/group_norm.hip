@@ -40,17 +40,24 @@ struct Segments {
                                     : load_global<std::int32_t>(static_cast<const std::int32_t*>(offsets) + s);
         return static_cast<std::uint64_t>(v < 0 ? 0 : min<std::uint64_t>(static_cast<std::uint64_t>(v), N));
     }
-    // The last segment that starts at or before `row`, for row < N.
+    // The last segment that starts at or before `row` (0 if there is none),
+    // for row < N, by a whole wave: 64 starts a round.
     __device__ __forceinline__ std::uint64_t find(std::uint64_t row) const {
         if (offsets == nullptr) return row / each;
-        std::uint64_t lo = 0, hi = B;
+        std::uint64_t lo = 0, hi = B;  // start(lo) <= row < start(hi), or lo = 0
         while (hi - lo > 1) {
-            const std::uint64_t m = (lo + hi) / 2;
-            if (start(m) <= row) lo = m;
-            else hi = m;
+            const std::uint64_t step = (hi - lo + kWave - 1) / kWave;
+            const std::uint64_t m = lo + (__lane_id() + 1) * step;
+            const std::uint64_t above = __ballot(m >= hi || start(m) > row);
+            const std::uint64_t k = above == 0 ? kWave : __builtin_ctzll(above);
+            hi = min(lo + (k + 1) * step, hi);
+            lo += k * step;
         }
         return lo;
     }
+    // Segments of more rows than this go tile by tile, the others whole.
+    std::uint64_t longest;
+    __device__ __forceinline__ bool whole(std::uint64_t s) const { return start(s + 1) - start(s) <= longest; }
 };
 
 struct NormArgs {
@@ -60,18 +67,33 @@ struct NormArgs {
     float *mean, *rstd;
     float2* part;      // [slots][G]: mean and squared deviations, or S1 and S2
     float2* sums;      // [B][G]: S1 / M and S2 / M
-    float2* channel;   // [tiles][C]: dBias and dWeight
+    float2* channel;   // [wholeRows + tiles][C]: dBias and dWeight
+    std::uint8_t* seen;  // [kWholeBlocks]: whether a whole segments' workgroup met one that goes by tiles
+    std::uint32_t seenCount;  // those workgroups; 0: tiles alone
     std::uint64_t ldx, lddy, ldo, tileRows;
     std::uint32_t C, G, K, colsV, rowLanes;  // K = C / G; colsV vectors a row, rowLanes rows at once
     std::uint32_t paramBytes, paramType, act;
     float eps;
 };
 
-__device__ __forceinline__ float param_at(const void* p, std::uint32_t type, std::uint32_t c, float none) {
-    if (p == nullptr) return none;
-    if (type == TCC_F32) return static_cast<const float*>(p)[c];
-    if (type == TCC_BF16) return static_cast<float>(static_cast<const bf16_t*>(p)[c]);
-    return static_cast<float>(static_cast<const f16_t*>(p)[c]);
+// Channels c .. c + N of a weight or bias: one branch and one load for all of
+// them (a branch for each put every load behind the one before).  c is a
+// multiple of N, but the caller's array need only be aligned to its elements.
+template <int N>
+__device__ __forceinline__ vec_t<float, N> load_params(const void* p, std::uint32_t type, std::uint32_t c, float none) {
+    vec_t<float, N> v(none);
+    if (p == nullptr) return v;
+    if (type == TCC_F32) {
+#pragma unroll
+        for (int q = 0; q < N; ++q) v[q] = load_global<float>(static_cast<const float*>(p) + c + q);
+    } else if (type == TCC_BF16) {
+#pragma unroll
+        for (int q = 0; q < N; ++q) v[q] = static_cast<float>(load_global<bf16_t>(static_cast<const bf16_t*>(p) + c + q));
+    } else {
+#pragma unroll
+        for (int q = 0; q < N; ++q) v[q] = static_cast<float>(load_global<f16_t>(static_cast<const f16_t*>(p) + c + q));
+    }
+    return v;
 }
 
 // z with a rounding after each operation, in the forward as in the gradient.
@@ -85,27 +107,65 @@ __device__ __forceinline__ float affine(float xh, float w, float b) {
     return m + b;
 }
 
-__device__ __forceinline__ float activate(std::uint32_t act, float z) {
-    if (act == TCC_ACT_NONE) return z;
-    if (act == TCC_ACT_RELU) return z > 0.0f ? z : z * 0.0f;  // keeps NaN
-    if (act == TCC_ACT_SILU) return z / (1.0f + expf(-z));
-    return z * (0.5f * (1.0f + erff(z * 0.70710678f)));
+// exp, and 1 / x, by the hardware's instructions: good to a few 2^-24 of the
+// exponent and of the quotient, which no activation below magnifies.
+__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
+__device__ __forceinline__ float fast_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
+
+// The normal distribution's Phi(z), and e = exp(-z^2 / 2), from which both
+// come: erf by Abramowitz and Stegun's 7.1.26, off by 1.5e-7 at most, with z
+// scaled once for both (v^2 log 2 = z^2 / 2) and the halves in the
+// coefficients.  The library's erff and expf cost the gradient twice the
+// instructions.
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+    const float v = z * 0.849321800f;                              // sqrt(log2(e) / 2)
+    const float t = fast_rcp(fmaf(0.272737481f, fabsf(v), 1.0f));  // 0.3275911 sqrt(log 2)
+    e = __builtin_amdgcn_exp2f(-v * v);
+    float q = fmaf(t, 0.5307027145f, -0.7265760135f);
+    q = fmaf(t, q, 0.7107068705f);
+    q = fmaf(t, q, -0.142248368f);
+    q = fmaf(t, q, 0.127414796f);
+    q = q * (t * e);
+    return z > 0.0f ? 1.0f - q : q;
 }
 
-__device__ __forceinline__ float slope(std::uint32_t act, float z) {
-    if (act == TCC_ACT_NONE) return 1.0f;
-    if (act == TCC_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
-    if (act == TCC_ACT_SILU) {
-        const float p = 1.0f / (1.0f + expf(-z));
-        return p * (1.0f + z * (1.0f - p));
+template <std::uint32_t ACT>
+__device__ __forceinline__ float activate(float z) {
+    if (ACT == TCC_ACT_NONE) return z;
+    if (ACT == TCC_ACT_RELU) return z > 0.0f ? z : z * 0.0f;  // keeps NaN
+    if (ACT == TCC_ACT_SILU) return z * fast_rcp(1.0f + fast_exp(-z));
+    float e;
+    return z * normal_cdf(z, e);
+}
+
+template <std::uint32_t ACT>
+__device__ __forceinline__ float slope(float z) {
+    if (ACT == TCC_ACT_NONE) return 1.0f;
+    if (ACT == TCC_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+    if (ACT == TCC_ACT_SILU) {
+        const float p = fast_rcp(1.0f + fast_exp(-z));
+        return p * fmaf(z, 1.0f - p, 1.0f);
     }
-    return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * expf(-0.5f * z * z) * 0.39894228f;
+    float e;
+    const float p = normal_cdf(z, e);
+    return fmaf(z * 0.39894228f, e, p);
 }
 
 // Rows a, a + rowLanes, ... below b that a row lane takes.
 __device__ __forceinline__ std::uint32_t lane_rows(std::uint64_t a, std::uint64_t b, std::uint32_t rl,
                                                    std::uint32_t rowLanes) {
     return a + rl < b ? static_cast<std::uint32_t>((b - a - rl + rowLanes - 1) / rowLanes) : 0u;
+}
+
+// Whether the tiles have anything to do, for a whole workgroup.
+__device__ __forceinline__ bool tiles_needed(const std::uint8_t* seen, std::uint32_t count) {
+    if (count == 0) return true;
+    std::uint32_t any = 0;
+    for (std::uint32_t i = threadIdx.x * 16; i < count; i += blockDim.x * 16) {
+        const vu4 v = load_global<vu4>(seen + i);
+        any |= v[0] | v[1] | v[2] | v[3];
+    }
+    return __syncthreads_or(static_cast<int>(any)) != 0;
 }
 
 __device__ __forceinline__ float wave_sum(float v) {
@@ -124,6 +184,7 @@ constexpr int kBatch = 4;  // rows whose deviations are taken from their own mea
 // difference of large sums, whatever the mean.
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads) stats_kernel(NormArgs a) {
+    if (!tiles_needed(a.seen, a.seenCount)) return;
     extern __shared__ float lds[];
     float* ldsMean = lds;
     float* ldsDev = lds + a.rowLanes * a.C;
@@ -137,7 +198,7 @@ __global__ void __launch_bounds__(kThreads) stats_kernel(NormArgs a) {
     for (std::uint64_t s = a.seg.find(lo); s < a.seg.B; ++s) {
         const std::uint64_t first = max(a.seg.start(s), lo), end = min(a.seg.start(s + 1), hi);
         if (a.seg.start(s) >= hi) break;
-        if (first >= end) continue;
+        if (first >= end || a.seg.whole(s)) continue;
         if (active) {
             for (std::uint32_t cv = cv0; cv < a.colsV; cv += kThreads) {
                 vec_t<float, N> mean(0.0f), dev(0.0f);
@@ -212,44 +273,57 @@ __device__ __forceinline__ float slot_rows(const NormArgs& a, std::uint64_t t, s
     return static_cast<float>(hi - lo);
 }
 
-// The sum of a workgroup's values, in the same order every time.
+// The groups of a segment's joins: with W > 1 a workgroup of W waves each
+// (few segments of many slots), else a wave each.
 template <int W>
-__device__ __forceinline__ float group_sum(float v, float* red) {
-    v = wave_sum(v);
-    if (W == 1) return v;
-    if (__lane_id() == 0) red[threadIdx.x / kWave] = v;
-    __syncthreads();
-    float s = 0.0f;
+struct JoinGroup {
+    static constexpr int threads = W > 1 ? W * kWave : kThreads;
+    static unsigned grid(std::uint32_t G) { return W > 1 ? G : (G + kWaves - 1) / kWaves; }
+    __device__ __forceinline__ static std::uint32_t group() {
+        return W > 1 ? blockIdx.y : blockIdx.y * kWaves + threadIdx.x / kWave;
+    }
+    __device__ __forceinline__ static std::uint32_t first() { return W > 1 ? threadIdx.x : __lane_id(); }
+    // The sum of the group's threads' values, in the same order every time.
+    __device__ __forceinline__ static float sum(float v, float* red) {
+        v = wave_sum(v);
+        if (W == 1) return v;
+        if (__lane_id() == 0) red[threadIdx.x / kWave] = v;
+        __syncthreads();
+        float s = 0.0f;
 #pragma unroll
-    for (int w = 0; w < W; ++w) s += red[w];
-    __syncthreads();
-    return s;
-}
+        for (int w = 0; w < W; ++w) s += red[w];
+        __syncthreads();
+        return s;
+    }
+};
 
-// mean and rstd of one segment's group from its slots.
+// mean and rstd of one segment's groups from its slots.
 template <int W>
-__global__ void __launch_bounds__(kWave* W) stats_join_kernel(NormArgs a) {
+__global__ void __launch_bounds__(JoinGroup<W>::threads) stats_join_kernel(NormArgs a) {
+    if (!tiles_needed(a.seen, a.seenCount)) return;
+    using Join = JoinGroup<W>;
     __shared__ float red[W];
-    const std::uint64_t s = blockIdx.x / a.G;
-    const std::uint32_t g = blockIdx.x - static_cast<std::uint32_t>(s * a.G);
+    const std::uint64_t s = blockIdx.x;
+    const std::uint32_t g = Join::group();
     const std::uint64_t first = a.seg.start(s), end = a.seg.start(s + 1);
+    if (g >= a.G || (first < end && a.seg.whole(s))) return;
     float mean = 0.0f, var = 0.0f;
     if (first < end) {
         const std::uint64_t t0 = first / a.tileRows, t1 = (end - 1) / a.tileRows;
         const float rows = static_cast<float>(end - first);
         float sum = 0.0f;
-        for (std::uint64_t t = t0 + threadIdx.x; t <= t1; t += kWave * W)
+        for (std::uint64_t t = t0 + Join::first(); t <= t1; t += kWave * W)
             sum += a.part[(t + s) * a.G + g].x * slot_rows(a, t, first, end);
-        mean = group_sum<W>(sum, red) / rows;
+        mean = Join::sum(sum, red) / rows;
         float dev = 0.0f;
-        for (std::uint64_t t = t0 + threadIdx.x; t <= t1; t += kWave * W) {
+        for (std::uint64_t t = t0 + Join::first(); t <= t1; t += kWave * W) {
             const float2 p = a.part[(t + s) * a.G + g];
             const float gap = p.x - mean;
             dev += p.y + gap * gap * slot_rows(a, t, first, end) * static_cast<float>(a.K);
         }
-        var = group_sum<W>(dev, red) / (rows * static_cast<float>(a.K));
+        var = Join::sum(dev, red) / (rows * static_cast<float>(a.K));
     }
-    if (threadIdx.x == 0) {
+    if (Join::first() == 0) {
         a.mean[s * a.G + g] = mean;
         a.rstd[s * a.G + g] = 1.0f / sqrtf(var + a.eps);
     }
@@ -257,29 +331,27 @@ __global__ void __launch_bounds__(kWave* W) stats_join_kernel(NormArgs a) {
 
 // ---------------------------------------------------------------- output
 
-template <typename T, int N>
+template <typename T, int N, std::uint32_t ACT>
 __global__ void __launch_bounds__(kThreads) apply_kernel(NormArgs a) {
+    if (!tiles_needed(a.seen, a.seenCount)) return;
     const std::uint64_t lo = blockIdx.x * a.tileRows, hi = min(lo + a.tileRows, a.seg.N);
     const std::uint32_t rl = threadIdx.x / a.colsV;
     const std::uint32_t cv0 = a.colsV > kThreads ? threadIdx.x : threadIdx.x - rl * a.colsV;
+    const std::uint64_t s0 = a.seg.find(lo);
     if (a.colsV <= kThreads && rl >= a.rowLanes) return;
     const std::uint32_t row = a.colsV > kThreads ? 0u : rl;
     const T* x = static_cast<const T*>(a.x);
     T* y = static_cast<T*>(a.out);
-    const std::uint64_t s0 = a.seg.find(lo);
     for (std::uint32_t cv = cv0; cv < a.colsV; cv += kThreads) {
-        float w[N], b[N];
+        const vec_t<float, N> w = load_params<N>(a.weight, a.paramType, cv * N, 1.0f);
+        const vec_t<float, N> b = load_params<N>(a.bias, a.paramType, cv * N, 0.0f);
         std::uint32_t g[N];
 #pragma unroll
-        for (int q = 0; q < N; ++q) {
-            w[q] = param_at(a.weight, a.paramType, cv * N + q, 1.0f);
-            b[q] = param_at(a.bias, a.paramType, cv * N + q, 0.0f);
-            g[q] = (cv * N + q) / a.K;
-        }
+        for (int q = 0; q < N; ++q) g[q] = (cv * N + q) / a.K;
         for (std::uint64_t s = s0; s < a.seg.B; ++s) {
             const std::uint64_t first = max(a.seg.start(s), lo), end = min(a.seg.start(s + 1), hi);
             if (a.seg.start(s) >= hi) break;
-            if (first >= end) continue;
+            if (first >= end || a.seg.whole(s)) continue;
             float mean[N], rstd[N];
 #pragma unroll
             for (int q = 0; q < N; ++q) {
@@ -291,7 +363,7 @@ __global__ void __launch_bounds__(kThreads) apply_kernel(NormArgs a) {
                 const vec_t<float, N> v = load_row<T, N>(x + r * a.ldx + cv * N);
                 vec_t<float, N> o;
 #pragma unroll
-                for (int q = 0; q < N; ++q) o[q] = activate(a.act, affine(normalise(v[q], mean[q], rstd[q]), w[q], b[q]));
+                for (int q = 0; q < N; ++q) o[q] = activate<ACT>(affine(normalise(v[q], mean[q], rstd[q]), w[q], b[q]));
                 store_row<T, N>(y + r * a.ldo + cv * N, o);
             }
         }
@@ -302,8 +374,9 @@ __global__ void __launch_bounds__(kThreads) apply_kernel(NormArgs a) {
 
 // S1 and S2 of each segment's rows in a tile, and the tile's dBias and
 // dWeight.  LDS: the segment's sums and the tile's, a place for each lane.
-template <typename T, int N>
+template <typename T, int N, std::uint32_t ACT>
 __global__ void __launch_bounds__(kThreads) grad_sums_kernel(NormArgs a) {
+    if (!tiles_needed(a.seen, a.seenCount)) return;
     extern __shared__ float lds[];
     const std::uint32_t plane = a.rowLanes * a.C;
     float *seg1 = lds, *seg2 = lds + plane, *all1 = lds + 2 * plane, *all2 = lds + 3 * plane;
@@ -320,16 +393,16 @@ __global__ void __launch_bounds__(kThreads) grad_sums_kernel(NormArgs a) {
     for (std::uint64_t s = a.seg.find(lo); s < a.seg.B; ++s) {
         const std::uint64_t first = max(a.seg.start(s), lo), end = min(a.seg.start(s + 1), hi);
         if (a.seg.start(s) >= hi) break;
-        if (first >= end) continue;
+        if (first >= end || a.seg.whole(s)) continue;
         if (active) {
             for (std::uint32_t cv = cv0; cv < a.colsV; cv += kThreads) {
-                float w[N], b[N], mean[N], rstd[N];
+                const vec_t<float, N> w = load_params<N>(a.weight, a.paramType, cv * N, 1.0f);
+                const vec_t<float, N> b = load_params<N>(a.bias, a.paramType, cv * N, 0.0f);
+                float mean[N], rstd[N];
                 vec_t<float, N> s1(0.0f), s2(0.0f);
 #pragma unroll
                 for (int q = 0; q < N; ++q) {
                     const std::uint32_t c = cv * N + q;
-                    w[q] = param_at(a.weight, a.paramType, c, 1.0f);
-                    b[q] = param_at(a.bias, a.paramType, c, 0.0f);
                     mean[q] = a.mean[s * a.G + c / a.K];
                     rstd[q] = a.rstd[s * a.G + c / a.K];
                 }
@@ -340,7 +413,7 @@ __global__ void __launch_bounds__(kThreads) grad_sums_kernel(NormArgs a) {
 #pragma unroll
                     for (int q = 0; q < N; ++q) {
                         const float xh = normalise(v[q], mean[q], rstd[q]);
-                        const float dz = d[q] * slope(a.act, affine(xh, w[q], b[q]));
+                        const float dz = d[q] * slope<ACT>(affine(xh, w[q], b[q]));
                         s1[q] += dz;
                         s2[q] += dz * xh;
                     }
@@ -379,38 +452,43 @@ __global__ void __launch_bounds__(kThreads) grad_sums_kernel(NormArgs a) {
     }
 }
 
-// S1 / M and S2 / M of one segment's group from its slots.
+// S1 / M and S2 / M of one segment's groups from its slots.
 template <int W>
-__global__ void __launch_bounds__(kWave* W) grad_join_kernel(NormArgs a) {
+__global__ void __launch_bounds__(JoinGroup<W>::threads) grad_join_kernel(NormArgs a) {
+    if (!tiles_needed(a.seen, a.seenCount)) return;
+    using Join = JoinGroup<W>;
     __shared__ float red[W];
-    const std::uint64_t s = blockIdx.x / a.G;
-    const std::uint32_t g = blockIdx.x - static_cast<std::uint32_t>(s * a.G);
+    const std::uint64_t s = blockIdx.x;
+    const std::uint32_t g = Join::group();
     const std::uint64_t first = a.seg.start(s), end = a.seg.start(s + 1);
-    if (first >= end) return;
+    if (g >= a.G || first >= end || a.seg.whole(s)) return;
     const std::uint64_t t0 = first / a.tileRows, t1 = (end - 1) / a.tileRows;
     float s1 = 0.0f, s2 = 0.0f;
-    for (std::uint64_t t = t0 + threadIdx.x; t <= t1; t += kWave * W) {
+    for (std::uint64_t t = t0 + Join::first(); t <= t1; t += kWave * W) {
         const float2 p = a.part[(t + s) * a.G + g];
         s1 += p.x;
         s2 += p.y;
     }
-    s1 = group_sum<W>(s1, red);
-    s2 = group_sum<W>(s2, red);
+    s1 = Join::sum(s1, red);
+    s2 = Join::sum(s2, red);
     const float size = static_cast<float>(end - first) * static_cast<float>(a.K);
-    if (threadIdx.x == 0) a.sums[s * a.G + g] = float2{s1 / size, s2 / size};
+    if (Join::first() == 0) a.sums[s * a.G + g] = float2{s1 / size, s2 / size};
 }
 
-// dBias and dWeight from the tiles' sums: 16 columns a workgroup, 16 threads
-// a column.
-constexpr std::uint32_t kParamCols = 16;
-__global__ void __launch_bounds__(kThreads) param_grad_kernel(const float2* channel, std::uint64_t tiles, std::uint32_t C,
-                                                             float* dWeight, float* dBias) {
-    __shared__ float2 red[kThreads];
-    const std::uint32_t c = blockIdx.x * kParamCols + threadIdx.x % kParamCols;
+// dBias and dWeight from `rows` rows of partial sums: 4 columns a workgroup,
+// 256 threads a column; the tiles' rows come after the whole segments'.
+constexpr std::uint32_t kParamCols = 4, kParamRows = 256;
+__global__ void __launch_bounds__(kParamCols* kParamRows) param_grad_kernel(NormArgs a, std::uint64_t wholeRows,
+                                                                           std::uint64_t tiles, float* dWeight,
+                                                                           float* dBias) {
+    __shared__ float2 red[kParamCols * kParamRows];
+    const std::uint32_t c = blockIdx.x * kParamCols + threadIdx.x % kParamCols, C = a.C;
+    const float2* channel = a.channel;
+    const std::uint64_t rows = wholeRows + (tiles > 0 && tiles_needed(a.seen, a.seenCount) ? tiles : 0);
     float2 s{0.0f, 0.0f};
     if (c < C) {
-#pragma unroll 4
-        for (std::uint64_t t = threadIdx.x / kParamCols; t < tiles; t += kThreads / kParamCols) {
+#pragma unroll 8
+        for (std::uint64_t t = threadIdx.x / kParamCols; t < rows; t += kParamRows) {
             const float2 p = channel[t * C + c];
             s.x += p.x;
             s.y += p.y;
@@ -418,40 +496,41 @@ __global__ void __launch_bounds__(kThreads) param_grad_kernel(const float2* chan
     }
     red[threadIdx.x] = s;
     __syncthreads();
-    if (threadIdx.x < kParamCols && c < C) {
-        for (std::uint32_t i = 1; i < kThreads / kParamCols; ++i) {
-            s.x += red[i * kParamCols + threadIdx.x].x;
-            s.y += red[i * kParamCols + threadIdx.x].y;
+    for (std::uint32_t half = kParamRows / 2; half > 0; half /= 2) {
+        if (threadIdx.x < half * kParamCols) {
+            red[threadIdx.x].x += red[threadIdx.x + half * kParamCols].x;
+            red[threadIdx.x].y += red[threadIdx.x + half * kParamCols].y;
         }
-        if (dBias != nullptr) dBias[c] = s.x;
-        if (dWeight != nullptr) dWeight[c] = s.y;
+        __syncthreads();
+    }
+    if (threadIdx.x < kParamCols && c < C) {
+        if (dBias != nullptr) dBias[c] = red[threadIdx.x].x;
+        if (dWeight != nullptr) dWeight[c] = red[threadIdx.x].y;
     }
 }
 
-template <typename T, int N>
+template <typename T, int N, std::uint32_t ACT>
 __global__ void __launch_bounds__(kThreads) grad_apply_kernel(NormArgs a) {
+    if (!tiles_needed(a.seen, a.seenCount)) return;
     const std::uint64_t lo = blockIdx.x * a.tileRows, hi = min(lo + a.tileRows, a.seg.N);
     const std::uint32_t rl = threadIdx.x / a.colsV;
     const std::uint32_t cv0 = a.colsV > kThreads ? threadIdx.x : threadIdx.x - rl * a.colsV;
+    const std::uint64_t s0 = a.seg.find(lo);
     if (a.colsV <= kThreads && rl >= a.rowLanes) return;
     const std::uint32_t row = a.colsV > kThreads ? 0u : rl;
     const T* x = static_cast<const T*>(a.x);
     const T* dy = static_cast<const T*>(a.dy);
     T* dx = static_cast<T*>(a.out);
-    const std::uint64_t s0 = a.seg.find(lo);
     for (std::uint32_t cv = cv0; cv < a.colsV; cv += kThreads) {
-        float w[N], b[N];
+        const vec_t<float, N> w = load_params<N>(a.weight, a.paramType, cv * N, 1.0f);
+        const vec_t<float, N> b = load_params<N>(a.bias, a.paramType, cv * N, 0.0f);
         std::uint32_t g[N];
 #pragma unroll
-        for (int q = 0; q < N; ++q) {
-            w[q] = param_at(a.weight, a.paramType, cv * N + q, 1.0f);
-            b[q] = param_at(a.bias, a.paramType, cv * N + q, 0.0f);
-            g[q] = (cv * N + q) / a.K;
-        }
+        for (int q = 0; q < N; ++q) g[q] = (cv * N + q) / a.K;
         for (std::uint64_t s = s0; s < a.seg.B; ++s) {
             const std::uint64_t first = max(a.seg.start(s), lo), end = min(a.seg.start(s + 1), hi);
             if (a.seg.start(s) >= hi) break;
-            if (first >= end) continue;
+            if (first >= end || a.seg.whole(s)) continue;
             float mean[N], rstd[N];
             float2 m[N];
 #pragma unroll
@@ -468,12 +547,345 @@ __global__ void __launch_bounds__(kThreads) grad_apply_kernel(NormArgs a) {
 #pragma unroll
                 for (int q = 0; q < N; ++q) {
                     const float xh = normalise(v[q], mean[q], rstd[q]);
-                    const float dz = d[q] * slope(a.act, affine(xh, w[q], b[q]));
+                    const float dz = d[q] * slope<ACT>(affine(xh, w[q], b[q]));
                     o[q] = (dz * w[q] - m[q].x - xh * m[q].y) * rstd[q];
                 }
                 store_row<T, N>(dx + r * a.ldo + cv * N, o);
             }
         }
+    }
+}
+
+// ---------------------------------------------------------------- whole segments
+
+// A workgroup takes a segment (a slice of whole groups of it) at a time.  Rows
+// that fit its registers are read once; of longer segments the statistics come
+// from a first reading and the output from a second, which the caches mostly
+// serve.  A vector of a lane lies in one group (N divides K).  What a short
+// segment costs is the wait for its offsets, its rows and its sums, so the
+// workgroup is a single wave where that holds the usual segment: as many of
+// them as fit a CU wait at the same time.
+constexpr int kWholeThreads = 256;  // at most; one wave where segments are short
+
+struct WholeArgs {
+    std::uint32_t blocks;     // workgroups of a slice: the segments a grid's step apart
+    std::uint32_t slices;
+    std::uint32_t threads;    // of a workgroup
+    std::uint32_t groups;     // of a slice
+    std::uint32_t cols;       // its vectors a row
+    std::uint32_t laneBits;   // lanes of a row: a power of two that holds them, at most `threads`
+    std::uint32_t groupCols;  // vectors of a group
+};
+
+constexpr int kHeld = 8;  // rows a lane holds, as they are in memory
+
+// Sums of a pair of values over the lanes of each group, each lane getting its
+// own group's, in the same order every time.  `red` is not read by the call
+// before the next one's first wait, so two places used in turn need one wait.
+struct GroupSum {
+    std::uint32_t threads, lanes, groupCols, cv, g0;  // g0: the group's first vector
+    bool tree;                               // groups of a power of two of vectors
+
+    __device__ __forceinline__ float2 operator()(float2 v, float2* red) const {
+        for (std::uint32_t d = lanes; d < kWave; d <<= 1) {
+            v.x += __shfl_xor(v.x, d, kWave);
+            v.y += __shfl_xor(v.y, d, kWave);
+        }
+        const std::uint32_t inWave = min(groupCols, static_cast<std::uint32_t>(kWave));
+        if (tree)
+            for (std::uint32_t d = 1; d < inWave; d <<= 1) {
+                v.x += __shfl_xor(v.x, d, kWave);
+                v.y += __shfl_xor(v.y, d, kWave);
+            }
+        if (tree && threads == kWave) return v;
+        // rows of places: a wave's lanes' columns, or a row of lanes
+        const std::uint32_t rows = lanes < kWave ? threads / kWave : threads / lanes;
+        const std::uint32_t at = lanes < kWave ? threadIdx.x / kWave * lanes + cv : threadIdx.x;
+        if (lanes >= kWave || __lane_id() < lanes) red[at] = v;
+        __syncthreads();
+        const std::uint32_t step = tree ? inWave : 1u;
+        float2 s{0.0f, 0.0f};
+        for (std::uint32_t r = 0; r < rows; ++r)
+            for (std::uint32_t c = g0; c < g0 + groupCols; c += step) {
+                const float2 p = red[r * lanes + c];
+                s.x += p.x;
+                s.y += p.y;
+            }
+        return s;
+    }
+};
+
+// What a lane of a slice works on.
+template <int N>
+struct WholeLane {
+    std::uint32_t cv, row, rowLanes, c;  // its vector of the slice, row lane, the rows at once, its first channel
+    std::uint32_t g;                     // its group
+    std::uint32_t block;                 // the first of its segments
+    bool active;
+    GroupSum sum;
+    __device__ __forceinline__ WholeLane(const NormArgs& a, const WholeArgs& k) {
+        // 8 segments' first slices, then their second ones: the slices of a
+        // segment meet on one XCD (workgroups go to the 8 of them in turn),
+        // whose L2 then holds the lines that they share
+        const std::uint32_t turn = blockIdx.x / (8 * k.slices), place = blockIdx.x - turn * 8 * k.slices;
+        const std::uint32_t slice = place / 8;
+        block = turn * 8 + place % 8;
+        const std::uint32_t lanes = 1u << k.laneBits;
+        cv = threadIdx.x & (lanes - 1u);
+        row = threadIdx.x >> k.laneBits;
+        rowLanes = k.threads >> k.laneBits;
+        active = cv < k.cols;
+        const std::uint32_t inSlice = cv / k.groupCols;
+        g = slice * k.groups + inSlice;
+        c = (slice * k.cols + cv) * N;
+        sum = GroupSum{k.threads, lanes, k.groupCols, cv, min(inSlice, k.groups - 1) * k.groupCols,
+                       (k.groupCols & (k.groupCols - 1)) == 0};
+    }
+    // The most that a lane of this wave holds: its first lane's (rows rise with
+    // the lanes, and a row's first vector is active).
+    __device__ __forceinline__ static int most(int got) { return __builtin_amdgcn_readfirstlane(got); }
+    // How many of a segment's first kHeld * rowLanes rows it holds.
+    __device__ __forceinline__ int held(std::uint64_t rows) const {
+        const std::uint32_t n = static_cast<std::uint32_t>(min(rows, static_cast<std::uint64_t>(kHeld * rowLanes)));
+        return active && row < n ? static_cast<int>((n - row + rowLanes - 1) / rowLanes) : 0;
+    }
+};
+
+// Calls body(v...) for a lane's rows r, r + rowLanes, ... below `rows`, kBatch
+// of them loaded before the first is used; p... go from row r on.  Past the end
+// the last row is loaded again and not used: a loop for the remainder waited
+// for each of its rows in turn.
+template <typename T, int N, typename Body>
+__device__ __forceinline__ void each_row(std::uint64_t r, std::uint64_t rows, std::uint32_t rowLanes, const T* p,
+                                         std::uint64_t step, Body body) {
+    for (; r < rows; r += kBatch * rowLanes) {
+        const int more = static_cast<int>(min<std::uint64_t>(kBatch, (rows - r + rowLanes - 1) / rowLanes));
+        vec_t<T, N> v[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            v[i] = load_global<vec_t<T, N>>(p);
+            if (i + 1 < more) p += step;
+        }
+        p += step;
+        body(v, more);
+    }
+}
+template <typename T, int N, typename Body>
+__device__ __forceinline__ void each_row(std::uint64_t r, std::uint64_t rows, std::uint32_t rowLanes, const T* p,
+                                         std::uint64_t step, const T* q, std::uint64_t stepQ, Body body) {
+    for (; r < rows; r += kBatch * rowLanes) {
+        const int more = static_cast<int>(min<std::uint64_t>(kBatch, (rows - r + rowLanes - 1) / rowLanes));
+        vec_t<T, N> v[kBatch], u[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            v[i] = load_global<vec_t<T, N>>(p);
+            u[i] = load_global<vec_t<T, N>>(q);
+            if (i + 1 < more) {
+                p += step;
+                q += stepQ;
+            }
+        }
+        p += step;
+        q += stepQ;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+            if (i < more) body(__builtin_convertvector(v[i], vec_t<float, N>), __builtin_convertvector(u[i], vec_t<float, N>));
+    }
+}
+
+// Keeps what was computed from v before this point from being held beside it
+// until after (N floats and N normalised values for each packed vector).
+template <typename V>
+__device__ __forceinline__ void forget(V& v) {
+    if constexpr (sizeof(V) == 2) {
+        std::uint32_t u = __builtin_bit_cast(std::uint16_t, v);
+        asm volatile("" : "+v"(u));
+        v = __builtin_bit_cast(V, static_cast<std::uint16_t>(u));
+    } else if constexpr (sizeof(V) == 4) {
+        std::uint32_t u = __builtin_bit_cast(std::uint32_t, v);
+        asm volatile("" : "+v"(u));
+        v = __builtin_bit_cast(V, u);
+    } else {
+        vec_t<std::uint32_t, sizeof(V) / 4> u = __builtin_bit_cast(decltype(u), v);
+        asm volatile("" : "+v"(u));
+        v = __builtin_bit_cast(V, u);
+    }
+}
+
+// A lane's values so far: their count, mean and squared deviations from it.
+struct Deviations {
+    float count = 0.0f, mean = 0.0f, dev = 0.0f;
+    // the first `got` of R vectors
+    template <int R, typename T, int N>
+    __device__ __forceinline__ void add(vec_t<T, N> (&v)[R], int got) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const vec_t<float, N> f = __builtin_convertvector(v[i], vec_t<float, N>);
+#pragma unroll
+            for (int q = 0; q < N; ++q) sum += i < got ? f[q] : 0.0f;
+        }
+        const float more = static_cast<float>(got * N);
+        const float m = sum / more;
+        float d = 0.0f;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            forget(v[i]);
+            const vec_t<float, N> f = __builtin_convertvector(v[i], vec_t<float, N>);
+#pragma unroll
+            for (int q = 0; q < N; ++q) {
+                const float e = i < got ? f[q] - m : 0.0f;
+                d = fmaf(e, e, d);
+            }
+        }
+        const float share = more / (count + more), gap = m - mean;
+        mean += gap * share;
+        dev += d + gap * gap * (count * share);
+        count += more;
+    }
+};
+
+template <typename T, int N, std::uint32_t ACT>
+__global__ void __launch_bounds__(kWholeThreads, 4) whole_kernel(NormArgs a, WholeArgs k) {
+    extern __shared__ float2 places[];  // two of a GroupSum
+    float2* const red[2] = {places, places + k.threads};
+    const WholeLane<N> me(a, k);
+    const std::uint32_t c = me.active ? me.c : 0u;
+    const vec_t<float, N> w = load_params<N>(a.weight, a.paramType, c, 1.0f), b = load_params<N>(a.bias, a.paramType, c, 0.0f);
+    std::uint8_t anyLong = 0;
+    for (std::uint64_t s = me.block; s < a.seg.B; s += k.blocks) {
+        const std::uint64_t first = a.seg.start(s), end = a.seg.start(s + 1);
+        if (first < end && end - first > a.seg.longest) {
+            anyLong = 1;
+            continue;
+        }
+        const std::uint64_t rows = first < end ? end - first : 0;
+        const T* x = static_cast<const T*>(a.x) + (first + me.row) * a.ldx + me.c;
+        T* y = static_cast<T*>(a.out) + (first + me.row) * a.ldo + me.c;
+        float gm = 0.0f, rs = 0.0f;
+        // the group's mean and rstd from the lanes' deviations, kept for the gradient
+        const auto settle = [&](const Deviations& mine) {
+            const float size = static_cast<float>(rows) * static_cast<float>(a.K);
+            if (rows > 0) {
+                gm = me.sum(float2{mine.count * mine.mean, 0.0f}, red[0]).x / size;
+                const float gap = mine.mean - gm;
+                rs = me.sum(float2{mine.dev + mine.count * gap * gap, 0.0f}, red[1]).x / size;
+            }
+            rs = 1.0f / sqrtf(rs + a.eps);
+            if (me.active && me.row == 0 && me.cv == me.sum.g0) {
+                a.mean[s * a.G + me.g] = gm;
+                a.rstd[s * a.G + me.g] = rs;
+            }
+        };
+        const auto apply = [&](vec_t<float, N> v, T* to) {
+            vec_t<float, N> o;
+#pragma unroll
+            for (int q = 0; q < N; ++q) o[q] = activate<ACT>(affine(normalise(v[q], gm, rs), w[q], b[q]));
+            store_row<T, N>(to, o);
+        };
+        Deviations mine;
+        if (me.active)
+            each_row<T, N>(me.row, rows, me.rowLanes, x, me.rowLanes * a.ldx,
+                           [&](vec_t<T, N>(&v)[kBatch], int more) { mine.template add<kBatch, T, N>(v, more); });
+        settle(mine);
+        if (me.active)
+            each_row<T, N>(me.row, rows, me.rowLanes, x, me.rowLanes * a.ldx, [&](vec_t<T, N>(&v)[kBatch], int more) {
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i)
+                    if (i < more) {
+                        apply(__builtin_convertvector(v[i], vec_t<float, N>), y);
+                        y += me.rowLanes * a.ldo;
+                    }
+            });
+    }
+    // places past `blocks` that the tiles' 16-byte loads take in
+    if (me.c == 0 && me.row == 0 && a.seenCount > 0) {
+        if (me.block < k.blocks) a.seen[me.block] = anyLong;
+        if (me.block + 1 == k.blocks)
+            for (std::uint32_t i = k.blocks; i % 16 != 0; ++i) a.seen[i] = 0;
+    }
+}
+
+// `partial`: where this workgroup's dBias and dWeight go ([blocks][C]).
+template <typename T, int N, std::uint32_t ACT>
+__global__ void __launch_bounds__(kWholeThreads, 3) whole_grad_kernel(NormArgs a, WholeArgs k, float2* partial) {
+    extern __shared__ float2 places[];  // two of a GroupSum, then dBias and dWeight of every lane
+    float2* const all = places + 2 * k.threads;
+    const WholeLane<N> me(a, k);
+    const std::uint32_t c = me.active ? me.c : 0u;
+    const vec_t<float, N> w = load_params<N>(a.weight, a.paramType, c, 1.0f), b = load_params<N>(a.bias, a.paramType, c, 0.0f);
+    vec_t<float, N> dw(0.0f), db(0.0f);
+    std::uint32_t turn = 0;
+    std::uint8_t anyLong = 0;
+    for (std::uint64_t s = me.block; s < a.seg.B; s += k.blocks) {
+        const std::uint64_t first = a.seg.start(s), end = a.seg.start(s + 1);
+        if (first >= end) continue;
+        if (end - first > a.seg.longest) {
+            anyLong = 1;
+            continue;
+        }
+        const std::uint64_t rows = end - first;
+        const float mean = me.active ? a.mean[s * a.G + me.g] : 0.0f, rstd = me.active ? a.rstd[s * a.G + me.g] : 0.0f;
+        const T* x = static_cast<const T*>(a.x) + (first + me.row) * a.ldx + me.c;
+        const T* dy = static_cast<const T*>(a.dy) + (first + me.row) * a.lddy + me.c;
+        T* dx = static_cast<T*>(a.out) + (first + me.row) * a.ldo + me.c;
+        float2 part{0.0f, 0.0f}, m{0.0f, 0.0f};
+        // dz, counted in the sums
+        const auto gather = [&](vec_t<float, N> v, vec_t<float, N> d) {
+#pragma unroll
+            for (int q = 0; q < N; ++q) {
+                const float xh = normalise(v[q], mean, rstd);
+                const float z = d[q] * slope<ACT>(affine(xh, w[q], b[q]));
+                db[q] += z;
+                dw[q] = fmaf(z, xh, dw[q]);
+                part.x = fmaf(z, w[q], part.x);
+                part.y = fmaf(z * w[q], xh, part.y);
+            }
+        };
+        const auto settle = [&] {
+            const float size = static_cast<float>(rows) * static_cast<float>(a.K);
+            m = me.sum(part, places + turn * k.threads);
+            turn ^= 1u;
+            m.x /= size;
+            m.y /= size;
+        };
+        const auto apply = [&](vec_t<float, N> v, vec_t<float, N> d, T* to) {
+            vec_t<float, N> o;
+#pragma unroll
+            for (int q = 0; q < N; ++q) {
+                const float xh = normalise(v[q], mean, rstd);
+                o[q] = (d[q] * slope<ACT>(affine(xh, w[q], b[q])) * w[q] - m.x - xh * m.y) * rstd;
+            }
+            store_row<T, N>(to, o);
+        };
+        if (me.active) each_row<T, N>(me.row, rows, me.rowLanes, x, me.rowLanes * a.ldx, dy, me.rowLanes * a.lddy, gather);
+        settle();
+        if (me.active)
+            each_row<T, N>(me.row, rows, me.rowLanes, x, me.rowLanes * a.ldx, dy, me.rowLanes * a.lddy,
+                           [&](vec_t<float, N> v, vec_t<float, N> d) {
+                               apply(v, d, dx);
+                               dx += me.rowLanes * a.ldo;
+                           });
+    }
+    // places past `blocks` that the tiles' 16-byte loads take in
+    if (me.c == 0 && me.row == 0 && a.seenCount > 0) {
+        if (me.block < k.blocks) a.seen[me.block] = anyLong;
+        if (me.block + 1 == k.blocks)
+            for (std::uint32_t i = k.blocks; i % 16 != 0; ++i) a.seen[i] = 0;
+    }
+    if (partial == nullptr || me.block >= k.blocks) return;
+#pragma unroll
+    for (int q = 0; q < N; ++q) all[threadIdx.x * N + q] = float2{db[q], dw[q]};
+    __syncthreads();
+    const std::uint32_t lanes = 1u << k.laneBits;
+    for (std::uint32_t i = threadIdx.x; i < k.cols * N; i += k.threads) {
+        float2 s{0.0f, 0.0f};
+        for (std::uint32_t r = 0; r < me.rowLanes; ++r) {
+            const float2 p = all[(r * lanes) * N + i];
+            s.x += p.x;
+            s.y += p.y;
+        }
+        partial[me.block * static_cast<std::uint64_t>(a.C) + (me.c - me.cv * N) + i] = s;
     }
 }
 
@@ -483,25 +895,91 @@ constexpr std::size_t align16(std::size_t b) { return (b + 15) & ~std::size_t(15
 
 // Tiles of at most this many, so that the tiles' sums stay few.
 constexpr std::uint64_t kTiles = 2048;
+// A segment that a workgroup walks in at most this many steps goes whole (some
+// 20 us; a longer one would end after all others), and all segments do where x
+// has no more than kSmallBytes.
+constexpr std::uint64_t kWholeSteps = 32, kSmallBytes = 1 << 20;
+// Workgroups of a slice of whole segments, each with its own dWeight and dBias.
+constexpr std::uint64_t kWholeBlocks = 4096;
+
+// Elements a lane takes in a whole segment, of `width` that the rows allow: a
+// power of two that divides a group.
+std::uint32_t whole_width(std::uint32_t K, std::uint32_t width) {
+    while (K % width != 0) width /= 2;
+    return width;
+}
+
+// How whole segments are cut, for lanes of n elements: into slices of whole
+// groups of at least 128 bytes a row (64 where fewer than 1024 segments have to
+// spread over the GPU), a wave for a slice where that takes the usual segment in
+// one step of loads, else four.  169,000 rows of 128 bf16 channels, forward and
+// gradient together: in segments of 21 rows 97 us with one wave and 268 us with
+// four, of 85 rows (four times as many) 224 us and 207 us; whole rows instead
+// of slices cost 2 to 10% more.
+WholeArgs whole_args(const tcc_group_norm_shape& s, std::uint32_t n) {
+    const std::uint32_t elem = dtype_bytes(s.dtype), K = s.C / s.G;
+    WholeArgs k{};
+    k.groupCols = K / n;
+    for (std::uint32_t g = 1; g <= s.G; ++g) {
+        if (s.G % g != 0) continue;
+        if (g > 1 && g * k.groupCols > kWholeThreads) break;
+        k.groups = g;
+        if (g * K * elem >= (s.B < 1024 ? 64 : 128)) break;
+    }
+    k.slices = s.G / k.groups;
+    k.cols = k.groups * k.groupCols;
+    while ((1u << k.laneBits) < k.cols) ++k.laneBits;
+    const bool wave = s.B >= 1024 && k.cols <= kWave && s.N / s.B <= kBatch * (kWave >> k.laneBits);
+    k.threads = wave ? kWave : kWholeThreads;
+    return k;
+}
+
+// Which segments go whole and which tile by tile, from what the host knows.
+struct Split {
+    std::uint64_t longest;  // rows of a segment that goes whole
+    bool whole, tiles;      // whether either kind may occur
+    // `width`: elements a lane can take at once, by the rows' alignment
+    Split(const tcc_group_norm_shape& s, std::uint32_t width) {
+        const std::uint32_t elem = dtype_bytes(s.dtype), K = s.C / s.G;
+        const std::uint64_t row = static_cast<std::uint64_t>(s.C) * elem;
+        const std::uint64_t most = s.offsets == nullptr ? (s.B > 0 ? s.N / s.B : 0) : s.maxRows > 0 ? s.maxRows : s.N;
+        const std::uint32_t aligned = whole_width(K, 16 / elem);
+        if (K / whole_width(K, width) > kWholeThreads || K / aligned > kWholeThreads) {
+            longest = 0;  // groups wider than a workgroup
+        } else if (s.N * row <= kSmallBytes) {
+            longest = s.N;
+        } else {
+            const WholeArgs k = whole_args(s, aligned);
+            longest = kWholeSteps * (k.threads >> k.laneBits);
+        }
+        tiles = s.N > 0 && (most > longest || s.N > s.B * most);
+        if (!tiles) longest = s.N;  // whatever maxRows says
+        whole = longest > 0 && (s.offsets != nullptr || most <= longest);
+    }
+};
 
 struct Layout {
-    std::uint64_t tileRows, tiles;
-    std::size_t part, sums, channel, bytes;
+    std::uint64_t tileRows, tiles, wholeRows;
+    std::size_t part, sums, channel, seen, bytes;
     Layout(const tcc_group_norm_shape& s, bool backward) {
+        const Split split(s, 16 / dtype_bytes(s.dtype));
+        const bool unaligned = s.C / s.G > kWholeThreads;  // room for rows that cannot go whole
         // at least 32 rows of a tile, however narrow the rows: a tile's own
         // reductions cost about as much
         tileRows = std::max<std::uint64_t>((s.N + kTiles - 1) / kTiles, 32);
-        tiles = (s.N + tileRows - 1) / tileRows;
+        tiles = split.tiles || unaligned ? (s.N + tileRows - 1) / tileRows : 0;
+        wholeRows = split.whole && backward ? std::min(s.B, kWholeBlocks) : 0;
         part = 0;
-        std::size_t at = align16((tiles + s.B) * s.G * sizeof(float2));
+        std::size_t at = tiles > 0 ? align16((tiles + s.B) * s.G * sizeof(float2)) : 0;
         sums = at;
         channel = at;
         if (backward) {
-            at += align16(s.B * s.G * sizeof(float2));
+            if (tiles > 0) at += align16(s.B * s.G * sizeof(float2));
             channel = at;
-            at += align16(tiles * s.C * sizeof(float2));
+            at += align16((wholeRows + tiles) * s.C * sizeof(float2));
         }
-        bytes = at;
+        seen = at;
+        bytes = at + kWholeBlocks;
     }
 };
 
@@ -524,60 +1002,85 @@ int check_shape(const tcc_group_norm_shape* s) {
     return TCC_OK;
 }
 
+// A kernel's form for the activation.
+#define TCC_BY_ACT(kernel, T, N, grid, threads, lds, st, ...)                                                   \
+    do {                                                                                                        \
+        auto* form = a.act == TCC_ACT_NONE   ? &kernel<T, N, TCC_ACT_NONE>                                      \
+                     : a.act == TCC_ACT_RELU ? &kernel<T, N, TCC_ACT_RELU>                                      \
+                     : a.act == TCC_ACT_SILU ? &kernel<T, N, TCC_ACT_SILU>                                      \
+                                             : &kernel<T, N, TCC_ACT_GELU>;                                     \
+        hipLaunchKernelGGL(form, grid, dim3(threads), lds, st, __VA_ARGS__);                                    \
+    } while (0)
+
+dim3 whole_grid(const WholeArgs& k) { return dim3((k.blocks + 7) / 8 * 8 * k.slices); }
+
 template <typename T, int N>
-int forward_launch(NormArgs a, const Layout& lay, std::uint64_t B, hipStream_t st) {
-    a.colsV = a.C / N;
-    a.rowLanes = std::max<std::uint32_t>(1, kThreads / a.colsV);
-    const unsigned tiles = static_cast<unsigned>(lay.tiles);
-    if (tiles > 0) {
-        hipLaunchKernelGGL((stats_kernel<T, N>), dim3(tiles), dim3(kThreads), 2 * a.rowLanes * a.C * sizeof(float), st, a);
-        TCC_LAUNCH_CHECK();
-    }
-    const unsigned groups = static_cast<unsigned>(B * a.G);
-    if (lay.tiles > 64 * B) hipLaunchKernelGGL(stats_join_kernel<4>, dim3(groups), dim3(4 * kWave), 0, st, a);
-    else hipLaunchKernelGGL(stats_join_kernel<1>, dim3(groups), dim3(kWave), 0, st, a);
+int whole_launch(const NormArgs& a, WholeArgs k, hipStream_t st) {
+    TCC_BY_ACT(whole_kernel, T, N, whole_grid(k), k.threads, 2 * k.threads * sizeof(float2), st, a, k);
     TCC_LAUNCH_CHECK();
-    if (tiles > 0) {
-        hipLaunchKernelGGL((apply_kernel<T, N>), dim3(tiles), dim3(kThreads), 0, st, a);
-        TCC_LAUNCH_CHECK();
-    }
     return TCC_OK;
 }
 
 template <typename T, int N>
-int backward_launch(NormArgs a, const Layout& lay, std::uint64_t B, float* dWeight, float* dBias, hipStream_t st) {
-    a.colsV = a.C / N;
-    a.rowLanes = std::max<std::uint32_t>(1, kThreads / a.colsV);
-    const unsigned tiles = static_cast<unsigned>(lay.tiles);
-    if (tiles > 0) {
-        hipLaunchKernelGGL((grad_sums_kernel<T, N>), dim3(tiles), dim3(kThreads), 4 * a.rowLanes * a.C * sizeof(float), st,
-                           a);
-        TCC_LAUNCH_CHECK();
-        const unsigned groups = static_cast<unsigned>(B * a.G);
-        if (lay.tiles > 64 * B) hipLaunchKernelGGL(grad_join_kernel<4>, dim3(groups), dim3(4 * kWave), 0, st, a);
-        else hipLaunchKernelGGL(grad_join_kernel<1>, dim3(groups), dim3(kWave), 0, st, a);
-        TCC_LAUNCH_CHECK();
-    }
-    if (dWeight != nullptr || dBias != nullptr) {
-        hipLaunchKernelGGL(param_grad_kernel, dim3((a.C + kParamCols - 1) / kParamCols), dim3(kThreads), 0, st, a.channel,
-                           lay.tiles, a.C, dWeight, dBias);
-        TCC_LAUNCH_CHECK();
-    }
-    if (tiles > 0) {
-        hipLaunchKernelGGL((grad_apply_kernel<T, N>), dim3(tiles), dim3(kThreads), 0, st, a);
-        TCC_LAUNCH_CHECK();
-    }
+int whole_grad_launch(const NormArgs& a, WholeArgs k, bool params, hipStream_t st) {
+    TCC_BY_ACT(whole_grad_kernel, T, N, whole_grid(k), k.threads, (2 + N) * k.threads * sizeof(float2), st, a, k,
+               params ? a.channel : nullptr);
+    TCC_LAUNCH_CHECK();
     return TCC_OK;
 }
 
-NormArgs base_args(const tcc_group_norm_shape& s, const Layout& lay, void* workspace) {
+int stats_join_launch(const NormArgs& a, const Layout& lay, std::uint64_t B, hipStream_t st) {
+    if (lay.tiles > 64 * B)
+        hipLaunchKernelGGL(stats_join_kernel<4>, dim3(static_cast<unsigned>(B), JoinGroup<4>::grid(a.G)),
+                           dim3(JoinGroup<4>::threads), 0, st, a);
+    else
+        hipLaunchKernelGGL(stats_join_kernel<1>, dim3(static_cast<unsigned>(B), JoinGroup<1>::grid(a.G)),
+                           dim3(JoinGroup<1>::threads), 0, st, a);
+    TCC_LAUNCH_CHECK();
+    return TCC_OK;
+}
+
+template <typename T, int N>
+int tiles_launch(NormArgs a, const Layout& lay, std::uint64_t B, hipStream_t st) {
+    a.colsV = a.C / N;
+    a.rowLanes = std::max<std::uint32_t>(1, kThreads / a.colsV);
+    const unsigned tiles = static_cast<unsigned>(lay.tiles);
+    hipLaunchKernelGGL((stats_kernel<T, N>), dim3(tiles), dim3(kThreads), 2 * a.rowLanes * a.C * sizeof(float), st, a);
+    TCC_LAUNCH_CHECK();
+    if (const int rc = stats_join_launch(a, lay, B, st)) return rc;
+    TCC_BY_ACT(apply_kernel, T, N, dim3(tiles), kThreads, 0, st, a);
+    TCC_LAUNCH_CHECK();
+    return TCC_OK;
+}
+
+template <typename T, int N>
+int tiles_grad_launch(NormArgs a, const Layout& lay, std::uint64_t B, hipStream_t st) {
+    a.colsV = a.C / N;
+    a.rowLanes = std::max<std::uint32_t>(1, kThreads / a.colsV);
+    const unsigned tiles = static_cast<unsigned>(lay.tiles);
+    TCC_BY_ACT(grad_sums_kernel, T, N, dim3(tiles), kThreads, 4 * a.rowLanes * a.C * sizeof(float), st, a);
+    TCC_LAUNCH_CHECK();
+    if (lay.tiles > 64 * B)
+        hipLaunchKernelGGL(grad_join_kernel<4>, dim3(static_cast<unsigned>(B), JoinGroup<4>::grid(a.G)),
+                           dim3(JoinGroup<4>::threads), 0, st, a);
+    else
+        hipLaunchKernelGGL(grad_join_kernel<1>, dim3(static_cast<unsigned>(B), JoinGroup<1>::grid(a.G)),
+                           dim3(JoinGroup<1>::threads), 0, st, a);
+    TCC_LAUNCH_CHECK();
+    TCC_BY_ACT(grad_apply_kernel, T, N, dim3(tiles), kThreads, 0, st, a);
+    TCC_LAUNCH_CHECK();
+    return TCC_OK;
+}
+
+NormArgs base_args(const tcc_group_norm_shape& s, const Layout& lay, const Split& split, void* workspace) {
     NormArgs a{};
-    a.seg = Segments{s.offsets, s.N, s.B, s.B > 0 ? s.N / s.B : 0, s.offsetBytes == 8};
+    a.seg = Segments{s.offsets, s.N, s.B, s.B > 0 ? s.N / s.B : 0, s.offsetBytes == 8, split.longest};
     if (s.offsets == nullptr && a.seg.each == 0) a.seg.each = 1;  // no rows: never read
     char* ws = static_cast<char*>(workspace);
     a.part = reinterpret_cast<float2*>(ws + lay.part);
     a.sums = reinterpret_cast<float2*>(ws + lay.sums);
     a.channel = reinterpret_cast<float2*>(ws + lay.channel);
+    a.seen = reinterpret_cast<std::uint8_t*>(ws + lay.seen);
     a.tileRows = lay.tileRows;
     a.C = s.C;
     a.G = s.G;
@@ -588,16 +1091,17 @@ NormArgs base_args(const tcc_group_norm_shape& s, const Layout& lay, void* works
     return a;
 }
 
-#define TCC_BY_WIDTH(T, MAXN, width, CALL)            \
-    do {                                              \
-        if ((MAXN) >= 8 && (width) >= 8) {            \
-            constexpr int N = (MAXN) >= 8 ? 8 : 1;    \
-            return CALL(T, N);                        \
-        }                                             \
-        if ((width) >= 4) return CALL(T, 4);          \
-        if ((width) >= 2) return CALL(T, 2);          \
-        return CALL(T, 1);                            \
-    } while (0)
+// CALL(T, N) for an element type and a lane's elements.
+#define TCC_BY_TYPE(dtype, n, CALL)                                                                      \
+    ((dtype) == TCC_F32    ? ((n) >= 4 ? CALL(float, 4) : (n) >= 2 ? CALL(float, 2) : CALL(float, 1))    \
+     : (dtype) == TCC_BF16 ? ((n) >= 8   ? CALL(bf16_t, 8)                                               \
+                              : (n) >= 4 ? CALL(bf16_t, 4)                                               \
+                              : (n) >= 2 ? CALL(bf16_t, 2)                                               \
+                                         : CALL(bf16_t, 1))                                              \
+                           : ((n) >= 8   ? CALL(f16_t, 8)                                                \
+                              : (n) >= 4 ? CALL(f16_t, 4)                                                \
+                              : (n) >= 2 ? CALL(f16_t, 2)                                                \
+                                         : CALL(f16_t, 1)))
 
 }  // namespace
 }  // namespace tcc
@@ -622,7 +1126,9 @@ int tcc_group_norm(const tcc_group_norm_shape* s, const void* x, uint64_t ldx, c
                     reinterpret_cast<std::uintptr_t>(workspace) % 16 == 0,
                 TCC_ERR_INVALID_ARGUMENT, "group norm workspace too small or unaligned (tcc_group_norm_workspace_bytes)");
     if (s->B == 0) return TCC_OK;
-    NormArgs a = base_args(*s, lay, workspace);
+    const std::uint32_t w = RowWidth(s->C, dtype_bytes(s->dtype)).with(x).with(y).stride(ldx).stride(ldy).elems();
+    const Split split(*s, w);
+    NormArgs a = base_args(*s, lay, split, workspace);
     a.x = x;
     a.ldx = ldx;
     a.weight = weight;
@@ -631,12 +1137,20 @@ int tcc_group_norm(const tcc_group_norm_shape* s, const void* x, uint64_t ldx, c
     a.ldo = ldy;
     a.mean = mean;
     a.rstd = rstd;
-    const std::uint32_t w = RowWidth(s->C, dtype_bytes(s->dtype)).with(x).with(y).stride(ldx).stride(ldy).elems();
     const hipStream_t st = as_stream(stream);
-#define CALL(T, N) (forward_launch<T, N>(a, lay, s->B, st))
-    if (s->dtype == TCC_F32) TCC_BY_WIDTH(float, 4, w, CALL);
-    if (s->dtype == TCC_BF16) TCC_BY_WIDTH(bf16_t, 8, w, CALL);
-    TCC_BY_WIDTH(f16_t, 8, w, CALL);
+    if (split.whole) {
+        const std::uint32_t n = whole_width(a.K, w);
+        WholeArgs k = whole_args(*s, n);
+        k.blocks = static_cast<std::uint32_t>(std::min(s->B, kWholeBlocks));
+        if (split.tiles) a.seenCount = k.blocks;
+#define CALL(T, N) (whole_launch<T, N>(a, k, st))
+        if (const int rc = TCC_BY_TYPE(s->dtype, n, CALL)) return rc;
+#undef CALL
+    }
+    if (s->N == 0) return stats_join_launch(a, lay, s->B, st);  // segments without rows
+    if (!split.tiles) return TCC_OK;
+#define CALL(T, N) (tiles_launch<T, N>(a, lay, s->B, st))
+    return TCC_BY_TYPE(s->dtype, w, CALL);
 #undef CALL
 }
 
@@ -652,7 +1166,10 @@ int tcc_group_norm_grad(const tcc_group_norm_shape* s, const void* dY, uint64_t 
     TCC_REQUIRE((workspace || lay.bytes == 0) && workspaceBytes >= lay.bytes &&
                     reinterpret_cast<std::uintptr_t>(workspace) % 16 == 0,
                 TCC_ERR_INVALID_ARGUMENT, "group norm workspace too small or unaligned (tcc_group_norm_workspace_bytes)");
-    NormArgs a = base_args(*s, lay, workspace);
+    const std::uint32_t w = RowWidth(s->C, dtype_bytes(s->dtype)).with(dY).with(x).with(dX).stride(lddy).stride(ldx)
+                                .stride(lddx).elems();
+    const Split split(*s, w);
+    NormArgs a = base_args(*s, lay, split, workspace);
     a.x = x;
     a.ldx = ldx;
     a.dy = dY;
@@ -663,14 +1180,31 @@ int tcc_group_norm_grad(const tcc_group_norm_shape* s, const void* dY, uint64_t 
     a.ldo = lddx;
     a.mean = const_cast<float*>(mean);
     a.rstd = const_cast<float*>(rstd);
-    const std::uint32_t w = RowWidth(s->C, dtype_bytes(s->dtype)).with(dY).with(x).with(dX).stride(lddy).stride(ldx)
-                                .stride(lddx).elems();
     const hipStream_t st = as_stream(stream);
-#define CALL(T, N) (backward_launch<T, N>(a, lay, s->B, dWeight, dBias, st))
-    if (s->dtype == TCC_F32) TCC_BY_WIDTH(float, 4, w, CALL);
-    if (s->dtype == TCC_BF16) TCC_BY_WIDTH(bf16_t, 8, w, CALL);
-    TCC_BY_WIDTH(f16_t, 8, w, CALL);
+    const bool params = dWeight != nullptr || dBias != nullptr;
+    const std::uint64_t wholeRows = split.whole ? lay.wholeRows : 0, tileRows = split.tiles ? lay.tiles : 0;
+    if (wholeRows > 0) {
+        const std::uint32_t n = whole_width(a.K, w);
+        WholeArgs k = whole_args(*s, n);
+        k.blocks = static_cast<std::uint32_t>(wholeRows);
+        if (split.tiles) a.seenCount = k.blocks;
+#define CALL(T, N) (whole_grad_launch<T, N>(a, k, params, st))
+        if (const int rc = TCC_BY_TYPE(s->dtype, n, CALL)) return rc;
 #undef CALL
+    }
+    if (tileRows > 0) {
+        NormArgs at = a;
+        at.channel += wholeRows * a.C;
+#define CALL(T, N) (tiles_grad_launch<T, N>(at, lay, s->B, st))
+        if (const int rc = TCC_BY_TYPE(s->dtype, w, CALL)) return rc;
+#undef CALL
+    }
+    if (params) {
+        hipLaunchKernelGGL(param_grad_kernel, dim3((a.C + kParamCols - 1) / kParamCols), dim3(kParamCols * kParamRows), 0,
+                           st, a, wholeRows, tileRows, dWeight, dBias);
+        TCC_LAUNCH_CHECK();
+    }
+    return TCC_OK;
 }
 
 }  // extern "C"

@@ -151,6 +151,35 @@ def test_both_passes(gpu, dtype, kind, N, C, G):
                 assert torch.equal(p, q), "the same inputs give the same bits"
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("long", [0, 9000])
+@pytest.mark.parametrize("N,C,G,mean_rows", [(30_000, 64, 8, 15), (30_000, 24, 2, 20), (40_000, 33, 11, 150),
+                                             (12_000, 520, 1, 7), (12_000, 606, 2, 100)])
+def test_many_short_segments_with_a_long_one(gpu, dtype, long, N, C, G, mean_rows):
+    """Over a thousand segments (a wave each) or hundreds (a workgroup each),
+    with empty ones, and one that is too long for either, whether the
+    longest is known or not."""
+    from tcc_amd import training
+
+    gen, x, w, b, d = inputs(N, C, dtype, N + C)
+    cuts = torch.randint(0, N - long, ((N - long) // mean_rows,), generator=gen)
+    at = torch.sort(torch.cat([torch.tensor([0, N - long, N]), cuts])).values
+    off, at = at.cuda(), at.tolist()
+    act = ["relu", "silu", "gelu"][TYPES.index(dtype)]
+    first = None
+    for rows in (None, max(hi - lo for lo, hi in zip(at[:-1], at[1:]))):
+        got = training.group_norm(x, G, w, b, offsets=off, activation=act, max_rows=rows)
+        back = training.group_norm_grad(d, x, got[1], got[2], G, w, b, offsets=off, activation=act, max_rows=rows)
+        if first is None:
+            first = got, back
+            check_forward(got, x, G, w, b, at, 1e-5, act)
+            check_grad(back, d, x, got[1], got[2], G, w, b, at, act)
+        else:  # another split at most: the same values
+            for p, q in zip(got + back, first[0] + first[1]):
+                assert bool(torch.isfinite(p).all())
+                assert float((p.double() - q.double()).norm() / q.double().norm()) <= (1e-6 if p.dtype == torch.float32 else 1e-3)
+
+
 @pytest.mark.parametrize("weight,bias,ptype", [(False, False, torch.float32), (True, False, torch.float32),
                                                (False, True, torch.bfloat16), (True, True, torch.bfloat16),
                                                (True, True, torch.float16)])
