@@ -50,11 +50,14 @@ __device__ __forceinline__ void report(std::uint32_t* err, bool bad) {
 constexpr int kLookupUnroll = 4;
 
 // The output as one run of n * colsV vectors, kThreads * kLookupUnroll of
-// them a workgroup, so that no lane idles whatever the width.
+// them a workgroup, so that no lane idles whatever the width.  Large outputs
+// are written past the caches' order, which leaves those to rows that come
+// again: 2.45M x 100 rows of bf16 248 us instead of 270, of fp32 323 instead
+// of 359 (4 vectors a lane; with 2 of them 257 and 318, with 8 over 600).
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads) lookup_kernel(const T* __restrict__ table, std::uint64_t ldt, Ids ids,
                                                          std::uint64_t n, std::uint32_t colsV, float scale,
-                                                         T* __restrict__ out, std::uint64_t ldo, std::uint32_t* err) {
+                                                         T* __restrict__ out, std::uint64_t ldo, bool once, std::uint32_t* err) {
     const std::uint64_t first = static_cast<std::uint64_t>(blockIdx.x) * (kThreads * kLookupUnroll);
     const std::uint64_t row0 = first / colsV;
     const std::uint32_t col0 = static_cast<std::uint32_t>(first - row0 * colsV);
@@ -78,7 +81,7 @@ __global__ void __launch_bounds__(kThreads) lookup_kernel(const T* __restrict__ 
     }
 #pragma unroll
     for (int u = 0; u < kLookupUnroll; ++u)
-        if (i[u] < n) store_row<T, N>(out + i[u] * ldo + c[u], x[u]);
+        if (i[u] < n) write_out<T, N>(once, out + i[u] * ldo + c[u], x[u]);
     report(err, bad);
 }
 
@@ -102,13 +105,14 @@ struct IdKeys {
     __device__ __forceinline__ void report(bool bad) const { tcc::report(err, bad); }
 };
 
-__global__ void __launch_bounds__(kThreads) mark_kernel(Ids ids, std::uint64_t n, std::uint8_t* __restrict__ mark) {
+// Marks the rows that occur, from the sorted keys: neighbours in memory (from
+// the ids as they come, 2.45M of them took 16 us instead of TODO).
+__global__ void __launch_bounds__(kThreads) mark_kernel(const std::uint64_t* __restrict__ keys, std::uint64_t n,
+                                                       std::uint64_t V, std::uint8_t* __restrict__ mark) {
     const std::uint64_t i = static_cast<std::uint64_t>(blockIdx.x) * kThreads + threadIdx.x;
-    bool bad = false;
-    if (i < n) {
-        const std::uint32_t v = ids.row(i, bad);
-        if (v != kNoRow) mark[v] = 1;
-    }
+    if (i >= n) return;
+    const std::uint32_t v = static_cast<std::uint32_t>(keys[i] >> 32);
+    if (v < V && (i == 0 || static_cast<std::uint32_t>(keys[i - 1] >> 32) != v)) mark[v] = 1;
 }
 
 struct GradArgs {
@@ -121,6 +125,7 @@ struct GradArgs {
     std::uint32_t D, chunk, chunks, laneBits, sumBlocks;
     float scale;
     int accumulate;
+    bool once;  // the gradient is too large for the caches
 };
 
 __device__ __forceinline__ std::uint32_t key_row(std::uint64_t k) { return static_cast<std::uint32_t>(k >> 32); }
@@ -130,15 +135,17 @@ __device__ __forceinline__ void write_sum(const GradArgs& a, std::uint32_t v, st
     T* p = static_cast<T*>(a.grad) + v * a.ldg + c;
     s *= a.scale;
     if (a.accumulate) s += load_row<T, N>(p);
-    store_row<T, N>(p, s);
+    write_out<T, N>(a.once, p, s);
 }
 
-constexpr int kGradUnroll = 8;
+constexpr int kGradUnroll = 4;  // rows a lane has in flight: with 8, half the waves fit and 2.45M x 100 take 585 us, not TODO
 
 // Blocks below sumBlocks: a team of 2^laneBits lanes sums one chunk of the
-// sorted rows.  The others write zeros to the rows that do not occur.
+// sorted rows, the block's keys in LDS.  The others write zeros to the rows
+// that do not occur.
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads) grad_kernel(GradArgs a) {
+    extern __shared__ std::uint64_t ldsKeys[];
     if (blockIdx.x >= a.sumBlocks) {
         const std::uint64_t w = static_cast<std::uint64_t>(blockIdx.x - a.sumBlocks) * (kThreads / kWave) +
                                 threadIdx.x / kWave;
@@ -150,83 +157,137 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(GradArgs a) {
             const std::uint32_t r = static_cast<std::uint32_t>(__builtin_ctzll(absent));
             absent &= absent - 1;
             T* p = static_cast<T*>(a.grad) + (v0 + r) * a.ldg;
-            for (std::uint32_t c = lane * N; c < a.D; c += kWave * N) store_row<T, N>(p + c, vec_t<float, N>(0.0f));
+            for (std::uint32_t c = lane * N; c < a.D; c += kWave * N) write_out<T, N>(a.once, p + c, vec_t<float, N>(0.0f));
         }
         return;
     }
-    const std::uint32_t team = (blockIdx.x * kThreads + threadIdx.x) >> a.laneBits;
-    const std::uint32_t lane = threadIdx.x & ((1u << a.laneBits) - 1u);
-    if (team >= a.chunks) return;
-    const std::uint64_t lo = static_cast<std::uint64_t>(team) * a.chunk;
-    const std::uint64_t hi = min(lo + a.chunk, a.n);
+    const std::uint32_t teams = kThreads >> a.laneBits;
+    const std::uint64_t base = static_cast<std::uint64_t>(blockIdx.x) * teams * a.chunk;
+    const std::uint32_t here = static_cast<std::uint32_t>(min(a.n - base, static_cast<std::uint64_t>(teams * a.chunk)));
+    for (std::uint32_t i = threadIdx.x; i < here; i += kThreads) ldsKeys[i] = a.keys[base + i];
     const std::uint32_t none = static_cast<std::uint32_t>(a.V);
-    const std::uint32_t before = lo > 0 ? key_row(a.keys[lo - 1]) : none;
-    const std::uint32_t after = hi < a.n ? key_row(a.keys[hi]) : none;
+    const std::uint32_t blockBefore = base > 0 ? key_row(a.keys[base - 1]) : none;
+    const std::uint32_t blockAfter = base + here < a.n ? key_row(a.keys[base + here]) : none;
+    __syncthreads();
+    const std::uint32_t mine = threadIdx.x >> a.laneBits;
+    const std::uint32_t lane = threadIdx.x & ((1u << a.laneBits) - 1u);
+    const std::uint32_t lo = mine * a.chunk, hi = min(lo + a.chunk, here);
+    if (lo >= hi) return;
+    const std::uint64_t team = static_cast<std::uint64_t>(blockIdx.x) * teams + mine;
+    const std::uint32_t before = lo > 0 ? key_row(ldsKeys[lo - 1]) : blockBefore;
+    const std::uint32_t after = hi < here ? key_row(ldsKeys[hi]) : blockAfter;
     const T* dOut = static_cast<const T*>(a.dOut);
+    float* headPart = a.parts + 2 * team * a.D;
     for (std::uint32_t c = lane * N; c < a.D; c += N << a.laneBits) {
         std::uint32_t cur = none;
         bool head = false;
         vec_t<float, N> s(0.0f);
-        for (std::uint64_t i = lo; i < hi; i += kGradUnroll) {
-            std::uint64_t k[kGradUnroll];
-            vec_t<float, N> x[kGradUnroll];
+        for (std::uint32_t i = lo; i < hi; i += kGradUnroll) {
+            std::uint32_t v[kGradUnroll];
+            vec_t<T, N> x[kGradUnroll];
 #pragma unroll
             for (int u = 0; u < kGradUnroll; ++u) {
-                k[u] = a.keys[min(i + u, hi - 1)];
-                x[u] = vec_t<float, N>(0.0f);
-                if (i + u < hi && key_row(k[u]) != none)
-                    x[u] = load_row<T, N>(dOut + (k[u] & 0xFFFFFFFFu) * a.ldd + c);
+                const std::uint64_t k = ldsKeys[min(i + u, hi - 1)];
+                v[u] = key_row(k);
+                x[u] = vec_t<T, N>(T(0.0f));
+                if (v[u] != none)  // rows that do not count are not read
+                    x[u] = load_global<vec_t<T, N>>(dOut + (k & 0xFFFFFFFFu) * a.ldd + c);
             }
 #pragma unroll
             for (int u = 0; u < kGradUnroll; ++u) {
                 if (i + u >= hi) break;
-                const std::uint32_t v = key_row(k[u]);
-                if (v != cur) {
-                    if (cur != none) {
-                        if (head) *reinterpret_cast<vec_t<float, N>*>(a.parts + 2ull * team * a.D + c) = s;
-                        else write_sum<T, N>(a, cur, c, s);
-                    }
-                    head = i + u == lo && v == before;
-                    cur = v;
-                    s = x[u];
-                } else {
-                    s += x[u];
+                const vec_t<float, N> f = __builtin_convertvector(x[u], vec_t<float, N>);
+                if (v[u] == cur) {
+                    s += f;
+                    continue;
                 }
+                if (cur != none) {
+                    if (head) *reinterpret_cast<vec_t<float, N>*>(headPart + c) = s;
+                    else write_sum<T, N>(a, cur, c, s);
+                }
+                head = i + u == lo && v[u] == before;
+                cur = v[u];
+                s = f;
             }
         }
         if (cur == none) continue;
-        if (head) *reinterpret_cast<vec_t<float, N>*>(a.parts + 2ull * team * a.D + c) = s;
-        else if (cur == after) *reinterpret_cast<vec_t<float, N>*>(a.parts + (2ull * team + 1) * a.D + c) = s;
+        if (head) *reinterpret_cast<vec_t<float, N>*>(headPart + c) = s;
+        else if (cur == after) *reinterpret_cast<vec_t<float, N>*>(headPart + a.D + c) = s;
         else write_sum<T, N>(a, cur, c, s);
     }
 }
 
-// A team for each chunk in which a row begins that goes on after it: adds the
-// row's parts, chunk by chunk.
+// Adds the parts of the rows that go on after the chunk they begin in, a team
+// for each such chunk; a row of many parts (a hub's) is added by the whole
+// workgroup, each of its teams taking every so many-th part.
+constexpr std::uint32_t kLongRow = 16;
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads) join_kernel(GradArgs a) {
-    const std::uint32_t team = (blockIdx.x * kThreads + threadIdx.x) >> a.laneBits;
+    __shared__ std::uint32_t rowOf[kThreads], partsOf[kThreads];
+    __shared__ float sums[kThreads * N];
+    const std::uint32_t teams = kThreads >> a.laneBits, mine = threadIdx.x >> a.laneBits;
     const std::uint32_t lane = threadIdx.x & ((1u << a.laneBits) - 1u);
-    if (team + 1 >= a.chunks) return;
-    const std::uint64_t lo = static_cast<std::uint64_t>(team) * a.chunk;
-    const std::uint64_t hi = lo + a.chunk;  // the next chunk's first
-    const std::uint32_t v = key_row(a.keys[hi - 1]);
-    if (v == a.V || key_row(a.keys[hi]) != v) return;
-    if (lo > 0 && key_row(a.keys[lo - 1]) == v) return;  // begun earlier
-    // the row's end: the first key past it
-    std::uint64_t l = hi, h = a.n;
-    while (l < h) {
-        const std::uint64_t m = (l + h) / 2;
-        if (key_row(a.keys[m]) <= v) l = m + 1;
-        else h = m;
+    const std::uint32_t first = blockIdx.x * teams, team = first + mine;
+    const std::uint32_t none = static_cast<std::uint32_t>(a.V);
+    std::uint32_t v = none, count = 0;  // parts after the first
+    if (team + 1 < a.chunks) {
+        const std::uint64_t lo = static_cast<std::uint64_t>(team) * a.chunk, hi = lo + a.chunk;
+        const std::uint32_t own = key_row(a.keys[hi - 1]), next = key_row(a.keys[hi]);
+        const std::uint32_t before = lo > 0 ? key_row(a.keys[lo - 1]) : none;
+        if (own != none && next == own && before != own) {
+            v = own;
+            std::uint64_t l = hi, h = a.n;  // the first key past the row
+            while (l < h) {
+                const std::uint64_t m = (l + h) / 2;
+                if (key_row(a.keys[m]) <= v) l = m + 1;
+                else h = m;
+            }
+            count = static_cast<std::uint32_t>((l - 1) / a.chunk) - team;
+        }
     }
-    const std::uint32_t last = static_cast<std::uint32_t>((l - 1) / a.chunk);
-    for (std::uint32_t c = lane * N; c < a.D; c += N << a.laneBits) {
-        vec_t<float, N> s = *reinterpret_cast<const vec_t<float, N>*>(a.parts + (2ull * team + 1) * a.D + c);
-        for (std::uint32_t k = team + 1; k <= last; ++k)
-            s += *reinterpret_cast<const vec_t<float, N>*>(a.parts + 2ull * k * a.D + c);
-        write_sum<T, N>(a, v, c, s);
+    if (lane == 0) {
+        rowOf[mine] = v;
+        partsOf[mine] = count;
     }
+    const auto part = [&](std::uint64_t k, std::uint32_t c) {
+        return load_global<vec_t<float, N>>(a.parts + k * a.D + c);
+    };
+    if (v != none && count <= kLongRow) {
+        for (std::uint32_t c = lane * N; c < a.D; c += N << a.laneBits) {
+            vec_t<float, N> s = part(2ull * team + 1, c);
+            for (std::uint32_t k = 1; k <= count; ++k) s += part(2ull * (team + k), c);
+            write_sum<T, N>(a, v, c, s);
+        }
+    }
+    __syncthreads();
+    for (std::uint32_t t = 0; t < teams; ++t) {
+        if (partsOf[t] <= kLongRow) continue;  // the same for the whole workgroup
+        const std::uint32_t many = partsOf[t];
+        for (std::uint32_t c0 = 0; c0 < a.D; c0 += N << a.laneBits) {
+            const std::uint32_t c = c0 + lane * N;
+            vec_t<float, N> s(0.0f);
+            if (c < a.D) {
+                if (mine == 0) s = part(2ull * (first + t) + 1, c);
+#pragma unroll 4
+                for (std::uint32_t k = 1 + mine; k <= many; k += teams) s += part(2ull * (first + t + k), c);
+            }
+            *reinterpret_cast<vec_t<float, N>*>(sums + threadIdx.x * N) = s;
+            __syncthreads();
+            if (mine == 0 && c < a.D) {
+                for (std::uint32_t o = 1; o < teams; ++o)
+                    s += *reinterpret_cast<const vec_t<float, N>*>(sums + ((o << a.laneBits) + lane) * N);
+                write_sum<T, N>(a, rowOf[t], c, s);
+            }
+            __syncthreads();
+        }
+    }
+}
+
+// The lanes of a team, as a power of two, for lanes of `width` elements.
+unsigned team_bits(std::uint32_t D, std::uint32_t width) {
+    unsigned bits = 0;
+    while (bits < 6 && (width << bits) < D) ++bits;
+    return bits;
 }
 
 // Rows a chunk: short ones give few rows enough teams, long ones keep the
@@ -269,20 +330,21 @@ int lookup_launch(const void* table, std::uint64_t ldt, const Ids& ids, std::uin
     const std::uint64_t blocks = (vecs + kThreads * kLookupUnroll - 1) / (kThreads * kLookupUnroll);
     TCC_REQUIRE(blocks < (1ull << 31), TCC_ERR_UNSUPPORTED, "embedding lookup output too large for one call");
     hipLaunchKernelGGL((lookup_kernel<T, N>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st,
-                       static_cast<const T*>(table), ldt, ids, n, colsV, scale, static_cast<T*>(out), ldo, err);
+                       static_cast<const T*>(table), ldt, ids, n, colsV, scale, static_cast<T*>(out), ldo,
+                       n * D * sizeof(T) > kCacheBytes, err);
     TCC_LAUNCH_CHECK();
     return TCC_OK;
 }
 
 template <typename T, int N>
 int grad_launch(GradArgs a, hipStream_t st) {
-    unsigned bits = 0;
-    while (bits < 6 && (static_cast<std::uint32_t>(N) << bits) < a.D) ++bits;
-    a.laneBits = bits;
-    a.sumBlocks = grid_for(static_cast<std::uint64_t>(a.chunks) << bits, kThreads);
+    a.laneBits = team_bits(a.D, N);
+    a.once = a.V * a.D * sizeof(T) > kCacheBytes;
+    a.sumBlocks = grid_for(static_cast<std::uint64_t>(a.chunks) << a.laneBits, kThreads);
+    const std::uint32_t lds = (kThreads >> a.laneBits) * a.chunk * sizeof(std::uint64_t);
     const unsigned fillBlocks = a.accumulate ? 0u : grid_for(a.V, kThreads);
     if (a.sumBlocks + fillBlocks > 0)
-        hipLaunchKernelGGL((grad_kernel<T, N>), dim3(a.sumBlocks + fillBlocks), dim3(kThreads), 0, st, a);
+        hipLaunchKernelGGL((grad_kernel<T, N>), dim3(a.sumBlocks + fillBlocks), dim3(kThreads), lds, st, a);
     TCC_LAUNCH_CHECK();
     if (a.chunks > 1) {
         hipLaunchKernelGGL((join_kernel<T, N>), dim3(a.sumBlocks), dim3(kThreads), 0, st, a);
@@ -363,7 +425,8 @@ int tcc_embedding_grad(const void* dOut, uint64_t ldd, uint32_t dtype, const voi
     std::uint8_t* mark = reinterpret_cast<std::uint8_t*>(ws + lay.mark);
     if (!accumulate) {
         TCC_HIP_CHECK(fill<std::uint8_t>(mark, V, 0, st));
-        if (n > 0) hipLaunchKernelGGL(mark_kernel, dim3(grid_for(n, kThreads)), dim3(kThreads), 0, st, rows, n, mark);
+        if (n > 0)
+            hipLaunchKernelGGL(mark_kernel, dim3(grid_for(n, kThreads)), dim3(kThreads), 0, st, a.keys, n, V, mark);
         TCC_LAUNCH_CHECK();
     }
     a.dOut = dOut;

@@ -184,11 +184,6 @@ __device__ __forceinline__ vec_t<float, N> load_once(const T* p) {
     const auto* g = (const __attribute__((address_space(1))) V*)(reinterpret_cast<std::uintptr_t>(p));
     return __builtin_convertvector(__builtin_nontemporal_load(g), vec_t<float, N>);
 }
-template <typename T, int N>
-__device__ __forceinline__ void write_out(bool once, T* p, vec_t<float, N> v) {
-    if (once) __builtin_nontemporal_store(__builtin_convertvector(v, vec_t<T, N>), reinterpret_cast<vec_t<T, N>*>(p));
-    else store_row<T, N>(p, v);
-}
 
 // What the channels c .. c + N need of their groups' values: one of each where
 // a vector lies in one group (N divides K), as it mostly does.
@@ -896,8 +891,6 @@ __global__ void __launch_bounds__(kWholeThreads, 3) whole_grad_kernel(NormArgs a
 
 constexpr std::size_t align16(std::size_t b) { return (b + 15) & ~std::size_t(15); }
 
-// Bytes that the last level of cache holds.
-constexpr std::uint64_t kCacheBytes = 256 << 20;
 // Tiles of at most this many, so that the tiles' sums stay few.
 constexpr std::uint64_t kTiles = 2048;
 // A segment that a workgroup walks in at most this many steps goes whole (some

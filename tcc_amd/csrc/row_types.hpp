@@ -24,6 +24,16 @@ __device__ __forceinline__ void store_row(T* p, vec_t<float, N> v) {
     *reinterpret_cast<vec_t<T, N>*>(p) = __builtin_convertvector(v, vec_t<T, N>);
 }
 
+// Bytes that the last level of cache holds: larger outputs are written past
+// its order.
+constexpr std::uint64_t kCacheBytes = 256 << 20;
+
+template <typename T, int N>
+__device__ __forceinline__ void write_out(bool once, T* p, vec_t<float, N> v) {
+    if (once) __builtin_nontemporal_store(__builtin_convertvector(v, vec_t<T, N>), reinterpret_cast<vec_t<T, N>*>(p));
+    else store_row<T, N>(p, v);
+}
+
 // Element bytes of a TCC_F32 / TCC_BF16 / TCC_F16 code, 0 for any other.
 inline std::uint32_t dtype_bytes(std::uint64_t dtype) { return dtype == 0 ? 4u : (dtype == 1 || dtype == 2) ? 2u : 0u; }
 
