@@ -31,13 +31,32 @@ struct Ids {
     std::int64_t padding;
     std::uint32_t wide;  // int64
     __device__ __forceinline__ std::uint32_t row(std::uint64_t i, bool& bad) const {
-        const std::int64_t id = wide ? load_global<std::int64_t>(static_cast<const std::int64_t*>(p) + i)
-                                     : load_global<std::int32_t>(static_cast<const std::int32_t*>(p) + i);
-        if (static_cast<std::uint64_t>(id) >= V) {
-            bad = true;
-            return kNoRow;
+        return row_of(wide ? load_global<std::int64_t>(static_cast<const std::int64_t*>(p) + i)
+                           : load_global<std::int32_t>(static_cast<const std::int32_t*>(p) + i),
+                      bad);
+    }
+    __device__ __forceinline__ std::uint32_t row_of(std::int64_t id, bool& bad) const {
+        const bool in = static_cast<std::uint64_t>(id) < V;
+        bad |= !in;
+        return in && id != padding ? static_cast<std::uint32_t>(id) : kNoRow;
+    }
+    // R ids, `step` apart from i on (the last id where they pass it), all
+    // loaded before the first is looked at.
+    template <int R>
+    __device__ __forceinline__ void rows(std::uint64_t i, std::uint64_t step, std::uint64_t n, std::uint32_t (&v)[R],
+                                         bool& bad) const {
+        std::int64_t id[R];
+        if (wide) {
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                id[r] = load_global<std::int64_t>(static_cast<const std::int64_t*>(p) + min(i + r * step, n - 1));
+        } else {
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                id[r] = load_global<std::int32_t>(static_cast<const std::int32_t*>(p) + min(i + r * step, n - 1));
         }
-        return id == padding ? kNoRow : static_cast<std::uint32_t>(id);
+#pragma unroll
+        for (int r = 0; r < R; ++r) v[r] = row_of(id[r], bad);
     }
 };
 
@@ -54,10 +73,10 @@ constexpr int kLookupUnroll = 4;
 // are written past the caches' order, which leaves those to rows that come
 // again: 2.45M x 100 rows of bf16 248 us instead of 270, of fp32 323 instead
 // of 359 (4 vectors a lane; with 2 of them 257 and 318, with 8 over 600).
-template <typename T, int N>
+template <typename T, int N, bool ONCE>
 __global__ void __launch_bounds__(kThreads) lookup_kernel(const T* __restrict__ table, std::uint64_t ldt, Ids ids,
                                                          std::uint64_t n, std::uint32_t colsV, float scale,
-                                                         T* __restrict__ out, std::uint64_t ldo, bool once, std::uint32_t* err) {
+                                                         T* __restrict__ out, std::uint64_t ldo, std::uint32_t* err) {
     const std::uint64_t first = static_cast<std::uint64_t>(blockIdx.x) * (kThreads * kLookupUnroll);
     const std::uint64_t row0 = first / colsV;
     const std::uint32_t col0 = static_cast<std::uint32_t>(first - row0 * colsV);
@@ -81,7 +100,7 @@ __global__ void __launch_bounds__(kThreads) lookup_kernel(const T* __restrict__ 
     }
 #pragma unroll
     for (int u = 0; u < kLookupUnroll; ++u)
-        if (i[u] < n) write_out<T, N>(once, out + i[u] * ldo + c[u], x[u]);
+        if (i[u] < n) write_out<ONCE, T, N>(out + i[u] * ldo + c[u], x[u]);
     report(err, bad);
 }
 
@@ -94,38 +113,26 @@ struct IdKeys {
     std::uint64_t n;
     std::uint32_t* err;
     __device__ __forceinline__ void load(std::uint64_t first, std::uint64_t (&k)[kPrimRounds], bool& bad) const {
-        const std::uint64_t last = n - 1;
+        std::uint32_t v[kPrimRounds];
+        ids.rows<kPrimRounds>(first, kWave, n, v, bad);
 #pragma unroll
-        for (int r = 0; r < kPrimRounds; ++r) {
-            const std::uint64_t i = min(first + static_cast<std::uint64_t>(r) * kWave, last);
-            const std::uint32_t v = ids.row(i, bad);
-            k[r] = (v == kNoRow ? ids.V : static_cast<std::uint64_t>(v)) << 32 | i;
-        }
+        for (int r = 0; r < kPrimRounds; ++r)
+            k[r] = (v[r] == kNoRow ? ids.V : static_cast<std::uint64_t>(v[r])) << 32 |
+                   min(first + static_cast<std::uint64_t>(r) * kWave, n - 1);
     }
     __device__ __forceinline__ void report(bool bad) const { tcc::report(err, bad); }
 };
-
-// Marks the rows that occur, from the sorted keys: neighbours in memory (from
-// the ids as they come, 2.45M of them took 16 us instead of TODO).
-__global__ void __launch_bounds__(kThreads) mark_kernel(const std::uint64_t* __restrict__ keys, std::uint64_t n,
-                                                       std::uint64_t V, std::uint8_t* __restrict__ mark) {
-    const std::uint64_t i = static_cast<std::uint64_t>(blockIdx.x) * kThreads + threadIdx.x;
-    if (i >= n) return;
-    const std::uint32_t v = static_cast<std::uint32_t>(keys[i] >> 32);
-    if (v < V && (i == 0 || static_cast<std::uint32_t>(keys[i - 1] >> 32) != v)) mark[v] = 1;
-}
 
 struct GradArgs {
     const std::uint64_t* keys;  // sorted
     const void* dOut;
     void* grad;
     float* parts;  // [2 * chunks][D]: sums of a chunk's first row (begun before it) and last row (going on after it)
-    const std::uint8_t* mark;
+    std::uint8_t* mark;  // [windows]: 1 where a row occurs
     std::uint64_t n, V, ldd, ldg;
-    std::uint32_t D, chunk, chunks, laneBits, sumBlocks;
+    std::uint32_t D, chunk, chunks, laneBits, joinBlocks;
     float scale;
     int accumulate;
-    bool once;  // the gradient is too large for the caches
 };
 
 __device__ __forceinline__ std::uint32_t key_row(std::uint64_t k) { return static_cast<std::uint32_t>(k >> 32); }
@@ -135,39 +142,45 @@ __device__ __forceinline__ void write_sum(const GradArgs& a, std::uint32_t v, st
     T* p = static_cast<T*>(a.grad) + v * a.ldg + c;
     s *= a.scale;
     if (a.accumulate) s += load_row<T, N>(p);
-    write_out<T, N>(a.once, p, s);
+    store_row<T, N>(p, s);
 }
 
-constexpr int kGradUnroll = 4;  // rows a lane has in flight: with 8, half the waves fit and 2.45M x 100 take 585 us, not TODO
+constexpr int kGradUnroll = 4;  // rows a lane has in flight
 
-// Blocks below sumBlocks: a team of 2^laneBits lanes sums one chunk of the
-// sorted rows, the block's keys in LDS.  The others write zeros to the rows
-// that do not occur.
+// Rows that do not occur are zeroed where they lie: those of a window of this
+// many rows that holds others, by the teams that write these (a row's lines
+// are then written whole, unless past the caches' order, which took 534 us for
+// 2.45M x 100 rows instead of 488; zeroed apart from the sums, they took 577),
+// those of empty windows by the join's launch.
+constexpr std::uint32_t kWindow = 16;
+
+// Zeros in the rows between q (kNoRow: none before) and r (V: none after)
+// that share a window with either.
+template <typename T, int N>
+__device__ __forceinline__ void zero_between(const GradArgs& a, std::uint32_t q, std::uint32_t r, std::uint32_t c) {
+    const std::uint32_t V = static_cast<std::uint32_t>(a.V);
+    std::uint32_t v = q + 1;  // 0 where none is before
+    const std::uint32_t endOfQ = q == kNoRow ? 0u : min(r, (q / kWindow + 1) * kWindow);
+    const std::uint32_t startOfR = r < V ? r / kWindow * kWindow : V;
+    for (; v < r; ++v) {
+        if (v >= endOfQ && v < startOfR) v = startOfR;  // an empty window begins
+        if (v >= r) break;
+        store_row<T, N>(static_cast<T*>(a.grad) + v * a.ldg + c, vec_t<float, N>(0.0f));
+    }
+}
+
+// A team of 2^laneBits lanes sums one chunk of the sorted rows, the block's
+// keys in LDS.
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads) grad_kernel(GradArgs a) {
     extern __shared__ std::uint64_t ldsKeys[];
-    if (blockIdx.x >= a.sumBlocks) {
-        const std::uint64_t w = static_cast<std::uint64_t>(blockIdx.x - a.sumBlocks) * (kThreads / kWave) +
-                                threadIdx.x / kWave;
-        const std::uint32_t lane = __lane_id();
-        const std::uint64_t v0 = w * kWave;
-        if (v0 >= a.V) return;
-        std::uint64_t absent = __ballot(v0 + lane < a.V && a.mark[min(v0 + lane, a.V - 1)] == 0);
-        while (absent != 0) {
-            const std::uint32_t r = static_cast<std::uint32_t>(__builtin_ctzll(absent));
-            absent &= absent - 1;
-            T* p = static_cast<T*>(a.grad) + (v0 + r) * a.ldg;
-            for (std::uint32_t c = lane * N; c < a.D; c += kWave * N) write_out<T, N>(a.once, p + c, vec_t<float, N>(0.0f));
-        }
-        return;
-    }
     const std::uint32_t teams = kThreads >> a.laneBits;
     const std::uint64_t base = static_cast<std::uint64_t>(blockIdx.x) * teams * a.chunk;
     const std::uint32_t here = static_cast<std::uint32_t>(min(a.n - base, static_cast<std::uint64_t>(teams * a.chunk)));
     for (std::uint32_t i = threadIdx.x; i < here; i += kThreads) ldsKeys[i] = a.keys[base + i];
     const std::uint32_t none = static_cast<std::uint32_t>(a.V);
-    const std::uint32_t blockBefore = base > 0 ? key_row(a.keys[base - 1]) : none;
-    const std::uint32_t blockAfter = base + here < a.n ? key_row(a.keys[base + here]) : none;
+    const std::uint32_t blockBefore = base > 0 ? key_row(a.keys[base - 1]) : kNoRow;
+    const std::uint32_t blockAfter = base + here < a.n ? key_row(a.keys[base + here]) : kNoRow;
     __syncthreads();
     const std::uint32_t mine = threadIdx.x >> a.laneBits;
     const std::uint32_t lane = threadIdx.x & ((1u << a.laneBits) - 1u);
@@ -179,7 +192,7 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(GradArgs a) {
     const T* dOut = static_cast<const T*>(a.dOut);
     float* headPart = a.parts + 2 * team * a.D;
     for (std::uint32_t c = lane * N; c < a.D; c += N << a.laneBits) {
-        std::uint32_t cur = none;
+        std::uint32_t cur = kNoRow;  // the row being summed; none: rows that do not count
         bool head = false;
         vec_t<float, N> s(0.0f);
         for (std::uint32_t i = lo; i < hi; i += kGradUnroll) {
@@ -201,30 +214,65 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(GradArgs a) {
                     s += f;
                     continue;
                 }
-                if (cur != none) {
+                if (cur < none) {
                     if (head) *reinterpret_cast<vec_t<float, N>*>(headPart + c) = s;
                     else write_sum<T, N>(a, cur, c, s);
                 }
+                const std::uint32_t last = i + u == lo ? before : cur;
                 head = i + u == lo && v[u] == before;
+                if (!head && !a.accumulate) {
+                    zero_between<T, N>(a, last, v[u], c);
+                    if (c == 0 && v[u] != none) a.mark[v[u] / kWindow] = 1;
+                }
                 cur = v[u];
                 s = f;
             }
         }
-        if (cur == none) continue;
+        if (cur >= none) continue;
+        if (base + hi == a.n && !a.accumulate) zero_between<T, N>(a, cur, none, c);
         if (head) *reinterpret_cast<vec_t<float, N>*>(headPart + c) = s;
         else if (cur == after) *reinterpret_cast<vec_t<float, N>*>(headPart + a.D + c) = s;
         else write_sum<T, N>(a, cur, c, s);
     }
 }
 
+// A workgroup's share of the empty windows: as many windows as its threads, a
+// wave for one at a time.
+template <typename T, int N>
+__device__ __forceinline__ void zero_windows(const GradArgs& a, std::uint32_t block) {
+    const std::uint64_t first = (static_cast<std::uint64_t>(block) * (kThreads / kWave) + threadIdx.x / kWave) * kWave;
+    const std::uint64_t w = first + __lane_id(), windows = (a.V + kWindow - 1) / kWindow;
+    std::uint64_t empty = __ballot(w < windows && a.mark[min(w, windows - 1)] == 0);
+    while (empty != 0) {
+        const std::uint64_t v0 = (first + __builtin_ctzll(empty)) * kWindow;
+        empty &= empty - 1;
+        const std::uint32_t cols = a.D / N, rows = static_cast<std::uint32_t>(min<std::uint64_t>(kWindow, a.V - v0));
+        T* p = static_cast<T*>(a.grad) + v0 * a.ldg;
+        if (a.ldg == a.D) {
+            for (std::uint32_t i = __lane_id(); i < rows * cols; i += kWave)
+                store_row<T, N>(p + static_cast<std::uint64_t>(i) * N, vec_t<float, N>(0.0f));
+        } else {
+            for (std::uint32_t i = __lane_id(); i < rows * cols; i += kWave) {
+                const std::uint32_t r = i / cols;
+                store_row<T, N>(p + r * a.ldg + (i - r * cols) * N, vec_t<float, N>(0.0f));
+            }
+        }
+    }
+}
+
 // Adds the parts of the rows that go on after the chunk they begin in, a team
-// for each such chunk; a row of many parts (a hub's) is added by the whole
+// for each such chunk, and zeroes the empty windows (blocks from joinBlocks
+// on); a row of many parts (a hub's) is added by the whole
 // workgroup, each of its teams taking every so many-th part.
 constexpr std::uint32_t kLongRow = 16;
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads) join_kernel(GradArgs a) {
     __shared__ std::uint32_t rowOf[kThreads], partsOf[kThreads];
     __shared__ float sums[kThreads * N];
+    if (blockIdx.x >= a.joinBlocks) {
+        zero_windows<T, N>(a, blockIdx.x - a.joinBlocks);
+        return;
+    }
     const std::uint32_t teams = kThreads >> a.laneBits, mine = threadIdx.x >> a.laneBits;
     const std::uint32_t lane = threadIdx.x & ((1u << a.laneBits) - 1u);
     const std::uint32_t first = blockIdx.x * teams, team = first + mine;
@@ -236,13 +284,18 @@ __global__ void __launch_bounds__(kThreads) join_kernel(GradArgs a) {
         const std::uint32_t before = lo > 0 ? key_row(a.keys[lo - 1]) : none;
         if (own != none && next == own && before != own) {
             v = own;
-            std::uint64_t l = hi, h = a.n;  // the first key past the row
-            while (l < h) {
-                const std::uint64_t m = (l + h) / 2;
-                if (key_row(a.keys[m]) <= v) l = m + 1;
-                else h = m;
+            // the last chunk that begins with the row: steps that double, then halve
+            std::uint32_t last = team + 1, step = 1;
+            const auto begins = [&](std::uint32_t k) {
+                return k < a.chunks && key_row(a.keys[static_cast<std::uint64_t>(k) * a.chunk]) == v;
+            };
+            while (begins(last + step)) {
+                last += step;
+                step *= 2;
             }
-            count = static_cast<std::uint32_t>((l - 1) / a.chunk) - team;
+            for (; step > 0; step /= 2)
+                if (begins(last + step)) last += step;
+            count = last - team;
         }
     }
     if (lane == 0) {
@@ -317,7 +370,7 @@ struct GradLayout {
         hist = take(partition_hist_elems(n) * 4);
         total = take(kRadixBins * 4);
         parts = take(2 * chunks * D * 4);
-        mark = take(V);
+        mark = take((V + kWindow - 1) / kWindow + 8);
         bytes = at;
     }
 };
@@ -329,9 +382,9 @@ int lookup_launch(const void* table, std::uint64_t ldt, const Ids& ids, std::uin
     const std::uint64_t vecs = n * colsV;
     const std::uint64_t blocks = (vecs + kThreads * kLookupUnroll - 1) / (kThreads * kLookupUnroll);
     TCC_REQUIRE(blocks < (1ull << 31), TCC_ERR_UNSUPPORTED, "embedding lookup output too large for one call");
-    hipLaunchKernelGGL((lookup_kernel<T, N>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st,
-                       static_cast<const T*>(table), ldt, ids, n, colsV, scale, static_cast<T*>(out), ldo,
-                       n * D * sizeof(T) > kCacheBytes, err);
+    auto* form = n * D * sizeof(T) > kCacheBytes ? &lookup_kernel<T, N, true> : &lookup_kernel<T, N, false>;
+    hipLaunchKernelGGL(form, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st, static_cast<const T*>(table), ldt,
+                       ids, n, colsV, scale, static_cast<T*>(out), ldo, err);
     TCC_LAUNCH_CHECK();
     return TCC_OK;
 }
@@ -339,15 +392,16 @@ int lookup_launch(const void* table, std::uint64_t ldt, const Ids& ids, std::uin
 template <typename T, int N>
 int grad_launch(GradArgs a, hipStream_t st) {
     a.laneBits = team_bits(a.D, N);
-    a.once = a.V * a.D * sizeof(T) > kCacheBytes;
-    a.sumBlocks = grid_for(static_cast<std::uint64_t>(a.chunks) << a.laneBits, kThreads);
-    const std::uint32_t lds = (kThreads >> a.laneBits) * a.chunk * sizeof(std::uint64_t);
-    const unsigned fillBlocks = a.accumulate ? 0u : grid_for(a.V, kThreads);
-    if (a.sumBlocks + fillBlocks > 0)
-        hipLaunchKernelGGL((grad_kernel<T, N>), dim3(a.sumBlocks + fillBlocks), dim3(kThreads), lds, st, a);
-    TCC_LAUNCH_CHECK();
-    if (a.chunks > 1) {
-        hipLaunchKernelGGL((join_kernel<T, N>), dim3(a.sumBlocks), dim3(kThreads), 0, st, a);
+    const unsigned blocks = grid_for(static_cast<std::uint64_t>(a.chunks) << a.laneBits, kThreads);
+    if (blocks > 0) {
+        const std::uint32_t lds = (kThreads >> a.laneBits) * a.chunk * sizeof(std::uint64_t);
+        hipLaunchKernelGGL((grad_kernel<T, N>), dim3(blocks), dim3(kThreads), lds, st, a);
+        TCC_LAUNCH_CHECK();
+    }
+    a.joinBlocks = a.chunks > 1 ? blocks : 0u;
+    const unsigned zeroBlocks = a.accumulate ? 0u : grid_for((a.V + kWindow - 1) / kWindow, kThreads);
+    if (a.joinBlocks + zeroBlocks > 0) {
+        hipLaunchKernelGGL((join_kernel<T, N>), dim3(a.joinBlocks + zeroBlocks), dim3(kThreads), 0, st, a);
         TCC_LAUNCH_CHECK();
     }
     return TCC_OK;
@@ -424,10 +478,7 @@ int tcc_embedding_grad(const void* dOut, uint64_t ldd, uint32_t dtype, const voi
     }
     std::uint8_t* mark = reinterpret_cast<std::uint8_t*>(ws + lay.mark);
     if (!accumulate) {
-        TCC_HIP_CHECK(fill<std::uint8_t>(mark, V, 0, st));
-        if (n > 0)
-            hipLaunchKernelGGL(mark_kernel, dim3(grid_for(n, kThreads)), dim3(kThreads), 0, st, a.keys, n, V, mark);
-        TCC_LAUNCH_CHECK();
+        TCC_HIP_CHECK(fill<std::uint64_t>(reinterpret_cast<std::uint64_t*>(mark), (V + 8 * kWindow - 1) / (8 * kWindow), 0, st));
     }
     a.dOut = dOut;
     a.grad = grad;

@@ -74,7 +74,6 @@ struct NormArgs {
     std::uint32_t C, G, K, colsV, rowLanes;  // K = C / G; colsV vectors a row, rowLanes rows at once
     std::uint32_t paramBytes, paramType, act;
     float eps;
-    bool once;  // the output is too large for the caches
 };
 
 // Channels c .. c + N of a weight or bias: one branch and one load for all of
@@ -175,9 +174,9 @@ __device__ __forceinline__ float wave_sum(float v) {
     return v;
 }
 
-// Rows of tiles are read and written past the caches' order: read as usual,
-// 2.45M x 256 fp32 rows took 479 us for the statistics instead of 400, and
-// their gradient's sums 843 instead of 747.
+// Rows of tiles are read past the caches' order: read as usual, 2.45M x 256 fp32
+// rows took 479 us for the statistics instead of 400, and their gradient's
+// sums 843 instead of 747.
 template <typename T, int N>
 __device__ __forceinline__ vec_t<float, N> load_once(const T* p) {
     using V = vec_t<T, N>;
@@ -402,7 +401,7 @@ __global__ void __launch_bounds__(kThreads) apply_kernel(NormArgs a) {
                 vec_t<float, N> o;
 #pragma unroll
                 for (int q = 0; q < N; ++q) o[q] = activate<ACT>(affine(normalise(v[q], of.mean[q], of.rstd[q]), w[q], b[q]));
-                write_out<T, N>(a.once, y + r * a.ldo + cv * N, o);
+                store_row<T, N>(y + r * a.ldo + cv * N, o);
             }
         }
     }
@@ -574,7 +573,7 @@ __global__ void __launch_bounds__(kThreads) grad_apply_kernel(NormArgs a) {
                     const float dz = d[q] * slope<ACT>(affine(xh, w[q], b[q]));
                     o[q] = (dz * w[q] - of.sums[q].x - xh * of.sums[q].y) * of.rstd[q];
                 }
-                write_out<T, N>(a.once, dx + r * a.ldo + cv * N, o);
+                store_row<T, N>(dx + r * a.ldo + cv * N, o);
             }
         }
     }
@@ -1093,7 +1092,6 @@ NormArgs base_args(const tcc_group_norm_shape& s, const Layout& lay, const Split
     a.channel = reinterpret_cast<float2*>(ws + lay.channel);
     a.seen = reinterpret_cast<std::uint8_t*>(ws + lay.seen);
     a.tileRows = lay.tileRows;
-    a.once = s.N * s.C * dtype_bytes(s.dtype) > kCacheBytes;
     a.C = s.C;
     a.G = s.G;
     a.K = s.C / s.G;

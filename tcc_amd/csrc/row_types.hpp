@@ -25,12 +25,13 @@ __device__ __forceinline__ void store_row(T* p, vec_t<float, N> v) {
 }
 
 // Bytes that the last level of cache holds: larger outputs are written past
-// its order.
+// its order (ONCE).  A constant, as the compiler makes one plain store of two
+// that a value at run time chooses between.
 constexpr std::uint64_t kCacheBytes = 256 << 20;
 
-template <typename T, int N>
-__device__ __forceinline__ void write_out(bool once, T* p, vec_t<float, N> v) {
-    if (once) __builtin_nontemporal_store(__builtin_convertvector(v, vec_t<T, N>), reinterpret_cast<vec_t<T, N>*>(p));
+template <bool ONCE, typename T, int N>
+__device__ __forceinline__ void write_out(T* p, vec_t<float, N> v) {
+    if constexpr (ONCE) __builtin_nontemporal_store(__builtin_convertvector(v, vec_t<T, N>), reinterpret_cast<vec_t<T, N>*>(p));
     else store_row<T, N>(p, v);
 }
 
