@@ -52,7 +52,7 @@ size_t tcc_embedding_grad_workspace_bytes(uint64_t n, uint64_t V, uint32_t D);
  * row of grad is written (accumulate = 0), or the sums are added to grad and
  * only rows that occur are touched (accumulate != 0).  Padding and refused
  * ids as in tcc_embedding_lookup: their rows of dOut are not read.  The rows
- * of one id are added in the order of their ids' stable sort. */
+ * of one id are added in an order that the ids alone decide. */
 int tcc_embedding_grad(const void* dOut, uint64_t ldd, uint32_t dtype, const void* ids, uint32_t idBytes, uint64_t n,
                        uint64_t V, uint32_t D, float scale, int64_t padding, void* grad, uint64_t ldg, int accumulate,
                        uint32_t* deviceError, void* workspace, size_t workspaceBytes, void* stream);

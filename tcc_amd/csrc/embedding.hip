@@ -130,7 +130,7 @@ struct GradArgs {
     float* parts;  // [2 * chunks][D]: sums of a chunk's first row (begun before it) and last row (going on after it)
     std::uint8_t* mark;  // [windows]: 1 where a row occurs
     std::uint64_t n, V, ldd, ldg;
-    std::uint32_t D, chunk, chunks, laneBits, joinBlocks;
+    std::uint32_t D, chunk, chunks, laneBits, joinBlocks, zeroRows;
     float scale;
     int accumulate;
 };
@@ -336,6 +336,94 @@ __global__ void __launch_bounds__(kThreads) join_kernel(GradArgs a) {
     }
 }
 
+// ---------------------------------------------------------------- few rows
+
+// Without a sort, in one launch: every workgroup holds the ids, and the wave of
+// the first position of each row looks for the others.  That is n^2 / 64
+// comparisons, which a few thousand rows spread over the GPU need less time for
+// than a sort's launches follow each other in: rows of 32 fp32 into a table of
+// 4,096, 8 us and sorted 52 for 1,000 of them, 12 and 45 for 2,048, 28 and 46
+// for 4,096 (of 256 values 38 and 39).
+constexpr std::uint64_t kFewRows = 4096;
+constexpr std::uint32_t kFewZeroRows = 256;  // rows of a workgroup that zeroes, at most
+
+template <typename T, int N>
+__global__ void __launch_bounds__(kThreads) few_grad_kernel(GradArgs a, Ids ids, std::uint32_t* err) {
+    extern __shared__ std::uint32_t rowOf[];  // [n], then a list of n positions for each wave
+    __shared__ std::uint32_t occurs[kFewZeroRows];
+    const std::uint32_t n = static_cast<std::uint32_t>(a.n);
+    bool bad = false;
+    for (std::uint32_t i = threadIdx.x; i < n; i += 8 * kThreads) {
+        std::uint32_t v[8];
+        ids.rows<8>(i, kThreads, n, v, bad);
+#pragma unroll
+        for (std::uint32_t r = 0; r < 8; ++r)
+            if (i + r * kThreads < n) rowOf[i + r * kThreads] = v[r];
+    }
+    if (blockIdx.x == 0) report(err, bad);
+    if (blockIdx.x >= a.joinBlocks) {  // zeros in the rows that do not occur
+        const std::uint64_t v0 = static_cast<std::uint64_t>(blockIdx.x - a.joinBlocks) * a.zeroRows;
+        occurs[threadIdx.x] = 0;
+        __syncthreads();
+        for (std::uint32_t i = threadIdx.x; i < n; i += kThreads) {
+            const std::uint64_t at = rowOf[i] - v0;  // past the rows for those before v0 too
+            if (rowOf[i] != kNoRow && at < a.zeroRows) occurs[at] = 1;
+        }
+        __syncthreads();
+        const std::uint32_t cols = a.D / N;
+        const std::uint32_t rows = static_cast<std::uint32_t>(min<std::uint64_t>(a.zeroRows, a.V - v0));
+        for (std::uint32_t i = threadIdx.x; i < rows * cols; i += kThreads) {
+            const std::uint32_t r = i / cols;
+            if (occurs[r] == 0)
+                store_row<T, N>(static_cast<T*>(a.grad) + (v0 + r) * a.ldg + (i - r * cols) * N, vec_t<float, N>(0.0f));
+        }
+        return;
+    }
+    __syncthreads();
+    constexpr std::uint32_t kWaves = kThreads / kWave;
+    const std::uint32_t wave = threadIdx.x / kWave, lane = __lane_id();
+    std::uint16_t* list = reinterpret_cast<std::uint16_t*>(rowOf + n) + wave * n;
+    const std::uint32_t team = lane >> a.laneBits, teams = kWave >> a.laneBits;
+    const std::uint32_t col = (lane & ((1u << a.laneBits) - 1u)) * N;
+    const T* dOut = static_cast<const T*>(a.dOut);
+    for (std::uint32_t i = blockIdx.x * kWaves + wave; i < n; i += a.joinBlocks * kWaves) {
+        const std::uint32_t v = uniform(rowOf[i]);
+        if (v == kNoRow) continue;
+        std::uint32_t found = 0;
+        bool first = true;
+        for (std::uint32_t j0 = 0; j0 < n; j0 += kWave) {
+            const std::uint32_t j = j0 + lane;
+            const std::uint64_t same = __ballot(j < n && rowOf[min(j, n - 1)] == v);
+            if (same == 0) continue;
+            if (found == 0 && j0 + __builtin_ctzll(same) != i) {  // another position's
+                first = false;
+                break;
+            }
+            if (same >> lane & 1) list[found + __popcll(same & lanemask_lt())] = static_cast<std::uint16_t>(j);
+            found += static_cast<std::uint32_t>(__popcll(same));
+        }
+        if (!first) continue;
+        for (std::uint32_t c = col; c < a.D; c += N << a.laneBits) {
+            vec_t<float, N> s(0.0f);
+            for (std::uint32_t k = team; k < found; k += 4 * teams) {
+                vec_t<T, N> x[4];
+#pragma unroll
+                for (std::uint32_t u = 0; u < 4; ++u)
+                    x[u] = load_global<vec_t<T, N>>(dOut + list[min(k + u * teams, found - 1)] * a.ldd + c);
+#pragma unroll
+                for (std::uint32_t u = 0; u < 4; ++u)
+                    if (k + u * teams < found) s += __builtin_convertvector(x[u], vec_t<float, N>);
+            }
+            for (std::uint32_t d = 1u << a.laneBits; d < kWave; d <<= 1)
+#pragma unroll
+                for (int q = 0; q < N; ++q) s[q] += __shfl_xor(s[q], d, kWave);
+            if (team == 0) write_sum<T, N>(a, v, c, s);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- host side
+
 // The lanes of a team, as a power of two, for lanes of `width` elements.
 unsigned team_bits(std::uint32_t D, std::uint32_t width) {
     unsigned bits = 0;
@@ -385,6 +473,18 @@ int lookup_launch(const void* table, std::uint64_t ldt, const Ids& ids, std::uin
     auto* form = n * D * sizeof(T) > kCacheBytes ? &lookup_kernel<T, N, true> : &lookup_kernel<T, N, false>;
     hipLaunchKernelGGL(form, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st, static_cast<const T*>(table), ldt,
                        ids, n, colsV, scale, static_cast<T*>(out), ldo, err);
+    TCC_LAUNCH_CHECK();
+    return TCC_OK;
+}
+
+template <typename T, int N>
+int few_grad_launch(GradArgs a, const Ids& ids, std::uint32_t* err, hipStream_t st) {
+    a.laneBits = team_bits(a.D, N);
+    a.joinBlocks = grid_for(a.n, kThreads / kWave);
+    a.zeroRows = static_cast<std::uint32_t>(std::clamp<std::uint64_t>(a.V / 1024, 4, kFewZeroRows));
+    const unsigned zeroBlocks = a.accumulate ? 0u : grid_for(a.V, a.zeroRows);
+    const std::size_t lds = a.n * (sizeof(std::uint32_t) + kThreads / kWave * sizeof(std::uint16_t));
+    hipLaunchKernelGGL((few_grad_kernel<T, N>), dim3(a.joinBlocks + zeroBlocks), dim3(kThreads), lds, st, a, ids, err);
     TCC_LAUNCH_CHECK();
     return TCC_OK;
 }
@@ -468,22 +568,10 @@ int tcc_embedding_grad(const void* dOut, uint64_t ldd, uint32_t dtype, const voi
     char* ws = static_cast<char*>(workspace);
     const Ids rows{ids, V, padding, idBytes == 8};
     GradArgs a{};
-    if (n > 0) {
-        std::uint64_t* sorted = nullptr;
-        TCC_HIP_CHECK(partition_by(IdKeys{rows, n, deviceError}, reinterpret_cast<std::uint64_t*>(ws + lay.keysA),
-                                   reinterpret_cast<std::uint64_t*>(ws + lay.keysB), n, 32, id_bits(V),
-                                   reinterpret_cast<std::uint32_t*>(ws + lay.hist),
-                                   reinterpret_cast<std::uint32_t*>(ws + lay.total), &sorted, st));
-        a.keys = sorted;
-    }
-    std::uint8_t* mark = reinterpret_cast<std::uint8_t*>(ws + lay.mark);
-    if (!accumulate) {
-        TCC_HIP_CHECK(fill<std::uint64_t>(reinterpret_cast<std::uint64_t*>(mark), (V + 8 * kWindow - 1) / (8 * kWindow), 0, st));
-    }
     a.dOut = dOut;
     a.grad = grad;
     a.parts = reinterpret_cast<float*>(ws + lay.parts);
-    a.mark = mark;
+    a.mark = reinterpret_cast<std::uint8_t*>(ws + lay.mark);
     a.n = n;
     a.V = V;
     a.ldd = ldd;
@@ -494,6 +582,24 @@ int tcc_embedding_grad(const void* dOut, uint64_t ldd, uint32_t dtype, const voi
     a.scale = scale;
     a.accumulate = accumulate;
     const std::uint32_t w = RowWidth(D, dtype_bytes(dtype)).with(dOut).with(grad).stride(ldd).stride(ldg).elems();
+    if (n > 0 && n <= kFewRows) {
+#define CALL(T, N) (few_grad_launch<T, N>(a, rows, deviceError, st))
+        if (dtype == TCC_F32) TCC_BY_WIDTH(float, 4, w, CALL);
+        if (dtype == TCC_BF16) TCC_BY_WIDTH(bf16_t, 8, w, CALL);
+        TCC_BY_WIDTH(f16_t, 8, w, CALL);
+#undef CALL
+    }
+    if (n > 0) {
+        std::uint64_t* sorted = nullptr;
+        TCC_HIP_CHECK(partition_by(IdKeys{rows, n, deviceError}, reinterpret_cast<std::uint64_t*>(ws + lay.keysA),
+                                   reinterpret_cast<std::uint64_t*>(ws + lay.keysB), n, 32, id_bits(V),
+                                   reinterpret_cast<std::uint32_t*>(ws + lay.hist),
+                                   reinterpret_cast<std::uint32_t*>(ws + lay.total), &sorted, st));
+        a.keys = sorted;
+    }
+    if (!accumulate)
+        TCC_HIP_CHECK(fill<std::uint64_t>(reinterpret_cast<std::uint64_t*>(a.mark), (V + 8 * kWindow - 1) / (8 * kWindow),
+                                          0, st));
 #define CALL(T, N) (grad_launch<T, N>(a, st))
     if (dtype == TCC_F32) TCC_BY_WIDTH(float, 4, w, CALL);
     if (dtype == TCC_BF16) TCC_BY_WIDTH(bf16_t, 8, w, CALL);
