@@ -4,6 +4,8 @@
   (``include/tcc_swtcf.h``, ``include/tcc_spmm_cnic.h``), no torch dependency.
 * ``tcc_amd/spmm_cnic*.so`` — the ``spmm_cnic`` PyTorch extension (pybind11,
   C++), a thin layer over the C-ABI (see ``csrc/spmm_cnic_ext.cpp``).
+* ``tcc_amd/_training*.so`` — the extension behind ``tcc_amd.training``
+  (``csrc/training_ext.cpp``), another one.
 
 Run ``python -m tcc_amd.build`` (or ``__graft_entry__.build()``).
 """
@@ -76,14 +78,14 @@ def build_library(jobs: int = 8) -> str:
     return out
 
 
-def build_extension() -> str:
-    """Compile the spmm_cnic pybind11 module against libtcc_swtcf.so."""
+def build_extension(name: str = "spmm_cnic", source: str = "spmm_cnic_ext.cpp") -> str:
+    """Compile a pybind11 module of torch tensors against libtcc_swtcf.so."""
     import pybind11
     import torch.utils.cpp_extension as cpp
 
     os.makedirs(BUILD, exist_ok=True)
     suffix = sysconfig.get_config_var("EXT_SUFFIX")
-    out = os.path.join(PKG, "spmm_cnic" + suffix)
+    out = os.path.join(PKG, name + suffix)
     tmp = out + ".tmp"
     torch_lib = os.path.join(os.path.dirname(cpp.__file__), "..", "lib")
     torch_lib = os.path.abspath(torch_lib)
@@ -93,9 +95,9 @@ def build_extension() -> str:
     ]
     cmd = [
         "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1",
-        "-DTORCH_EXTENSION_NAME=spmm_cnic", "-DTORCH_API_INCLUDE_EXTENSION_H",
+        f"-DTORCH_EXTENSION_NAME={name}", "-DTORCH_API_INCLUDE_EXTENSION_H",
         "-D_GLIBCXX_USE_CXX11_ABI=1", *inc,
-        os.path.join(CSRC, "spmm_cnic_ext.cpp"), "-o", tmp,
+        os.path.join(CSRC, source), "-o", tmp,
         f"-L{PKG}", "-ltcc_swtcf", f"-L{torch_lib}", "-lc10", "-ltorch", "-ltorch_cpu",
         "-ltorch_python", "-lc10_hip", "-ltorch_hip", "-L/opt/rocm/lib", "-lamdhip64",
         "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}", "-Wl,-rpath,/opt/rocm/lib",
@@ -103,6 +105,11 @@ def build_extension() -> str:
     _run(cmd)
     os.replace(tmp, out)
     return out
+
+
+def build_training() -> str:
+    """The extension behind tcc_amd.training."""
+    return build_extension("_training", "training_ext.cpp")
 
 
 CLI_SOURCES = ["swtcf_convert_run.cpp", "swtcf_spmm_run.cpp"]
@@ -132,6 +139,7 @@ def main(argv=None) -> int:
         print("building", out, flush=True)
     if "--no-ext" not in argv:
         print("building", build_extension(), flush=True)
+        print("building", build_training(), flush=True)
     return 0
 
 
