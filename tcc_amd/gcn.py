@@ -33,6 +33,12 @@ GCN = conv1 (first layer, F_in -> hidden), ReLU, dropout, conv_final
 trained with cross-entropy and Adam (:448-449).  Without dropout and with at
 most 8 classes the two layers run as one autograd node whose backward forms
 both weight gradients in one pass (TwoLayerFunction).
+
+EmbeddingGCN is the model where the node rows are learned (graphs without
+features): rows of an embedding table (NodeEmbedding), conv1, a group norm
+over the node rows of each graph with its activation (NodeGroupNorm),
+conv_final, trained by ClippedAdam, over tcc_amd.training.  The reference,
+whose features are given, has no counterpart.
 """
 from __future__ import annotations
 
@@ -223,6 +229,153 @@ class GCN(torch.nn.Module):
         return self.conv_final(g2, x=x)
 
 
+class EmbeddingFunction(torch.autograd.Function):
+    """scale * table[ids] with the gradient of the table by sorted ids
+    (tcc_amd.training.embedding_lookup / embedding_grad)."""
+
+    @staticmethod
+    def forward(ctx, table, ids, scale, padding_idx, device_error):
+        from . import training
+
+        ctx.save_for_backward(ids)
+        ctx.args = table.shape[0], scale, padding_idx
+        return training.embedding_lookup(table, ids, scale=scale, padding_idx=padding_idx, device_error=device_error)
+
+    @staticmethod
+    def backward(ctx, d_out):
+        from . import training
+
+        (ids,) = ctx.saved_tensors
+        num_rows, scale, padding_idx = ctx.args
+        return training.embedding_grad(d_out, ids, num_rows, scale=scale, padding_idx=padding_idx), None, None, None, None
+
+
+class GroupNormFunction(torch.autograd.Function):
+    """act(group_norm(x)) over the rows of each segment, channels last
+    (tcc_amd.training.group_norm / group_norm_grad)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, num_groups, offsets, eps, activation, max_rows):
+        from . import training
+
+        y, mean, rstd = training.group_norm(x, num_groups, weight, bias, offsets=offsets, eps=eps, activation=activation,
+                                            max_rows=max_rows)
+        ctx.save_for_backward(x, weight, bias, offsets, mean, rstd)
+        ctx.args = num_groups, activation, max_rows
+        return y
+
+    @staticmethod
+    def backward(ctx, d_y):
+        from . import training
+
+        x, weight, bias, offsets, mean, rstd = ctx.saved_tensors
+        num_groups, activation, max_rows = ctx.args
+        dx, dw, db = training.group_norm_grad(d_y, x, mean, rstd, num_groups, weight, bias, offsets=offsets,
+                                              activation=activation, max_rows=max_rows)
+        dw = None if dw is None else dw.to(weight.dtype)
+        db = None if db is None else db.to(bias.dtype)
+        return dx, dw, db, None, None, None, None, None
+
+
+class NodeEmbedding(torch.nn.Module):
+    """A learned row of `dim` values for each of `num_nodes` nodes; forward
+    gives scale * rows of `ids` (sqrt(dim) times rows that begin at
+    1 / sqrt(dim) have unit variance).  The row of `padding_idx` stays zero.
+    error() reports ids outside the table, as FeatureTable's does."""
+
+    def __init__(self, num_nodes: int, dim: int, scale: float | None = None, padding_idx: int | None = None,
+                 device="cuda", dtype=torch.float32):
+        super().__init__()
+        self.scale = dim**0.5 if scale is None else scale
+        self.padding_idx = padding_idx
+        self.weight = torch.nn.Parameter(torch.randn((num_nodes, dim), device=device).div_(dim**0.5).to(dtype))
+        if padding_idx is not None:
+            with torch.no_grad():
+                self.weight[padding_idx].zero_()
+        self.device_error = torch.zeros(1, dtype=torch.int32, device=device)
+
+    def forward(self, ids: torch.Tensor) -> torch.Tensor:
+        return EmbeddingFunction.apply(self.weight, ids, self.scale, self.padding_idx, self.device_error)
+
+    def error(self) -> int:
+        """TCC_DEVERR_FEATURE_INDEX if an id fell outside the table since the
+        last call, else 0; synchronises the device and clears the word."""
+        v = int(self.device_error.item())
+        self.device_error.zero_()
+        return v
+
+
+class NodeGroupNorm(torch.nn.Module):
+    """Group norm over the node rows of each graph (the rows offsets[b] ..
+    offsets[b+1] of x; all rows without offsets) with its activation."""
+
+    def __init__(self, num_groups: int, channels: int, activation: str = "none", eps: float = 1e-5, device="cuda"):
+        super().__init__()
+        self.num_groups, self.activation, self.eps = num_groups, activation, eps
+        self.weight = torch.nn.Parameter(torch.ones(channels, device=device))
+        self.bias = torch.nn.Parameter(torch.zeros(channels, device=device))
+
+    def forward(self, x: torch.Tensor, offsets: torch.Tensor | None = None, max_rows: int | None = None) -> torch.Tensor:
+        return GroupNormFunction.apply(x, self.weight, self.bias, self.num_groups, offsets, self.eps, self.activation,
+                                       max_rows)
+
+
+class EmbeddingGCN(torch.nn.Module):
+    """conv_final(act(norm(conv1(embedding[ids])))) over a batch of graphs
+    (their block-diagonal A as one LayerGraph, `offsets` their first rows) or
+    one graph (no offsets)."""
+
+    def __init__(self, num_nodes: int, dim: int, hidden_dim: int, num_classes: int, num_groups: int = 8,
+                 activation: str = "relu", padding_idx: int | None = None):
+        super().__init__()
+        self.embedding = NodeEmbedding(num_nodes, dim, padding_idx=padding_idx)
+        self.conv1 = GCNConv(dim, hidden_dim).cuda()
+        self.norm = NodeGroupNorm(num_groups, hidden_dim, activation)
+        self.conv_final = GCNConv(hidden_dim, num_classes).cuda()
+
+    def forward(self, graph: LayerGraph, ids: torch.Tensor, offsets: torch.Tensor | None = None,
+                max_rows: int | None = None) -> torch.Tensor:
+        x = self.conv1(graph, x=self.embedding(ids))
+        return self.conv_final(graph, x=self.norm(x, offsets, max_rows))
+
+
+class ClippedAdam(torch.optim.Optimizer):
+    """Adam over one group of parameters whose gradients are clipped to
+    `max_norm` as the update reads them (tcc_amd.training.adam_step): step()
+    leaves the gradients as they are and returns their norm, a device scalar
+    (None without max_norm).  Nothing synchronises."""
+
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.0,
+                 decoupled: bool = True, max_norm: float | None = None):
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, decoupled=decoupled,
+                                      max_norm=max_norm))
+        if len(self.param_groups) != 1:
+            raise ValueError("ClippedAdam takes one group of parameters: the norm is over all of them")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        from . import training
+
+        if closure is not None:
+            with torch.enable_grad():
+                closure()
+        group = self.param_groups[0]
+        params = [p for p in group["params"] if p.grad is not None]
+        if not params:
+            return None
+        if "step" not in group:
+            group["step"] = torch.zeros((), dtype=torch.int64, device=params[0].device)
+        for p in params:
+            state = self.state[p]
+            if not state:
+                state["exp_avg"] = torch.zeros_like(p, dtype=torch.float32)
+                state["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32)
+        return training.adam_step(params, [p.grad for p in params], [self.state[p]["exp_avg"] for p in params],
+                                  [self.state[p]["exp_avg_sq"] for p in params], group["step"], lr=group["lr"],
+                                  betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
+                                  decoupled=group["decoupled"], max_norm=group["max_norm"])
+
+
 class FeatureTable:
     """Features of every node: the hot rows (top `hot_fraction` of nodes by
     in-degree as a source, ties by id) in an HBM cache, all rows in mapped
@@ -306,6 +459,17 @@ def train_epoch(model: GCN, g1: LayerGraph, g2: LayerGraph, source, labels: torc
     loss.backward()
     optimizer.step()
     return loss
+
+
+def train_embedding_epoch(model: EmbeddingGCN, graph: LayerGraph, ids: torch.Tensor, labels: torch.Tensor,
+                          optimizer: torch.optim.Optimizer, offsets: torch.Tensor | None = None,
+                          max_rows: int | None = None, loss_fcn=cross_entropy):
+    """One step of EmbeddingGCN: forward, loss, backward, clipped update.
+    Returns (loss, gradient norm), both on the device."""
+    loss = loss_fcn(model(graph, ids, offsets, max_rows), labels)
+    optimizer.zero_grad()
+    loss.backward()
+    return loss.detach(), optimizer.step()
 
 
 def synthetic_labels(n: int, num_classes: int, seed: int) -> torch.Tensor:

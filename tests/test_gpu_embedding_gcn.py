@@ -1,0 +1,129 @@
+"""The GCN with learned node rows (tcc_amd.gcn.EmbeddingGCN) against a dense
+64-bit evaluation, its optimizer, and the example that trains it.
+
+The forward SpMM rounds its input to TF32 (2^-11 of each value); the dense
+evaluation does the same where the model does, so that what is left is fp32
+arithmetic: rel-L2 1e-4, as for the GCN with given features."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+REL = 1e-4
+
+
+def rel_l2(a, b):
+    a = a.detach().double().cpu()
+    return float((a - b).norm() / b.norm().clamp(min=1e-30))
+
+
+class TF32(torch.autograd.Function):
+    """Rounding to TF32 in the forward pass, the identity backwards."""
+
+    @staticmethod
+    def forward(ctx, x):
+        b = x.float().numpy().view(np.uint32).astype(np.uint64)
+        return torch.from_numpy(((b + 0x1000) & 0xFFFFE000).astype(np.uint32).view(np.float32)).double()
+
+    @staticmethod
+    def backward(ctx, d):
+        return d
+
+
+def dense_step(A, table, ids, W1, w, b, W2, labels, at, groups, scale):
+    t = [v.detach().double().cpu().requires_grad_(True) for v in (table, W1, w, b, W2)]
+    x = t[0][ids] * scale
+    h = (A @ TF32.apply(x)) @ t[1] if W1.shape[1] >= W1.shape[0] else A @ TF32.apply(x @ t[1])
+    parts = []
+    for lo, hi in zip(at[:-1], at[1:]):
+        v = h[lo:hi].view(hi - lo, groups, -1)
+        d = v - v.mean((0, 2), keepdim=True)
+        parts.append((d / torch.sqrt(d.pow(2).mean((0, 2), keepdim=True) + 1e-5)).reshape(hi - lo, -1))
+    r = torch.relu(torch.cat(parts) * t[2] + t[3])
+    out = A @ TF32.apply(r @ t[4])
+    loss = torch.nn.functional.cross_entropy(out, labels)
+    return out.detach(), loss.detach(), torch.autograd.grad(loss, t)
+
+
+@pytest.mark.parametrize("batch", [True, False])
+def test_step_matches_dense_reference(gpu, batch):
+    from tcc_amd import gcn
+    from tcc_amd.train_embeddings import batch_of_graphs
+
+    torch.manual_seed(1)
+    nodes, dim, hidden, classes, groups = 700, 24, 48, 3, 6
+    rows, cols, ids, offsets, longest = batch_of_graphs(nodes, 25, 40, 3)
+    n = ids.numel()
+    graph = gcn.LayerGraph(rows, cols, n, n)
+    model = gcn.EmbeddingGCN(nodes, dim, hidden, classes, num_groups=groups)
+    labels = gcn.synthetic_labels(n, classes, 5)
+    with torch.no_grad():
+        model.norm.weight.uniform_(0.5, 1.5)
+        model.norm.bias.normal_()
+    off = offsets.cuda() if batch else None
+    out = model(graph, ids.cuda(), off, longest if batch else None)
+    loss = gcn.cross_entropy(out, labels)
+    loss.backward()
+    assert model.embedding.error() == 0
+    A = torch.zeros((n, n), dtype=torch.float64)
+    A[rows, cols] = 1.0
+    at = offsets.tolist() if batch else [0, n]
+    params = (model.embedding.weight, model.conv1.weights, model.norm.weight, model.norm.bias, model.conv_final.weights)
+    want, want_loss, grads = dense_step(A, params[0], ids, params[1], params[2], params[3], params[4], labels.cpu(), at,
+                                        groups, model.embedding.scale)
+    assert rel_l2(out, want) < REL and abs(float(loss) - float(want_loss)) < REL
+    for p, g in zip(params, grads):
+        assert rel_l2(p.grad, g) < REL
+    untouched = torch.ones(nodes, dtype=torch.bool)
+    untouched[ids] = False
+    assert int(torch.count_nonzero(model.embedding.weight.grad.cpu()[untouched])) == 0
+
+
+def test_padding_row_stays_and_bad_ids_are_reported(gpu):
+    from tcc_amd import gcn, swtcf
+
+    e = gcn.NodeEmbedding(20, 8, padding_idx=3)
+    ids = torch.tensor([3, 5, 3, 7], device="cuda")
+    y = e(ids)
+    assert torch.equal(y[0], torch.zeros(8, device="cuda"))
+    y.sum().backward()
+    assert int(torch.count_nonzero(e.weight.grad[3])) == 0 and int(torch.count_nonzero(e.weight.grad[5])) == 8
+    assert e.error() == 0
+    e(torch.tensor([25], device="cuda"))
+    assert e.error() == swtcf.DEVERR_FEATURE_INDEX and e.error() == 0
+
+
+def test_optimizer_follows_torch(gpu):
+    """ClippedAdam against clip_grad_norm_ and torch.optim.AdamW over steps with
+    gradients above and below the largest norm."""
+    from tcc_amd import gcn
+
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    new = lambda: [torch.nn.Parameter(torch.randn(s, generator=gen, device="cuda")) for s in ((30, 7), (11,))]  # noqa: E731
+    mine = new()
+    twin = [torch.nn.Parameter(p.detach().clone()) for p in mine]
+    unused = torch.nn.Parameter(torch.ones(4, device="cuda"))
+    a = gcn.ClippedAdam(mine + [unused], lr=0.02, weight_decay=0.1, max_norm=1.0)
+    b = torch.optim.AdamW(twin, lr=0.02, weight_decay=0.1)
+    for k in range(6):
+        for p, q in zip(mine, twin):
+            p.grad = torch.randn(p.shape, generator=gen, device="cuda") * (0.01 if k % 2 else 1.0)
+            q.grad = p.grad.clone()
+        norm = a.step()
+        want = torch.nn.utils.clip_grad_norm_(twin, 1.0)
+        b.step()
+        assert abs(float(norm) - float(want)) <= 1e-6 * float(want)
+        for p, q in zip(mine, twin):
+            assert float((p - q).abs().max()) <= 1e-6 * (k + 1) * 4
+    assert torch.equal(unused, torch.ones(4, device="cuda"))
+    with pytest.raises(ValueError):
+        gcn.ClippedAdam([{"params": mine}, {"params": [unused]}])
+
+
+def test_example_trains(gpu):
+    from tcc_amd import train_embeddings
+
+    losses, norms, _ = train_embeddings.train(nodes=2000, graphs=60, mean_rows=30, dim=16, hidden=32, steps=30,
+                                              log=lambda s: None)
+    assert all(np.isfinite(losses)) and all(np.isfinite(norms))
+    assert losses[-1] < 0.8 * losses[0]
