@@ -123,6 +123,72 @@ struct IdKeys {
     __device__ __forceinline__ void report(bool bad) const { tcc::report(err, bad); }
 };
 
+// The sort of up to kRankRows keys in one launch: a key's place is the number of
+// keys before it, counted against all of them, which every workgroup holds.
+// n^2 / 64 comparisons of two instructions each, over a wave for every 64 keys
+// and 16th of the keys they are compared with; it also clears the windows'
+// marks.  With the passes by digits, five launches more, a gradient of 8,000
+// rows of 32 takes 45 us instead of 34, of 16,384 the same 44.
+constexpr std::uint64_t kRankRows = 12288;
+constexpr int kRankThreads = 1024, kRankWaves = kRankThreads / kWave;
+__global__ void __launch_bounds__(kRankThreads) rank_kernel(IdKeys src, std::uint64_t* __restrict__ out,
+                                                           std::uint64_t* __restrict__ marks, std::uint64_t markWords) {
+    extern __shared__ __attribute__((aligned(16))) std::uint32_t rowOf[];  // padded to whole 64s
+    __shared__ std::uint32_t counts[kRankWaves][kWave];
+    const std::uint32_t n = static_cast<std::uint32_t>(src.n), padded = (n + kWave - 1) / kWave * kWave;
+    const std::uint32_t none = static_cast<std::uint32_t>(src.ids.V);
+    for (std::uint64_t i = static_cast<std::uint64_t>(blockIdx.x) * kRankThreads + threadIdx.x; i < markWords;
+         i += static_cast<std::uint64_t>(gridDim.x) * kRankThreads)
+        marks[i] = 0;
+    bool bad = false;
+    for (std::uint32_t i = threadIdx.x; i < padded; i += 8 * kRankThreads) {
+        std::uint32_t v[8];
+        src.ids.rows<8>(i, kRankThreads, n, v, bad);
+#pragma unroll
+        for (std::uint32_t r = 0; r < 8; ++r) {
+            const std::uint32_t at = i + r * kRankThreads;
+            // past the end: after every key
+            if (at < padded) rowOf[at] = at >= n ? kNoRow : v[r] == kNoRow ? none : v[r];
+        }
+    }
+    if (blockIdx.x == 0) src.report(bad);
+    __syncthreads();
+    const std::uint32_t wave = uniform(threadIdx.x / kWave), lane = __lane_id();
+    const std::uint32_t i0 = blockIdx.x * kWave, i = i0 + lane, mine = rowOf[i];
+    // this wave's share of the 64s, a lane's key against each of their keys
+    const std::uint32_t tiles = padded / kWave;
+    std::uint32_t before = 0;
+    for (std::uint32_t t = wave; t < tiles; t += kRankWaves) {
+        const vu4* keys = reinterpret_cast<const vu4*>(rowOf + t * kWave);
+        if (t * kWave < i0) {  // equal rows come before
+#pragma unroll 4
+            for (std::uint32_t j = 0; j < kWave / 4; ++j) {
+                const vu4 k = keys[j];
+                before += (k[0] <= mine) + (k[1] <= mine) + (k[2] <= mine) + (k[3] <= mine);
+            }
+        } else if (t * kWave > i0) {  // and after
+#pragma unroll 4
+            for (std::uint32_t j = 0; j < kWave / 4; ++j) {
+                const vu4 k = keys[j];
+                before += (k[0] < mine) + (k[1] < mine) + (k[2] < mine) + (k[3] < mine);
+            }
+        } else {
+            for (std::uint32_t j = 0; j < kWave; ++j) {
+                const std::uint32_t k = rowOf[i0 + j];
+                before += k < mine || (k == mine && j < lane) ? 1u : 0u;
+            }
+        }
+    }
+    counts[wave][lane] = before;
+    __syncthreads();
+    if (wave == 0 && i < n) {
+        std::uint32_t place = 0;
+#pragma unroll
+        for (int w = 0; w < kRankWaves; ++w) place += counts[w][lane];
+        out[place] = static_cast<std::uint64_t>(mine) << 32 | i;
+    }
+}
+
 struct GradArgs {
     const std::uint64_t* keys;  // sorted
     const void* dOut;
@@ -342,8 +408,8 @@ __global__ void __launch_bounds__(kThreads) join_kernel(GradArgs a) {
 // the first position of each row looks for the others.  That is n^2 / 64
 // comparisons, which a few thousand rows spread over the GPU need less time for
 // than a sort's launches follow each other in: rows of 32 fp32 into a table of
-// 4,096, 8 us and sorted 52 for 1,000 of them, 12 and 45 for 2,048, 28 and 46
-// for 4,096 (of 256 values 38 and 39).
+// 4,096, 8 us and sorted 38 for 1,000 of them, 12 and 32 for 2,000, 28 and 32
+// for 4,096.
 constexpr std::uint64_t kFewRows = 4096;
 constexpr std::uint32_t kFewZeroRows = 256;  // rows of a workgroup that zeroes, at most
 
@@ -589,17 +655,26 @@ int tcc_embedding_grad(const void* dOut, uint64_t ldd, uint32_t dtype, const voi
         TCC_BY_WIDTH(f16_t, 8, w, CALL);
 #undef CALL
     }
-    if (n > 0) {
-        std::uint64_t* sorted = nullptr;
-        TCC_HIP_CHECK(partition_by(IdKeys{rows, n, deviceError}, reinterpret_cast<std::uint64_t*>(ws + lay.keysA),
-                                   reinterpret_cast<std::uint64_t*>(ws + lay.keysB), n, 32, id_bits(V),
-                                   reinterpret_cast<std::uint32_t*>(ws + lay.hist),
-                                   reinterpret_cast<std::uint32_t*>(ws + lay.total), &sorted, st));
-        a.keys = sorted;
+    const std::uint64_t markWords = accumulate ? 0 : (V + 8 * kWindow - 1) / (8 * kWindow);
+    std::uint64_t* const marks = reinterpret_cast<std::uint64_t*>(a.mark);
+    std::uint64_t* const keys = reinterpret_cast<std::uint64_t*>(ws + lay.keysA);
+    if (n > 0 && n <= kRankRows) {
+        const unsigned blocks = grid_for(n, kWave);
+        hipLaunchKernelGGL(rank_kernel, dim3(blocks), dim3(kRankThreads), blocks * kWave * sizeof(std::uint32_t), st,
+                           IdKeys{rows, n, deviceError}, keys, marks, markWords);
+        TCC_LAUNCH_CHECK();
+        a.keys = keys;
+    } else {
+        if (n > 0) {
+            std::uint64_t* sorted = nullptr;
+            TCC_HIP_CHECK(partition_by(IdKeys{rows, n, deviceError}, keys,
+                                       reinterpret_cast<std::uint64_t*>(ws + lay.keysB), n, 32, id_bits(V),
+                                       reinterpret_cast<std::uint32_t*>(ws + lay.hist),
+                                       reinterpret_cast<std::uint32_t*>(ws + lay.total), &sorted, st));
+            a.keys = sorted;
+        }
+        TCC_HIP_CHECK(fill<std::uint64_t>(marks, markWords, 0, st));
     }
-    if (!accumulate)
-        TCC_HIP_CHECK(fill<std::uint64_t>(reinterpret_cast<std::uint64_t*>(a.mark), (V + 8 * kWindow - 1) / (8 * kWindow),
-                                          0, st));
 #define CALL(T, N) (grad_launch<T, N>(a, st))
     if (dtype == TCC_F32) TCC_BY_WIDTH(float, 4, w, CALL);
     if (dtype == TCC_BF16) TCC_BY_WIDTH(bf16_t, 8, w, CALL);

@@ -322,7 +322,11 @@ __device__ __forceinline__ float slot_rows(const NormArgs& a, std::uint64_t t, s
 template <int W>
 struct JoinGroup {
     static constexpr int threads = W > 1 ? W * kWave : kThreads;
-    static unsigned grid(std::uint32_t G) { return W > 1 ? G : (G + kWaves - 1) / kWaves; }
+    // few workgroups, each with many segments: most have none to join
+    static dim3 grid(std::uint64_t B, std::uint32_t G) {
+        const std::uint32_t y = W > 1 ? G : (G + kWaves - 1) / kWaves;
+        return dim3(static_cast<unsigned>(std::min<std::uint64_t>(B, std::max(1u, 2048 / y))), y);
+    }
     __device__ __forceinline__ static std::uint32_t group() {
         return W > 1 ? blockIdx.y : blockIdx.y * kWaves + threadIdx.x / kWave;
     }
@@ -347,29 +351,30 @@ __global__ void __launch_bounds__(JoinGroup<W>::threads) stats_join_kernel(NormA
     if (!tiles_needed(a.seen, a.seenCount)) return;
     using Join = JoinGroup<W>;
     __shared__ float red[W];
-    const std::uint64_t s = blockIdx.x;
     const std::uint32_t g = Join::group();
-    const std::uint64_t first = a.seg.start(s), end = a.seg.start(s + 1);
-    if (g >= a.G || (first < end && a.seg.whole(s))) return;
-    float mean = 0.0f, var = 0.0f;
-    if (first < end) {
-        const std::uint64_t t0 = first / a.tileRows, t1 = (end - 1) / a.tileRows;
-        const float rows = static_cast<float>(end - first);
-        float sum = 0.0f;
-        for (std::uint64_t t = t0 + Join::first(); t <= t1; t += kWave * W)
-            sum += a.part[(t + s) * a.G + g].x * slot_rows(a, t, first, end);
-        mean = Join::sum(sum, red) / rows;
-        float dev = 0.0f;
-        for (std::uint64_t t = t0 + Join::first(); t <= t1; t += kWave * W) {
-            const float2 p = a.part[(t + s) * a.G + g];
-            const float gap = p.x - mean;
-            dev += p.y + gap * gap * slot_rows(a, t, first, end) * static_cast<float>(a.K);
+    for (std::uint64_t s = blockIdx.x; s < a.seg.B; s += gridDim.x) {
+        const std::uint64_t first = a.seg.start(s), end = a.seg.start(s + 1);
+        if (g >= a.G || (first < end && a.seg.whole(s))) continue;
+        float mean = 0.0f, var = 0.0f;
+        if (first < end) {
+            const std::uint64_t t0 = first / a.tileRows, t1 = (end - 1) / a.tileRows;
+            const float rows = static_cast<float>(end - first);
+            float sum = 0.0f;
+            for (std::uint64_t t = t0 + Join::first(); t <= t1; t += kWave * W)
+                sum += a.part[(t + s) * a.G + g].x * slot_rows(a, t, first, end);
+            mean = Join::sum(sum, red) / rows;
+            float dev = 0.0f;
+            for (std::uint64_t t = t0 + Join::first(); t <= t1; t += kWave * W) {
+                const float2 p = a.part[(t + s) * a.G + g];
+                const float gap = p.x - mean;
+                dev += p.y + gap * gap * slot_rows(a, t, first, end) * static_cast<float>(a.K);
+            }
+            var = Join::sum(dev, red) / (rows * static_cast<float>(a.K));
         }
-        var = Join::sum(dev, red) / (rows * static_cast<float>(a.K));
-    }
-    if (Join::first() == 0) {
-        a.mean[s * a.G + g] = mean;
-        a.rstd[s * a.G + g] = 1.0f / sqrtf(var + a.eps);
+        if (Join::first() == 0) {
+            a.mean[s * a.G + g] = mean;
+            a.rstd[s * a.G + g] = 1.0f / sqrtf(var + a.eps);
+        }
     }
 }
 
@@ -490,21 +495,22 @@ __global__ void __launch_bounds__(JoinGroup<W>::threads) grad_join_kernel(NormAr
     if (!tiles_needed(a.seen, a.seenCount)) return;
     using Join = JoinGroup<W>;
     __shared__ float red[W];
-    const std::uint64_t s = blockIdx.x;
     const std::uint32_t g = Join::group();
-    const std::uint64_t first = a.seg.start(s), end = a.seg.start(s + 1);
-    if (g >= a.G || first >= end || a.seg.whole(s)) return;
-    const std::uint64_t t0 = first / a.tileRows, t1 = (end - 1) / a.tileRows;
-    float s1 = 0.0f, s2 = 0.0f;
-    for (std::uint64_t t = t0 + Join::first(); t <= t1; t += kWave * W) {
-        const float2 p = a.part[(t + s) * a.G + g];
-        s1 += p.x;
-        s2 += p.y;
+    for (std::uint64_t s = blockIdx.x; s < a.seg.B; s += gridDim.x) {
+        const std::uint64_t first = a.seg.start(s), end = a.seg.start(s + 1);
+        if (g >= a.G || first >= end || a.seg.whole(s)) continue;
+        const std::uint64_t t0 = first / a.tileRows, t1 = (end - 1) / a.tileRows;
+        float s1 = 0.0f, s2 = 0.0f;
+        for (std::uint64_t t = t0 + Join::first(); t <= t1; t += kWave * W) {
+            const float2 p = a.part[(t + s) * a.G + g];
+            s1 += p.x;
+            s2 += p.y;
+        }
+        s1 = Join::sum(s1, red);
+        s2 = Join::sum(s2, red);
+        const float size = static_cast<float>(end - first) * static_cast<float>(a.K);
+        if (Join::first() == 0) a.sums[s * a.G + g] = float2{s1 / size, s2 / size};
     }
-    s1 = Join::sum(s1, red);
-    s2 = Join::sum(s2, red);
-    const float size = static_cast<float>(end - first) * static_cast<float>(a.K);
-    if (Join::first() == 0) a.sums[s * a.G + g] = float2{s1 / size, s2 / size};
 }
 
 // dBias and dWeight from `rows` rows of partial sums: 4 columns a workgroup,
@@ -598,7 +604,7 @@ struct WholeArgs {
     std::uint32_t groups;     // of a slice
     std::uint32_t cols;       // its vectors a row
     std::uint32_t laneBits;   // lanes of a row: a power of two that holds them, at most `threads`
-    std::uint32_t groupCols;  // vectors of a group
+    std::uint32_t groupCols;  // vectors of a group (1 where they straddle groups)
 };
 
 // Sums of a pair of values over the lanes of each group, each lane getting its
@@ -641,7 +647,7 @@ struct GroupSum {
 template <int N>
 struct WholeLane {
     std::uint32_t cv, row, rowLanes, c;  // its vector of the slice, row lane, the rows at once, its first channel
-    std::uint32_t g;                     // its group
+    std::uint32_t g0, g;                 // the slice's first group; the lane's (where a vector lies in one)
     std::uint32_t block;                 // the first of its segments
     bool active;
     GroupSum sum;
@@ -657,9 +663,10 @@ struct WholeLane {
         row = threadIdx.x >> k.laneBits;
         rowLanes = k.threads >> k.laneBits;
         active = cv < k.cols;
-        const std::uint32_t inSlice = cv / k.groupCols;
-        g = slice * k.groups + inSlice;
+        g0 = slice * k.groups;
         c = (slice * k.cols + cv) * N;
+        const std::uint32_t inSlice = cv / k.groupCols;
+        g = g0 + inSlice;
         sum = GroupSum{k.threads, lanes, k.groupCols, cv, min(inSlice, k.groups - 1) * k.groupCols,
                        (k.groupCols & (k.groupCols - 1)) == 0};
     }
@@ -705,6 +712,16 @@ __device__ __forceinline__ void each_row(std::uint64_t r, std::uint64_t rows, st
         for (int i = 0; i < kBatch; ++i)
             if (i < more) body(__builtin_convertvector(v[i], vec_t<float, N>), __builtin_convertvector(u[i], vec_t<float, N>), i);
     }
+}
+
+// What a workgroup saw, told by one of its segments' workgroups (`teller`).
+__device__ __forceinline__ void tell_seen(const NormArgs& a, const WholeArgs& k, std::uint32_t block, bool teller,
+                                          std::uint8_t anyLong) {
+    if (!teller || a.seenCount == 0) return;
+    if (block < k.blocks) a.seen[block] = anyLong;
+    // places past `blocks` that the tiles' 16-byte loads take in
+    if (block + 1 == k.blocks)
+        for (std::uint32_t i = k.blocks; i % 16 != 0; ++i) a.seen[i] = 0;
 }
 
 // A lane's values so far: what they exceed the mean of its first vector by, and
@@ -795,12 +812,7 @@ __global__ void __launch_bounds__(kWholeThreads, 4) whole_kernel(NormArgs a, Who
                     }
             });
     }
-    // places past `blocks` that the tiles' 16-byte loads take in
-    if (me.c == 0 && me.row == 0 && a.seenCount > 0) {
-        if (me.block < k.blocks) a.seen[me.block] = anyLong;
-        if (me.block + 1 == k.blocks)
-            for (std::uint32_t i = k.blocks; i % 16 != 0; ++i) a.seen[i] = 0;
-    }
+    tell_seen(a, k, me.block, me.c == 0 && me.row == 0, anyLong);
 }
 
 // Whether the first batch's dz w stay in LDS between the two readings: where the
@@ -899,12 +911,7 @@ __global__ void __launch_bounds__(kWholeThreads, 4) whole_grad_kernel(NormArgs a
                            });
         }
     }
-    // places past `blocks` that the tiles' 16-byte loads take in
-    if (me.c == 0 && me.row == 0 && a.seenCount > 0) {
-        if (me.block < k.blocks) a.seen[me.block] = anyLong;
-        if (me.block + 1 == k.blocks)
-            for (std::uint32_t i = k.blocks; i % 16 != 0; ++i) a.seen[i] = 0;
-    }
+    tell_seen(a, k, me.block, me.c == 0 && me.row == 0, anyLong);
     if (partial == nullptr || me.block >= k.blocks) return;
     __syncthreads();
 #pragma unroll
@@ -922,6 +929,238 @@ __global__ void __launch_bounds__(kWholeThreads, 4) whole_grad_kernel(NormArgs a
     }
 }
 
+// ---------------------------------------------------------------- groups of odd sizes
+
+// Whole segments where a lane's vector straddles groups (C / G of 3 or 25, say):
+// channels are summed apart and joined to groups in LDS.  Lanes as narrow as
+// such groups allow, a channel each at worst, took 5 to 13 times the time that
+// the bytes need.
+
+// The lanes' pairs for each channel, summed over the rows of a workgroup: the
+// places of `rows` partial sums of channel c of the slice are c, c + stride, ...
+template <int N>
+struct ChannelSums {
+    float2* places;
+    std::uint32_t rows, stride;
+    __device__ __forceinline__ ChannelSums(const WholeArgs& k, float2* p) : places(p) {
+        const std::uint32_t lanes = 1u << k.laneBits;
+        rows = lanes < kWave ? k.threads / kWave : k.threads / lanes;
+        stride = lanes * N;
+    }
+    __device__ __forceinline__ void put(const WholeArgs& k, vec_t<float, N> x, vec_t<float, N> y) const {
+        const std::uint32_t lanes = 1u << k.laneBits;
+        for (std::uint32_t d = lanes; d < kWave; d <<= 1)
+#pragma unroll
+            for (int q = 0; q < N; ++q) {
+                x[q] += __shfl_xor(x[q], d, kWave);
+                y[q] += __shfl_xor(y[q], d, kWave);
+            }
+        const std::uint32_t at = lanes < kWave ? threadIdx.x / kWave * lanes + __lane_id() : threadIdx.x;
+        if (lanes >= kWave || __lane_id() < lanes)
+#pragma unroll
+            for (int q = 0; q < N; ++q) places[at * N + q] = float2{x[q], y[q]};
+    }
+    __device__ __forceinline__ float2 of(std::uint32_t c) const {
+        float2 s{0.0f, 0.0f};
+        for (std::uint32_t r = 0; r < rows; ++r) {
+            const float2 p = places[r * stride + c];
+            s.x += p.x;
+            s.y += p.y;
+        }
+        return s;
+    }
+};
+
+// The threads of a workgroup as teams, one for a group of the slice at a time.
+struct GroupTeam {
+    std::uint32_t size, first, step, lane;
+    __device__ __forceinline__ explicit GroupTeam(const WholeArgs& k) {
+        size = 1;
+        while (size < kWave && 2 * size * k.groups <= k.threads) size *= 2;
+        first = threadIdx.x / size;
+        step = k.threads / size;
+        lane = threadIdx.x % size;
+    }
+    __device__ __forceinline__ float sum(float v) const {
+        for (std::uint32_t d = 1; d < size; d <<= 1) v += __shfl_xor(v, d, kWave);
+        return v;
+    }
+};
+
+// LDS: the channels' places, [lanes * N] floats of their shifts, a pair for each group.
+template <int N>
+std::uint32_t spread_lds(const WholeArgs& k) {
+    return (k.threads * N + ((1u << k.laneBits) * N + 1) / 2 + k.groups) * static_cast<std::uint32_t>(sizeof(float2));
+}
+
+template <typename T, int N, std::uint32_t ACT>
+__global__ void __launch_bounds__(kWholeThreads, 4) spread_kernel(NormArgs a, WholeArgs k) {
+    extern __shared__ float2 places[];
+    float* const shifts = reinterpret_cast<float*>(places + k.threads * N);
+    float2* const groups = places + k.threads * N + ((1u << k.laneBits) * N + 1) / 2;
+    const WholeLane<N> me(a, k);
+    const ChannelSums<N> channels(k, places);
+    const GroupTeam team(k);
+    const std::uint32_t c = me.active ? me.c : 0u, own = me.cv * N;  // the channel in the slice
+    const vec_t<float, N> w = load_params<N>(a.weight, a.paramType, c, 1.0f), b = load_params<N>(a.bias, a.paramType, c, 0.0f);
+    std::uint8_t anyLong = 0;
+    for (std::uint64_t s = me.block; s < a.seg.B; s += k.blocks) {
+        const std::uint64_t first = a.seg.start(s), end = a.seg.start(s + 1);
+        if (first < end && end - first > a.seg.longest) {
+            anyLong = 1;
+            continue;
+        }
+        const std::uint64_t rows = first < end ? end - first : 0;
+        const T* x = static_cast<const T*>(a.x) + (first + me.row) * a.ldx + me.c;
+        T* y = static_cast<T*>(a.out) + (first + me.row) * a.ldo + me.c;
+        vec_t<float, N> shift(0.0f), sum(0.0f), square(0.0f);
+        if (me.active && rows > 0) {
+            // the same for every lane of these channels: the mean of four rows
+            const T* p = static_cast<const T*>(a.x) + first * a.ldx + me.c;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) shift += load_row<T, N>(p + rows * i / 4 * a.ldx);
+            shift *= 0.25f;
+            each_row<T, N>(me.row, rows, me.rowLanes, x, me.rowLanes * a.ldx, [&](vec_t<T, N>(&v)[kBatch], int more) {
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i)
+                    if (i < more) {
+                        const vec_t<float, N> e = __builtin_convertvector(v[i], vec_t<float, N>) - shift;
+                        sum += e;
+                        square += e * e;
+                    }
+            });
+            if (me.row == 0)
+#pragma unroll
+                for (int q = 0; q < N; ++q) shifts[own + q] = shift[q];
+        }
+        channels.put(k, sum, square);
+        __syncthreads();
+        const float n = static_cast<float>(rows), size = n * static_cast<float>(a.K);
+        for (std::uint32_t g = team.first; g < k.groups; g += team.step) {
+            float mean = 0.0f, var = 0.0f;
+            if (rows > 0) {
+                for (std::uint32_t e = g * a.K + team.lane; e < (g + 1) * a.K; e += team.size)
+                    mean += shifts[e] + channels.of(e).x / n;
+                mean = team.sum(mean) / static_cast<float>(a.K);
+                for (std::uint32_t e = g * a.K + team.lane; e < (g + 1) * a.K; e += team.size) {
+                    const float2 p = channels.of(e);
+                    const float part = p.x / n, gap = (shifts[e] - mean) + part;
+                    var += (p.y - p.x * part) + n * gap * gap;
+                }
+                var = team.sum(var) / size;
+                var = var < 0.0f ? 0.0f : var;  // NaN stays
+            }
+            if (team.lane == 0) {
+                const float rs = 1.0f / sqrtf(var + a.eps);
+                groups[g] = float2{mean, rs};
+                a.mean[s * a.G + me.g0 + g] = mean;
+                a.rstd[s * a.G + me.g0 + g] = rs;
+            }
+        }
+        __syncthreads();
+        if (!me.active || rows == 0) continue;
+        float2 of[N];
+#pragma unroll
+        for (int q = 0; q < N; ++q) of[q] = groups[(own + q) / a.K];
+        each_row<T, N>(me.row, rows, me.rowLanes, x, me.rowLanes * a.ldx, [&](vec_t<T, N>(&v)[kBatch], int more) {
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i)
+                if (i < more) {
+                    const vec_t<float, N> f = __builtin_convertvector(v[i], vec_t<float, N>);
+                    vec_t<float, N> o;
+#pragma unroll
+                    for (int q = 0; q < N; ++q) o[q] = activate<ACT>(affine(normalise(f[q], of[q].x, of[q].y), w[q], b[q]));
+                    store_row<T, N>(y, o);
+                    y += me.rowLanes * a.ldo;
+                }
+        });
+    }
+    tell_seen(a, k, me.block, me.c == 0 && me.row == 0, anyLong);
+}
+
+// `partial` as in whole_grad_kernel.
+template <typename T, int N, std::uint32_t ACT>
+__global__ void __launch_bounds__(kWholeThreads, 4) spread_grad_kernel(NormArgs a, WholeArgs k, float2* partial) {
+    extern __shared__ float2 places[];
+    float2* const groups = places + k.threads * N + ((1u << k.laneBits) * N + 1) / 2;
+    const WholeLane<N> me(a, k);
+    const ChannelSums<N> channels(k, places);
+    const GroupTeam team(k);
+    const std::uint32_t c = me.active ? me.c : 0u, own = me.cv * N;
+    const vec_t<float, N> w = load_params<N>(a.weight, a.paramType, c, 1.0f), b = load_params<N>(a.bias, a.paramType, c, 0.0f);
+    vec_t<float, N> dw(0.0f), db(0.0f);
+    std::uint8_t anyLong = 0;
+    for (std::uint64_t s = me.block; s < a.seg.B; s += k.blocks) {
+        const std::uint64_t first = a.seg.start(s), end = a.seg.start(s + 1);
+        if (first >= end) continue;
+        if (end - first > a.seg.longest) {
+            anyLong = 1;
+            continue;
+        }
+        const std::uint64_t rows = end - first;
+        const T* x = static_cast<const T*>(a.x) + (first + me.row) * a.ldx + me.c;
+        const T* dy = static_cast<const T*>(a.dy) + (first + me.row) * a.lddy + me.c;
+        T* dx = static_cast<T*>(a.out) + (first + me.row) * a.ldo + me.c;
+        const std::uint64_t stepX = me.rowLanes * a.ldx, stepD = me.rowLanes * a.lddy;
+        float mean[N], rstd[N];
+#pragma unroll
+        for (int q = 0; q < N; ++q) {
+            const std::uint64_t at = s * a.G + (me.active ? me.g0 + (own + q) / a.K : 0u);
+            mean[q] = a.mean[at];
+            rstd[q] = a.rstd[at];
+        }
+        vec_t<float, N> s1(0.0f), s2(0.0f);
+        if (me.active)
+            each_row<T, N>(me.row, rows, me.rowLanes, x, stepX, dy, stepD, [&](vec_t<float, N> v, vec_t<float, N> d, int) {
+#pragma unroll
+                for (int q = 0; q < N; ++q) {
+                    const float xh = normalise(v[q], mean[q], rstd[q]);
+                    const float z = d[q] * slope<ACT>(affine(xh, w[q], b[q]));
+                    s1[q] += z;
+                    s2[q] = fmaf(z, xh, s2[q]);
+                }
+            });
+        db += s1;
+        dw += s2;
+        channels.put(k, s1 * w, s2 * w);
+        __syncthreads();
+        const float size = static_cast<float>(rows) * static_cast<float>(a.K);
+        for (std::uint32_t g = team.first; g < k.groups; g += team.step) {
+            float2 m{0.0f, 0.0f};
+            for (std::uint32_t e = g * a.K + team.lane; e < (g + 1) * a.K; e += team.size) {
+                const float2 p = channels.of(e);
+                m.x += p.x;
+                m.y += p.y;
+            }
+            m.x = team.sum(m.x);
+            m.y = team.sum(m.y);
+            if (team.lane == 0) groups[g] = float2{m.x / size, m.y / size};
+        }
+        __syncthreads();
+        if (!me.active) continue;
+        float2 of[N];
+#pragma unroll
+        for (int q = 0; q < N; ++q) of[q] = groups[(own + q) / a.K];
+        each_row<T, N>(me.row, rows, me.rowLanes, x, stepX, dy, stepD, [&](vec_t<float, N> v, vec_t<float, N> d, int) {
+            vec_t<float, N> o;
+#pragma unroll
+            for (int q = 0; q < N; ++q) {
+                const float xh = normalise(v[q], mean[q], rstd[q]);
+                o[q] = (d[q] * slope<ACT>(affine(xh, w[q], b[q])) * w[q] - of[q].x - xh * of[q].y) * rstd[q];
+            }
+            store_row<T, N>(dx, o);
+            dx += me.rowLanes * a.ldo;
+        });
+    }
+    tell_seen(a, k, me.block, me.c == 0 && me.row == 0, anyLong);
+    if (partial == nullptr || me.block >= k.blocks) return;
+    __syncthreads();
+    channels.put(k, me.active ? db : vec_t<float, N>(0.0f), me.active ? dw : vec_t<float, N>(0.0f));
+    __syncthreads();
+    for (std::uint32_t i = threadIdx.x; i < k.cols * N; i += k.threads)
+        partial[me.block * static_cast<std::uint64_t>(a.C) + me.g0 * a.K + i] = channels.of(i);
+}
+
 // ---------------------------------------------------------------- host side
 
 constexpr std::size_t align16(std::size_t b) { return (b + 15) & ~std::size_t(15); }
@@ -929,43 +1168,60 @@ constexpr std::size_t align16(std::size_t b) { return (b + 15) & ~std::size_t(15
 // Tiles of at most this many, so that the tiles' sums stay few.
 constexpr std::uint64_t kTiles = 2048;
 // A segment that a workgroup walks in at most this many steps goes whole (some
-// 20 us; a longer one would end after all others), and all segments do where x
-// has no more than kSmallBytes.
-constexpr std::uint64_t kWholeSteps = 32, kSmallBytes = 1 << 20;
+// 20 us; a longer one would end after all others): kManySteps where a thousand
+// and more take longer in all, kWaveSteps for waves, of which thousands are
+// under way at once.  All segments do, for the
+// launches that this saves, where no more than kSmallSteps could make one of
+// them and kSkew times the mean would still be short; none do where a segment of
+// kUneven times the mean, as batches have them, would be too long anyway.
+constexpr std::uint64_t kWholeSteps = 32, kManySteps = 64, kWaveSteps = 128, kSmallSteps = 256, kSkew = 8, kUneven = 4;
 // Workgroups of a slice of whole segments, each with its own dWeight and dBias.
 constexpr std::uint64_t kWholeBlocks = 4096;
 
 // Elements a lane takes in a whole segment, of `width` that the rows allow: a
-// power of two that divides a group.
-std::uint32_t whole_width(std::uint32_t K, std::uint32_t width) {
-    while (K % width != 0) width /= 2;
-    return width;
-}
+// power of two that divides a group, or up to four that straddle groups where
+// these have no such divisor.
+struct WholeWidth {
+    std::uint32_t n;
+    bool spread;
+    WholeWidth(std::uint32_t K, std::uint32_t width) : n(width), spread(false) {
+        while (K % n != 0) n /= 2;
+        const std::uint32_t wide = std::min(width, 4u);
+        if (n < wide) {
+            n = wide;
+            spread = true;
+        }
+    }
+};
 
-// How whole segments are cut, for lanes of n elements: into slices of whole
-// groups of at least 128 bytes a row (64 where fewer than 1024 segments have to
+// How whole segments are cut, for such lanes: into slices of whole groups (and
+// lanes) of at least 128 bytes a row (64 where fewer than 1024 segments have to
 // spread over the GPU), a wave for a slice where that takes the usual segment in
-// one step of loads, else four.  169,000 rows of 128 bf16 channels, forward and
+// two batches of loads, else four.  169,000 rows of 128 bf16 channels, forward and
 // gradient together: in segments of 21 rows 97 us with one wave and 268 us with
 // four, of 85 rows (four times as many) 224 us and 207 us; whole rows instead
-// of slices cost 2 to 10% more.
-WholeArgs whole_args(const tcc_group_norm_shape& s, std::uint32_t n) {
-    const std::uint32_t elem = dtype_bytes(s.dtype), K = s.C / s.G;
+// of slices cost 2 to 10% more.  No groups: a slice is wider than a workgroup.
+WholeArgs whole_args(const tcc_group_norm_shape& s, const WholeWidth& width) {
+    const std::uint32_t elem = dtype_bytes(s.dtype), K = s.C / s.G, n = width.n;
     WholeArgs k{};
-    k.groupCols = K / n;
+    k.groupCols = width.spread ? 1 : K / n;
     for (std::uint32_t g = 1; g <= s.G; ++g) {
-        if (s.G % g != 0) continue;
-        if (g > 1 && g * k.groupCols > kWholeThreads) break;
+        if (s.G % g != 0 || g * K % n != 0) continue;
+        if (g * K / n > kWholeThreads) break;
         k.groups = g;
         if (g * K * elem >= (s.B < 1024 ? 64 : 128)) break;
     }
+    if (k.groups == 0) return k;
     k.slices = s.G / k.groups;
-    k.cols = k.groups * k.groupCols;
+    k.cols = k.groups * K / n;
     while ((1u << k.laneBits) < k.cols) ++k.laneBits;
-    const bool wave = s.B >= 1024 && k.cols <= kWave && s.N / s.B <= kBatch * (kWave >> k.laneBits);
+    const bool wave = s.B >= 1024 && k.cols <= kWave && s.N / s.B <= 2 * kBatch * (kWave >> k.laneBits);
     k.threads = wave ? kWave : kWholeThreads;
     return k;
 }
+
+// The width of aligned rows of C elements.
+std::uint32_t full_width(std::uint32_t C, std::uint32_t elem) { return RowWidth(C, elem).elems(); }
 
 // Which segments go whole and which tile by tile, from what the host knows.
 struct Split {
@@ -973,17 +1229,18 @@ struct Split {
     bool whole, tiles;      // whether either kind may occur
     // `width`: elements a lane can take at once, by the rows' alignment
     Split(const tcc_group_norm_shape& s, std::uint32_t width) {
-        const std::uint32_t elem = dtype_bytes(s.dtype), K = s.C / s.G;
-        const std::uint64_t row = static_cast<std::uint64_t>(s.C) * elem;
-        const std::uint64_t most = s.offsets == nullptr ? (s.B > 0 ? s.N / s.B : 0) : s.maxRows > 0 ? s.maxRows : s.N;
-        const std::uint32_t aligned = whole_width(K, 16 / elem);
-        if (K / whole_width(K, width) > kWholeThreads || K / aligned > kWholeThreads) {
-            longest = 0;  // groups wider than a workgroup
-        } else if (s.N * row <= kSmallBytes) {
-            longest = s.N;
+        const std::uint32_t K = s.C / s.G;
+        const bool known = s.offsets == nullptr || s.maxRows > 0;
+        const std::uint64_t each = s.B > 0 ? s.N / s.B : 0;
+        const std::uint64_t most = s.offsets == nullptr ? each : known ? s.maxRows : s.N;
+        const WholeArgs k = whole_args(s, WholeWidth(K, full_width(s.C, dtype_bytes(s.dtype))));
+        if (k.groups == 0 || whole_args(s, WholeWidth(K, width)).groups == 0) {
+            longest = 0;
         } else {
-            const WholeArgs k = whole_args(s, aligned);
-            longest = kWholeSteps * (k.threads >> k.laneBits);
+            const std::uint64_t rowLanes = k.threads >> k.laneBits;
+            longest = (k.threads == kWave ? kWaveSteps : s.B >= 1024 ? kManySteps : kWholeSteps) * rowLanes;
+            if (!known && s.N <= kSmallSteps * rowLanes && kSkew * each <= 2 * longest) longest = s.N;
+            else if (!known && kUneven * each > longest) longest = 0;
         }
         tiles = s.N > 0 && (most > longest || s.N > s.B * most);
         if (!tiles) longest = s.N;  // whatever maxRows says
@@ -997,20 +1254,21 @@ struct Split {
 // elements have twice the weights to load before they begin: bf16 rows took
 // 458 us with 16 steps and 570 with 4, their gradient 632 with 4 and 946 with 2
 // (fp32 rows 940 and 835, 1,283 and 1,260).
-template <int N>
-constexpr std::uint32_t kOutSteps = N == 8 ? 16 : 4;
-template <int N>
-constexpr std::uint32_t kGradSteps = N == 8 ? 4 : 2;
+// Narrower lanes take as many more steps.
+template <typename T, int N>
+constexpr std::uint32_t kOutSteps = (N == 8 ? 16 : 4) * (16 / (N * sizeof(T)));
+template <typename T, int N>
+constexpr std::uint32_t kGradSteps = (N == 8 ? 4 : 2) * (16 / (N * sizeof(T)));
 
 struct Layout {
     std::uint64_t tileRows, tiles, wholeRows;
     std::size_t part, sums, channel, seen, bytes;
     Layout(const tcc_group_norm_shape& s, bool backward) {
-        const Split split(s, 16 / dtype_bytes(s.dtype));
+        const Split split(s, full_width(s.C, dtype_bytes(s.dtype)));
         const bool unaligned = s.C / s.G > kWholeThreads;  // room for rows that cannot go whole
-        // at least 32 rows of a tile, however narrow the rows: a tile's own
-        // reductions cost about as much
-        tileRows = std::max<std::uint64_t>((s.N + kTiles - 1) / kTiles, 32);
+        // 16 rows of a tile at least and 64 where there are plenty, however narrow
+        // the rows: a tile's own reductions cost about as much
+        tileRows = std::max<std::uint64_t>((s.N + kTiles - 1) / kTiles, std::clamp<std::uint64_t>(s.N / 512, 16, 64));
         tiles = split.tiles || unaligned ? (s.N + tileRows - 1) / tileRows : 0;
         wholeRows = split.whole && backward ? std::min(s.B, kWholeBlocks) : 0;
         part = 0;
@@ -1059,7 +1317,14 @@ int check_shape(const tcc_group_norm_shape* s) {
 dim3 whole_grid(const WholeArgs& k) { return dim3((k.blocks + 7) / 8 * 8 * k.slices); }
 
 template <typename T, int N>
-int whole_launch(const NormArgs& a, WholeArgs k, hipStream_t st) {
+int whole_launch(const NormArgs& a, WholeArgs k, bool spread, hipStream_t st) {
+    if constexpr (N <= 4) {
+        if (spread) {
+            TCC_BY_ACT(spread_kernel, T, N, whole_grid(k), k.threads, spread_lds<N>(k), st, a, k);
+            TCC_LAUNCH_CHECK();
+            return TCC_OK;
+        }
+    }
     TCC_BY_ACT(whole_kernel, T, N, whole_grid(k), k.threads, 2 * k.threads * sizeof(float2), st, a, k);
     TCC_LAUNCH_CHECK();
     return TCC_OK;
@@ -1073,7 +1338,15 @@ std::uint32_t grad_lds(std::uint32_t act, std::uint32_t threads) {
 }
 
 template <typename T, int N>
-int whole_grad_launch(const NormArgs& a, WholeArgs k, bool params, hipStream_t st) {
+int whole_grad_launch(const NormArgs& a, WholeArgs k, bool spread, bool params, hipStream_t st) {
+    if constexpr (N <= 4) {
+        if (spread) {
+            TCC_BY_ACT(spread_grad_kernel, T, N, whole_grid(k), k.threads, spread_lds<N>(k), st, a, k,
+                       params ? a.channel : nullptr);
+            TCC_LAUNCH_CHECK();
+            return TCC_OK;
+        }
+    }
     TCC_BY_ACT(whole_grad_kernel, T, N, whole_grid(k), k.threads, grad_lds<N>(a.act, k.threads), st, a, k,
                params ? a.channel : nullptr);
     TCC_LAUNCH_CHECK();
@@ -1082,10 +1355,10 @@ int whole_grad_launch(const NormArgs& a, WholeArgs k, bool params, hipStream_t s
 
 int stats_join_launch(const NormArgs& a, const Layout& lay, std::uint64_t B, hipStream_t st) {
     if (lay.tiles > 64 * B)
-        hipLaunchKernelGGL(stats_join_kernel<4>, dim3(static_cast<unsigned>(B), JoinGroup<4>::grid(a.G)),
+        hipLaunchKernelGGL(stats_join_kernel<4>, JoinGroup<4>::grid(B, a.G),
                            dim3(JoinGroup<4>::threads), 0, st, a);
     else
-        hipLaunchKernelGGL(stats_join_kernel<1>, dim3(static_cast<unsigned>(B), JoinGroup<1>::grid(a.G)),
+        hipLaunchKernelGGL(stats_join_kernel<1>, JoinGroup<1>::grid(B, a.G),
                            dim3(JoinGroup<1>::threads), 0, st, a);
     TCC_LAUNCH_CHECK();
     return TCC_OK;
@@ -1099,8 +1372,8 @@ int tiles_launch(NormArgs a, const Layout& lay, std::uint64_t B, hipStream_t st)
     hipLaunchKernelGGL((stats_kernel<T, N>), dim3(tiles), dim3(kThreads), 2 * a.rowLanes * a.C * sizeof(float), st, a);
     TCC_LAUNCH_CHECK();
     if (const int rc = stats_join_launch(a, lay, B, st)) return rc;
-    a.outRows = kOutSteps<N> * a.rowLanes;
-    TCC_BY_ACT(apply_kernel, T, N, dim3(grid_for(a.seg.N, kOutSteps<N> * a.rowLanes)), kThreads, 0, st, a);
+    a.outRows = kOutSteps<T, N> * a.rowLanes;
+    TCC_BY_ACT(apply_kernel, T, N, dim3(grid_for(a.seg.N, kOutSteps<T, N> * a.rowLanes)), kThreads, 0, st, a);
     TCC_LAUNCH_CHECK();
     return TCC_OK;
 }
@@ -1113,14 +1386,14 @@ int tiles_grad_launch(NormArgs a, const Layout& lay, std::uint64_t B, hipStream_
     TCC_BY_ACT(grad_sums_kernel, T, N, dim3(tiles), kThreads, 4 * a.rowLanes * a.C * sizeof(float), st, a);
     TCC_LAUNCH_CHECK();
     if (lay.tiles > 64 * B)
-        hipLaunchKernelGGL(grad_join_kernel<4>, dim3(static_cast<unsigned>(B), JoinGroup<4>::grid(a.G)),
+        hipLaunchKernelGGL(grad_join_kernel<4>, JoinGroup<4>::grid(B, a.G),
                            dim3(JoinGroup<4>::threads), 0, st, a);
     else
-        hipLaunchKernelGGL(grad_join_kernel<1>, dim3(static_cast<unsigned>(B), JoinGroup<1>::grid(a.G)),
+        hipLaunchKernelGGL(grad_join_kernel<1>, JoinGroup<1>::grid(B, a.G),
                            dim3(JoinGroup<1>::threads), 0, st, a);
     TCC_LAUNCH_CHECK();
-    a.outRows = kGradSteps<N> * a.rowLanes;
-    TCC_BY_ACT(grad_apply_kernel, T, N, dim3(grid_for(a.seg.N, kGradSteps<N> * a.rowLanes)), kThreads, 0, st, a);
+    a.outRows = kGradSteps<T, N> * a.rowLanes;
+    TCC_BY_ACT(grad_apply_kernel, T, N, dim3(grid_for(a.seg.N, kGradSteps<T, N> * a.rowLanes)), kThreads, 0, st, a);
     TCC_LAUNCH_CHECK();
     return TCC_OK;
 }
@@ -1192,12 +1465,12 @@ int tcc_group_norm(const tcc_group_norm_shape* s, const void* x, uint64_t ldx, c
     a.rstd = rstd;
     const hipStream_t st = as_stream(stream);
     if (split.whole) {
-        const std::uint32_t n = whole_width(a.K, w);
-        WholeArgs k = whole_args(*s, n);
+        const WholeWidth width(a.K, w);
+        WholeArgs k = whole_args(*s, width);
         k.blocks = static_cast<std::uint32_t>(std::min(s->B, kWholeBlocks));
         if (split.tiles) a.seenCount = k.blocks;
-#define CALL(T, N) (whole_launch<T, N>(a, k, st))
-        if (const int rc = TCC_BY_TYPE(s->dtype, n, CALL)) return rc;
+#define CALL(T, N) (whole_launch<T, N>(a, k, width.spread, st))
+        if (const int rc = TCC_BY_TYPE(s->dtype, width.n, CALL)) return rc;
 #undef CALL
     }
     if (s->N == 0) return stats_join_launch(a, lay, s->B, st);  // segments without rows
@@ -1237,12 +1510,12 @@ int tcc_group_norm_grad(const tcc_group_norm_shape* s, const void* dY, uint64_t 
     const bool params = dWeight != nullptr || dBias != nullptr;
     const std::uint64_t wholeRows = split.whole ? lay.wholeRows : 0, tileRows = split.tiles ? lay.tiles : 0;
     if (wholeRows > 0) {
-        const std::uint32_t n = whole_width(a.K, w);
-        WholeArgs k = whole_args(*s, n);
+        const WholeWidth width(a.K, w);
+        WholeArgs k = whole_args(*s, width);
         k.blocks = static_cast<std::uint32_t>(wholeRows);
         if (split.tiles) a.seenCount = k.blocks;
-#define CALL(T, N) (whole_grad_launch<T, N>(a, k, params, st))
-        if (const int rc = TCC_BY_TYPE(s->dtype, n, CALL)) return rc;
+#define CALL(T, N) (whole_grad_launch<T, N>(a, k, width.spread, params, st))
+        if (const int rc = TCC_BY_TYPE(s->dtype, width.n, CALL)) return rc;
 #undef CALL
     }
     if (tileRows > 0) {

@@ -154,7 +154,8 @@ def test_both_passes(gpu, dtype, kind, N, C, G):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("long", [0, 9000])
 @pytest.mark.parametrize("N,C,G,mean_rows", [(30_000, 64, 8, 15), (30_000, 24, 2, 20), (40_000, 33, 11, 150),
-                                             (12_000, 520, 1, 7), (12_000, 606, 2, 100)])
+                                             (12_000, 520, 1, 7), (12_000, 606, 2, 100),
+                                             (30_000, 48, 16, 15), (25_000, 308, 4, 120), (31_000, 36, 4, 9)])
 def test_many_short_segments_with_a_long_one(gpu, dtype, long, N, C, G, mean_rows):
     """Over a thousand segments (a wave each) or hundreds (a workgroup each),
     with empty ones, and one that is too long for either, whether the
