@@ -96,7 +96,8 @@ int tcc_group_norm(const tcc_group_norm_shape* s, const void* x, uint64_t ldx, c
 /* dX [N x C] (lddx) of x's type, and dWeight and dBias [C] fp32 (either may
  * be NULL), from dY [N x C] (lddy) of x's type, x and the forward's mean and
  * rstd.  z is formed with the forward's roundings, so that relu's mask is
- * that of the forward's output. */
+ * that of the forward's output; what it masks counts as 0, infinities and
+ * NaN too. */
 int tcc_group_norm_grad(const tcc_group_norm_shape* s, const void* dY, uint64_t lddy, const void* x, uint64_t ldx,
                         const float* mean, const float* rstd, const void* weight, const void* bias, void* dX,
                         uint64_t lddx, float* dWeight, float* dBias, void* workspace, size_t workspaceBytes,

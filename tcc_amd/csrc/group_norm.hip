@@ -132,23 +132,24 @@ __device__ __forceinline__ float normal_cdf(float z, float& e) {
 template <std::uint32_t ACT>
 __device__ __forceinline__ float activate(float z) {
     if (ACT == TCC_ACT_NONE) return z;
-    if (ACT == TCC_ACT_RELU) return z > 0.0f ? z : z * 0.0f;  // keeps NaN
+    if (ACT == TCC_ACT_RELU) return z <= 0.0f ? 0.0f : z;  // keeps NaN
     if (ACT == TCC_ACT_SILU) return z * fast_rcp(1.0f + fast_exp(-z));
     float e;
     return z * normal_cdf(z, e);
 }
 
+// d act'(z).  What relu masks is 0 whatever it is, an infinity too.
 template <std::uint32_t ACT>
-__device__ __forceinline__ float slope(float z) {
-    if (ACT == TCC_ACT_NONE) return 1.0f;
-    if (ACT == TCC_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+__device__ __forceinline__ float through(float d, float z) {
+    if (ACT == TCC_ACT_NONE) return d;
+    if (ACT == TCC_ACT_RELU) return z <= 0.0f ? 0.0f : d;
     if (ACT == TCC_ACT_SILU) {
         const float p = fast_rcp(1.0f + fast_exp(-z));
-        return p * fmaf(z, 1.0f - p, 1.0f);
+        return d * (p * fmaf(z, 1.0f - p, 1.0f));
     }
     float e;
     const float p = normal_cdf(z, e);
-    return fmaf(z * 0.39894228f, e, p);
+    return d * fmaf(z * 0.39894228f, e, p);
 }
 
 // Rows a, a + rowLanes, ... below b that a row lane takes.
@@ -450,7 +451,7 @@ __global__ void __launch_bounds__(kThreads) grad_sums_kernel(NormArgs a) {
 #pragma unroll
                     for (int q = 0; q < N; ++q) {
                         const float xh = normalise(v[q], of.mean[q], of.rstd[q]);
-                        const float dz = d[q] * slope<ACT>(affine(xh, w[q], b[q]));
+                        const float dz = through<ACT>(d[q], affine(xh, w[q], b[q]));
                         s1[q] += dz;
                         s2[q] += dz * xh;
                     }
@@ -576,7 +577,7 @@ __global__ void __launch_bounds__(kThreads) grad_apply_kernel(NormArgs a) {
 #pragma unroll
                 for (int q = 0; q < N; ++q) {
                     const float xh = normalise(v[q], of.mean[q], of.rstd[q]);
-                    const float dz = d[q] * slope<ACT>(affine(xh, w[q], b[q]));
+                    const float dz = through<ACT>(d[q], affine(xh, w[q], b[q]));
                     o[q] = (dz * w[q] - of.sums[q].x - xh * of.sums[q].y) * of.rstd[q];
                 }
                 store_row<T, N>(dx + r * a.ldo + cv * N, o);
@@ -856,7 +857,7 @@ __global__ void __launch_bounds__(kWholeThreads, 4) whole_grad_kernel(NormArgs a
 #pragma unroll
             for (int q = 0; q < N; ++q) {
                 const float xh = normalise(v[q], mean, rstd);
-                d[q] *= slope<ACT>(affine(xh, w[q], b[q]));
+                d[q] = through<ACT>(d[q], affine(xh, w[q], b[q]));
                 db[q] += d[q];
                 dw[q] = fmaf(d[q], xh, dw[q]);
                 d[q] *= w[q];
@@ -905,7 +906,7 @@ __global__ void __launch_bounds__(kWholeThreads, 4) whole_grad_kernel(NormArgs a
                            [&](vec_t<float, N> v, vec_t<float, N> d, int) {
 #pragma unroll
                                for (int q = 0; q < N; ++q)
-                                   d[q] *= slope<ACT>(affine(normalise(v[q], mean, rstd), w[q], b[q])) * w[q];
+                                   d[q] = through<ACT>(d[q], affine(normalise(v[q], mean, rstd), w[q], b[q])) * w[q];
                                apply(v, d, dx);
                                dx += stepO;
                            });
@@ -1115,7 +1116,7 @@ __global__ void __launch_bounds__(kWholeThreads, 4) spread_grad_kernel(NormArgs 
 #pragma unroll
                 for (int q = 0; q < N; ++q) {
                     const float xh = normalise(v[q], mean[q], rstd[q]);
-                    const float z = d[q] * slope<ACT>(affine(xh, w[q], b[q]));
+                    const float z = through<ACT>(d[q], affine(xh, w[q], b[q]));
                     s1[q] += z;
                     s2[q] = fmaf(z, xh, s2[q]);
                 }
@@ -1146,7 +1147,7 @@ __global__ void __launch_bounds__(kWholeThreads, 4) spread_grad_kernel(NormArgs 
 #pragma unroll
             for (int q = 0; q < N; ++q) {
                 const float xh = normalise(v[q], mean[q], rstd[q]);
-                o[q] = (d[q] * slope<ACT>(affine(xh, w[q], b[q])) * w[q] - of[q].x - xh * of[q].y) * rstd[q];
+                o[q] = (through<ACT>(d[q], affine(xh, w[q], b[q])) * w[q] - of[q].x - xh * of[q].y) * rstd[q];
             }
             store_row<T, N>(dx, o);
             dx += me.rowLanes * a.ldo;

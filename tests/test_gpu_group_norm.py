@@ -314,6 +314,31 @@ def test_relu_mask_is_the_forward_s(gpu):
     assert bool((db == 0).all()) and bool((dx == 0).all())
 
 
+@pytest.mark.parametrize("maxRows, C, G", [(40, 32, 4), (None, 32, 4), (40, 30, 10), (5000, 32, 4)])
+def test_relu_masks_infinities(gpu, maxRows, C, G):
+    """An infinite dy where relu masks is as good as none, and a bias of -inf
+    leaves zeros: in whole segments, in groups that vectors straddle, in tiles."""
+    from tcc_amd import training
+
+    each = maxRows or 40
+    gen, x, w, b, d = inputs(5 * each, C, torch.float32, 12)
+    off = None if maxRows else torch.arange(0, 5 * each + 1, each, device="cuda")
+    if off is None:
+        x, d = x.view(5, each, C), d.view(5, each, C)
+    y, mean, rstd = training.group_norm(x, G, w, b, offsets=off, activation="relu")
+    at = [each * i for i in range(6)]
+    none = torch.where(y > 0, d, 0.0)
+    flat = lambda t: t.reshape(5 * each, C)  # noqa: E731
+    for masked in (float("inf"), -float("inf"), float("nan")):
+        got = training.group_norm_grad(torch.where(y > 0, d, masked), x, mean, rstd, G, w, b, offsets=off,
+                                       activation="relu")
+        check_grad((flat(got[0]), *got[1:]), flat(none), flat(x), mean, rstd, G, w, b, at, "relu")
+    b[3] = -float("inf")
+    y2 = training.group_norm(x, G, w, b, offsets=off, activation="relu")[0]
+    y[..., 3] = 0.0
+    assert torch.equal(y2, y)
+
+
 def test_replayed_graph_and_other_stream(gpu):
     from tcc_amd import training
 
