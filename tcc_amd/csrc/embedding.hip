@@ -3,12 +3,22 @@
 //   lookup:   out[i]  = scale * table[ids[i]]
 //   gradient: grad[v] = scale * sum over {i : ids[i] = v} of dOut[i]
 //
-// Both move bytes and compute next to nothing.  The gradient sorts the ids
-// with their positions (stable, so that a row's terms have one order and the
-// sums the same bits every time), then walks the sorted positions in chunks
-// of equal length, whatever the ids' frequencies: a hub node with thousands
-// of rows is spread over as many chunks as it needs, and its parts are joined
-// afterwards in chunk order.
+// Both move bytes and compute next to nothing.  The lookup is bound by the
+// lines of 128 bytes that its rows lie in: 2.45M rows of 100 bf16 from a table
+// of as many take 243 us, 735 MB of ids, rows and output (3.0 TB/s) or 1.09 GB
+// with the lines that two rows share (4.5).
+//
+// The gradient sorts the ids with their positions (stable, so that a row's
+// terms have one order and the sums the same bits every time), then walks the
+// sorted positions in chunks of equal length, whatever the ids' frequencies:
+// a hub node with thousands of rows is spread over as many chunks as it needs,
+// and its parts are joined afterwards in chunk order.  Atomics on the rows
+// would spare the sort, but add in no fixed order and round every partial sum
+// of a bf16 row.  A few rows need no sort (few_grad_kernel), some more one of
+// a single launch (rank_kernel), the others passes by digits of the rows:
+// 2.45M rows of 100 fp32 into as many take 608 us, of which the sums are 488
+// (1.96 GB, 4.0 TB/s: rows of 400 bytes in the sorted order are read at random
+// and share lines), the sort 95 and the parts 25.
 #include <algorithm>
 
 #include "../../include/tcc_spmm_cnic.h"
