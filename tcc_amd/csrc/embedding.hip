@@ -14,11 +14,11 @@
 // a hub node with thousands of rows is spread over as many chunks as it needs,
 // and its parts are joined afterwards in chunk order.  Atomics on the rows
 // would spare the sort, but add in no fixed order and round every partial sum
-// of a bf16 row.  A few rows need no sort (few_grad_kernel), some more one of
-// a single launch (rank_kernel), the others passes by digits of the rows:
-// 2.45M rows of 100 fp32 into as many take 608 us, of which the sums are 488
-// (1.96 GB, 4.0 TB/s: rows of 400 bytes in the sorted order are read at random
-// and share lines), the sort 95 and the parts 25.
+// of a bf16 row.  A few rows need no sort (few_grad_kernel), up to 65,536 one
+// of a launch for each 11 bits of the rows (pass_kernel), the others passes of
+// 8 bits and three launches: 2.45M rows of 100 fp32 into as many take 595 us,
+// of which the sums are 488 (1.96 GB, 4.0 TB/s: rows of 400 bytes in the sorted
+// order are read at random and share lines), the sort 90 and the parts 20.
 #include <algorithm>
 
 #include "../../include/tcc_spmm_cnic.h"
@@ -133,70 +133,123 @@ struct IdKeys {
     __device__ __forceinline__ void report(bool bad) const { tcc::report(err, bad); }
 };
 
-// The sort of up to kRankRows keys in one launch: a key's place is the number of
-// keys before it, counted against all of them, which every workgroup holds.
-// n^2 / 64 comparisons of two instructions each, over a wave for every 64 keys
-// and 16th of the keys they are compared with; it also clears the windows'
-// marks.  With the passes by digits, five launches more, a gradient of 8,000
-// rows of 32 takes 45 us instead of 34, of 16,384 the same 44.
-constexpr std::uint64_t kRankRows = 12288;
-constexpr int kRankThreads = 1024, kRankWaves = kRankThreads / kWave;
-__global__ void __launch_bounds__(kRankThreads) rank_kernel(IdKeys src, std::uint64_t* __restrict__ out,
-                                                           std::uint64_t* __restrict__ marks, std::uint64_t markWords) {
-    extern __shared__ __attribute__((aligned(16))) std::uint32_t rowOf[];  // padded to whole 64s
-    __shared__ std::uint32_t counts[kRankWaves][kWave];
-    const std::uint32_t n = static_cast<std::uint32_t>(src.n), padded = (n + kWave - 1) / kWave * kWave;
-    const std::uint32_t none = static_cast<std::uint32_t>(src.ids.V);
-    for (std::uint64_t i = static_cast<std::uint64_t>(blockIdx.x) * kRankThreads + threadIdx.x; i < markWords;
-         i += static_cast<std::uint64_t>(gridDim.x) * kRankThreads)
-        marks[i] = 0;
+// A pass of the sort of up to kPassRows rows by a digit of up to kDigitBits
+// bits, in one launch: every workgroup counts the digits of all keys, apart for
+// those before its own, and so knows where each digit's run begins and its own
+// keys' places in it.  The first pass also clears the windows' marks.  Counting
+// costs a workgroup what its CU can read, so that it grows with n, while passes
+// of three launches cost what these follow each other in: a gradient of rows of
+// 32 fp32 into 1,500 takes (one pass) 18 us for 12,000 rows, 32 for 65,000 and
+// 46 for 100,000, with passes of three launches 31, 41 and 45; into 70,000
+// (two passes) 31, 50 and 75, with three launches 54, 59 and 67.
+constexpr int kDigitBits = 11;
+constexpr std::uint32_t kDigits = 1u << kDigitBits;
+constexpr int kPassThreads = 1024, kPassWaves = kPassThreads / kWave, kPassUnroll = 8;
+constexpr std::uint64_t kPassRows = 65536;
+
+// The lanes of `mask` below this one.
+__device__ __forceinline__ std::uint32_t rank_in(std::uint64_t mask) {
+    return __builtin_popcountll(mask & ((1ull << __lane_id()) - 1ull));
+}
+
+struct SortedKeys {
+    const std::uint64_t* keys;
+    __device__ __forceinline__ std::uint64_t key(std::uint64_t i, bool&) const { return load_global<std::uint64_t>(keys + i); }
+    template <int R>
+    __device__ __forceinline__ void rows(std::uint64_t i, std::uint64_t step, std::uint64_t n, std::uint32_t (&v)[R],
+                                         bool&) const {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            v[r] = static_cast<std::uint32_t>(load_global<std::uint64_t>(keys + min(i + r * step, n - 1)) >> 32);
+    }
+};
+
+struct FirstKeys {
+    Ids ids;
+    __device__ __forceinline__ std::uint64_t key(std::uint64_t i, bool& bad) const {
+        const std::uint32_t v = ids.row(i, bad);
+        return (v == kNoRow ? ids.V : static_cast<std::uint64_t>(v)) << 32 | i;
+    }
+    template <int R>
+    __device__ __forceinline__ void rows(std::uint64_t i, std::uint64_t step, std::uint64_t n, std::uint32_t (&v)[R],
+                                         bool& bad) const {
+        ids.rows<R>(i, step, n, v, bad);
+#pragma unroll
+        for (int r = 0; r < R; ++r) v[r] = v[r] == kNoRow ? static_cast<std::uint32_t>(ids.V) : v[r];
+    }
+};
+
+template <typename Src>
+__global__ void __launch_bounds__(kPassThreads) pass_kernel(Src src, std::uint32_t n, std::uint32_t shift,
+                                                           std::uint32_t bits, std::uint64_t* __restrict__ out,
+                                                           std::uint64_t* __restrict__ marks, std::uint64_t markWords,
+                                                           std::uint32_t* err) {
+    __shared__ std::uint32_t before[kDigits], rest[kDigits], waveSums[kPassWaves];
+    const std::uint32_t t = threadIdx.x, first = blockIdx.x * kPassThreads, mask = (1u << bits) - 1u;
+    for (std::uint64_t i = first + t; i < markWords; i += static_cast<std::uint64_t>(gridDim.x) * kPassThreads) marks[i] = 0;
     bool bad = false;
-    for (std::uint32_t i = threadIdx.x; i < padded; i += 8 * kRankThreads) {
-        std::uint32_t v[8];
-        src.ids.rows<8>(i, kRankThreads, n, v, bad);
+    const bool have = first + t < n;
+    std::uint64_t key = 0;
+    if (have) key = src.key(first + t, bad);
 #pragma unroll
-        for (std::uint32_t r = 0; r < 8; ++r) {
-            const std::uint32_t at = i + r * kRankThreads;
-            // past the end: after every key
-            if (at < padded) rowOf[at] = at >= n ? kNoRow : v[r] == kNoRow ? none : v[r];
-        }
-    }
-    if (blockIdx.x == 0) src.report(bad);
+    for (std::uint32_t d = 0; d < kDigits; d += kPassThreads) before[d + t] = rest[d + t] = 0;
     __syncthreads();
-    const std::uint32_t wave = uniform(threadIdx.x / kWave), lane = __lane_id();
-    const std::uint32_t i0 = blockIdx.x * kWave, i = i0 + lane, mine = rowOf[i];
-    // this wave's share of the 64s, a lane's key against each of their keys
-    const std::uint32_t tiles = padded / kWave;
-    std::uint32_t before = 0;
-    for (std::uint32_t t = wave; t < tiles; t += kRankWaves) {
-        const vu4* keys = reinterpret_cast<const vu4*>(rowOf + t * kWave);
-        if (t * kWave < i0) {  // equal rows come before
-#pragma unroll 4
-            for (std::uint32_t j = 0; j < kWave / 4; ++j) {
-                const vu4 k = keys[j];
-                before += (k[0] <= mine) + (k[1] <= mine) + (k[2] <= mine) + (k[3] <= mine);
-            }
-        } else if (t * kWave > i0) {  // and after
-#pragma unroll 4
-            for (std::uint32_t j = 0; j < kWave / 4; ++j) {
-                const vu4 k = keys[j];
-                before += (k[0] < mine) + (k[1] < mine) + (k[2] < mine) + (k[3] < mine);
-            }
-        } else {
-            for (std::uint32_t j = 0; j < kWave; ++j) {
-                const std::uint32_t k = rowOf[i0 + j];
-                before += k < mine || (k == mine && j < lane) ? 1u : 0u;
+    for (std::uint32_t i = t; i < n; i += kPassUnroll * kPassThreads) {
+        std::uint32_t v[kPassUnroll];
+        src.template rows<kPassUnroll>(i, kPassThreads, n, v, bad);
+#pragma unroll
+        for (int r = 0; r < kPassUnroll; ++r) {
+            const std::uint32_t at = i + r * kPassThreads;  // a wave's are all before the workgroup's or none
+            if (at >= n) continue;
+            const std::uint32_t d = v[r] >> shift & mask;
+            std::uint32_t* const c = at < first ? before : rest;
+            const std::uint64_t active = __ballot(1);
+            if (__ballot(d == uniform(d)) == active) {  // one digit for all, as a hub's are: not one after the other
+                if (rank_in(active) == 0) atomicAdd(c + d, static_cast<std::uint32_t>(__builtin_popcountll(active)));
+            } else {
+                atomicAdd(c + d, 1u);
             }
         }
     }
-    counts[wave][lane] = before;
+    if (blockIdx.x == 0) report(err, bad);
     __syncthreads();
-    if (wave == 0 && i < n) {
-        std::uint32_t place = 0;
+    // where each digit's run begins for this workgroup: the digits below, and its own before
+    constexpr int E = kDigits / kPassThreads;
+    std::uint32_t c[E], b[E], sum = 0;
 #pragma unroll
-        for (int w = 0; w < kRankWaves; ++w) place += counts[w][lane];
-        out[place] = static_cast<std::uint64_t>(mine) << 32 | i;
+    for (int e = 0; e < E; ++e) {
+        b[e] = before[t * E + e];
+        c[e] = b[e] + rest[t * E + e];
+        sum += c[e];
     }
+    const std::uint32_t inc = wave_inclusive_scan(sum);
+    const std::uint32_t wave = uniform(t / kWave), lane = __lane_id();
+    if (lane == kWave - 1) waveSums[wave] = inc;
+    __syncthreads();
+    std::uint32_t at = inc - sum;
+    for (std::uint32_t w = 0; w < wave; ++w) at += waveSums[w];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        before[t * E + e] = at + b[e];
+        at += c[e];
+    }
+    // keys of the same digit in a wave by lanes, the waves in turn
+    const std::uint32_t digit = static_cast<std::uint32_t>(key >> 32) >> shift & mask;
+    std::uint64_t same = __ballot(have);
+    for (std::uint32_t k = 0; k < bits; ++k) {
+        const bool one = digit >> k & 1u;
+        const std::uint64_t ones = __ballot(one);
+        same &= one ? ones : ~ones;
+    }
+    const std::uint32_t rank = rank_in(same);
+    std::uint32_t place = 0;
+    for (std::uint32_t w = 0; w < kPassWaves; ++w) {
+        __syncthreads();
+        if (w != wave || !have) continue;
+        place = before[digit] + rank;
+        if (rank == 0) before[digit] = place + __builtin_popcountll(same);
+    }
+    if (have) out[place] = key;
 }
 
 struct GradArgs {
@@ -206,7 +259,7 @@ struct GradArgs {
     float* parts;  // [2 * chunks][D]: sums of a chunk's first row (begun before it) and last row (going on after it)
     std::uint8_t* mark;  // [windows]: 1 where a row occurs
     std::uint64_t n, V, ldd, ldg;
-    std::uint32_t D, chunk, chunks, laneBits, joinBlocks, zeroRows;
+    std::uint32_t D, chunk, chunks, laneBits, joinBlocks, zeroRows, waveWindows;
     float scale;
     int accumulate;
 };
@@ -312,13 +365,14 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(GradArgs a) {
     }
 }
 
-// A workgroup's share of the empty windows: as many windows as its threads, a
-// wave for one at a time.
+// A workgroup's share of the empty windows: a wave zeroes one of its own after
+// the other.
 template <typename T, int N>
 __device__ __forceinline__ void zero_windows(const GradArgs& a, std::uint32_t block) {
-    const std::uint64_t first = (static_cast<std::uint64_t>(block) * (kThreads / kWave) + threadIdx.x / kWave) * kWave;
-    const std::uint64_t w = first + __lane_id(), windows = (a.V + kWindow - 1) / kWindow;
-    std::uint64_t empty = __ballot(w < windows && a.mark[min(w, windows - 1)] == 0);
+    const std::uint64_t wave = static_cast<std::uint64_t>(block) * (kThreads / kWave) + threadIdx.x / kWave;
+    const std::uint64_t first = wave * a.waveWindows, windows = (a.V + kWindow - 1) / kWindow, w = first + __lane_id();
+    const bool mine = __lane_id() < a.waveWindows && w < windows;
+    std::uint64_t empty = __ballot(mine && a.mark[min(w, windows - 1)] == 0);
     while (empty != 0) {
         const std::uint64_t v0 = (first + __builtin_ctzll(empty)) * kWindow;
         empty &= empty - 1;
@@ -340,7 +394,7 @@ __device__ __forceinline__ void zero_windows(const GradArgs& a, std::uint32_t bl
 // for each such chunk, and zeroes the empty windows (blocks from joinBlocks
 // on); a row of many parts (a hub's) is added by the whole
 // workgroup, each of its teams taking every so many-th part.
-constexpr std::uint32_t kLongRow = 16;
+constexpr std::uint32_t kLongRow = 16, kJoinUnroll = 8;
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads) join_kernel(GradArgs a) {
     __shared__ std::uint32_t rowOf[kThreads], partsOf[kThreads];
@@ -381,10 +435,23 @@ __global__ void __launch_bounds__(kThreads) join_kernel(GradArgs a) {
     const auto part = [&](std::uint64_t k, std::uint32_t c) {
         return load_global<vec_t<float, N>>(a.parts + k * a.D + c);
     };
+    // the first parts of the chunks t + k, t + k + step, ... up to t + last, kJoinUnroll
+    // of them loaded before the first is added
+    const auto add_parts = [&](vec_t<float, N>& s, std::uint32_t t, std::uint32_t k, std::uint32_t step, std::uint32_t last,
+                               std::uint32_t c) {
+        for (; k <= last; k += kJoinUnroll * step) {
+            vec_t<float, N> x[kJoinUnroll];
+#pragma unroll
+            for (std::uint32_t u = 0; u < kJoinUnroll; ++u) x[u] = part(2ull * (t + min(k + u * step, last)), c);
+#pragma unroll
+            for (std::uint32_t u = 0; u < kJoinUnroll; ++u)
+                if (k + u * step <= last) s += x[u];
+        }
+    };
     if (v != none && count <= kLongRow) {
         for (std::uint32_t c = lane * N; c < a.D; c += N << a.laneBits) {
             vec_t<float, N> s = part(2ull * team + 1, c);
-            for (std::uint32_t k = 1; k <= count; ++k) s += part(2ull * (team + k), c);
+            add_parts(s, team, 1, 1, count, c);
             write_sum<T, N>(a, v, c, s);
         }
     }
@@ -397,8 +464,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(GradArgs a) {
             vec_t<float, N> s(0.0f);
             if (c < a.D) {
                 if (mine == 0) s = part(2ull * (first + t) + 1, c);
-#pragma unroll 4
-                for (std::uint32_t k = 1 + mine; k <= many; k += teams) s += part(2ull * (first + t + k), c);
+                add_parts(s, first + t, 1 + mine, teams, many, c);
             }
             *reinterpret_cast<vec_t<float, N>*>(sums + threadIdx.x * N) = s;
             __syncthreads();
@@ -417,10 +483,10 @@ __global__ void __launch_bounds__(kThreads) join_kernel(GradArgs a) {
 // Without a sort, in one launch: every workgroup holds the ids, and the wave of
 // the first position of each row looks for the others.  That is n^2 / 64
 // comparisons, which a few thousand rows spread over the GPU need less time for
-// than a sort's launches follow each other in: rows of 32 fp32 into a table of
-// 4,096, 8 us and sorted 38 for 1,000 of them, 12 and 32 for 2,000, 28 and 32
-// for 4,096.
-constexpr std::uint64_t kFewRows = 4096;
+// than a sort's launches follow each other in: rows of 32 fp32 into 1,500 (and
+// 70,000) take 6 us (7) for 1,000 of them, 14 (16) for 3,000 and 26 (27) for
+// 4,000, sorted 15 (29) for any of these.
+constexpr std::uint64_t kFewRows = 3000;
 constexpr std::uint32_t kFewZeroRows = 256;  // rows of a workgroup that zeroes, at most
 
 template <typename T, int N>
@@ -508,8 +574,10 @@ unsigned team_bits(std::uint32_t D, std::uint32_t width) {
 }
 
 // Rows a chunk: short ones give few rows enough teams, long ones keep the
-// parts few.
-std::uint32_t grad_chunk(std::uint64_t n) { return n < (1u << 16) ? 16u : n < (1u << 19) ? 32u : 64u; }
+// parts few.  12,000 rows of 32 into 70,000: the sums 12 us with chunks of 4, 19
+// with 8, 32 with 16; 250,000 rows of 32 into 400,000 together 68 us with 8, 70
+// with 16, 80 with 32, and 520,000 rows of 100 150, 143, 140.
+std::uint32_t grad_chunk(std::uint64_t n) { return n < (1u << 15) ? 4u : n < (1u << 17) ? 8u : n < (1u << 19) ? 16u : 64u; }
 
 unsigned id_bits(std::uint64_t V) {  // of the values 0 .. V
     unsigned b = 1;
@@ -565,6 +633,10 @@ int few_grad_launch(GradArgs a, const Ids& ids, std::uint32_t* err, hipStream_t 
     return TCC_OK;
 }
 
+// Waves that the windows are spread over where there are as many (with 4,096 of
+// them 2M rows of 100 take 176 us instead of 169 where nearly all are zero).
+constexpr std::uint64_t kZeroWaves = 16384;
+
 template <typename T, int N>
 int grad_launch(GradArgs a, hipStream_t st) {
     a.laneBits = team_bits(a.D, N);
@@ -575,7 +647,9 @@ int grad_launch(GradArgs a, hipStream_t st) {
         TCC_LAUNCH_CHECK();
     }
     a.joinBlocks = a.chunks > 1 ? blocks : 0u;
-    const unsigned zeroBlocks = a.accumulate ? 0u : grid_for((a.V + kWindow - 1) / kWindow, kThreads);
+    const std::uint64_t windows = (a.V + kWindow - 1) / kWindow;
+    a.waveWindows = static_cast<std::uint32_t>(std::clamp<std::uint64_t>(windows / kZeroWaves, 1, kWave));
+    const unsigned zeroBlocks = a.accumulate ? 0u : grid_for(windows, a.waveWindows * (kThreads / kWave));
     if (a.joinBlocks + zeroBlocks > 0) {
         hipLaunchKernelGGL((join_kernel<T, N>), dim3(a.joinBlocks + zeroBlocks), dim3(kThreads), 0, st, a);
         TCC_LAUNCH_CHECK();
@@ -668,12 +742,23 @@ int tcc_embedding_grad(const void* dOut, uint64_t ldd, uint32_t dtype, const voi
     const std::uint64_t markWords = accumulate ? 0 : (V + 8 * kWindow - 1) / (8 * kWindow);
     std::uint64_t* const marks = reinterpret_cast<std::uint64_t*>(a.mark);
     std::uint64_t* const keys = reinterpret_cast<std::uint64_t*>(ws + lay.keysA);
-    if (n > 0 && n <= kRankRows) {
-        const unsigned blocks = grid_for(n, kWave);
-        hipLaunchKernelGGL(rank_kernel, dim3(blocks), dim3(kRankThreads), blocks * kWave * sizeof(std::uint32_t), st,
-                           IdKeys{rows, n, deviceError}, keys, marks, markWords);
-        TCC_LAUNCH_CHECK();
-        a.keys = keys;
+    if (n > 0 && n <= kPassRows) {
+        const std::uint32_t bits = id_bits(V), passes = (bits + kDigitBits - 1) / kDigitBits, digit = (bits + passes - 1) / passes;
+        std::uint64_t* const other = reinterpret_cast<std::uint64_t*>(ws + lay.keysB);
+        const dim3 grid(grid_for(n, kPassThreads)), block(kPassThreads);
+        const std::uint32_t count = static_cast<std::uint32_t>(n);
+        for (std::uint32_t p = 0; p < passes; ++p) {
+            const std::uint32_t width = std::min(digit, bits - p * digit);
+            std::uint64_t* const to = p % 2 == 0 ? keys : other;
+            if (p == 0)
+                hipLaunchKernelGGL(pass_kernel<FirstKeys>, grid, block, 0, st, FirstKeys{rows}, count, 0u, width, to, marks,
+                                   markWords, deviceError);
+            else
+                hipLaunchKernelGGL(pass_kernel<SortedKeys>, grid, block, 0, st, SortedKeys{a.keys}, count, p * digit, width,
+                                   to, marks, std::uint64_t(0), static_cast<std::uint32_t*>(nullptr));
+            TCC_LAUNCH_CHECK();
+            a.keys = to;
+        }
     } else {
         if (n > 0) {
             std::uint64_t* sorted = nullptr;

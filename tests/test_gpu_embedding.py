@@ -121,7 +121,8 @@ def test_lookup_refused_ids_and_non_finite_rows(gpu):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("kind", ["uniform", "hubs", "one", "ordered"])
 @pytest.mark.parametrize("V,n,D", [(1, 1, 1), (7, 2, 5), (300, 1000, 32), (4096, 777, 100), (50, 3001, 33), (9, 4097, 130),
-                                   (70_000, 20_011, 16), (100, 70_000, 20), (40, 300, 602)])
+                                   (70_000, 20_011, 16), (100, 70_000, 20), (40, 300, 602),
+                                   (5_000_000, 5001, 2), (2047, 65_536, 3), (2048, 65_537, 3), (3, 3000, 9), (60, 40_000, 36)])
 def test_grad(gpu, dtype, kind, V, n, D):
     from tcc_amd import training
 
