@@ -1182,14 +1182,17 @@ constexpr std::size_t align16(std::size_t b) { return (b + 15) & ~std::size_t(15
 
 // Tiles of at most this many, so that the tiles' sums stay few.
 constexpr std::uint64_t kTiles = 2048;
-// A segment that a workgroup walks in at most this many steps goes whole (some
-// 20 us; a longer one would end after all others): kManySteps where a thousand
-// and more take longer in all, kWaveSteps for waves, of which thousands are
-// under way at once.  All segments do, for the
-// launches that this saves, where no more than kSmallSteps could make one of
-// them and kSkew times the mean would still be short; none do where a segment of
-// kUneven times the mean, as batches have them, would be too long anyway.
-constexpr std::uint64_t kWholeSteps = 32, kManySteps = 64, kWaveSteps = 128, kSmallSteps = 256, kSkew = 8, kUneven = 4;
+// A segment that a workgroup walks in at most kWholeSteps steps goes whole (some
+// 30 us; a longer one would end after all others), or in kManySteps where kMany
+// segments and more take longer in all.  Where the longest is not known, it is
+// taken for kUneven times the mean (kManyUneven with many, of which few go by
+// tiles then): none goes whole if that is too long, as the kernels for both cost
+// more than either.  Where no more than kSmallSteps could make one segment and
+// the mean is half of what goes whole, all do, for the launches that this
+// saves.  780 segments of 324,652 x 32 bf16 rows, gradient: 62 us with 128 steps,
+// 89 with 64, 140 with 32; 70 of 17,559 x 42 rows: 35 by tiles, 70 whole; 5 of
+// 665 x 96 rows: 12 whole, 39 by tiles.
+constexpr std::uint64_t kWholeSteps = 64, kManySteps = 128, kMany = 512, kUneven = 8, kManyUneven = 4, kSmallSteps = 256;
 // Workgroups of a slice of whole segments, each with its own dWeight and dBias.
 constexpr std::uint64_t kWholeBlocks = 4096;
 
@@ -1253,9 +1256,10 @@ struct Split {
             longest = 0;
         } else {
             const std::uint64_t rowLanes = k.threads >> k.laneBits;
-            longest = (k.threads == kWave ? kWaveSteps : s.B >= 1024 ? kManySteps : kWholeSteps) * rowLanes;
-            if (!known && s.N <= kSmallSteps * rowLanes && kSkew * each <= 2 * longest) longest = s.N;
-            else if (!known && kUneven * each > longest) longest = 0;
+            const bool many = s.B >= kMany;
+            longest = (many ? kManySteps : kWholeSteps) * rowLanes;
+            if (!known && s.N <= kSmallSteps * rowLanes && 2 * each <= longest) longest = s.N;
+            else if (!known && (many ? kManyUneven : kUneven) * each > longest) longest = 0;
         }
         tiles = s.N > 0 && (most > longest || s.N > s.B * most);
         if (!tiles) longest = s.N;  // whatever maxRows says
