@@ -1190,9 +1190,10 @@ constexpr std::uint64_t kTiles = 2048;
 // more than either.  Where no more than kSmallSteps could make one segment and
 // the mean is half of what goes whole, all do, for the launches that this
 // saves.  780 segments of 324,652 x 32 bf16 rows, gradient: 62 us with 128 steps,
-// 89 with 64, 140 with 32; 70 of 17,559 x 42 rows: 35 by tiles, 70 whole; 5 of
-// 665 x 96 rows: 12 whole, 39 by tiles.
-constexpr std::uint64_t kWholeSteps = 64, kManySteps = 128, kMany = 512, kUneven = 8, kManyUneven = 4, kSmallSteps = 256;
+// 89 with 64, 140 with 32; 70 of 17,559 x 42 rows (31 steps in the mean): 35 by
+// tiles, 70 whole; 395 of 13,842 x 592 (9 steps): 71 by tiles, 49 mostly whole; 5
+// of 665 x 96 rows: 12 whole, 39 by tiles.
+constexpr std::uint64_t kWholeSteps = 64, kManySteps = 128, kMany = 512, kUneven = 5, kManyUneven = 4, kSmallSteps = 256;
 // Workgroups of a slice of whole segments, each with its own dWeight and dBias.
 constexpr std::uint64_t kWholeBlocks = 4096;
 
@@ -1285,9 +1286,12 @@ struct Layout {
     Layout(const tcc_group_norm_shape& s, bool backward) {
         const Split split(s, full_width(s.C, dtype_bytes(s.dtype)));
         const bool unaligned = s.C / s.G > kWholeThreads;  // room for rows that cannot go whole
-        // 16 rows of a tile at least and 64 where there are plenty, however narrow
-        // the rows: a tile's own reductions cost about as much
-        tileRows = std::max<std::uint64_t>((s.N + kTiles - 1) / kTiles, std::clamp<std::uint64_t>(s.N / 512, 16, 64));
+        // 16 rows of a tile at least and 64 where there are plenty, more where rows
+        // are narrow: a tile's own reductions cost about as much (one segment of
+        // 91,413 x 32 fp32 rows, gradient, 38 us with tiles of 128, 46 with 64)
+        const std::uint64_t rowLanes = kThreads * full_width(s.C, dtype_bytes(s.dtype)) / s.C;
+        tileRows = std::max<std::uint64_t>((s.N + kTiles - 1) / kTiles,
+                                           std::clamp<std::uint64_t>(s.N / 512, 16, std::max<std::uint64_t>(64, 4 * rowLanes)));
         tiles = split.tiles || unaligned ? (s.N + tileRows - 1) / tileRows : 0;
         wholeRows = split.whole && backward ? std::min(s.B, kWholeBlocks) : 0;
         part = 0;
