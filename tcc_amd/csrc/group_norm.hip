@@ -55,7 +55,8 @@ struct Segments {
         return static_cast<std::uint64_t>(v < 0 ? 0 : min<std::uint64_t>(static_cast<std::uint64_t>(v), N));
     }
     // The last segment that starts at or before `row` (0 if there is none),
-    // for row < N, by a whole wave: 64 starts a round.
+    // for row < N (so that segments of one size have rows), by a whole wave:
+    // 64 starts a round.
     __device__ __forceinline__ std::uint64_t find(std::uint64_t row) const {
         if (offsets == nullptr) return row / each;
         std::uint64_t lo = 0, hi = B;  // start(lo) <= row < start(hi), or lo = 0
@@ -1424,7 +1425,6 @@ int tiles_grad_launch(NormArgs a, const Layout& lay, std::uint64_t B, hipStream_
 NormArgs base_args(const tcc_group_norm_shape& s, const Layout& lay, const Split& split, void* workspace) {
     NormArgs a{};
     a.seg = Segments{s.offsets, s.N, s.B, s.B > 0 ? s.N / s.B : 0, s.offsetBytes == 8, split.longest};
-    if (s.offsets == nullptr && a.seg.each == 0) a.seg.each = 1;  // no rows: never read
     char* ws = static_cast<char*>(workspace);
     a.part = reinterpret_cast<float2*>(ws + lay.part);
     a.sums = reinterpret_cast<float2*>(ws + lay.sums);

@@ -278,6 +278,21 @@ def test_no_rows(gpu):
     assert dx.shape == (0, 12) and bool((dw == 0).all()) and bool((db == 0).all())
 
 
+@pytest.mark.parametrize("shape,G", [((0, 12), 3), ((1, 0, 12), 3), ((7, 0, 12), 12), ((1000, 0, 2, 24), 24), ((0, 5, 12), 3)])
+def test_segments_of_one_size_without_rows(gpu, shape, G):
+    """No offsets and no rows: every segment is empty, in number above what
+    the workspace has room for beside slots."""
+    from tcc_amd import training
+
+    B = 1 if len(shape) == 2 else shape[0]
+    x, w = torch.empty(shape, device="cuda"), torch.ones(shape[-1], device="cuda")
+    y, mean, rstd = training.group_norm(x, G, w, w, eps=0.25)
+    assert y.shape == shape and mean.shape == (B, G)
+    assert bool((mean == 0).all()) and bool((rstd == 2.0).all())
+    dx, dw, db = training.group_norm_grad(x, x, mean, rstd, G, w, w)
+    assert dx.shape == shape and bool((dw == 0).all()) and bool((db == 0).all())
+
+
 @pytest.mark.parametrize("act", ["none", "silu", "gelu"])
 def test_gradient_against_differences(gpu, act):
     """The change of sum(d * y) along e, for x, weight and bias: central
