@@ -42,11 +42,50 @@ whose features are given, has no counterpart.
 """
 from __future__ import annotations
 
+import functools
+
 import numpy as np
 import torch
 
 from . import swtcf
 from .hostmem import PinnedArray
+
+
+class _FirstOrder(torch.autograd.Function):
+    """A gradient that is no constant (it depends on `sources`) but cannot be
+    differentiated again."""
+
+    @staticmethod
+    def forward(ctx, name, grad, *sources):
+        ctx.name = name
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError(f"{ctx.name} has no second derivative: its gradient was asked for with create_graph=True "
+                           "and then differentiated")
+
+
+def _first_order(backward):
+    """For the backward of a node whose gradients are computed outside
+    autograd: under create_graph=True they would count as constants.  Here a
+    second differentiation raises instead."""
+
+    @functools.wraps(backward)
+    def checked(ctx, *grads):
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return out
+        sources = [t for t in (*grads, *ctx.saved_tensors) if t is not None and t.requires_grad]
+        if not sources:
+            return out
+        several = isinstance(out, tuple)
+        name = type(ctx).__name__.removesuffix("Backward")
+        out = [t if t is None else _FirstOrder.apply(name, t, *sources) for t in (out if several else (out,))]
+        return tuple(out) if several else out[0]
+
+    return checked
 
 
 class LayerGraph:
@@ -124,6 +163,7 @@ class CNICSPMMFunction(torch.autograd.Function):
         return torch.mm(AX, weights)
 
     @staticmethod
+    @_first_order
     def backward(ctx, d_output):
         AX, weights = ctx.saved_tensors
         grad_weights = swtcf.dense_tn(AX, d_output)  # AXᵀ·dY (:150)
@@ -150,6 +190,7 @@ class TransformFirstFunction(torch.autograd.Function):
         return out
 
     @staticmethod
+    @_first_order
     def backward(ctx, d_output):
         x, weights = ctx.saved_tensors
         grad_sp = ctx.graph.transpose_aggregate(d_output)
@@ -199,6 +240,7 @@ class TwoLayerFunction(torch.autograd.Function):
         return out
 
     @staticmethod
+    @_first_order
     def backward(ctx, d_output):
         AX, H, w2 = ctx.saved_tensors
         G = ctx.g2.transpose_aggregate(d_output)
@@ -242,6 +284,7 @@ class EmbeddingFunction(torch.autograd.Function):
         return training.embedding_lookup(table, ids, scale=scale, padding_idx=padding_idx, device_error=device_error)
 
     @staticmethod
+    @_first_order
     def backward(ctx, d_out):
         from . import training
 
@@ -265,6 +308,7 @@ class GroupNormFunction(torch.autograd.Function):
         return y
 
     @staticmethod
+    @_first_order
     def backward(ctx, d_y):
         from . import training
 

@@ -79,6 +79,38 @@ def test_step_matches_dense_reference(gpu, batch):
     assert int(torch.count_nonzero(model.embedding.weight.grad.cpu()[untouched])) == 0
 
 
+def test_second_derivatives_are_refused(gpu):
+    """A gradient that is taken with create_graph=True has its value, and a
+    second differentiation raises: nothing counts as a constant silently."""
+    from tcc_amd import gcn
+
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    leaf = lambda *s: torch.randn(s, generator=gen, device="cuda").requires_grad_(True)  # noqa: E731
+    table, x, w, b, w1, wide = leaf(9, 16), leaf(30, 16), leaf(16), leaf(16), leaf(16, 24), leaf(24, 2)
+    ids = torch.randint(0, 9, (30,), generator=gen, device="cuda")
+    graph, small = (gcn.LayerGraph(torch.arange(n), (torch.arange(n) * 7) % n, n, n) for n in (30, 16))
+    norm = lambda act: gcn.GroupNormFunction.apply(x, w, b, 4, None, 1e-5, act, None)  # noqa: E731
+    nodes = [
+        (lambda: gcn.EmbeddingFunction.apply(table, ids, 1.0, None, None).square().sum(), (table,)),
+        (lambda: norm("silu").square().sum(), (x, w, b)),
+        (lambda: norm("none").sum(), (x, w, b)),  # the slope depends on x and w alone
+        (lambda: gcn.CNICSPMMFunction.apply(graph, None, x, w1).square().sum(), (x, w1)),
+        (lambda: gcn.TransformFirstFunction.apply(small, w1, wide).square().sum(), (w1, wide)),
+    ]
+    for f, leaves in nodes:
+        plain = torch.autograd.grad(f(), leaves)
+        grads = torch.autograd.grad(f(), leaves, create_graph=True)
+        for g, p in zip(grads, plain):
+            assert torch.equal(g, p)
+        for g, t in zip(grads, leaves):
+            with pytest.raises(RuntimeError, match="second derivative"):
+                torch.autograd.grad((g * t).sum(), t, retain_graph=True)
+    # a gradient that is a constant stays one: the lookup is linear
+    (g,) = torch.autograd.grad(gcn.EmbeddingFunction.apply(table, ids, 1.0, None, None).sum(), table, create_graph=True)
+    (again,) = torch.autograd.grad((g * table).sum(), table)
+    assert torch.equal(again, g)
+
+
 def test_padding_row_stays_and_bad_ids_are_reported(gpu):
     from tcc_amd import gcn, swtcf
 
