@@ -393,8 +393,11 @@ class ClippedAdam(torch.optim.Optimizer):
                  decoupled: bool = True, max_norm: float | None = None):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, decoupled=decoupled,
                                       max_norm=max_norm))
-        if len(self.param_groups) != 1:
+
+    def add_param_group(self, param_group):
+        if self.param_groups:
             raise ValueError("ClippedAdam takes one group of parameters: the norm is over all of them")
+        super().add_param_group(param_group)
 
     @torch.no_grad()
     def step(self, closure=None):

@@ -123,3 +123,15 @@ def test_list_refusals():
     assert L.tcc_adam_step(good, good, half, good, 1, ctypes.byref(a), P, P, P, need, None) == INVALID
     assert L.tcc_adam_step(good, good, good, good, 1, ctypes.byref(a), None, P, P, need, None) == INVALID
     assert L.tcc_adam_step(good, good, good, good, 1, None, P, P, P, need, None) == INVALID
+
+
+def test_optimizer_takes_one_group():
+    from tcc_amd import gcn
+
+    first, second = (torch.nn.Parameter(torch.zeros(3)) for _ in range(2))
+    with pytest.raises(ValueError):
+        gcn.ClippedAdam([{"params": [first]}, {"params": [second]}])
+    optimizer = gcn.ClippedAdam([first])
+    with pytest.raises(ValueError):  # later too: step() would pass over it
+        optimizer.add_param_group({"params": [second]})
+    assert len(optimizer.param_groups) == 1
