@@ -387,7 +387,10 @@ class ClippedAdam(torch.optim.Optimizer):
     """Adam over one group of parameters whose gradients are clipped to
     `max_norm` as the update reads them (tcc_amd.training.adam_step): step()
     leaves the gradients as they are and returns their norm, a device scalar
-    (None without max_norm).  Nothing synchronises."""
+    (None without max_norm).  Steps are counted for each parameter, from its
+    first gradient on; where the counts differ, the clipped gradients are
+    written once, in their type, for an update a count.  Nothing
+    synchronises."""
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.0,
                  decoupled: bool = True, max_norm: float | None = None):
@@ -410,17 +413,43 @@ class ClippedAdam(torch.optim.Optimizer):
         params = [p for p in group["params"] if p.grad is not None]
         if not params:
             return None
-        if "step" not in group:
-            group["step"] = torch.zeros((), dtype=torch.int64, device=params[0].device)
+        ages = self._ages(params)
+        grads, max_norm, norm = {p: p.grad for p in params}, group["max_norm"], None
+        if max_norm is not None and len(ages) > 1:  # one norm for several updates
+            out = [torch.empty_like(g) for g in grads.values()]
+            norm = training.clip_grad_norm(list(grads.values()), max_norm, out=out)
+            grads, max_norm = dict(zip(params, out)), None
+        for some in ages:
+            states = [self.state[p] for p in some]
+            total = training.adam_step(some, [grads[p] for p in some], [s["exp_avg"] for s in states],
+                                       [s["exp_avg_sq"] for s in states], states[0]["step"], lr=group["lr"],
+                                       betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
+                                       decoupled=group["decoupled"], max_norm=max_norm)
+            norm = total if norm is None else norm
+        return norm
+
+    def _ages(self, params):
+        """`params` by the steps they have taken.  A count on the device serves
+        all parameters that were always updated together; those that go on
+        without the others get a copy of it."""
+        fresh, ages = None, {}
         for p in params:
             state = self.state[p]
             if not state:
+                if fresh is None:
+                    fresh = torch.zeros((), dtype=torch.int64, device=p.device)
+                state["step"] = fresh
                 state["exp_avg"] = torch.zeros_like(p, dtype=torch.float32)
                 state["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32)
-        return training.adam_step(params, [p.grad for p in params], [self.state[p]["exp_avg"] for p in params],
-                                  [self.state[p]["exp_avg_sq"] for p in params], group["step"], lr=group["lr"],
-                                  betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
-                                  decoupled=group["decoupled"], max_norm=group["max_norm"])
+            ages.setdefault(id(state["step"]), []).append(p)
+        here = set(params)
+        left = {id(s["step"]) for p, s in self.state.items() if p not in here}
+        for count, some in ages.items():
+            if count in left:
+                own = self.state[some[0]]["step"].clone()
+                for p in some:
+                    self.state[p]["step"] = own
+        return list(ages.values())
 
 
 class FeatureTable:

@@ -152,6 +152,37 @@ def test_optimizer_follows_torch(gpu):
         gcn.ClippedAdam([{"params": mine}, {"params": [unused]}])
 
 
+@pytest.mark.parametrize("max_norm", [None, 1.0])
+def test_optimizer_counts_steps_for_each_parameter(gpu, max_norm):
+    """Parameters whose gradients begin late or miss a step, against
+    torch.optim.AdamW: fp32 rounding of the update is below 1e-6 a step at
+    this rate, as in test_optimizer_follows_torch."""
+    from tcc_amd import gcn
+
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    sizes = ((30, 7), (11,), (64,), (5, 5))
+    mine = [torch.nn.Parameter(torch.randn(s, generator=gen, device="cuda")) for s in sizes]
+    twin = [torch.nn.Parameter(p.detach().clone()) for p in mine]
+    a = gcn.ClippedAdam(mine, lr=0.02, weight_decay=0.1, max_norm=max_norm)
+    b = torch.optim.AdamW(twin, lr=0.02, weight_decay=0.1)
+    for k in range(9):
+        for i, (p, q) in enumerate(zip(mine, twin)):
+            p.grad = q.grad = None
+            if (i == 1 and k < 3) or (i == 2 and k % 3 == 1) or (i == 3 and k in (0, 5)):
+                continue
+            p.grad = torch.randn(p.shape, generator=gen, device="cuda")
+            q.grad = p.grad.clone()
+        norm = a.step()
+        if max_norm is None:
+            assert norm is None
+        else:
+            want = torch.nn.utils.clip_grad_norm_(twin, max_norm)
+            assert abs(float(norm) - float(want)) <= 1e-6 * float(want)
+        b.step()
+        for p, q in zip(mine, twin):
+            assert float((p - q).abs().max()) <= 1e-6 * (k + 1) * 4
+
+
 def test_example_trains(gpu):
     from tcc_amd import train_embeddings
 
