@@ -402,6 +402,30 @@ class ClippedAdam(torch.optim.Optimizer):
             raise ValueError("ClippedAdam takes one group of parameters: the norm is over all of them")
         super().add_param_group(param_group)
 
+    def load_state_dict(self, state_dict):
+        """The moments come back in fp32 whatever the parameters' type, and the
+        counts on their device: torch would round the first to the parameters'
+        type and leave the second where the checkpoint was loaded to."""
+        seen = []
+        last = self.register_load_state_dict_pre_hook(lambda _, d: seen.append(d))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            last.remove()
+        (group,), state = seen[0]["param_groups"], seen[0]["state"]
+        # checkpoints made while one count served all parameters have it in the group
+        common = self.param_groups[0].pop("step", None)
+        counts = {}
+        for k, p in zip(group["params"], self.param_groups[0]["params"]):
+            if not state.get(k):
+                continue
+            t = int(state[k].get("step", common))
+            if t not in counts:
+                counts[t] = torch.tensor(t, dtype=torch.int64, device=p.device)
+            self.state[p]["step"] = counts[t]
+            for name in ("exp_avg", "exp_avg_sq"):
+                self.state[p][name] = state[k][name].to(p.device, torch.float32, copy=True)
+
     @torch.no_grad()
     def step(self, closure=None):
         from . import training

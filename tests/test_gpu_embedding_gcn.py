@@ -183,6 +183,74 @@ def test_optimizer_counts_steps_for_each_parameter(gpu, max_norm):
             assert float((p - q).abs().max()) <= 1e-6 * (k + 1) * 4
 
 
+@pytest.mark.parametrize("where", ["memory", "cpu"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_optimizer_resumes(gpu, dtype, where):
+    """A run that goes on from a checkpoint has the bits of one that was not
+    interrupted: moments in fp32, counts, parameters without a gradient so far."""
+    import io
+
+    from tcc_amd import gcn
+
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    grads = [[(torch.randn(s, generator=gen, device="cuda") * 0.1).to(dtype) for s in ((40, 8), (9,), (3,))]
+             for _ in range(6)]
+    start = [torch.randn(g.shape, generator=gen, device="cuda").to(dtype) for g in grads[0]]
+
+    def make(values):
+        params = [torch.nn.Parameter(v.detach().clone()) for v in values]
+        return params, gcn.ClippedAdam(params, lr=0.02, weight_decay=0.1, max_norm=0.5)
+
+    def run(params, optimizer, steps):
+        for k in steps:
+            for i, p in enumerate(params):
+                p.grad = None if i == 2 or (i == 1 and k == 0) else grads[k][i]  # the last one never, the second later
+            optimizer.step()
+
+    whole, one = make(start)
+    run(whole, one, range(6))
+    half, two = make(start)
+    run(half, two, range(3))
+    state = two.state_dict()
+    if where == "cpu":
+        buffer = io.BytesIO()
+        torch.save(state, buffer)
+        buffer.seek(0)
+        state = torch.load(buffer, map_location="cpu", weights_only=True)
+    rest, three = make(half)
+    three.load_state_dict(state)
+    run(half, two, range(3, 6))  # the checkpoint's own run goes on: nothing is shared with it
+    run(rest, three, range(3, 6))
+    for p, q, r in zip(whole, half, rest):
+        assert torch.equal(p, q) and torch.equal(p, r)
+        a, b = one.state[p], three.state[r]
+        assert set(a) == set(b)
+        for name in a:
+            assert a[name].dtype == b[name].dtype and b[name].device == r.device and torch.equal(a[name], b[name])
+
+
+def test_optimizer_takes_checkpoints_with_one_count(gpu):
+    """The count of all parameters in their group, as it once was kept."""
+    from tcc_amd import gcn
+
+    p = torch.nn.Parameter(torch.ones(5, device="cuda"))
+    q = torch.nn.Parameter(torch.ones(5, device="cuda"))
+    a, b = gcn.ClippedAdam([p], lr=0.1), gcn.ClippedAdam([q], lr=0.1)
+    p.grad = q.grad = torch.linspace(-1, 1, 5, device="cuda")
+    for _ in range(3):
+        a.step()
+    state = a.state_dict()
+    state["param_groups"][0]["step"] = state["state"][0].pop("step")
+    b.load_state_dict(state)
+    with torch.no_grad():
+        q.copy_(p)
+    assert int(b.state[q]["step"]) == 3 and "step" not in b.param_groups[0]
+    state["state"][0]["step"] = state["param_groups"][0].pop("step")
+    a.step()
+    b.step()
+    assert torch.equal(p, q)
+
+
 def test_example_trains(gpu):
     from tcc_amd import train_embeddings
 
