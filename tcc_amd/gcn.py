@@ -387,10 +387,13 @@ class ClippedAdam(torch.optim.Optimizer):
     """Adam over one group of parameters whose gradients are clipped to
     `max_norm` as the update reads them (tcc_amd.training.adam_step): step()
     leaves the gradients as they are and returns their norm, a device scalar
-    (None without max_norm).  Steps are counted for each parameter, from its
+    (None without max_norm).  step(closure) returns the closure's loss, as
+    torch's optimizers do; the norm is in `norm` after either.  Steps are counted for each parameter, from its
     first gradient on; where the counts differ, the clipped gradients are
     written once, in their type, for an update a count.  Nothing
     synchronises."""
+
+    norm = None
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.0,
                  decoupled: bool = True, max_norm: float | None = None):
@@ -428,11 +431,16 @@ class ClippedAdam(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None):
-        from . import training
-
+        loss = None
         if closure is not None:
             with torch.enable_grad():
-                closure()
+                loss = closure()
+        self.norm = self._update()
+        return self.norm if closure is None else loss
+
+    def _update(self):
+        from . import training
+
         group = self.param_groups[0]
         params = [p for p in group["params"] if p.grad is not None]
         if not params:

@@ -251,6 +251,26 @@ def test_optimizer_takes_checkpoints_with_one_count(gpu):
     assert torch.equal(p, q)
 
 
+def test_optimizer_returns_the_closures_loss(gpu):
+    from tcc_amd import gcn
+
+    p = torch.nn.Parameter(torch.full((4,), 3.0, device="cuda"))
+    optimizer = gcn.ClippedAdam([p], max_norm=1.0)
+
+    def closure():
+        optimizer.zero_grad()
+        loss = p.square().sum()
+        loss.backward()
+        return loss
+
+    assert float(optimizer.step(closure)) == 36.0
+    assert float(optimizer.norm) == 12.0  # sqrt(4 * 6^2)
+    optimizer.zero_grad()
+    p.sum().backward()
+    norm = optimizer.step()
+    assert float(norm) == 2.0 and norm is optimizer.norm
+
+
 def test_example_trains(gpu):
     from tcc_amd import train_embeddings
 
