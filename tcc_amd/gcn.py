@@ -336,7 +336,8 @@ class NodeEmbedding(torch.nn.Module):
         if padding_idx is not None:
             with torch.no_grad():
                 self.weight[padding_idx].zero_()
-        self.device_error = torch.zeros(1, dtype=torch.int32, device=device)
+        # a buffer, so that it moves with the module; no part of checkpoints
+        self.register_buffer("device_error", torch.zeros(1, dtype=torch.int32, device=device), persistent=False)
 
     def forward(self, ids: torch.Tensor) -> torch.Tensor:
         return EmbeddingFunction.apply(self.weight, ids, self.scale, self.padding_idx, self.device_error)

@@ -135,3 +135,14 @@ def test_optimizer_takes_one_group():
     with pytest.raises(ValueError):  # later too: step() would pass over it
         optimizer.add_param_group({"params": [second]})
     assert len(optimizer.param_groups) == 1
+
+
+def test_embedding_moves_as_a_whole():
+    """The error word goes where the table goes, and is in no checkpoint."""
+    from tcc_amd import gcn
+
+    e = gcn.NodeEmbedding(6, 4, device="cpu")
+    assert list(e.state_dict()) == ["weight"]
+    e = e.to("meta").to(torch.bfloat16)
+    assert e.weight.dtype == torch.bfloat16
+    assert e.device_error.device.type == "meta" and e.device_error.dtype == torch.int32
