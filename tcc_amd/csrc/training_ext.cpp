@@ -94,6 +94,15 @@ Tensor workspace(std::size_t bytes, const Tensor& like) {
     return empty({static_cast<std::int64_t>(bytes)}, like.options().dtype(at::kByte));
 }
 
+// Autograd has to know of what a call wrote in place: a graph that saved the
+// tensor refuses its backward pass then, instead of taking the new values.
+void written(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+void written(const std::vector<Tensor>& list) {
+    for (const Tensor& t : list) written(t);
+}
+
 void* ptr(const MaybeTensor& t) { return t ? t->data_ptr() : nullptr; }
 
 // A matrix whose rows are contiguous, and its row stride (a copy where the
@@ -159,6 +168,7 @@ Tensor embedding_lookup(const Tensor& table, const Tensor& ids, double scale, st
     check(tcc_embedding_lookup(rows.t.data_ptr(), rows.ld, code, flat.data_ptr(), width, flat.numel(), V,
                                static_cast<std::uint32_t>(D), static_cast<float>(scale), pad, to.data_ptr(), ldo, err,
                                stream_of(table)));
+    if (out) written(to);
     return to;
 }
 
@@ -194,6 +204,7 @@ Tensor embedding_grad(const Tensor& dOut, const Tensor& ids, std::int64_t V, dou
     check(tcc_embedding_grad(rows.t.data_ptr(), rows.ld, code, flat.data_ptr(), width, n, V,
                              static_cast<std::uint32_t>(D), static_cast<float>(scale), pad, to.data_ptr(), ldg, accumulate,
                              err, ws.data_ptr(), need, stream_of(dOut)));
+    if (grad) written(to);
     return to;
 }
 
@@ -422,6 +433,7 @@ Tensor clip_grad_norm(const TensorList& grads, double maxNorm, const std::option
     const NormPlace p(true);
     check(tcc_clip_grad_norm(lists[0].data(), lists[1].data(), static_cast<std::uint32_t>(grads.size()),
                              static_cast<float>(maxNorm), p.at(), p.ws.data_ptr(), p.bytes, stream_of(p.ws)));
+    written(to);
     return p.norm;
 }
 
@@ -443,6 +455,8 @@ MaybeTensor adam_step(const TensorList& params, const TensorList& grads, const T
     check(tcc_adam_step(lists[0].data(), lists[1].data(), lists[2].data(), lists[3].data(),
                         static_cast<std::uint32_t>(params.size()), &a, step.data_ptr<std::int64_t>(), p.at(),
                         p.ws.data_ptr(), p.bytes, stream_of(p.ws)));
+    for (const TensorList* l : {&params, &expAvg, &expAvgSq}) written(*l);
+    written(step);
     return maxNorm ? MaybeTensor(p.norm) : std::nullopt;
 }
 

@@ -271,6 +271,39 @@ def test_optimizer_returns_the_closures_loss(gpu):
     assert float(norm) == 2.0 and norm is optimizer.norm
 
 
+def test_autograd_sees_what_is_written_in_place(gpu):
+    """A graph that saved a parameter refuses its backward pass once a step
+    has changed it, as with torch's optimizers, and every tensor that a call
+    writes has a new version (one that it only reads has not)."""
+    from tcc_amd import gcn, training
+
+    p = torch.nn.Parameter(torch.randn(6, device="cuda"))
+    optimizer = gcn.ClippedAdam([p], max_norm=1.0)
+    loss = (p * p).sum()
+    loss.backward(retain_graph=True)
+    optimizer.step()
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        loss.backward()
+    new = lambda *s: torch.rand(s, device="cuda")  # noqa: E731
+    table, ids, room, grads, out = new(9, 4), torch.arange(3, device="cuda"), new(3, 4), [new(5), new(2, 2)], [new(5), new(2, 2)]
+    moments = [new(5), new(2, 2)], [new(5), new(2, 2)]
+    step = torch.zeros((), dtype=torch.int64, device="cuda")
+    calls = [
+        (lambda: training.embedding_lookup(table, ids, out=room), [room], [table, ids]),
+        (lambda: training.embedding_grad(room, ids, 9, grad=table, accumulate=True), [table], [room, ids]),
+        (lambda: training.clip_grad_norm(grads, 0.1, out=out), out, grads),
+        (lambda: training.clip_grad_norm(grads, 0.1), grads, out),
+        (lambda: training.adam_step(out, grads, *moments, step, max_norm=1.0), out + moments[0] + moments[1] + [step], grads),
+    ]
+    for call, written, read in calls:
+        before = [t._version for t in written], [t._version for t in read]
+        call()
+        assert all(t._version > v for t, v in zip(written, before[0]))
+        assert [t._version for t in read] == before[1]
+    with torch.inference_mode():  # tensors without versions
+        training.clip_grad_norm([new(5)], 0.1)
+
+
 def test_example_trains(gpu):
     from tcc_amd import train_embeddings
 
