@@ -39,7 +39,8 @@ extern "C" {
  * out [n x D] (ldo), both of `dtype`; ids int32 (idBytes 4) or int64 (8).
  * Rows whose id is `padding` (-1: no such id) are zeros.  So are rows whose
  * id is outside [0, V): they set TCC_DEVERR_FEATURE_INDEX in *deviceError,
- * if it is not NULL.  n and V below 2^32 - 1. */
+ * if it is not NULL.  n and V below 2^32 - 1 and D below 2^32 - 1025
+ * (TCC_ERR_UNSUPPORTED above). */
 int tcc_embedding_lookup(const void* table, uint64_t ldt, uint32_t dtype, const void* ids, uint32_t idBytes, uint64_t n,
                          uint64_t V, uint32_t D, float scale, int64_t padding, void* out, uint64_t ldo,
                          uint32_t* deviceError, void* stream);
@@ -52,7 +53,7 @@ size_t tcc_embedding_grad_workspace_bytes(uint64_t n, uint64_t V, uint32_t D);
  * row of grad is written (accumulate = 0), or the sums are added to grad and
  * only rows that occur are touched (accumulate != 0).  Padding and refused
  * ids as in tcc_embedding_lookup: their rows of dOut are not read.  The rows
- * of one id are added in an order that the ids alone decide. */
+ * of one id are added in an order that the ids alone decide.  D below 2^28. */
 int tcc_embedding_grad(const void* dOut, uint64_t ldd, uint32_t dtype, const void* ids, uint32_t idBytes, uint64_t n,
                        uint64_t V, uint32_t D, float scale, int64_t padding, void* grad, uint64_t ldg, int accumulate,
                        uint32_t* deviceError, void* workspace, size_t workspaceBytes, void* stream);

@@ -585,6 +585,10 @@ unsigned id_bits(std::uint64_t V) {  // of the values 0 .. V
     return b;
 }
 
+// Columns of a gradient: a window's elements are counted in 32 bits.
+constexpr std::uint32_t kMaxGradCols = (1u << 28) - 1;
+static_assert(kMaxGradCols <= 0xFFFFFFFFu / kWindow);
+
 constexpr std::size_t align16(std::size_t b) { return (b + 15) & ~std::size_t(15); }
 
 struct GradLayout {
@@ -611,6 +615,7 @@ template <typename T, int N>
 int lookup_launch(const void* table, std::uint64_t ldt, const Ids& ids, std::uint64_t n, std::uint32_t D, float scale,
                   void* out, std::uint64_t ldo, std::uint32_t* err, hipStream_t st) {
     const std::uint32_t colsV = D / N;
+    TCC_REQUIRE(colsV < kNoRow - kThreads * kLookupUnroll, TCC_ERR_UNSUPPORTED, "embedding rows too wide for a lookup");
     const std::uint64_t vecs = n * colsV;
     const std::uint64_t blocks = (vecs + kThreads * kLookupUnroll - 1) / (kThreads * kLookupUnroll);
     TCC_REQUIRE(blocks < (1ull << 31), TCC_ERR_UNSUPPORTED, "embedding lookup output too large for one call");
@@ -706,6 +711,7 @@ int tcc_embedding_grad(const void* dOut, uint64_t ldd, uint32_t dtype, const voi
                        uint64_t V, uint32_t D, float scale, int64_t padding, void* grad, uint64_t ldg, int accumulate,
                        uint32_t* deviceError, void* workspace, size_t workspaceBytes, void* stream) {
     if (const int rc = check_ids(ids, idBytes, n, V, D, dtype)) return rc;
+    TCC_REQUIRE(D <= kMaxGradCols, TCC_ERR_UNSUPPORTED, "embedding rows too wide for a gradient (2^28 - 1 elements at most)");
     const GradLayout lay(n, V, D);
     TCC_REQUIRE(ldd >= D && ldg >= D && (dOut || n == 0) && (grad || V == 0), TCC_ERR_INVALID_ARGUMENT,
                 "invalid embedding gradient arguments");

@@ -133,6 +133,12 @@ std::int64_t padding_of(std::optional<std::int64_t> padding, std::int64_t rows) 
     return *padding;
 }
 
+// The columns of a table; the C-ABI counts them in 32 bits.
+std::uint32_t columns_of(std::int64_t D) {
+    if (D > 0xFFFFFFFFll) value_error("a table of " + std::to_string(D) + " columns is too wide");
+    return static_cast<std::uint32_t>(D);
+}
+
 std::uint32_t* error_word(const MaybeTensor& t) {
     if (!t) return nullptr;
     if (!t->is_cuda() || t->scalar_type() != at::kInt || t->numel() < 1) type_error("device_error must be an int32 device tensor");
@@ -146,6 +152,7 @@ Tensor embedding_lookup(const Tensor& table, const Tensor& ids, double scale, st
                         const MaybeTensor& out, const MaybeTensor& deviceError) {
     const std::uint32_t code = dtype_of(table, "table");
     const std::uint32_t width = index_bytes(ids, "ids");
+    const std::uint32_t cols = table.dim() == 2 ? columns_of(table.size(1)) : 0;
     const Rows rows(table, "table");
     const Tensor flat = ids.contiguous();
     const std::int64_t V = table.size(0), D = table.size(1), pad = padding_of(padding, V);
@@ -165,9 +172,8 @@ Tensor embedding_lookup(const Tensor& table, const Tensor& ids, double scale, st
     } else {
         to = empty(shape, table.options());
     }
-    check(tcc_embedding_lookup(rows.t.data_ptr(), rows.ld, code, flat.data_ptr(), width, flat.numel(), V,
-                               static_cast<std::uint32_t>(D), static_cast<float>(scale), pad, to.data_ptr(), ldo, err,
-                               stream_of(table)));
+    check(tcc_embedding_lookup(rows.t.data_ptr(), rows.ld, code, flat.data_ptr(), width, flat.numel(), V, cols,
+                               static_cast<float>(scale), pad, to.data_ptr(), ldo, err, stream_of(table)));
     if (out) written(to);
     return to;
 }
@@ -181,6 +187,7 @@ Tensor embedding_grad(const Tensor& dOut, const Tensor& ids, std::int64_t V, dou
         value_error("d_out " + shape_of(dOut) + " does not have a row for each of the ids " + shape_of(ids));
     if (V < 0) value_error("num_rows is not negative");
     const std::int64_t n = ids.numel(), D = dOut.size(-1);
+    const std::uint32_t cols = columns_of(D);
     const Rows rows(dOut.dim() == 2 ? dOut : dOut.reshape({n, D}), "d_out");
     const Tensor flat = ids.contiguous();
     const std::int64_t pad = padding_of(padding, V);
@@ -199,11 +206,11 @@ Tensor embedding_grad(const Tensor& dOut, const Tensor& ids, std::int64_t V, dou
         if (accumulate) value_error("accumulate=True needs a gradient to add to");
         to = empty({V, D}, dOut.options());
     }
-    const std::size_t need = tcc_embedding_grad_workspace_bytes(n, V, static_cast<std::uint32_t>(D));
+    const std::size_t need = tcc_embedding_grad_workspace_bytes(n, V, cols);
     const Tensor ws = workspace(need, dOut);
-    check(tcc_embedding_grad(rows.t.data_ptr(), rows.ld, code, flat.data_ptr(), width, n, V,
-                             static_cast<std::uint32_t>(D), static_cast<float>(scale), pad, to.data_ptr(), ldg, accumulate,
-                             err, ws.data_ptr(), need, stream_of(dOut)));
+    check(tcc_embedding_grad(rows.t.data_ptr(), rows.ld, code, flat.data_ptr(), width, n, V, cols,
+                             static_cast<float>(scale), pad, to.data_ptr(), ldg, accumulate, err, ws.data_ptr(), need,
+                             stream_of(dOut)));
     if (grad) written(to);
     return to;
 }

@@ -202,6 +202,18 @@ def test_places_past_32_bits(gpu):
     assert torch.equal(g[V - 2], d[2]) and int(torch.count_nonzero(g[V - 3])) == 0
 
 
+def test_columns_past_32_bits_are_refused(gpu):
+    """Tables without a row, so that nothing of that width is in memory."""
+    from tcc_amd import training
+
+    none = torch.empty(0, dtype=torch.int64, device="cuda")
+    wide = torch.empty((0, 2**32 + 8), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError):
+        training.embedding_lookup(wide, none)
+    with pytest.raises(ValueError):
+        training.embedding_grad(wide, none, 0)
+
+
 def test_gradient_against_differences(gpu):
     """<grad, e> is the change of sum(w * lookup) along e: the lookup is
     linear, so the difference quotient is exact up to rounding."""

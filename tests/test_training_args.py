@@ -146,3 +146,12 @@ def test_embedding_moves_as_a_whole():
     e = e.to("meta").to(torch.bfloat16)
     assert e.weight.dtype == torch.bfloat16
     assert e.device_error.device.type == "meta" and e.device_error.dtype == torch.int32
+
+
+def test_rows_too_wide_are_refused():
+    """Column counts that the kernels' 32-bit arithmetic does not hold."""
+    L = lib()
+    for D in (0xFFFFFFFF, 0xFFFFFFFF - 100):
+        assert L.tcc_embedding_lookup(P, D, 1, P, 4, 3, 5, D, 1.0, -1, ctypes.c_void_p(66), D, None, None) == UNSUPPORTED
+    for D in (1 << 28, 0xFFFFFFFF):
+        assert L.tcc_embedding_grad(P, D, 0, P, 4, 3, 5, D, 1.0, -1, P, D, 0, None, P, 1 << 40, None) == UNSUPPORTED
