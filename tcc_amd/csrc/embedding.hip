@@ -83,11 +83,13 @@ constexpr int kLookupUnroll = 4;
 // are written past the caches' order, which leaves those to rows that come
 // again: 2.45M x 100 rows of bf16 248 us instead of 270, of fp32 323 instead
 // of 359 (4 vectors a lane; with 2 of them 257 and 318, with 8 over 600).
+// `from`: the launch's first vector.
 template <typename T, int N, bool ONCE>
 __global__ void __launch_bounds__(kThreads) lookup_kernel(const T* __restrict__ table, std::uint64_t ldt, Ids ids,
                                                          std::uint64_t n, std::uint32_t colsV, float scale,
-                                                         T* __restrict__ out, std::uint64_t ldo, std::uint32_t* err) {
-    const std::uint64_t first = static_cast<std::uint64_t>(blockIdx.x) * (kThreads * kLookupUnroll);
+                                                         T* __restrict__ out, std::uint64_t ldo, std::uint32_t* err,
+                                                         std::uint64_t from) {
+    const std::uint64_t first = from + static_cast<std::uint64_t>(blockIdx.x) * (kThreads * kLookupUnroll);
     const std::uint64_t row0 = first / colsV;
     const std::uint32_t col0 = static_cast<std::uint32_t>(first - row0 * colsV);
     std::uint64_t i[kLookupUnroll];
@@ -617,12 +619,14 @@ int lookup_launch(const void* table, std::uint64_t ldt, const Ids& ids, std::uin
     const std::uint32_t colsV = D / N;
     TCC_REQUIRE(colsV < kNoRow - kThreads * kLookupUnroll, TCC_ERR_UNSUPPORTED, "embedding rows too wide for a lookup");
     const std::uint64_t vecs = n * colsV;
-    const std::uint64_t blocks = (vecs + kThreads * kLookupUnroll - 1) / (kThreads * kLookupUnroll);
-    TCC_REQUIRE(blocks < (1ull << 31), TCC_ERR_UNSUPPORTED, "embedding lookup output too large for one call");
+    constexpr std::uint64_t kVecs = kThreads * kLookupUnroll, kMost = kVecs << 22;  // of a launch: 2^30 threads
     auto* form = n * D * sizeof(T) > kCacheBytes ? &lookup_kernel<T, N, true> : &lookup_kernel<T, N, false>;
-    hipLaunchKernelGGL(form, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st, static_cast<const T*>(table), ldt,
-                       ids, n, colsV, scale, static_cast<T*>(out), ldo, err);
-    TCC_LAUNCH_CHECK();
+    for (std::uint64_t from = 0; from < vecs; from += kMost) {
+        const unsigned blocks = grid_for(std::min(vecs - from, kMost), kVecs);
+        hipLaunchKernelGGL(form, dim3(blocks), dim3(kThreads), 0, st, static_cast<const T*>(table), ldt, ids, n, colsV, scale,
+                           static_cast<T*>(out), ldo, err, from);
+        TCC_LAUNCH_CHECK();
+    }
     return TCC_OK;
 }
 

@@ -202,6 +202,20 @@ def test_places_past_32_bits(gpu):
     assert torch.equal(g[V - 2], d[2]) and int(torch.count_nonzero(g[V - 3])) == 0
 
 
+def test_lookup_of_more_than_a_launch(gpu):
+    """17.3e9 elements that lanes take one by one (35 GB): more than one launch
+    has threads for, with the launches' ends inside rows."""
+    from tcc_amd import training
+
+    V, n, D = 1000, 171_000_007, 101
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    table = torch.randn((V, D), generator=gen, device="cuda").to(torch.float16)
+    ids = torch.randint(0, V, (n,), generator=gen, device="cuda", dtype=torch.int32)
+    got = training.embedding_lookup(table, ids)
+    for at in range(0, n, 10_000_000):
+        assert torch.equal(got[at:at + 10_000_000], table[ids[at:at + 10_000_000].long()])
+
+
 def test_columns_past_32_bits_are_refused(gpu):
     """Tables without a row, so that nothing of that width is in memory."""
     from tcc_amd import training
