@@ -1309,6 +1309,13 @@ struct Layout {
     }
 };
 
+// The rows of a workgroup of the output, doubled until a launch has fewer
+// than 2^32 threads (more, HIP takes for the remainder without an error).
+std::uint64_t out_rows(std::uint64_t N, std::uint64_t rows) {
+    while (N / rows >= (1ull << 32) / kThreads - 1) rows *= 2;
+    return rows;
+}
+
 int check_shape(const tcc_group_norm_shape* s) {
     TCC_REQUIRE(s != nullptr, TCC_ERR_INVALID_ARGUMENT, "group norm: no shape");
     TCC_REQUIRE(s->G >= 1 && s->C >= 1 && s->C % s->G == 0, TCC_ERR_INVALID_ARGUMENT,
@@ -1396,8 +1403,8 @@ int tiles_launch(NormArgs a, const Layout& lay, std::uint64_t B, hipStream_t st)
     hipLaunchKernelGGL((stats_kernel<T, N>), dim3(tiles), dim3(kThreads), 2 * a.rowLanes * a.C * sizeof(float), st, a);
     TCC_LAUNCH_CHECK();
     if (const int rc = stats_join_launch(a, lay, B, st)) return rc;
-    a.outRows = kOutSteps<T, N> * a.rowLanes;
-    TCC_BY_ACT(apply_kernel, T, N, dim3(grid_for(a.seg.N, kOutSteps<T, N> * a.rowLanes)), kThreads, 0, st, a);
+    a.outRows = out_rows(a.seg.N, kOutSteps<T, N> * a.rowLanes);
+    TCC_BY_ACT(apply_kernel, T, N, dim3(grid_for(a.seg.N, static_cast<unsigned>(a.outRows))), kThreads, 0, st, a);
     TCC_LAUNCH_CHECK();
     return TCC_OK;
 }
@@ -1416,8 +1423,8 @@ int tiles_grad_launch(NormArgs a, const Layout& lay, std::uint64_t B, hipStream_
         hipLaunchKernelGGL(grad_join_kernel<1>, JoinGroup<1>::grid(B, a.G),
                            dim3(JoinGroup<1>::threads), 0, st, a);
     TCC_LAUNCH_CHECK();
-    a.outRows = kGradSteps<T, N> * a.rowLanes;
-    TCC_BY_ACT(grad_apply_kernel, T, N, dim3(grid_for(a.seg.N, kGradSteps<T, N> * a.rowLanes)), kThreads, 0, st, a);
+    a.outRows = out_rows(a.seg.N, kGradSteps<T, N> * a.rowLanes);
+    TCC_BY_ACT(grad_apply_kernel, T, N, dim3(grid_for(a.seg.N, static_cast<unsigned>(a.outRows))), kThreads, 0, st, a);
     TCC_LAUNCH_CHECK();
     return TCC_OK;
 }

@@ -314,6 +314,21 @@ def test_gradient_against_differences(gpu, act):
     assert abs(along - quotient) <= tol
 
 
+def test_gradient_of_more_than_a_launch(gpu):
+    """Rows of 129 vectors, two to a workgroup: more workgroups than one launch
+    has threads for (69 GB each of x and dx).  x = dy = +-1 in turn with mean 0
+    and rstd 1/2: dx = (x - 0 - x / 4) / 2, off by what the sums' fp32 is."""
+    from tcc_amd import training
+
+    N, C = 2**25 + 999, 516
+    x = torch.ones((N, C), device="cuda")
+    x[1::2] = -1
+    mean, rstd = torch.zeros((1, 1), device="cuda"), torch.full((1, 1), 0.5, device="cuda")
+    dx, _, _ = training.group_norm_grad(x, x, mean, rstd, 1)
+    for at in range(0, N, 2**22):
+        assert float((dx[at:at + 2**22] - 0.375 * x[at:at + 2**22]).abs().max()) < 1e-3
+
+
 def test_relu_mask_is_the_forward_s(gpu):
     """Values that land on zero or beside it: dy passes exactly where y > 0."""
     from tcc_amd import training
