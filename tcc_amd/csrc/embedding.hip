@@ -489,6 +489,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(GradArgs a) {
 // 70,000) take 6 us (7) for 1,000 of them, 14 (16) for 3,000 and 26 (27) for
 // 4,000, sorted 15 (29) for any of these.
 constexpr std::uint64_t kFewRows = 3000;
+constexpr std::uint64_t kFewTableRows = 1ull << 31;  // so that those that zero stay far below 2^32 threads
 constexpr std::uint32_t kFewZeroRows = 256;  // rows of a workgroup that zeroes, at most
 
 template <typename T, int N>
@@ -742,7 +743,7 @@ int tcc_embedding_grad(const void* dOut, uint64_t ldd, uint32_t dtype, const voi
     a.scale = scale;
     a.accumulate = accumulate;
     const std::uint32_t w = RowWidth(D, dtype_bytes(dtype)).with(dOut).with(grad).stride(ldd).stride(ldg).elems();
-    if (n > 0 && n <= kFewRows) {
+    if (n > 0 && n <= kFewRows && V <= kFewTableRows) {
 #define CALL(T, N) (few_grad_launch<T, N>(a, rows, deviceError, st))
         if (dtype == TCC_F32) TCC_BY_WIDTH(float, 4, w, CALL);
         if (dtype == TCC_BF16) TCC_BY_WIDTH(bf16_t, 8, w, CALL);

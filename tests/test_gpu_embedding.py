@@ -216,6 +216,23 @@ def test_lookup_of_more_than_a_launch(gpu):
         assert torch.equal(got[at:at + 10_000_000], table[ids[at:at + 10_000_000].long()])
 
 
+@pytest.mark.parametrize("n", [50])
+def test_grad_of_the_longest_table(gpu, n):
+    """2^32 - 2 rows of one fp16 element: ids at both ends and between, every
+    other row zeroed, the last windows' too."""
+    from tcc_amd import training
+
+    V = 2**32 - 2
+    gen = torch.Generator().manual_seed(n)
+    ids = torch.cat([torch.randint(0, V, (n - 6,), generator=gen), torch.tensor([0, 3, V - 20, V - 9, V - 9, V - 5])]).cuda()
+    d = torch.ones((n, 1), dtype=torch.float16, device="cuda")
+    grad = torch.full((V, 1), 7.0, dtype=torch.float16, device="cuda")
+    training.embedding_grad(d, ids, V, grad=grad)
+    rows, count = torch.unique(ids, return_counts=True)
+    assert torch.equal(grad[rows, 0], count.to(torch.float16))
+    assert sum(int(torch.count_nonzero(grad[at:at + 2**29])) for at in range(0, V, 2**29)) == rows.numel()
+
+
 def test_columns_past_32_bits_are_refused(gpu):
     """Tables without a row, so that nothing of that width is in memory."""
     from tcc_amd import training
