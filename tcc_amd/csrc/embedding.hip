@@ -291,7 +291,7 @@ template <typename T, int N>
 __device__ __forceinline__ void zero_between(const GradArgs& a, std::uint32_t q, std::uint32_t r, std::uint32_t c) {
     const std::uint32_t V = static_cast<std::uint32_t>(a.V);
     std::uint32_t v = q + 1;  // 0 where none is before
-    const std::uint32_t endOfQ = q == kNoRow ? 0u : min(r, (q / kWindow + 1) * kWindow);
+    const std::uint32_t endOfQ = q == kNoRow ? 0u : q + min(r - q, kWindow - q % kWindow);
     const std::uint32_t startOfR = r < V ? r / kWindow * kWindow : V;
     for (; v < r; ++v) {
         if (v >= endOfQ && v < startOfR) v = startOfR;  // an empty window begins

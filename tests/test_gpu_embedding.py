@@ -216,7 +216,7 @@ def test_lookup_of_more_than_a_launch(gpu):
         assert torch.equal(got[at:at + 10_000_000], table[ids[at:at + 10_000_000].long()])
 
 
-@pytest.mark.parametrize("n", [50])
+@pytest.mark.parametrize("n", [50, 5000, 70_000])
 def test_grad_of_the_longest_table(gpu, n):
     """2^32 - 2 rows of one fp16 element: ids at both ends and between, every
     other row zeroed, the last windows' too."""
