@@ -282,7 +282,8 @@ struct AdamFactors {
 
 __device__ __forceinline__ void adam_one(float& p, float g, float& m, float& v, const AdamArgs& a,
                                          const AdamFactors& f) {
-    g = g * f.clip + a.decay * p;
+    g *= f.clip;
+    if (a.decay != 0.0f) g += a.decay * p;  // without decay an infinite parameter is none of the moments'
     m = a.beta1 * m + a.rest1 * g;
     v = a.beta2 * v + a.rest2 * g * g;
     p = a.keep * p - f.size * (m / (sqrtf(v) / f.root2 + a.eps));

@@ -239,3 +239,20 @@ def test_replayed_graph_and_other_stream(gpu):
         want = training.adam_step(twin[0], g, twin[1], twin[2], twin_step, max_norm=1.0)
         assert torch.equal(norm, want) and int(step) == int(twin_step) == k + 2
         assert all(torch.equal(a, b) for a, b in zip(p + m + v, twin[0] + twin[1] + twin[2]))
+
+
+@pytest.mark.parametrize("decoupled,decay", [(True, 0.1), (True, 0.0), (False, 0.0)])
+@pytest.mark.parametrize("n", [5, 5000])
+def test_infinite_parameters_leave_the_moments(gpu, decoupled, decay, n):
+    """The gradient holds no parameter unless its decay does: the moments stay
+    those of the gradients beside an infinite or NaN parameter."""
+    from tcc_amd import training
+
+    p, g = tensors([(n,)], [torch.float32], 3)[0], tensors([(n,)], [torch.float32], 4)[0]
+    m, v = torch.zeros_like(p), torch.zeros_like(p)
+    p[0], p[3] = float("inf"), float("nan")
+    training.adam_step([p], [g], [m], [v], torch.zeros((), dtype=torch.int64, device="cuda"), weight_decay=decay,
+                       decoupled=decoupled)
+    assert bool(p[0].isinf()) and bool(p[3].isnan()) and int(p.isfinite().sum()) == n - 2
+    assert bool(((m - 0.1 * g).abs() <= 4 * U * g.abs()).all())
+    assert bool(((v - 0.001 * g * g).abs() <= 8 * U * g * g).all())
