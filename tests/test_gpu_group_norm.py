@@ -252,6 +252,28 @@ def test_large_means_lose_nothing(gpu, dtype, level):
     assert bool(((got[2].double().cpu()[0] ** -2 - 1e-5 - var).abs() <= 2 * off + 1e-9).all())
 
 
+@pytest.mark.parametrize("size", [100.0, 1e4, 1e6])
+@pytest.mark.parametrize("N,C,G,B", [(40_000, 64, 8, 1), (20_000, 30, 10, 1), (3000, 64, 8, 10), (3500, 12, 4, 2),
+                                     (510, 100, 4, 3), (510, 150, 6, 600), (20, 64, 4, 1500), (300, 33, 11, 40)])
+def test_outliers_among_the_first_rows(gpu, N, C, G, B, size):
+    """Rows of many standard deviations where the kernels take what deviations
+    are measured from: the first rows, and those at the quarters.  A lane adds
+    some hundred deviations, whose roundings come as independent ones to 8 u of
+    the sum and of the squares; joins add a few u more.  32 u for the standard
+    deviation, and for the mean in units of it."""
+    from tcc_amd import training
+
+    gen = torch.Generator().manual_seed(17)
+    for rows in ([0], [0, N // 4, N // 2, 3 * N // 4], list(range(min(N // 2, 40)))):
+        x = torch.randn((B, N, C), generator=gen) + 0.5
+        x[:, rows] *= size
+        got = training.group_norm(x.cuda(), G)
+        v = x.double().view(B, N, G, C // G)
+        mean, var = v.mean((1, 3)), v.var((1, 3), unbiased=False)
+        assert bool(((got[1].double().cpu() - mean).abs() <= 32 * 2.0**-24 * (var.sqrt() + mean.abs())).all())
+        assert bool((got[2].double().cpu() * (var + 1e-5).sqrt() - 1).abs().max() <= 32 * 2.0**-24)
+
+
 def test_constant_and_non_finite_groups(gpu):
     from tcc_amd import training
 
