@@ -184,6 +184,39 @@ def test_grad_of_broadcast_and_transposed_rows(gpu):
     check_grad(training.embedding_grad(cols, ids, 30), cols, ids, 30, 1.0)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,V", [(200_000, 3000), (600_000, 400_000), (1_000_003, 70)])
+@pytest.mark.parametrize("D", [1, 4, 8, 33])
+def test_grad_of_long_lists(gpu, dtype, n, V, D):
+    """Chunks of 16 and 64 rows, with the most keys a workgroup can hold where
+    a row is one vector; hubs of many parts; accumulated too."""
+    from tcc_amd import training
+
+    gen = torch.Generator().manual_seed(n + D)
+    ids = ids_of("hubs", n, V, gen).to(torch.int32)
+    d = torch.randn((n, D), generator=gen).to(dtype).cuda()
+    got = training.embedding_grad(d, ids.cuda(), V, scale=0.5)
+    check_grad(got, d, ids, V, 0.5)
+    assert torch.equal(got, training.embedding_grad(d, ids.cuda(), V, scale=0.5))
+    base = torch.randn((V, D), generator=gen).to(dtype).cuda()
+    check_grad(training.embedding_grad(d, ids.cuda(), V, scale=0.5, grad=base.clone(), accumulate=True), d, ids, V, 0.5,
+               base=base)
+
+
+@pytest.mark.parametrize("n,D,dtype", [(700_003, 101, torch.float32), (600_001, 232, torch.bfloat16)])
+def test_lookup_past_the_caches(gpu, n, D, dtype):
+    """Outputs larger than the last level of cache (256 MB)."""
+    from tcc_amd import training
+
+    gen = torch.Generator(device="cuda").manual_seed(D)
+    table = torch.randn((5000, D), generator=gen, device="cuda").to(dtype)
+    ids = torch.randint(0, 5000, (n,), generator=gen, device="cuda")
+    got = training.embedding_lookup(table, ids, scale=0.3, padding_idx=7)
+    want = (table[ids].float() * 0.3).to(dtype)
+    want[ids == 7] = 0
+    assert torch.equal(got, want)
+
+
 def test_places_past_32_bits(gpu):
     """A table of over 2^32 elements: its last rows, and their gradient."""
     from tcc_amd import training

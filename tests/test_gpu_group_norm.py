@@ -274,6 +274,57 @@ def test_outliers_among_the_first_rows(gpu, N, C, G, B, size):
         assert bool((got[2].double().cpu() * (var + 1e-5).sqrt() - 1).abs().max() <= 32 * 2.0**-24)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("G", [1, 16, 4096])
+@pytest.mark.parametrize("first", [0, 1])
+def test_the_most_channels(gpu, dtype, G, first):
+    """4,096 channels, in rows that begin aligned and in rows that do not."""
+    from tcc_amd import training
+
+    gen, x, w, b, d = inputs(70, 4104, dtype, G + first)
+    cols = slice(first, first + 4096)
+    x, w, b, d = x[:, cols], w[cols], b[cols], d[:, cols]
+    for kind in ("one", "ragged"):
+        off, at = segments(kind, 70, gen)
+        off = None if off is None else off.cuda()
+        got = training.group_norm(x, G, w, b, offsets=off, activation="silu")
+        check_forward(got, x, G, w, b, at, 1e-5, "silu")
+        back = training.group_norm_grad(d, x, got[1], got[2], G, w, b, offsets=off, activation="silu")
+        check_grad(back, d, x, got[1], got[2], G, w, b, at, "silu")
+
+
+@pytest.mark.parametrize("tail", [300, 200_000])
+def test_places_past_32_bits(gpu, tail):
+    """4.5e9 elements: the last segment's, whole and by tiles."""
+    from tcc_amd import training
+
+    N, C, G = 1_100_000, 4096, 8
+    x, d = (torch.empty((N, C), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    x.normal_()
+    d.normal_()
+    x[N - tail:] += 2
+    cuts = [0, N - tail, N] if tail > 1000 else list(range(0, N - tail, 1000)) + [N - tail, N]
+    off = torch.tensor(cuts, device="cuda")
+    y, mean, rstd = training.group_norm(x, G, offsets=off, activation="relu", max_rows=max(np.diff(cuts)).item())
+    dx = training.group_norm_grad(d, x, mean, rstd, G, offsets=off, activation="relu", max_rows=max(np.diff(cuts)).item())[0]
+    v, xt = x[N - tail:].view(tail, G, C // G), x[N - tail:]
+    m64 = torch.stack([v[:, g].double().mean() for g in range(G)])
+    s64 = torch.stack([v[:, g].double().var(unbiased=False) for g in range(G)])
+    assert bool(((mean[-1].double() - m64).abs() <= K * 8).all())
+    assert bool((rstd[-1].double() * (s64 + 1e-5).sqrt() - 1).abs().max() <= K * 8)
+    m, r = (t[-1].view(G, 1).expand(G, C // G).reshape(C) for t in (mean, rstd))
+    xh = (xt[-200:].float() - m) * r
+    want = xh.clamp(min=0).to(torch.bfloat16)
+    assert torch.equal(y[-200:], want)
+    dz = torch.where((v.float() - mean[-1].view(1, G, 1)) * rstd[-1].view(1, G, 1) > 0, d[N - tail:].view(v.shape).float(), 0.0)
+    xv = (v.float() - mean[-1].view(1, G, 1)) * rstd[-1].view(1, G, 1)
+    s1 = dz.double().mean((0, 2)).view(G, 1).expand(G, C // G).reshape(C)
+    s2 = torch.stack([(dz[:, g].double() * xv[:, g].double()).mean() for g in range(G)]).view(G, 1).expand(G, C // G).reshape(C)
+    want = (dz[-200:].reshape(200, C).double() - s1 - xh.double() * s2) * r.double()
+    tol = 2.0**-8 * want.abs() + K * (s1.abs() + s2.abs() * xh.abs() + dz[-200:].reshape(200, C).abs() + 1) * r.double()
+    assert bool(((dx[-200:].double() - want).abs() <= tol).all())
+
+
 def test_constant_and_non_finite_groups(gpu):
     from tcc_amd import training
 
