@@ -87,7 +87,7 @@ struct NormArgs {
     std::uint32_t seenCount;  // those workgroups; 0: tiles alone
     std::uint64_t ldx, lddy, ldo, tileRows, outRows;  // rows of a tile of the sums, and of the output
     std::uint32_t C, G, K, colsV, rowLanes;  // K = C / G; colsV vectors a row, rowLanes rows at once
-    std::uint32_t paramBytes, paramType, act;
+    std::uint32_t paramType, act;
     float eps;
 };
 

@@ -29,9 +29,7 @@ except ImportError as e:
 
 _lib.lib()  # its errors are raised as _lib.TccError
 
-F32, BF16, F16 = 0, 1, 2  # TCC_F32, TCC_BF16, TCC_F16
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}  # TCC_ACT_*
-MAX_CHANNELS = 4096
 
 
 def _call(stream, f, *args):
