@@ -13,8 +13,10 @@
  * pointers are aligned to their element.  Every function is asynchronous on
  * `stream` (a hipStream_t; NULL = the null stream), allocates nothing and
  * records no memset, so that it can be captured into a HIP graph.  Sums run
- * in an order that depends on sizes alone: the same inputs give the same
- * bits.  Workspaces are device memory, 16-byte aligned, not shared with a
+ * in an order that sizes, ids, offsets, maxRows and the alignment of addresses
+ * and row strides (which decides how many elements a lane takes) fix: the same
+ * call gives the same bits, a copy at another alignment may differ in the last
+ * ones.  Workspaces are device memory, 16-byte aligned, not shared with a
  * concurrent call, with any contents.
  *
  * Errors as in tcc_swtcf.h: 0 or a TCC_ERR_* code, text in tcc_last_error().
@@ -68,7 +70,8 @@ int tcc_embedding_grad(const void* dOut, uint64_t ldd, uint32_t dtype, const voi
 /* The rows and channels of a group norm.  Segment b (a graph) holds the rows
  * offsets[b] .. offsets[b+1] (B + 1 non-decreasing device values from 0 to
  * N, int32 or int64 by offsetBytes 4 or 8), or, with offsets NULL, the N / B
- * rows from b * (N / B); a segment may be empty.  Group g of its C channels
+ * rows from b * (N / B); a segment may be empty.  Offsets are not checked, only
+ * kept within [0, N]: rows that no segment holds are not written.  Group g of its C channels
  * are the C / G from g * (C / G).  x [N x C], row stride ldx, of `dtype`;
  * weight and bias [C] of `paramDtype`, either may be NULL (ones, zeros).
  * `maxRows` is the longest segment's rows where the caller knows it (0: not
@@ -97,8 +100,8 @@ int tcc_group_norm(const tcc_group_norm_shape* s, const void* x, uint64_t ldx, c
 /* dX [N x C] (lddx) of x's type, and dWeight and dBias [C] fp32 (either may
  * be NULL), from dY [N x C] (lddy) of x's type, x and the forward's mean and
  * rstd.  z is formed with the forward's roundings, so that relu's mask is
- * that of the forward's output; what it masks counts as 0, infinities and
- * NaN too. */
+ * that of the forward's z (an fp16 output may round to 0 where z does not);
+ * what it masks counts as 0, infinities and NaN too. */
 int tcc_group_norm_grad(const tcc_group_norm_shape* s, const void* dY, uint64_t lddy, const void* x, uint64_t ldx,
                         const float* mean, const float* rstd, const void* weight, const void* bias, void* dX,
                         uint64_t lddx, float* dWeight, float* dBias, void* workspace, size_t workspaceBytes,

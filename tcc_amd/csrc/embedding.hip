@@ -5,20 +5,26 @@
 //
 // Both move bytes and compute next to nothing.  The lookup is bound by the
 // lines of 128 bytes that its rows lie in: 2.45M rows of 100 bf16 from a table
-// of as many take 243 us, 735 MB of ids, rows and output (3.0 TB/s) or 1.09 GB
-// with the lines that two rows share (4.5).
+// of as many take 243 us, 735 MB of ids, distinct rows and output (3.0 TB/s), or
+// 1.17 GB past the L2 by the counters (4.8 TB/s).  A lane takes what the rows'
+// alignment allows, so that odd widths go element by element: 101 columns take
+// 539 us, 102 take 353 (fp32: 318 for 100 columns, 727 and 481), and their
+// gradients 770 and 389 where 100 columns take 396 (fp32: 622, 951, 616).
 //
 // The gradient sorts the ids with their positions (stable, so that a row's
 // terms have one order and the sums the same bits every time), then walks the
 // sorted positions in chunks of equal length, whatever the ids' frequencies:
 // a hub node with thousands of rows is spread over as many chunks as it needs,
-// and its parts are joined afterwards in chunk order.  Atomics on the rows
+// and its parts are joined afterwards in chunk order (by one workgroup for each
+// hub: 2.45M rows of 100 fp32 take 665 us with a tenth of them in one, 950 with
+// all of them).  Atomics on the rows
 // would spare the sort, but add in no fixed order and round every partial sum
 // of a bf16 row.  A few rows need no sort (few_grad_kernel), up to 65,536 one
 // of a launch for each 11 bits of the rows (pass_kernel), the others passes of
-// 8 bits and three launches: 2.45M rows of 100 fp32 into as many take 595 us,
-// of which the sums are 488 (1.96 GB, 4.0 TB/s: rows of 400 bytes in the sorted
-// order are read at random and share lines), the sort 90 and the parts 20.
+// 8 bits and three launches: 2.45M rows of 100 fp32 into as many take 600 us,
+// of which the sums are 486 (1.96 GB, 4.0 TB/s: rows of 400 bytes in the sorted
+// order are read at random and share lines), the sort 95, the parts 20 and the
+// windows' marks 5.
 #include <algorithm>
 
 #include "../../include/tcc_spmm_cnic.h"
@@ -301,7 +307,9 @@ __device__ __forceinline__ void zero_between(const GradArgs& a, std::uint32_t q,
 }
 
 // A team of 2^laneBits lanes sums one chunk of the sorted rows, the block's
-// keys in LDS.
+// keys in LDS: 128 KB of them, one workgroup a CU, where a row is one vector and a
+// chunk 64 rows (600,000 rows into 400,000 take 138 us with 4 fp32 columns, 111
+// with 8 and 101 with 16).
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads) grad_kernel(GradArgs a) {
     extern __shared__ std::uint64_t ldsKeys[];
@@ -487,7 +495,10 @@ __global__ void __launch_bounds__(kThreads) join_kernel(GradArgs a) {
 // comparisons, which a few thousand rows spread over the GPU need less time for
 // than a sort's launches follow each other in: rows of 32 fp32 into 1,500 (and
 // 70,000) take 6 us (7) for 1,000 of them, 14 (16) for 3,000 and 26 (27) for
-// 4,000, sorted 15 (29) for any of these.
+// 4,000, sorted 15 (29) for any of these.  One wave adds all rows of an id here,
+// column by column, so that a hub is not spread: 3,000 rows of one id take 38, 108
+// and 1,573 us for 32, 128 and 602 fp32 columns (sorted 20, 22 and 85), where
+// 1,500 ids take 14, 14 and 16 (sorted 15, 14 and 22).
 constexpr std::uint64_t kFewRows = 3000;
 constexpr std::uint64_t kFewTableRows = 1ull << 31;  // so that those that zero stay far below 2^32 threads
 constexpr std::uint32_t kFewZeroRows = 256;  // rows of a workgroup that zeroes, at most

@@ -22,12 +22,13 @@
 // two moves on at every step, so the slots of all pairs are distinct and those
 // of a segment are consecutive.
 //
-// What bounds it: memory.  One segment of 2.45M x 256 fp32 rows takes 1,250 us
-// forward (7.5 GB, 6.0 TB/s: the statistics 390, the output 845) and 2,000 us
-// backward (12.5 GB, 6.2 TB/s: the sums 735, dx 1,265).  2,000 ragged graphs of
-// 169,000 x 128 bf16 rows together, 130 MB, take 85 us backward with gelu: 63
-// in the whole segments' kernel, half of it vector instructions, and 22 in
-// dWeight's and the three empty launches.
+// What bounds it: memory.  One segment of 2.45M x 256 fp32 rows takes 1,240 us
+// forward (7.5 GB, 6.1 TB/s: the statistics 385, the output 852) and 2,000 us
+// backward (12.5 GB, 6.2 TB/s: the sums 731, dx 1,292); bf16 rows 690 and 1,140
+// (3.8 and 6.3 GB, 5.5 TB/s).  2,000 ragged graphs of 169,000 x 128 bf16 rows
+// together, 130 MB, take 82 us backward with gelu: 61 in the whole segments'
+// kernel, half of it vector instructions, 8 in dWeight's and 14 in three empty
+// launches, which a caller who knows the longest graph is spared.
 #include <algorithm>
 
 #include "../../include/tcc_swtcf.h"
@@ -295,7 +296,7 @@ __device__ __forceinline__ bool shift_is_far(float count, float shift, float sum
 
 // The mean and squared deviations of each segment's rows in a tile, group by
 // group, first channel by channel for a lane's rows; a mean of every batch,
-// joined, instead of one shift, took 2.45M x 256 bf16 rows 394 us, not 205.
+// joined, instead of one shift, took 2.45M x 256 bf16 rows 394 us, not 217.
 template <typename T, int N>
 __global__ void __launch_bounds__(kThreads, 4) stats_kernel(NormArgs a) {
     if (!tiles_needed(a.seen, a.seenCount)) return;

@@ -10,8 +10,10 @@ learned node rows trains with.
 Tensors are fp32, bf16 or fp16 on the current device; sums, statistics and
 moments are fp32 or wider inside, and outputs are rounded once.  All work runs
 on torch's current stream or on `stream`, whose pool the outputs and
-workspaces then come from; nothing synchronises.  Tensors of another type or
-place raise TypeError, sizes and strides that no call takes ValueError.  The
+workspaces then come from; nothing synchronises, and a caller who passes
+`stream` has it wait for the inputs and keeps them until it is done.  What a
+call writes in place has a new version for autograd.  Tensors of another type
+or place raise TypeError, sizes and strides that no call takes ValueError.  The
 autograd nodes, modules and the model over these are in tcc_amd.gcn; the
 checks and calls are in csrc/training_ext.cpp.
 """
@@ -73,8 +75,9 @@ def group_norm(x: torch.Tensor, num_groups: int, weight: torch.Tensor | None = N
     """(y, mean, rstd) of act(group_norm(x)), channels last (tcc_group_norm).
 
     x [N x C] holds the node rows of a batch of graphs: segment b is the rows
-    offsets[b] .. offsets[b+1] (int32 or int64, from 0 to N, never falling;
-    empty segments allowed); without offsets all rows are one segment.  x
+    offsets[b] .. offsets[b+1] (int32 or int64, from 0 to N, never falling,
+    which is not checked: rows outside all segments are not written; empty
+    segments allowed); without offsets all rows are one segment.  x
     [B x ... x C] holds B segments of the same size.  Statistics run over a
     segment's rows and the channels of each of `num_groups` groups; mean and
     rstd are [B x G] fp32.  `weight` and `bias` [C] are of any one of the
