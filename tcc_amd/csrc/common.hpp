@@ -34,6 +34,17 @@ void clear_last_error();
 
 #define TCC_LAUNCH_CHECK() TCC_HIP_CHECK(hipGetLastError())
 
+// The grid, or none where the launch would have 2^32 threads or more in a
+// dimension: HIP runs the remainder of those and reports no error, while a launch
+// without a grid leaves hipErrorInvalidConfiguration for the check after it.
+inline dim3 launch_grid(dim3 grid, dim3 block) {
+    const auto fits = [](std::uint64_t g, std::uint64_t b) { return g * b <= 0xFFFFFFFFull; };
+    return fits(grid.x, block.x) && fits(grid.y, block.y) && fits(grid.z, block.z) ? grid : dim3(0, 0, 0);
+}
+#undef hipLaunchKernelGGL
+#define hipLaunchKernelGGL(kernel, grid, block, lds, stream, ...) \
+    kernel<<<::tcc::launch_grid((grid), (block)), (block), (lds), (stream)>>>(__VA_ARGS__)
+
 inline hipStream_t as_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
 constexpr int kWave = 64;
