@@ -389,10 +389,10 @@ class ClippedAdam(torch.optim.Optimizer):
     `max_norm` as the update reads them (tcc_amd.training.adam_step): step()
     leaves the gradients as they are and returns their norm, a device scalar
     (None without max_norm).  step(closure) returns the closure's loss, as
-    torch's optimizers do; the norm is in `norm` after either.  Steps are counted for each parameter, from its
-    first gradient on; where the counts differ, the clipped gradients are
-    written once, in their type, for an update a count.  Nothing
-    synchronises."""
+    torch's optimizers do; the norm is in `norm` after either.  Steps are
+    counted for each parameter, from its first gradient on; where the counts
+    differ, the clipped gradients are written once, in their type, for an
+    update a count.  Nothing synchronises but load_state_dict."""
 
     norm = None
 
@@ -476,7 +476,7 @@ class ClippedAdam(torch.optim.Optimizer):
                 state["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32)
             ages.setdefault(id(state["step"]), []).append(p)
         here = set(params)
-        left = {id(s["step"]) for p, s in self.state.items() if p not in here}
+        left = {id(s["step"]) for p, s in self.state.items() if s and p not in here}
         for count, some in ages.items():
             if count in left:
                 own = self.state[some[0]]["step"].clone()

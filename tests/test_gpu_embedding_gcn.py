@@ -165,6 +165,7 @@ def test_optimizer_counts_steps_for_each_parameter(gpu, max_norm):
     twin = [torch.nn.Parameter(p.detach().clone()) for p in mine]
     a = gcn.ClippedAdam(mine, lr=0.02, weight_decay=0.1, max_norm=max_norm)
     b = torch.optim.AdamW(twin, lr=0.02, weight_decay=0.1)
+    assert not a.state[mine[3]]  # a look at a state that is not there yet changes nothing
     for k in range(9):
         for i, (p, q) in enumerate(zip(mine, twin)):
             p.grad = q.grad = None
