@@ -107,6 +107,44 @@ int tcc_group_norm_grad(const tcc_group_norm_shape* s, const void* dY, uint64_t 
                         uint64_t lddx, float* dWeight, float* dBias, void* workspace, size_t workspaceBytes,
                         void* stream);
 
+/* -------------------------------------------------------------- layer norm */
+
+/* The rows of a layer norm: x [N x C] of `dtype`, weight and bias [C] of
+ * `paramDtype`, either may be NULL (ones, zeros).  C <= 16384, N below 2^40
+ * (TCC_ERR_UNSUPPORTED above).  Row addresses need only be aligned to their
+ * element, and no result depends on them. */
+typedef struct tcc_layer_norm_shape {
+    uint64_t N;
+    uint32_t C;
+    uint32_t dtype, paramDtype, activation;
+    float eps;
+} tcc_layer_norm_shape;
+
+/* y = act(z), z = ((h - mean) * rstd) * weight + bias, of h = x + residual
+ * (rounded to x's type; h = x where residual is NULL), with mean and
+ * rstd = 1 / sqrt(var + eps) over the channels of each row.  residual, y and
+ * sum of x's type, row strides ldr, ldy and lds; h is written to `sum` unless
+ * that is NULL.  mean and rstd [N] fp32, for the gradient.  Outputs overlap no
+ * input. */
+int tcc_layer_norm(const tcc_layer_norm_shape* s, const void* x, uint64_t ldx, const void* residual, uint64_t ldr,
+                   const void* weight, const void* bias, void* y, uint64_t ldy, void* sum, uint64_t lds, float* mean,
+                   float* rstd, void* stream);
+
+/* Bytes of workspace for dWeight or dBias on the current device. */
+size_t tcc_layer_norm_grad_workspace_bytes(const tcc_layer_norm_shape* s);
+
+/* dX [N x C] (lddx) of x's type, the gradient of x and of residual alike, and
+ * dWeight and dBias [C] fp32 (either may be NULL; without both no workspace is
+ * needed), from dY [N x C] (lddy), h (ldh) and the forward's mean and rstd.
+ * dSum [N x C] (ldds), if not NULL, is the gradient that h has from elsewhere:
+ * it is added to dX before that is rounded.  z is formed with the forward's
+ * roundings, so that relu masks what the forward masked; what it masks counts
+ * as 0, infinities and NaN too. */
+int tcc_layer_norm_grad(const tcc_layer_norm_shape* s, const void* dY, uint64_t lddy, const void* h, uint64_t ldh,
+                        const float* mean, const float* rstd, const void* weight, const void* bias, const void* dSum,
+                        uint64_t ldds, void* dX, uint64_t lddx, float* dWeight, float* dBias, void* workspace,
+                        size_t workspaceBytes, void* stream);
+
 /* ------------------------------------------------ gradient norm, clip, Adam */
 
 /* One tensor of a list, as rows of `cols` elements `ld` apart (a tensor that

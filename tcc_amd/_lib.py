@@ -89,6 +89,11 @@ class GroupNormShape(ctypes.Structure):
     ]
 
 
+class LayerNormShape(ctypes.Structure):
+    """tcc_layer_norm_shape."""
+    _fields_ = [("N", u64), ("C", u32), ("dtype", u32), ("paramDtype", u32), ("activation", u32), ("eps", ctypes.c_float)]
+
+
 class Adam(ctypes.Structure):
     """tcc_adam."""
     _fields_ = [
@@ -168,6 +173,11 @@ SIGNATURES = {
                                       ctypes.c_size_t, vp]),
     "tcc_group_norm_grad": (ctypes.c_int, [ctypes.POINTER(GroupNormShape), vp, u64, vp, u64, vp, vp, vp, vp, vp, u64,
                                            vp, vp, vp, ctypes.c_size_t, vp]),
+    "tcc_layer_norm": (ctypes.c_int, [ctypes.POINTER(LayerNormShape), vp, u64, vp, u64, vp, vp, vp, u64, vp, u64, vp, vp,
+                                      vp]),
+    "tcc_layer_norm_grad_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(LayerNormShape)]),
+    "tcc_layer_norm_grad": (ctypes.c_int, [ctypes.POINTER(LayerNormShape), vp, u64, vp, u64, vp, vp, vp, vp, vp, u64, vp,
+                                           u64, vp, vp, vp, ctypes.c_size_t, vp]),
     "tcc_grad_norm_workspace_bytes": (ctypes.c_size_t, []),
     "tcc_grad_norm": (ctypes.c_int, [vp, u32, vp, vp, ctypes.c_size_t, vp]),
     "tcc_clip_grad_norm": (ctypes.c_int, [vp, vp, u32, ctypes.c_float, vp, vp, ctypes.c_size_t, vp]),

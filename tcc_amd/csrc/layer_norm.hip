@@ -1,0 +1,451 @@
+// Layer norm of node rows with the sum before it and the activation after it
+// (include/tcc_training.h).
+//
+//   h = x + residual (rounded to x's type), over the C channels of a row:
+//   mean = sum h / C,  rstd = 1 / sqrt(sum (h - mean)^2 / C + eps)
+//   z = ((h - mean) * rstd) * weight + bias,  y = act(z)
+//
+// and with dz = dY act'(z), xh = (h - mean) rstd, a = dz weight:
+//   dBias = sum dz,  dWeight = sum dz xh  over the rows
+//   dX = rstd (a - (sum a + xh sum a xh) / C) + dSum
+//
+// A team of lanes holds a row in registers, so that memory is read once: 16
+// bytes a lane at a time, whatever the alignment (the last vector of a row that
+// does not divide into them is moved back to end with it; what it shares with
+// the one before counts once in every sum, and is written twice with the same
+// value).  Teams are as small as 16 elements a lane allow, which saves
+// reductions, at least four lanes, at most the 1,024 threads of a workgroup.
+// The mean is taken twice, the second time of the differences from the first:
+// what the first lost to rows far from zero comes back, and the sums of both
+// need one reduction.
+//
+// The gradient's teams walk the rows in equal steps and keep the sums of dz and
+// dz xh of their channels in registers; a workgroup adds its teams' in LDS and
+// writes one row, and a second kernel adds the rows in 64 bits.
+#include <algorithm>
+
+#include "../../include/tcc_swtcf.h"
+#include "../../include/tcc_training.h"
+#include "activations.hpp"
+#include "row_types.hpp"
+#include "teams.hpp"
+
+namespace tcc {
+namespace {
+
+constexpr std::uint32_t kMaxChannels = 16384;
+
+struct Args {
+    const void *x, *residual, *dy, *dSum, *weight, *bias;
+    void *out, *sum;  // y or dx, h
+    float *mean, *rstd, *part;  // part: [workgroups][2][C], dBias and dWeight
+    std::uint64_t N, ldx, ldr, lddy, ldds, ldo, lds;
+    std::uint32_t C, paramType, act;
+    float eps;
+};
+
+template <int TEAM>
+constexpr int kThreads = TEAM > 256 ? TEAM : 256;
+template <int TEAM>
+constexpr int kTeams = kThreads<TEAM> / TEAM;  // of a workgroup
+
+// The channels that a lane holds of every row: E vectors of V.
+template <int V, int E, int TEAM>
+struct Columns {
+    std::uint32_t c[E];     // first channel
+    std::uint32_t skip[E];  // elements that are another vector's (all: no vector)
+    __device__ __forceinline__ explicit Columns(std::uint32_t C) {
+        const std::uint32_t lane = threadIdx.x % TEAM;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const std::uint32_t at = (lane + e * TEAM) * V;
+            c[e] = min(at, C - V);
+            skip[e] = min(at - c[e], static_cast<std::uint32_t>(V));
+        }
+    }
+    __device__ __forceinline__ bool any(int e) const { return skip[e] < V; }
+    // v with 0 where another vector counts.
+    __device__ __forceinline__ vec_t<float, V> own(int e, vec_t<float, V> v) const {
+        if (skip[e] != 0) {
+#pragma unroll
+            for (int q = 0; q < V; ++q) v[q] = static_cast<std::uint32_t>(q) < skip[e] ? 0.0f : v[q];
+        }
+        return v;
+    }
+};
+
+template <std::uint32_t ACT, bool FINE, int N>
+__device__ __forceinline__ vec_t<float, N> activate_all(vec_t<float, N> z) {
+#pragma unroll
+    for (int q = 0; q < N; ++q) z[q] = activate<ACT, FINE>(z[q]);
+    return z;
+}
+template <bool FINE, int N>
+__device__ __forceinline__ vec_t<float, N> activate_by(std::uint32_t act, vec_t<float, N> z) {
+    if (act == TCC_ACT_NONE) return z;
+    if (act == TCC_ACT_RELU) return activate_all<TCC_ACT_RELU, FINE, N>(z);
+    if (act == TCC_ACT_SILU) return activate_all<TCC_ACT_SILU, FINE, N>(z);
+    return activate_all<TCC_ACT_GELU, FINE, N>(z);
+}
+template <std::uint32_t ACT, bool FINE, int N>
+__device__ __forceinline__ vec_t<float, N> through_all(vec_t<float, N> d, vec_t<float, N> z) {
+#pragma unroll
+    for (int q = 0; q < N; ++q) d[q] = through<ACT, FINE>(d[q], z[q]);
+    return d;
+}
+template <bool FINE, int N>
+__device__ __forceinline__ vec_t<float, N> through_by(std::uint32_t act, vec_t<float, N> d, vec_t<float, N> z) {
+    if (act == TCC_ACT_NONE) return d;
+    if (act == TCC_ACT_RELU) return through_all<TCC_ACT_RELU, FINE, N>(d, z);
+    if (act == TCC_ACT_SILU) return through_all<TCC_ACT_SILU, FINE, N>(d, z);
+    return through_all<TCC_ACT_GELU, FINE, N>(d, z);
+}
+
+// Rounded to T, as memory holds it.
+template <typename T, int N>
+__device__ __forceinline__ vec_t<float, N> rounded(vec_t<float, N> v) {
+    return __builtin_convertvector(__builtin_convertvector(v, vec_t<T, N>), vec_t<float, N>);
+}
+
+template <typename T, int V, int E, int TEAM>
+__global__ void __launch_bounds__(kThreads<TEAM>) forward_kernel(Args a) {
+    using F = vec_t<float, V>;
+    __shared__ typename TeamSum<TEAM>::Shared shared;
+    TeamSum<TEAM> sum(shared);
+    const Columns<V, E, TEAM> cols(a.C);
+    F w[E], b[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        if (!cols.any(e)) continue;
+        w[e] = load_params<V>(a.weight, a.paramType, cols.c[e], 1.0f);
+        b[e] = load_params<V>(a.bias, a.paramType, cols.c[e], 0.0f);
+    }
+    const float perC = 1.0f / static_cast<float>(a.C);
+    const std::uint64_t step = static_cast<std::uint64_t>(gridDim.x) * kTeams<TEAM>;
+    for (std::uint64_t r = static_cast<std::uint64_t>(blockIdx.x) * kTeams<TEAM> + threadIdx.x / TEAM; r < a.N; r += step) {
+        const T* x = static_cast<const T*>(a.x) + r * a.ldx;
+        F h[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) h[e] = cols.any(e) ? load_any<T, V>(x + cols.c[e]) : F(0.0f);
+        if (a.residual != nullptr) {
+            const T* res = static_cast<const T*>(a.residual) + r * a.ldr;
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (cols.any(e)) h[e] = rounded<T, V>(h[e] + load_any<T, V>(res + cols.c[e]));
+        }
+        float total = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const F own = cols.own(e, h[e]);
+#pragma unroll
+            for (int q = 0; q < V; ++q) total += own[q];
+        }
+        const float first = sum(total, 0.0f).x * perC;
+        float left = 0.0f, squares = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const F d = cols.own(e, h[e] - first);
+#pragma unroll
+            for (int q = 0; q < V; ++q) {
+                left += d[q];
+                squares = fmaf(d[q], d[q], squares);
+            }
+        }
+        const float2 both = sum(left, squares);
+        const float shift = both.x * perC, mean = first + shift;
+        const float var = fmaf(-shift, shift, both.y * perC);
+        const float rstd = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + a.eps);  // keeps NaN
+        T* y = static_cast<T*>(a.out) + r * a.ldo;
+        T* s = static_cast<T*>(a.sum) + r * a.lds;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            if (!cols.any(e)) continue;
+            if (a.sum != nullptr) store_any<T, V>(s + cols.c[e], h[e]);
+            F z;
+#pragma unroll
+            for (int q = 0; q < V; ++q) z[q] = affine(normalise(h[e][q], mean, rstd), w[e][q], b[e][q]);
+            store_any<T, V>(y + cols.c[e], activate_by<kFine<T>, V>(a.act, z));
+        }
+        if (threadIdx.x % TEAM == 0) {
+            a.mean[r] = mean;
+            a.rstd[r] = rstd;
+        }
+    }
+}
+
+template <typename T, int V, int E, int TEAM>
+__global__ void __launch_bounds__(kThreads<TEAM>) grad_kernel(Args a) {
+    using F = vec_t<float, V>;
+    __shared__ typename TeamSum<TEAM>::Shared shared;
+    TeamSum<TEAM> sum(shared);
+    const Columns<V, E, TEAM> cols(a.C);
+    F w[E], b[E], dw[E], db[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        dw[e] = db[e] = F(0.0f);
+        if (!cols.any(e)) continue;
+        w[e] = load_params<V>(a.weight, a.paramType, cols.c[e], 1.0f);
+        b[e] = load_params<V>(a.bias, a.paramType, cols.c[e], 0.0f);
+    }
+    const float perC = 1.0f / static_cast<float>(a.C);
+    const std::uint64_t step = static_cast<std::uint64_t>(gridDim.x) * kTeams<TEAM>;
+    for (std::uint64_t r = static_cast<std::uint64_t>(blockIdx.x) * kTeams<TEAM> + threadIdx.x / TEAM; r < a.N; r += step) {
+        const T* x = static_cast<const T*>(a.x) + r * a.ldx;
+        const T* dy = static_cast<const T*>(a.dy) + r * a.lddy;
+        F xh[E], dz[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            xh[e] = cols.any(e) ? load_any<T, V>(x + cols.c[e]) : F(0.0f);
+            dz[e] = cols.any(e) ? load_any<T, V>(dy + cols.c[e]) : F(0.0f);
+        }
+        const float mean = a.mean[r], rstd = a.rstd[r];
+        float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            if (!cols.any(e)) continue;
+            F z;
+#pragma unroll
+            for (int q = 0; q < V; ++q) {
+                xh[e][q] = normalise(xh[e][q], mean, rstd);
+                z[q] = affine(xh[e][q], w[e][q], b[e][q]);
+            }
+            dz[e] = through_by<kFine<T>, V>(a.act, dz[e], z);
+            const F d = cols.own(e, dz[e]);
+            db[e] += d;
+#pragma unroll
+            for (int q = 0; q < V; ++q) {
+                const float dx = d[q] * xh[e][q];
+                dw[e][q] += dx;
+                s1 = fmaf(d[q], w[e][q], s1);
+                s2 = fmaf(dx, w[e][q], s2);
+            }
+        }
+        const float2 both = sum(s1, s2);
+        const float m1 = both.x * perC, m2 = both.y * perC;
+        T* out = static_cast<T*>(a.out) + r * a.ldo;
+        const T* add = static_cast<const T*>(a.dSum) + r * a.ldds;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            if (!cols.any(e)) continue;
+            F v;
+#pragma unroll
+            for (int q = 0; q < V; ++q) v[q] = rstd * (fmaf(dz[e][q], w[e][q], -m1) - xh[e][q] * m2);
+            if (a.dSum != nullptr) v += load_any<T, V>(add + cols.c[e]);
+            store_any<T, V>(out + cols.c[e], v);
+        }
+    }
+    if (a.part == nullptr) return;
+    // the workgroup's sums: its teams', one after the other
+    float* to = a.part + static_cast<std::uint64_t>(blockIdx.x) * 2 * a.C;
+    if constexpr (kTeams<TEAM> == 1) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+            for (int q = 0; q < V; ++q)
+                if (static_cast<std::uint32_t>(q) >= cols.skip[e]) {
+                    to[cols.c[e] + q] = db[e][q];
+                    to[a.C + cols.c[e] + q] = dw[e][q];
+                }
+    } else {
+        __shared__ float total[2][TEAM * E * V];
+        for (int k = 0; k < kTeams<TEAM>; ++k) {
+            if (threadIdx.x / TEAM == k) {
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+#pragma unroll
+                    for (int q = 0; q < V; ++q)
+                        if (static_cast<std::uint32_t>(q) >= cols.skip[e]) {
+                            const std::uint32_t c = cols.c[e] + q;
+                            total[0][c] = k == 0 ? db[e][q] : total[0][c] + db[e][q];
+                            total[1][c] = k == 0 ? dw[e][q] : total[1][c] + dw[e][q];
+                        }
+            }
+            __syncthreads();
+        }
+        for (std::uint32_t i = threadIdx.x; i < 2 * a.C; i += kThreads<TEAM>)
+            to[i] = i < a.C ? total[0][i] : total[1][i - a.C];
+    }
+}
+
+// dBias and dWeight: the workgroups' sums added in 64 bits, kParamCols columns a
+// workgroup.
+constexpr std::uint32_t kParamCols = 8, kParamRows = 32;
+__global__ void __launch_bounds__(kParamCols* kParamRows) params_kernel(const float* part, std::uint32_t parts,
+                                                                        std::uint32_t C, float* dBias, float* dWeight) {
+    const std::uint32_t i = blockIdx.x * kParamCols + threadIdx.x % kParamCols, first = threadIdx.x / kParamCols;
+    double v = 0.0;
+    if (i < 2 * C)
+        for (std::uint32_t p = first; p < parts; p += kParamRows) v += part[static_cast<std::uint64_t>(p) * 2 * C + i];
+    __shared__ double all[kParamRows][kParamCols];
+    all[first][threadIdx.x % kParamCols] = v;
+    __syncthreads();
+    if (first != 0 || i >= 2 * C) return;
+    for (std::uint32_t k = 1; k < kParamRows; ++k) v += all[k][threadIdx.x];
+    float* to = i < C ? dBias : dWeight;
+    if (to != nullptr) to[i < C ? i : i - C] = static_cast<float>(v);
+}
+
+// ---------------------------------------------------------------- launches
+
+// Teams for rows of C elements; f is called with their <V, E, TEAM>.  Sixteen
+// elements a lane at most.
+template <typename T, typename F>
+void with_team(std::uint32_t C, F f) {
+    constexpr int V = kVec<T>, most = 16 / V;
+    const auto fits = [&](std::uint64_t team, std::uint64_t e) { return C <= team * e * V; };
+    if (C < V) return f.template operator()<1, 2, 4>();
+    if (fits(4, 1)) return f.template operator()<V, 1, 4>();
+    if (fits(16, 1)) return f.template operator()<V, 1, 16>();
+    if (fits(16, 2)) return f.template operator()<V, 2, 16>();
+    if constexpr (most == 4) {
+        if (fits(16, 4)) return f.template operator()<V, 4, 16>();
+    }
+    if (fits(64, 1)) return f.template operator()<V, 1, 64>();
+    if (fits(64, 2)) return f.template operator()<V, 2, 64>();
+    if constexpr (most == 4) {
+        if (fits(64, 4)) return f.template operator()<V, 4, 64>();
+    }
+    if (fits(256, 1)) return f.template operator()<V, 1, 256>();
+    if (fits(256, 2)) return f.template operator()<V, 2, 256>();
+    return f.template operator()<V, most, 1024>();
+}
+
+// Workgroups of the gradient: eight a compute unit, as many rows each.
+std::uint64_t grad_blocks(std::uint64_t N, std::uint64_t rows) {
+    return std::min<std::uint64_t>((N + rows - 1) / rows, 8ull * device_cus());
+}
+
+template <typename T>
+struct Forward {
+    const Args& a;
+    hipStream_t st;
+    template <int V, int E, int TEAM>
+    void operator()() const {
+            // four rows a team where there are plenty, for one reading of the parameters
+        const std::uint64_t all = (a.N + kTeams<TEAM> - 1) / kTeams<TEAM>;
+        const std::uint64_t blocks = std::min<std::uint64_t>(std::min<std::uint64_t>(all, std::max<std::uint64_t>(all / 4, 2048)), 1u << 21);
+        hipLaunchKernelGGL((forward_kernel<T, V, E, TEAM>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads<TEAM>), 0, st, a);
+    }
+};
+template <typename T>
+struct Backward {
+    const Args& a;
+    hipStream_t st;
+    std::uint64_t& blocks;
+    template <int V, int E, int TEAM>
+    void operator()() const {
+            blocks = grad_blocks(a.N, kTeams<TEAM>);
+        hipLaunchKernelGGL((grad_kernel<T, V, E, TEAM>), dim3(static_cast<unsigned>(blocks)), dim3(kThreads<TEAM>), 0, st, a);
+    }
+};
+
+int check_shape(const tcc_layer_norm_shape* s) {
+    TCC_REQUIRE(s != nullptr, TCC_ERR_INVALID_ARGUMENT, "layer norm: no shape");
+    TCC_REQUIRE(s->C >= 1, TCC_ERR_INVALID_ARGUMENT, "layer norm: rows have channels");
+    TCC_REQUIRE(dtype_bytes(s->dtype) != 0 && dtype_bytes(s->paramDtype) != 0, TCC_ERR_INVALID_ARGUMENT,
+                "layer norm: unknown element type");
+    TCC_REQUIRE(s->activation <= TCC_ACT_GELU, TCC_ERR_INVALID_ARGUMENT, "layer norm: unknown activation");
+    TCC_REQUIRE(s->eps >= 0.0f, TCC_ERR_INVALID_ARGUMENT, "layer norm: eps is not negative");
+    TCC_REQUIRE(s->C <= kMaxChannels, TCC_ERR_UNSUPPORTED, "layer norm: at most 16384 channels");
+    TCC_REQUIRE(s->N < (1ull << 40), TCC_ERR_UNSUPPORTED, "layer norm: fewer than 2^40 rows");
+    return TCC_OK;
+}
+
+Args args_of(const tcc_layer_norm_shape& s) {
+    Args a{};
+    a.N = s.N;
+    a.C = s.C;
+    a.paramType = s.paramDtype;
+    a.act = s.activation;
+    a.eps = s.eps;
+    return a;
+}
+
+template <template <typename> class Launch, typename... More>
+void launch_typed(std::uint32_t dtype, const Args& a, hipStream_t st, More&... more) {
+    if (dtype == TCC_F32) with_team<float>(a.C, Launch<float>{a, st, more...});
+    else if (dtype == TCC_BF16) with_team<bf16_t>(a.C, Launch<bf16_t>{a, st, more...});
+    else with_team<f16_t>(a.C, Launch<f16_t>{a, st, more...});
+}
+
+}  // namespace
+}  // namespace tcc
+
+extern "C" int tcc_layer_norm(const tcc_layer_norm_shape* s, const void* x, uint64_t ldx, const void* residual,
+                              uint64_t ldr, const void* weight, const void* bias, void* y, uint64_t ldy, void* sum,
+                              uint64_t lds, float* mean, float* rstd, void* stream) {
+    using namespace tcc;
+    clear_last_error();
+    if (const int rc = check_shape(s)) return rc;
+    if (s->N == 0) return TCC_OK;
+    TCC_REQUIRE(x != nullptr && y != nullptr && mean != nullptr && rstd != nullptr, TCC_ERR_INVALID_ARGUMENT,
+                "layer norm: a null pointer");
+    TCC_REQUIRE(ldx >= s->C && ldy >= s->C && (residual == nullptr || ldr >= s->C) && (sum == nullptr || lds >= s->C),
+                TCC_ERR_INVALID_ARGUMENT, "layer norm: a row stride below the channels");
+    Args a = args_of(*s);
+    a.x = x;
+    a.ldx = ldx;
+    a.residual = residual;
+    a.ldr = ldr;
+    a.weight = weight;
+    a.bias = bias;
+    a.out = y;
+    a.ldo = ldy;
+    a.sum = sum;
+    a.lds = lds;
+    a.mean = mean;
+    a.rstd = rstd;
+    launch_typed<Forward>(s->dtype, a, as_stream(stream));
+    TCC_LAUNCH_CHECK();
+    return TCC_OK;
+}
+
+extern "C" size_t tcc_layer_norm_grad_workspace_bytes(const tcc_layer_norm_shape* s) {
+    using namespace tcc;
+    if (check_shape(s) != TCC_OK) return 0;
+    // the most workgroups of any team, which has one row or more
+    return grad_blocks(s->N, 1) * 2 * s->C * sizeof(float);
+}
+
+extern "C" int tcc_layer_norm_grad(const tcc_layer_norm_shape* s, const void* dY, uint64_t lddy, const void* h,
+                                   uint64_t ldh, const float* mean, const float* rstd, const void* weight,
+                                   const void* bias, const void* dSum, uint64_t ldds, void* dX, uint64_t lddx,
+                                   float* dWeight, float* dBias, void* workspace, size_t workspaceBytes, void* stream) {
+    using namespace tcc;
+    clear_last_error();
+    if (const int rc = check_shape(s)) return rc;
+    TCC_REQUIRE(s->N == 0 || (dY != nullptr && h != nullptr && dX != nullptr && mean != nullptr && rstd != nullptr),
+                TCC_ERR_INVALID_ARGUMENT, "layer norm gradient: a null pointer");
+    TCC_REQUIRE(lddy >= s->C && ldh >= s->C && lddx >= s->C && (dSum == nullptr || ldds >= s->C),
+                TCC_ERR_INVALID_ARGUMENT, "layer norm gradient: a row stride below the channels");
+    const bool params = dWeight != nullptr || dBias != nullptr;
+    TCC_REQUIRE(!params || s->N == 0 ||
+                    (workspace != nullptr && (reinterpret_cast<std::uintptr_t>(workspace) & 15) == 0 &&
+                     workspaceBytes >= tcc_layer_norm_grad_workspace_bytes(s)),
+                TCC_ERR_INVALID_ARGUMENT, "layer norm gradient: the workspace is too small or not 16-byte aligned");
+    Args a = args_of(*s);
+    a.dy = dY;
+    a.lddy = lddy;
+    a.x = h;
+    a.ldx = ldh;
+    a.mean = const_cast<float*>(mean);
+    a.rstd = const_cast<float*>(rstd);
+    a.weight = weight;
+    a.bias = bias;
+    a.dSum = dSum;
+    a.ldds = ldds;
+    a.out = dX;
+    a.ldo = lddx;
+    a.part = params ? static_cast<float*>(workspace) : nullptr;
+    std::uint64_t blocks = 0;
+    if (s->N > 0) {
+        launch_typed<Backward>(s->dtype, a, as_stream(stream), blocks);
+        TCC_LAUNCH_CHECK();
+    }
+    if (params) {
+        hipLaunchKernelGGL(params_kernel, dim3(grid_for(2ull * s->C, kParamCols)), dim3(kParamCols * kParamRows), 0,
+                           as_stream(stream), a.part, static_cast<std::uint32_t>(blocks), s->C, dBias, dWeight);
+        TCC_LAUNCH_CHECK();
+    }
+    return TCC_OK;
+}

@@ -318,6 +318,97 @@ std::tuple<Tensor, MaybeTensor, MaybeTensor> group_norm_grad(const Tensor& dy, c
     return {dx, dw, db};
 }
 
+// ---------------------------------------------------------------- layer norm
+
+// Rows of x's last dimension (a view or a copy).
+Tensor rows_of(const Tensor& x, const char* name) {
+    if (x.dim() < 1 || x.size(-1) == 0) value_error(std::string(name) + " must have channels (got " + shape_of(x) + ")");
+    return x.dim() == 2 ? x : x.reshape({x.numel() / x.size(-1), x.size(-1)});
+}
+
+// A tensor of x's type, shape and device, as rows.
+Rows rows_like(const Tensor& t, const Tensor& x, const char* name) {
+    if (t.scalar_type() != x.scalar_type() || t.sizes() != x.sizes() || !t.is_cuda())
+        value_error(std::string(name) + " must be of x's type, shape " + shape_of(x) + " and device");
+    on_current_device(t);
+    return Rows(rows_of(t, name), name);
+}
+
+// A layer norm's tensors as the C-ABI takes them.
+struct LayerNorm {
+    tcc_layer_norm_shape s{};
+    Rows rows;
+    MaybeTensor weight, bias;  // kept until the launch
+
+    LayerNorm(const Tensor& x, const MaybeTensor& w, const MaybeTensor& b, double eps, std::uint32_t activation)
+        : rows(((void)dtype_of(x, "x"), rows_of(x, "x")), "x") {
+        s.dtype = dtype_of(x, "x");
+        const std::int64_t C = x.size(-1);
+        if (C > 16384) value_error("at most 16384 channels (got " + std::to_string(C) + ")");
+        if (!(eps >= 0)) value_error("eps is not negative (got " + std::to_string(eps) + ")");
+        s.N = rows.t.size(0);
+        s.C = static_cast<std::uint32_t>(C);
+        s.paramDtype = TCC_F32;
+        for (const auto& [p, name, to] : {std::tuple{&w, "weight", &weight}, std::tuple{&b, "bias", &bias}}) {
+            if (!*p) continue;
+            s.paramDtype = dtype_of(**p, name);
+            if ((*p)->dim() != 1 || (*p)->size(0) != C)
+                value_error(std::string(name) + " must hold a value for each of the " + std::to_string(C) + " channels (got " +
+                            shape_of(**p) + ")");
+            on_current_device(**p);
+            *to = (*p)->contiguous();
+        }
+        if (w && b && w->scalar_type() != b->scalar_type()) value_error("weight and bias must be of one type");
+        on_current_device(x);
+        s.activation = activation;
+        s.eps = static_cast<float>(eps);
+    }
+};
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> layer_norm(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias,
+                                                      const MaybeTensor& residual, double eps, std::uint32_t activation) {
+    const LayerNorm k(x, weight, bias, eps, activation);
+    std::optional<Rows> res;
+    if (residual) res.emplace(rows_like(*residual, x, "residual"));
+    const Tensor y = empty(x.sizes(), x.options());
+    const Tensor h = residual ? empty(x.sizes(), x.options()) : x;
+    const auto stats = x.sizes().slice(0, x.dim() - 1);
+    const auto f32 = x.options().dtype(at::kFloat);
+    const Tensor mean = empty(stats, f32), rstd = empty(stats, f32);
+    check(tcc_layer_norm(&k.s, k.rows.t.data_ptr(), k.rows.ld, res ? res->t.data_ptr() : nullptr, res ? res->ld : 0,
+                         ptr(k.weight), ptr(k.bias), y.data_ptr(), k.s.C, residual ? h.data_ptr() : nullptr, k.s.C,
+                         mean.data_ptr<float>(), rstd.data_ptr<float>(), stream_of(x)));
+    return {y, h, mean, rstd};
+}
+
+std::tuple<Tensor, MaybeTensor, MaybeTensor> layer_norm_grad(const Tensor& dy, const Tensor& h, const Tensor& mean,
+                                                             const Tensor& rstd, const MaybeTensor& weight,
+                                                             const MaybeTensor& bias, const MaybeTensor& dSum,
+                                                             std::uint32_t activation) {
+    const LayerNorm k(h, weight, bias, 0.0, activation);
+    const Rows rows = rows_like(dy, h, "d_y");
+    std::optional<Rows> add;
+    if (dSum) add.emplace(rows_like(*dSum, h, "d_sum"));
+    const auto stats = h.sizes().slice(0, h.dim() - 1);
+    for (const auto& [t, name] : {std::pair{&mean, "mean"}, std::pair{&rstd, "rstd"}}) {
+        if (!t->is_cuda() || t->scalar_type() != at::kFloat || !t->is_contiguous() || t->sizes() != stats)
+            value_error(std::string(name) + " must be contiguous float32, a value for each row of x");
+        on_current_device(*t);
+    }
+    const Tensor dx = empty(h.sizes(), h.options());
+    const auto f32 = h.options().dtype(at::kFloat);
+    MaybeTensor dw, db, ws;
+    if (weight) dw = empty({h.size(-1)}, f32);
+    if (bias) db = empty({h.size(-1)}, f32);
+    const std::size_t need = weight || bias ? tcc_layer_norm_grad_workspace_bytes(&k.s) : 0;
+    if (need > 0) ws = workspace(need, h);
+    check(tcc_layer_norm_grad(&k.s, rows.t.data_ptr(), rows.ld, k.rows.t.data_ptr(), k.rows.ld, mean.data_ptr<float>(),
+                              rstd.data_ptr<float>(), ptr(k.weight), ptr(k.bias), add ? add->t.data_ptr() : nullptr,
+                              add ? add->ld : 0, dx.data_ptr(), k.s.C, static_cast<float*>(ptr(dw)),
+                              static_cast<float*>(ptr(db)), ptr(ws), need, stream_of(h)));
+    return {dx, dw, db};
+}
+
 // ---------------------------------------------------------------- lists
 
 using TensorList = std::vector<Tensor>;
@@ -475,6 +566,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("embedding_grad", &embedding_grad);
     m.def("group_norm", &group_norm);
     m.def("group_norm_grad", &group_norm_grad);
+    m.def("layer_norm", &layer_norm);
+    m.def("layer_norm_grad", &layer_norm_grad);
     m.def("grad_norm", &grad_norm);
     m.def("clip_grad_norm", &clip_grad_norm);
     m.def("adam_step", &adam_step);

@@ -1,9 +1,11 @@
 """Python host API of include/tcc_training.h: the operators that a GCN with
-learned node rows trains with.
+learned node rows, or a deep one, trains with.
 
   embedding_lookup / embedding_grad   rows of a table, and their gradient
   group_norm / group_norm_grad        group norm over the node rows of each
                                       graph, channels last, with its activation
+  layer_norm / layer_norm_grad        layer norm of every row, with the residual
+                                      sum before it and its activation
   grad_norm / clip_grad_norm          the global gradient norm, and clipping
   adam_step                           the Adam update, clipping as it reads
 
@@ -95,6 +97,28 @@ def group_norm_grad(d_y: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd
     dweight and dbias [C] fp32 (None where there is no weight or bias)."""
     return _call(stream, _ext.group_norm_grad, d_y, x, mean, rstd, num_groups, weight, bias, offsets,
                  _activation(activation), max_rows)
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+               residual: torch.Tensor | None = None, eps: float = 1e-5, activation: str = "none",
+               stream=None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(y, h, mean, rstd) of act(layer_norm(h)) over the last dimension
+    (tcc_layer_norm), with h = x + residual rounded to x's type, or x itself
+    where there is no residual (of x's shape and type).  mean and rstd are fp32
+    of shape x.shape[:-1].  `weight` and `bias` [C] are of any one of the types."""
+    return _call(stream, _ext.layer_norm, x, weight, bias, residual, eps, _activation(activation))
+
+
+def layer_norm_grad(d_y: torch.Tensor, h: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
+                    weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+                    d_sum: torch.Tensor | None = None, activation: str = "none",
+                    stream=None) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
+    """(dx, dweight, dbias) of layer_norm (tcc_layer_norm_grad), from d_y of
+    h's shape and type, the forward's h, mean and rstd, and `d_sum`, the
+    gradient that h has from its other uses: dx of h's type is the gradient of
+    x and of residual alike, dweight and dbias [C] are fp32 (None where there
+    is no weight or bias)."""
+    return _call(stream, _ext.layer_norm_grad, d_y, h, mean, rstd, weight, bias, d_sum, _activation(activation))
 
 
 def grad_norm(grads, stream=None) -> torch.Tensor:
