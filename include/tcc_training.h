@@ -1,10 +1,11 @@
 /*
- * tcc_training.h — C-ABI of the operators that a GCN with learned node rows
- * trains with on MI355X (gfx950), beside the block-sparse SpMM of
- * tcc_spmm_cnic.h and the dense products of tcc_gcn.h: rows of an embedding
- * table and their gradient, a group norm over the node rows of each graph
- * with its activation, the global gradient norm with clipping, and the Adam
- * update that takes the clipped gradient.  The reference trains on a fixed
+ * tcc_training.h — C-ABI of the operators that a GCN with learned node rows, a
+ * deep one or one with a teacher trains with on MI355X (gfx950), beside the
+ * block-sparse SpMM of tcc_spmm_cnic.h and the dense products of tcc_gcn.h:
+ * rows of an embedding table and their gradient, a group norm over the node
+ * rows of each graph and a layer norm of each row, with their activation, a
+ * teacher's top logits and the loss against them, the global gradient norm with
+ * clipping, and the Adam update that takes the clipped gradient.  The reference trains on a fixed
  * feature table (train/tcgnn_conv_release.py:284-329) and has none of them.
  *
  * Element types (TCC_F32, TCC_BF16, TCC_F16) are those of the tensors in
@@ -144,6 +145,67 @@ int tcc_layer_norm_grad(const tcc_layer_norm_shape* s, const void* dY, uint64_t 
                         const float* mean, const float* rstd, const void* weight, const void* bias, const void* dSum,
                         uint64_t ldds, void* dX, uint64_t lddx, float* dWeight, float* dBias, void* workspace,
                         size_t workspaceBytes, void* stream);
+
+/* ------------------------------------------------------------ distillation */
+
+/* values and ids [n x K] (row strides ldv, ldi): the K largest of the C logits
+ * of each row (ldz) and their classes, largest first, the lowest class first
+ * among equals, NaN above all; values of the logits' type.  rest [n], unless it
+ * is NULL, is one logit that stands for the other classes at this temperature:
+ * rest = T log(sum of exp(z_j / T) over them), -inf where there are none.
+ * 1 <= K <= C, K <= 64 (TCC_ERR_UNSUPPORTED above), C below 2^31.  Row
+ * addresses of the logits need only be aligned to their element. */
+int tcc_top_logits(const void* logits, uint64_t ldz, uint32_t dtype, uint64_t n, uint32_t C, uint32_t K,
+                   float temperature, void* values, uint64_t ldv, int32_t* ids, uint64_t ldi, float* rest, void* stream);
+
+#define TCC_REDUCE_NONE 0u
+#define TCC_REDUCE_MEAN 1u
+#define TCC_REDUCE_SUM 2u
+
+/* A distillation of n rows of C logits of `dtype`, each against K entries of a
+ * teacher: values of `valueDtype` and ids (classes), int32 or int64 by idBytes 4
+ * or 8.  K <= 64, C below 2^31, n below 2^40 (TCC_ERR_UNSUPPORTED above). */
+typedef struct tcc_distill_shape {
+    uint64_t n;
+    uint32_t C, K;
+    uint32_t dtype, valueDtype, idBytes, reduction;
+    float temperature;
+} tcc_distill_shape;
+
+/* Bytes of workspace for tcc_distill_loss on the current device. */
+size_t tcc_distill_loss_workspace_bytes(const tcc_distill_shape* s);
+
+/* With p = softmax(t / T) over a row's entries t (and its `rest`, if not NULL)
+ * and q = softmax(z / T) over its classes, q_rest the sum of q over those that
+ * are no entry's:
+ *   row loss = w T^2 (sum_k p_k log(p_k / q_id_k) + p_rest log(p_rest / q_rest))
+ * with w = weight[row] (1 where weight is NULL).  Terms with p = 0 are 0.  An id
+ * of -1 is no entry, and so is any other that is no class: that sets
+ * TCC_DEVERR_FEATURE_INDEX in *deviceError, if it is not NULL.  A class may
+ * occur in several entries.  A row whose weight is 0 is not read, and it and a
+ * row without an entry or rest above -inf have no loss.
+ *
+ * *loss is the sum of the rows' losses (TCC_REDUCE_SUM) or that divided by the
+ * sum of the weights (TCC_REDUCE_MEAN; by n without weights; 0 where that is 0),
+ * summed in 64 bits, or loss [n] holds the rows' (TCC_REDUCE_NONE).  *total, if
+ * not NULL and the loss is summed, is the sum of the weights.  stats [n][4],
+ * 16-byte aligned, is for the gradient: the maximum of the logits, the sum of
+ * exp((z - maximum) / T), and both over the classes that are no entry's (0
+ * without rest); zeros for rows without a loss. */
+int tcc_distill_loss(const tcc_distill_shape* s, const void* logits, uint64_t ldz, const void* values, uint64_t ldv,
+                     const void* ids, uint64_t ldi, const float* rest, const float* weight, float* loss, float* total,
+                     float* stats, uint32_t* deviceError, void* workspace, size_t workspaceBytes, void* stream);
+
+/* dLogits [n x C] (ldd) of the logits' type, from *dLoss (dLoss [n] with
+ * TCC_REDUCE_NONE), the loss's arguments and its stats, and its total where it
+ * is a mean with weights (else NULL).  With g = dLoss w T (/ n or / total):
+ *   g (q_j - p_j)                  for the entries' classes, p_j the sum over them,
+ *   g (q_j - p_rest q_j / q_rest)  for the others (p_rest = 0 without rest).
+ * Rows without a loss have zeros.  dLogits overlaps no input. */
+int tcc_distill_grad(const tcc_distill_shape* s, const float* dLoss, const void* logits, uint64_t ldz,
+                     const void* values, uint64_t ldv, const void* ids, uint64_t ldi, const float* rest,
+                     const float* weight, const float* total, const float* stats, void* dLogits, uint64_t ldd,
+                     void* stream);
 
 /* ------------------------------------------------ gradient norm, clip, Adam */
 

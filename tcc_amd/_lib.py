@@ -94,6 +94,12 @@ class LayerNormShape(ctypes.Structure):
     _fields_ = [("N", u64), ("C", u32), ("dtype", u32), ("paramDtype", u32), ("activation", u32), ("eps", ctypes.c_float)]
 
 
+class DistillShape(ctypes.Structure):
+    """tcc_distill_shape."""
+    _fields_ = [("n", u64), ("C", u32), ("K", u32), ("dtype", u32), ("valueDtype", u32), ("idBytes", u32),
+                ("reduction", u32), ("temperature", ctypes.c_float)]
+
+
 class Adam(ctypes.Structure):
     """tcc_adam."""
     _fields_ = [
@@ -178,6 +184,12 @@ SIGNATURES = {
     "tcc_layer_norm_grad_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(LayerNormShape)]),
     "tcc_layer_norm_grad": (ctypes.c_int, [ctypes.POINTER(LayerNormShape), vp, u64, vp, u64, vp, vp, vp, vp, vp, u64, vp,
                                            u64, vp, vp, vp, ctypes.c_size_t, vp]),
+    "tcc_top_logits": (ctypes.c_int, [vp, u64, u32, u64, u32, u32, ctypes.c_float, vp, u64, vp, u64, vp, vp]),
+    "tcc_distill_loss_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(DistillShape)]),
+    "tcc_distill_loss": (ctypes.c_int, [ctypes.POINTER(DistillShape), vp, u64, vp, u64, vp, u64, vp, vp, vp, vp, vp, vp, vp,
+                                        ctypes.c_size_t, vp]),
+    "tcc_distill_grad": (ctypes.c_int, [ctypes.POINTER(DistillShape), vp, vp, u64, vp, u64, vp, u64, vp, vp, vp, vp, vp, u64,
+                                        vp]),
     "tcc_grad_norm_workspace_bytes": (ctypes.c_size_t, []),
     "tcc_grad_norm": (ctypes.c_int, [vp, u32, vp, vp, ctypes.c_size_t, vp]),
     "tcc_clip_grad_norm": (ctypes.c_int, [vp, vp, u32, ctypes.c_float, vp, vp, ctypes.c_size_t, vp]),

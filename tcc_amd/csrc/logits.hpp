@@ -1,0 +1,43 @@
+// Softmax sums over rows of logits (distill.hip, top_logits.hip).
+#pragma once
+
+#include "row_types.hpp"
+
+namespace tcc {
+
+constexpr float kLn2 = 0.693147181f;
+constexpr float kNone = -__builtin_huge_valf();  // the logit of nothing
+
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float log2_of(float x) { return __builtin_amdgcn_logf(x); }
+// A maximum as it is subtracted: 0 for that of nothing.
+__device__ __forceinline__ float base_of(float m) { return m == kNone ? 0.0f : m; }
+
+// The maximum m of some logits and s = sum of 2^((z - m) c).
+struct Share {
+    float m = kNone, s = 0.0f;
+    __device__ __forceinline__ void scale_to(float top, float c) {
+        s *= exp2_of((m - base_of(top)) * c);
+        m = top;
+    }
+    __device__ __forceinline__ Share with(Share o, float c) const {
+        const float top = fmaxf(m, o.m);
+        const float b = base_of(top);
+        return {top, s * exp2_of((m - b) * c) + o.s * exp2_of((o.m - b) * c)};
+    }
+};
+
+// A vector of V of a row's elements; the last one is moved back to end with the
+// row.
+template <int V>
+struct Place {
+    std::uint32_t at, skip;  // first element, and how many of them are another vector's (V: all)
+    __device__ __forceinline__ Place(std::uint32_t vector, std::uint32_t C) {
+        const std::uint64_t c = static_cast<std::uint64_t>(vector) * V;
+        at = static_cast<std::uint32_t>(min<std::uint64_t>(c, C - V));
+        skip = static_cast<std::uint32_t>(min<std::uint64_t>(c - at, V));
+    }
+    __device__ __forceinline__ bool any() const { return skip < V; }
+};
+
+}  // namespace tcc

@@ -409,6 +409,125 @@ std::tuple<Tensor, MaybeTensor, MaybeTensor> layer_norm_grad(const Tensor& dy, c
     return {dx, dw, db};
 }
 
+// ---------------------------------------------------------------- distillation
+
+void temperature_is_positive(double t) {
+    if (!(t > 0 && t < 1e18)) value_error("the temperature is positive (got " + std::to_string(t) + ")");
+}
+
+std::tuple<Tensor, Tensor, Tensor> top_logits(const Tensor& logits, std::int64_t k, double temperature) {
+    const std::uint32_t code = dtype_of(logits, "logits");
+    const Rows rows(logits, "logits");
+    const std::int64_t n = logits.size(0), C = logits.size(1);
+    if (C > 0x7FFFFFFFll) value_error("rows of " + std::to_string(C) + " logits are too long");
+    if (k < 1 || k > std::min<std::int64_t>(C, 64))
+        value_error("k must be between 1 and the " + std::to_string(C) + " classes, and at most 64 (got " + std::to_string(k) + ")");
+    temperature_is_positive(temperature);
+    on_current_device(logits);
+    const Tensor values = empty({n, k}, logits.options()), ids = empty({n, k}, logits.options().dtype(at::kInt));
+    const Tensor rest = empty({n}, logits.options().dtype(at::kFloat));
+    check(tcc_top_logits(rows.t.data_ptr(), rows.ld, code, n, static_cast<std::uint32_t>(C), static_cast<std::uint32_t>(k),
+                         static_cast<float>(temperature), values.data_ptr(), k, ids.data_ptr<std::int32_t>(), k,
+                         rest.data_ptr<float>(), stream_of(logits)));
+    return {values, ids, rest};
+}
+
+// A distillation's tensors as the C-ABI takes them.
+struct Distill {
+    tcc_distill_shape s{};
+    Rows z;
+    std::optional<Rows> values, ids;
+    MaybeTensor rest, weight;  // kept until the launch
+
+    Distill(const Tensor& logits, const Tensor& v, const Tensor& i, const MaybeTensor& r, const MaybeTensor& w,
+            double temperature, std::uint32_t reduction)
+        : z(((void)dtype_of(logits, "logits"), logits), "logits") {
+        s.dtype = dtype_of(logits, "logits");
+        s.valueDtype = dtype_of(v, "values");
+        s.idBytes = index_bytes(i, "ids");
+        s.reduction = reduction;
+        const std::int64_t n = logits.size(0), C = logits.size(1);
+        if (v.dim() != 2 || v.size(0) != n || v.size(1) < 1 || v.size(1) > 64 || i.sizes() != v.sizes())
+            value_error("values " + shape_of(v) + " and ids " + shape_of(i) + " must be 1 to 64 entries for each of the " +
+                        std::to_string(n) + " rows");
+        if (C > 0x7FFFFFFFll) value_error("rows of " + std::to_string(C) + " logits are too long");
+        temperature_is_positive(temperature);
+        values.emplace(v, "values");
+        ids.emplace(i, "ids");
+        for (const auto& [t, name, to] : {std::tuple{&r, "rest", &rest}, std::tuple{&w, "weight", &weight}}) {
+            if (!*t) continue;
+            if (!(*t)->is_cuda() || (*t)->scalar_type() != at::kFloat)
+                type_error(std::string(name) + " must be a float32 device tensor (got " + place_of(**t) + ")");
+            if ((*t)->dim() != 1 || (*t)->size(0) != n)
+                value_error(std::string(name) + " must hold a value for each of the " + std::to_string(n) + " rows (got " +
+                            shape_of(**t) + ")");
+            on_current_device(**t);
+            *to = (*t)->contiguous();
+        }
+        on_current_device(logits);
+        on_current_device(v);
+        on_current_device(i);
+        s.n = static_cast<std::uint64_t>(n);
+        s.C = static_cast<std::uint32_t>(C);
+        s.K = static_cast<std::uint32_t>(v.size(1));
+        s.temperature = static_cast<float>(temperature);
+    }
+};
+
+std::tuple<Tensor, Tensor, MaybeTensor> distill_loss(const Tensor& logits, const Tensor& values, const Tensor& ids,
+                                                     const MaybeTensor& rest, double temperature, const MaybeTensor& weight,
+                                                     std::uint32_t reduction, const MaybeTensor& deviceError) {
+    const Distill k(logits, values, ids, rest, weight, temperature, reduction);
+    std::uint32_t* err = error_word(deviceError);
+    const auto f32 = logits.options().dtype(at::kFloat);
+    const std::int64_t n = logits.size(0);
+    const Tensor loss = reduction == TCC_REDUCE_NONE ? empty({n}, f32) : empty({}, f32);
+    const Tensor stats = empty({n, 4}, f32);
+    MaybeTensor total, ws;
+    if (weight && reduction == TCC_REDUCE_MEAN) total = empty({}, f32);
+    const std::size_t need = tcc_distill_loss_workspace_bytes(&k.s);
+    if (need > 0) ws = workspace(need, logits);
+    check(tcc_distill_loss(&k.s, k.z.t.data_ptr(), k.z.ld, k.values->t.data_ptr(), k.values->ld, k.ids->t.data_ptr(),
+                           k.ids->ld, static_cast<const float*>(ptr(k.rest)), static_cast<const float*>(ptr(k.weight)),
+                           loss.data_ptr<float>(), static_cast<float*>(ptr(total)), stats.data_ptr<float>(), err, ptr(ws),
+                           need, stream_of(logits)));
+    if (deviceError) written(*deviceError);
+    return {loss, stats, total};
+}
+
+Tensor distill_grad(const Tensor& dLoss, const Tensor& logits, const Tensor& values, const Tensor& ids, const Tensor& stats,
+                    const MaybeTensor& rest, double temperature, const MaybeTensor& weight, const MaybeTensor& total,
+                    std::uint32_t reduction) {
+    const Distill k(logits, values, ids, rest, weight, temperature, reduction);
+    const std::int64_t n = logits.size(0);
+    const bool each = reduction == TCC_REDUCE_NONE;
+    const auto is_float = [](const Tensor& t, const char* name) {
+        if (!t.is_cuda() || t.scalar_type() != at::kFloat)
+            type_error(std::string(name) + " must be a float32 device tensor (got " + place_of(t) + ")");
+        on_current_device(t);
+    };
+    is_float(dLoss, "d_loss");
+    is_float(stats, "stats");
+    if (each ? dLoss.dim() != 1 || dLoss.size(0) != n : dLoss.numel() != 1)
+        value_error("d_loss " + shape_of(dLoss) + " must be of the loss's shape");
+    if (stats.dim() != 2 || stats.size(0) != n || stats.size(1) != 4) value_error("stats must be those of the loss");
+    if (weight && reduction == TCC_REDUCE_MEAN) {
+        if (!total) value_error("a mean with weights needs their total");
+        is_float(*total, "total");
+        if (total->numel() != 1) value_error("total must be that of the loss");
+    }
+    const Tensor d = dLoss.contiguous();
+    Tensor st = stats.contiguous();
+    if ((reinterpret_cast<std::uintptr_t>(st.data_ptr()) & 15) != 0) st = st.clone();
+    const Tensor dz = empty(logits.sizes(), logits.options());
+    const float* sum = weight && reduction == TCC_REDUCE_MEAN ? total->data_ptr<float>() : nullptr;
+    check(tcc_distill_grad(&k.s, d.data_ptr<float>(), k.z.t.data_ptr(), k.z.ld, k.values->t.data_ptr(), k.values->ld,
+                           k.ids->t.data_ptr(), k.ids->ld, static_cast<const float*>(ptr(k.rest)),
+                           static_cast<const float*>(ptr(k.weight)), sum, st.data_ptr<float>(), dz.data_ptr(), k.s.C,
+                           stream_of(logits)));
+    return dz;
+}
+
 // ---------------------------------------------------------------- lists
 
 using TensorList = std::vector<Tensor>;
@@ -568,6 +687,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("group_norm_grad", &group_norm_grad);
     m.def("layer_norm", &layer_norm);
     m.def("layer_norm_grad", &layer_norm_grad);
+    m.def("top_logits", &top_logits);
+    m.def("distill_loss", &distill_loss);
+    m.def("distill_grad", &distill_grad);
     m.def("grad_norm", &grad_norm);
     m.def("clip_grad_norm", &clip_grad_norm);
     m.def("adam_step", &adam_step);

@@ -1,11 +1,13 @@
 """Python host API of include/tcc_training.h: the operators that a GCN with
-learned node rows, or a deep one, trains with.
+learned node rows, a deep one or one with a teacher trains with.
 
   embedding_lookup / embedding_grad   rows of a table, and their gradient
   group_norm / group_norm_grad        group norm over the node rows of each
                                       graph, channels last, with its activation
   layer_norm / layer_norm_grad        layer norm of every row, with the residual
                                       sum before it and its activation
+  top_logits                          a teacher's largest logits of every row
+  distill_loss / distill_grad         the loss against them, and its gradient
   grad_norm / clip_grad_norm          the global gradient norm, and clipping
   adam_step                           the Adam update, clipping as it reads
 
@@ -34,6 +36,7 @@ except ImportError as e:
 _lib.lib()  # its errors are raised as _lib.TccError
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}  # TCC_ACT_*
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}  # TCC_REDUCE_*
 
 
 def _call(stream, f, *args):
@@ -43,11 +46,15 @@ def _call(stream, f, *args):
         return f(*args)
 
 
-def _activation(name: str) -> int:
-    code = ACTIVATIONS.get(name)
+def _code(codes: dict, kind: str, name: str) -> int:
+    code = codes.get(name)
     if code is None:
-        raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)} (got {name!r})")
+        raise ValueError(f"{kind} must be one of {sorted(codes)} (got {name!r})")
     return code
+
+
+def _activation(name: str) -> int:
+    return _code(ACTIVATIONS, "activation", name)
 
 
 def embedding_lookup(table: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, padding_idx: int | None = None,
@@ -119,6 +126,46 @@ def layer_norm_grad(d_y: torch.Tensor, h: torch.Tensor, mean: torch.Tensor, rstd
     x and of residual alike, dweight and dbias [C] are fp32 (None where there
     is no weight or bias)."""
     return _call(stream, _ext.layer_norm_grad, d_y, h, mean, rstd, weight, bias, d_sum, _activation(activation))
+
+
+def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0,
+               stream=None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(values, ids, rest) of logits [n x C] (tcc_top_logits): the `k` largest of
+    each row and their classes (int32), largest first, the lowest class first
+    among equals, NaN above all, and one fp32 logit that stands for the other
+    classes at this temperature (-inf where there are none).  k is at most 64."""
+    return _call(stream, _ext.top_logits, logits, k, temperature)
+
+
+def distill_loss(logits: torch.Tensor, values: torch.Tensor, ids: torch.Tensor, rest: torch.Tensor | None = None,
+                 temperature: float = 1.0, weight: torch.Tensor | None = None, reduction: str = "mean",
+                 device_error: torch.Tensor | None = None,
+                 stream=None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+    """(loss, stats, total) of a student's logits [n x C] against a teacher's
+    entries (tcc_distill_loss): T^2 times the divergence KL(p || q) of each row,
+    p the softmax of values / T over the row's entries, q that of logits / T over
+    all classes.  With `rest` (of the same temperature) both have one more class,
+    which holds what the entries leave; without it p is that of the entries alone
+    (a single entry at temperature 1: cross-entropy).  `weight` [n] fp32 weighs
+    the rows; those of weight 0 are not read.  The loss is the mean over the
+    weights, the sum, or the rows' own (reduction="none").  An id of -1 is no
+    entry; others that are no class are none either and set
+    TCC_DEVERR_FEATURE_INDEX in `device_error` (one int32 on the device).
+    stats [n x 4] and total (None unless the loss is a mean with weights) are
+    for the gradient."""
+    return _call(stream, _ext.distill_loss, logits, values, ids, rest, temperature, weight,
+                 _code(REDUCTIONS, "reduction", reduction), device_error)
+
+
+def distill_grad(d_loss: torch.Tensor, logits: torch.Tensor, values: torch.Tensor, ids: torch.Tensor,
+                 stats: torch.Tensor, rest: torch.Tensor | None = None, temperature: float = 1.0,
+                 weight: torch.Tensor | None = None, total: torch.Tensor | None = None, reduction: str = "mean",
+                 stream=None) -> torch.Tensor:
+    """The gradient of distill_loss in the logits, of their type
+    (tcc_distill_grad), from d_loss (fp32, of the loss's shape), the loss's
+    arguments, and the stats and total that it gave."""
+    return _call(stream, _ext.distill_grad, d_loss, logits, values, ids, stats, rest, temperature, weight, total,
+                 _code(REDUCTIONS, "reduction", reduction))
 
 
 def grad_norm(grads, stream=None) -> torch.Tensor:
