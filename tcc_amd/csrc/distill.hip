@@ -275,20 +275,19 @@ __global__ void __launch_bounds__(kThreads) loss_kernel(Args a) {
             }
             const Share others = team.join(v);
             const Share all = REST ? others.with(team.join(firsts), a.c) : others;
-            const float logAll = log2_of(all.s), logTop = log2_of(team.sum), b = base_of(all.m), tb = base_of(team.top);
+            const Log2 logAll(all.s), logTop(team.sum);
+            const float b = base_of(all.m), tb = base_of(team.top), sums = logAll.over(logTop);
             float sum = 0.0f;
 #pragma unroll
             for (int e = 0; e < kEntries<TEAM>; ++e) {
                 if (team.id[e] < 0 || team.p[e] == 0.0f) continue;
-                const float logP = (team.t[e] - tb) * a.c - logTop;
-                const float logQ = (static_cast<float>(z[team.id[e]]) - b) * a.c - logAll;
-                sum += team.p[e] * (logP - logQ);
+                const float apart = (team.t[e] - tb) * a.c - (static_cast<float>(z[team.id[e]]) - b) * a.c;
+                sum += team.p[e] * (apart + sums);
             }
             sum = wave_join<Team<TEAM>::inWave>(sum, Add());
             if (REST && team.pRest != 0.0f) {
-                const float logP = (team.rest - tb) * a.c - logTop;
-                const float logQ = (base_of(others.m) - b) * a.c + log2_of(others.s) - logAll;
-                sum += team.pRest * (logP - logQ);
+                const float apart = (team.rest - tb) * a.c - (base_of(others.m) - b) * a.c;
+                sum += team.pRest * (apart + (sums - Log2(others.s).over(Log2(1.0f))));
             }
             loss = w * (sum * (a.T * a.T * kLn2));
             stats = make_float4(b, all.s, REST ? base_of(others.m) : 0.0f, REST ? others.s : 0.0f);

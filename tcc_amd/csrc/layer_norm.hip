@@ -15,9 +15,10 @@
 // the one before counts once in every sum, and is written twice with the same
 // value).  Teams are as small as 16 elements a lane allow, which saves
 // reductions, at least four lanes, at most the 1,024 threads of a workgroup.
-// The mean is taken twice, the second time of the differences from the first:
-// what the first lost to rows far from zero comes back, and the sums of both
-// need one reduction.
+// A lane adds its elements in pairs, and the lanes' sums are added in 64 bits: the
+// mean comes out rounded once for most rows.  The variance is the mean square of
+// the differences from that, less the square of their mean, which is what rows
+// far from zero have lost.
 //
 // The gradient's teams walk the rows in equal steps and keep the sums of dz and
 // dz xh of their channels in registers; a workgroup adds its teams' in LDS and
@@ -101,6 +102,19 @@ __device__ __forceinline__ vec_t<float, N> through_by(std::uint32_t act, vec_t<f
     return through_all<TCC_ACT_GELU, FINE, N>(d, z);
 }
 
+// The sum of N elements (a power of two), pairs before pairs of pairs.
+template <int N, typename A>
+__device__ __forceinline__ float in_pairs(const A& v) {
+    float s[N];
+#pragma unroll
+    for (int q = 0; q < N; ++q) s[q] = v[q];
+#pragma unroll
+    for (int d = 1; d < N; d <<= 1)
+#pragma unroll
+        for (int q = 0; q + d < N; q += 2 * d) s[q] += s[q + d];
+    return s[0];
+}
+
 // Rounded to T, as memory holds it.
 template <typename T, int N>
 __device__ __forceinline__ vec_t<float, N> rounded(vec_t<float, N> v) {
@@ -120,7 +134,8 @@ __global__ void __launch_bounds__(kThreads<TEAM>) forward_kernel(Args a) {
         w[e] = load_params<V>(a.weight, a.paramType, cols.c[e], 1.0f);
         b[e] = load_params<V>(a.bias, a.paramType, cols.c[e], 0.0f);
     }
-    const float perC = 1.0f / static_cast<float>(a.C);
+    const double perC = 1.0 / a.C;
+    const float inverse = static_cast<float>(perC);
     const std::uint64_t step = static_cast<std::uint64_t>(gridDim.x) * kTeams<TEAM>;
     for (std::uint64_t r = static_cast<std::uint64_t>(blockIdx.x) * kTeams<TEAM> + threadIdx.x / TEAM; r < a.N; r += step) {
         const T* x = static_cast<const T*>(a.x) + r * a.ldx;
@@ -133,18 +148,15 @@ __global__ void __launch_bounds__(kThreads<TEAM>) forward_kernel(Args a) {
             for (int e = 0; e < E; ++e)
                 if (cols.any(e)) h[e] = rounded<T, V>(h[e] + load_any<T, V>(res + cols.c[e]));
         }
-        float total = 0.0f;
+        float pairs[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const F own = cols.own(e, h[e]);
-#pragma unroll
-            for (int q = 0; q < V; ++q) total += own[q];
-        }
-        const float first = sum(total, 0.0f).x * perC;
+        for (int e = 0; e < E; ++e) pairs[e] = in_pairs<V>(cols.own(e, h[e]));
+        const double mean64 = sum(static_cast<double>(in_pairs<E>(pairs))) * perC;
+        const float mean = static_cast<float>(mean64);
         float left = 0.0f, squares = 0.0f;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const F d = cols.own(e, h[e] - first);
+            const F d = cols.own(e, h[e] - mean);
 #pragma unroll
             for (int q = 0; q < V; ++q) {
                 left += d[q];
@@ -152,8 +164,7 @@ __global__ void __launch_bounds__(kThreads<TEAM>) forward_kernel(Args a) {
             }
         }
         const float2 both = sum(left, squares);
-        const float shift = both.x * perC, mean = first + shift;
-        const float var = fmaf(-shift, shift, both.y * perC);
+        const float off = both.x * inverse, var = fmaf(-off, off, both.y * inverse);
         const float rstd = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + a.eps);  // keeps NaN
         T* y = static_cast<T*>(a.out) + r * a.ldo;
         T* s = static_cast<T*>(a.sum) + r * a.lds;

@@ -10,6 +10,15 @@ constexpr float kNone = -__builtin_huge_valf();  // the logit of nothing
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log2_of(float x) { return __builtin_amdgcn_logf(x); }
+// log2(x) as a whole number and a fraction of [-1, 0): differences of two keep the
+// digits that the logarithm of a large sum rounds away (v_log_f32 does so to one
+// side, which the mean of many rows does not even out).
+struct Log2 {
+    float whole, part;
+    __device__ __forceinline__ explicit Log2(float x)
+        : whole(static_cast<float>(__builtin_amdgcn_frexp_expf(x))), part(log2_of(__builtin_amdgcn_frexp_mantf(x))) {}
+    __device__ __forceinline__ float over(const Log2& o) const { return (whole - o.whole) + (part - o.part); }
+};
 // A maximum as it is subtracted: 0 for that of nothing.
 __device__ __forceinline__ float base_of(float m) { return m == kNone ? 0.0f : m; }
 
