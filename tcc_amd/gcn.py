@@ -37,8 +37,11 @@ both weight gradients in one pass (TwoLayerFunction).
 EmbeddingGCN is the model where the node rows are learned (graphs without
 features): rows of an embedding table (NodeEmbedding), conv1, a group norm
 over the node rows of each graph with its activation (NodeGroupNorm),
-conv_final, trained by ClippedAdam, over tcc_amd.training.  The reference,
-whose features are given, has no counterpart.
+conv_final, trained by ClippedAdam, over tcc_amd.training.  With layer norms
+(NodeLayerNorm) it may have residual blocks between the two convolutions.  A
+smaller model learns from a larger one's largest logits (top_logits of
+tcc_amd.training, DistillationLoss).  The reference, whose features are given
+and whose labels are classes, has no counterpart.
 """
 from __future__ import annotations
 
@@ -321,6 +324,60 @@ class GroupNormFunction(torch.autograd.Function):
         return dx, dw, db, None, None, None, None, None
 
 
+class LayerNormFunction(torch.autograd.Function):
+    """act(layer_norm(x)), or (act(layer_norm(h)), h) of h = x + residual
+    (tcc_amd.training.layer_norm / layer_norm_grad)."""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, eps, activation):
+        from . import training
+
+        y, h, mean, rstd = training.layer_norm(x, weight, bias, residual=residual, eps=eps, activation=activation)
+        ctx.save_for_backward(h, weight, bias, mean, rstd)
+        ctx.activation, ctx.summed = activation, residual is not None
+        ctx.set_materialize_grads(False)
+        return (y, h) if ctx.summed else y
+
+    @staticmethod
+    @_first_order
+    def backward(ctx, d_y, d_sum=None):
+        from . import training
+
+        if d_y is None:  # only the sum was used
+            return d_sum, d_sum, None, None, None, None
+        h, weight, bias, mean, rstd = ctx.saved_tensors
+        dx, dw, db = training.layer_norm_grad(d_y, h, mean, rstd, weight, bias, d_sum=d_sum, activation=ctx.activation)
+        dw = None if dw is None else dw.to(weight.dtype)
+        db = None if db is None else db.to(bias.dtype)
+        return dx, dx if ctx.summed else None, dw, db, None, None
+
+
+class DistillationFunction(torch.autograd.Function):
+    """tcc_amd.training.distill_loss with its gradient in the logits; the
+    teacher's entries and the weights are constants."""
+
+    @staticmethod
+    def forward(ctx, logits, values, ids, rest, weight, temperature, reduction, device_error):
+        from . import training
+
+        loss, stats, total = training.distill_loss(logits, values, ids, rest=rest, temperature=temperature, weight=weight,
+                                                   reduction=reduction, device_error=device_error)
+        ctx.save_for_backward(logits, values, ids, rest, weight, stats, total)
+        ctx.args = temperature, reduction
+        return loss
+
+    @staticmethod
+    @_first_order
+    def backward(ctx, d_loss):
+        from . import training
+
+        logits, values, ids, rest, weight, stats, total = ctx.saved_tensors
+        temperature, reduction = ctx.args
+        d = training.distill_grad(d_loss, logits, values, ids, stats, rest=rest, temperature=temperature, weight=weight,
+                                  total=total, reduction=reduction)
+        return d, None, None, None, None, None, None, None
+
+
 class NodeEmbedding(torch.nn.Module):
     """A learned row of `dim` values for each of `num_nodes` nodes; forward
     gives scale * rows of `ids` (sqrt(dim) times rows that begin at
@@ -365,23 +422,79 @@ class NodeGroupNorm(torch.nn.Module):
                                        max_rows)
 
 
+class NodeLayerNorm(torch.nn.Module):
+    """Layer norm of every row with its activation.  With `residual`, the norm of
+    x + residual and that sum: (y, h)."""
+
+    def __init__(self, channels: int, activation: str = "none", eps: float = 1e-5, device="cuda"):
+        super().__init__()
+        self.activation, self.eps = activation, eps
+        self.weight = torch.nn.Parameter(torch.ones(channels, device=device))
+        self.bias = torch.nn.Parameter(torch.zeros(channels, device=device))
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None):
+        return LayerNormFunction.apply(x, residual, self.weight, self.bias, self.eps, self.activation)
+
+
 class EmbeddingGCN(torch.nn.Module):
     """conv_final(act(norm(conv1(embedding[ids])))) over a batch of graphs
     (their block-diagonal A as one LayerGraph, `offsets` their first rows) or
-    one graph (no offsets)."""
+    one graph (no offsets).  The norm is a group norm over each graph's rows, or
+    norm="layer" one of each row; between that and conv_final lie then `blocks`
+    residual ones, h = h + conv(act(norm(h)))."""
 
     def __init__(self, num_nodes: int, dim: int, hidden_dim: int, num_classes: int, num_groups: int = 8,
-                 activation: str = "relu", padding_idx: int | None = None):
+                 activation: str = "relu", padding_idx: int | None = None, norm: str = "group", blocks: int = 0):
         super().__init__()
+        if norm not in ("group", "layer"):
+            raise ValueError(f"norm must be 'group' or 'layer' (got {norm!r})")
+        if blocks < 0 or (blocks > 0 and norm != "layer"):
+            raise ValueError("residual blocks go with layer norms")
         self.embedding = NodeEmbedding(num_nodes, dim, padding_idx=padding_idx)
         self.conv1 = GCNConv(dim, hidden_dim).cuda()
-        self.norm = NodeGroupNorm(num_groups, hidden_dim, activation)
+        self.layer_norm = norm == "layer"
+        self.norm = (NodeLayerNorm(hidden_dim, activation) if self.layer_norm
+                     else NodeGroupNorm(num_groups, hidden_dim, activation))
+        self.convs = torch.nn.ModuleList(GCNConv(hidden_dim, hidden_dim).cuda() for _ in range(blocks))
+        self.norms = torch.nn.ModuleList(NodeLayerNorm(hidden_dim, activation) for _ in range(blocks))
         self.conv_final = GCNConv(hidden_dim, num_classes).cuda()
 
     def forward(self, graph: LayerGraph, ids: torch.Tensor, offsets: torch.Tensor | None = None,
                 max_rows: int | None = None) -> torch.Tensor:
-        x = self.conv1(graph, x=self.embedding(ids))
-        return self.conv_final(graph, x=self.norm(x, offsets, max_rows))
+        h = self.conv1(graph, x=self.embedding(ids))
+        y = self.norm(h) if self.layer_norm else self.norm(h, offsets, max_rows)
+        for conv, norm in zip(self.convs, self.norms):
+            y, h = norm(conv(graph, x=y), h)
+        return self.conv_final(graph, x=y)
+
+
+class DistillationLoss(torch.nn.Module):
+    """The loss of logits against a teacher's entries, (values, ids, rest) as
+    tcc_amd.training.top_logits gives them at this temperature (rest may be None:
+    then the teacher's probabilities are those of the entries alone).  It takes
+    the place of the class labels' loss in train_epoch and
+    train_embedding_epoch, and the entries that of the labels.  Rows of weight 0
+    do not count.  error() reports ids that are no class."""
+
+    def __init__(self, temperature: float = 1.0, weight: torch.Tensor | None = None, reduction: str = "mean", device="cuda"):
+        super().__init__()
+        self.temperature, self.reduction = temperature, reduction
+        self.register_buffer("weight", weight, persistent=False)
+        self.register_buffer("device_error", torch.zeros(1, dtype=torch.int32, device=device), persistent=False)
+
+    def forward(self, pred: torch.Tensor, entries) -> torch.Tensor:
+        values, ids, rest = entries
+        if any(t is not None and t.requires_grad for t in (values, rest, self.weight)):
+            raise ValueError("the teacher's entries and the weights are constants: detach them")
+        return DistillationFunction.apply(pred, values, ids, rest, self.weight, self.temperature, self.reduction,
+                                          self.device_error)
+
+    def error(self) -> int:
+        """TCC_DEVERR_FEATURE_INDEX if an id was no class (and not -1) since the
+        last call, else 0; synchronises the device and clears the word."""
+        v = int(self.device_error.item())
+        self.device_error.zero_()
+        return v
 
 
 class ClippedAdam(torch.optim.Optimizer):

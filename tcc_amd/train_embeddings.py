@@ -1,11 +1,14 @@
 """Trains a GCN with learned node rows on a batch of synthetic graphs:
 
     python -m tcc_amd.train_embeddings --graphs 200 --nodes 50000 --steps 20
+    python -m tcc_amd.train_embeddings --norm layer --blocks 2 --distill 4
 
 Every graph is a random subset of the nodes of one table with R-MAT edges
-among them, and its nodes' labels follow two hidden classes of the table, so
-that only the embeddings can tell them apart.  Prints the loss and the gradient
-norm of every step.
+among them, and its nodes' labels follow hidden classes of the table (two, or
+--classes), so that only the embeddings can tell them apart.  Prints the loss and
+the gradient norm of every step.  With --norm layer the model has layer norms and
+--blocks residual ones; with --distill K a model of one quarter of its widths then
+learns from its K largest logits of every node.
 """
 from __future__ import annotations
 
@@ -13,7 +16,7 @@ import argparse
 
 import torch
 
-from . import gcn
+from . import gcn, training
 from .graphs import rmat_graph
 
 
@@ -35,25 +38,37 @@ def batch_of_graphs(num_nodes: int, graphs: int, mean_rows: int, seed: int):
 
 
 def train(nodes: int = 50_000, graphs: int = 200, mean_rows: int = 60, dim: int = 64, hidden: int = 128, steps: int = 20,
-          lr: float = 1e-2, max_norm: float = 1.0, seed: int = 0, log=print):
-    """The losses and gradient norms of `steps` steps, and the model."""
+          lr: float = 1e-2, max_norm: float = 1.0, seed: int = 0, log=print, norm: str = "group", blocks: int = 0,
+          classes: int = 2, distill: int = 0, temperature: float = 2.0):
+    """The losses and gradient norms of `steps` steps, and the model; with
+    `distill`, those of the student that learns from its `distill` largest logits,
+    and the student."""
     torch.manual_seed(seed)
     rows, cols, ids, offsets, max_rows = batch_of_graphs(nodes, graphs, mean_rows, seed)
     n = ids.numel()
     graph = gcn.LayerGraph(rows, cols, n, n)
-    labels = (ids % 2).cuda()
+    labels = (ids % classes).cuda()
     ids, offsets = ids.cuda(), offsets.cuda()
-    model = gcn.EmbeddingGCN(nodes, dim, hidden, 2)
-    optimizer = gcn.ClippedAdam(model.parameters(), lr=lr, max_norm=max_norm)
-    losses, norms = [], []
-    for step in range(steps):
-        loss, norm = gcn.train_embedding_epoch(model, graph, ids, labels, optimizer, offsets, max_rows)
-        losses.append(float(loss))
-        norms.append(float(norm))
-        log(f"step {step}: loss {losses[-1]:.4f}, gradient norm {norms[-1]:.3f}")
-    if model.embedding.error():
-        raise RuntimeError("a node id lies outside the embedding table")
-    return losses, norms, model
+
+    def run(model, targets, loss_fcn, name):
+        optimizer = gcn.ClippedAdam(model.parameters(), lr=lr, max_norm=max_norm)
+        losses, norms = [], []
+        for step in range(steps):
+            loss, total = gcn.train_embedding_epoch(model, graph, ids, targets, optimizer, offsets, max_rows, loss_fcn)
+            losses.append(float(loss))
+            norms.append(float(total))
+            log(f"{name}step {step}: loss {losses[-1]:.4f}, gradient norm {norms[-1]:.3f}")
+        if model.embedding.error():
+            raise RuntimeError("a node id lies outside the embedding table")
+        return losses, norms, model
+
+    teacher = run(gcn.EmbeddingGCN(nodes, dim, hidden, classes, norm=norm, blocks=blocks), labels, gcn.cross_entropy, "")
+    if distill == 0:
+        return teacher
+    with torch.no_grad():
+        entries = training.top_logits(teacher[2](graph, ids, offsets, max_rows), distill, temperature=temperature)
+    small = [max(8, w // 4 // 8 * 8) for w in (dim, hidden)]  # 8 groups, where they are asked for
+    return run(gcn.EmbeddingGCN(nodes, *small, classes, norm=norm), entries, gcn.DistillationLoss(temperature), "student: ")
 
 
 def main(argv=None) -> int:
@@ -66,9 +81,15 @@ def main(argv=None) -> int:
     p.add_argument("--steps", type=int, default=20)
     p.add_argument("--lr", type=float, default=1e-2)
     p.add_argument("--max-norm", type=float, default=1.0)
+    p.add_argument("--norm", choices=("group", "layer"), default="group")
+    p.add_argument("--blocks", type=int, default=0, help="residual blocks (with --norm layer)")
+    p.add_argument("--classes", type=int, default=2)
+    p.add_argument("--distill", type=int, default=0, metavar="K", help="train a student from the K largest logits")
+    p.add_argument("--temperature", type=float, default=2.0)
     a = p.parse_args(argv)
     train(a.nodes, a.graphs, a.mean_rows, a.dim, a.hidden, a.steps, a.lr, a.max_norm,
-          log=lambda s: print(s, flush=True))
+          log=lambda s: print(s, flush=True), norm=a.norm, blocks=a.blocks, classes=a.classes, distill=a.distill,
+          temperature=a.temperature)
     return 0
 
 
