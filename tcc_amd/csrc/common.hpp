@@ -66,6 +66,19 @@ inline std::uint32_t device_cus() {
     return cache[dev];
 }
 
+// Workgroups of a kernel that the current device runs at once (asked once a
+// kernel): a grid of as many, each at an equal share of the work, leaves no
+// compute unit waiting for a last round.
+template <typename Kernel>
+std::uint32_t resident_blocks(Kernel kernel, int threads, std::uint32_t& perCu) {
+    if (perCu == 0) {
+        int n = 0;
+        const hipError_t e = hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, reinterpret_cast<const void*>(kernel), threads, 0);
+        perCu = e == hipSuccess && n > 0 ? static_cast<std::uint32_t>(n) : 1u;
+    }
+    return perCu * device_cus();
+}
+
 // ---------------------------------------------------------------- numerics
 // cvt.rna.tf32.f32 restated from its definition: round to nearest with ties
 // away from zero, keeping 10 explicit mantissa bits; inf and NaN unchanged.

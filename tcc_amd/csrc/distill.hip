@@ -61,14 +61,15 @@ __device__ __forceinline__ void team_sync() {
 }
 
 template <int TEAM>
-constexpr int kEntries = TEAM >= 64 ? 1 : 4;  // of a lane; TEAM * kEntries >= K
-
-template <int TEAM>
 constexpr int kTeams = kThreads / TEAM;
 
 // Classes whose bits a team holds at once, a multiple of 32.
 template <int TEAM>
 constexpr std::uint32_t kWindow = TEAM == 4 ? 128 : TEAM == 16 ? 512 : TEAM == 64 ? 4096 : 1u << 17;
+
+__device__ __forceinline__ float weight_of(const Args& a, std::uint64_t r) {
+    return a.weight == nullptr ? 1.0f : r < a.n ? a.weight[r] : 0.0f;
+}
 
 // LDS of the workgroup.
 template <int TEAM>
@@ -79,22 +80,22 @@ struct Shared {
     double2 sums[kThreads / kWave];
 };
 
-// One team at its rows.
-template <int TEAM>
+// One team at its rows; a lane holds E of their entries.
+template <int TEAM, int E>
 struct Team {
     static constexpr int inWave = TEAM < kWave ? TEAM : kWave;
     Shared<TEAM>& lds;
     const Args& a;
     std::uint32_t* bits;
     std::uint32_t lane;
-    int turn = 0, row = 0;  // places in LDS alternate, so that one barrier a use is enough
+    int turn = 0, odd = 0;  // places in LDS alternate, so that one barrier a use is enough
     __device__ __forceinline__ Team(Shared<TEAM>& shared, const Args& args)
         : lds(shared), a(args), bits(shared.bits[threadIdx.x / TEAM]), lane(threadIdx.x % TEAM) {}
 
     // The entries of a row: lane + e TEAM < K.  Only the first wave of a
     // workgroup holds any.
-    std::int64_t id[kEntries<TEAM>];  // -1: no entry
-    float t[kEntries<TEAM>], p[kEntries<TEAM>];
+    std::int64_t id[E];  // -1: no entry
+    float t[E], p[E], z[E];  // the teacher's value and probability, the student's logit
     float top, sum, pRest, rest;  // of the teacher's values
     bool twice;  // some id occurs again
 
@@ -114,32 +115,37 @@ struct Team {
     // The maximum of a NaN is an infinity, so that its differences are NaN.
     static __device__ __forceinline__ float bound(float v) { return v != v ? -kNone : v; }
 
-    // Loads the entries of row r and the teacher's probabilities; false where
-    // the row has no target.
-    __device__ __forceinline__ bool load(std::uint64_t r) {
+    // Loads the entries of row r, with logits at `row`, and the teacher's
+    // probabilities; false where the row has no target.
+    template <typename T>
+    __device__ __forceinline__ bool load(std::uint64_t r, const T* row) {
         float m = kNone;
         bool bad = false;
 #pragma unroll
-        for (int e = 0; e < kEntries<TEAM>; ++e) {
+        for (int e = 0; e < E; ++e) {
             const std::uint32_t k = lane + e * TEAM;
             id[e] = -1;
             t[e] = kNone;
             if (k < a.K) {
-                const std::int64_t i = id_at(r, k);
-                if (is_class(i)) {
-                    id[e] = i;
-                    t[e] = value_at(r, k);
-                } else if (i != -1) {
-                    bad = true;
-                }
+                id[e] = id_at(r, k);
+                t[e] = value_at(r, k);
             }
-            m = fmaxf(m, bound(t[e]));
         }
         rest = a.rest == nullptr ? kNone : a.rest[r];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            if (!is_class(id[e])) {
+                bad |= id[e] != -1;
+                id[e] = -1;
+                t[e] = kNone;
+            }
+            z[e] = id[e] < 0 ? kNone : static_cast<float>(row[id[e]]);
+            m = fmaxf(m, bound(t[e]));
+        }
         m = fmaxf(wave_join<inWave>(m, Larger()), bound(rest));
         float s = 0.0f;
 #pragma unroll
-        for (int e = 0; e < kEntries<TEAM>; ++e) {
+        for (int e = 0; e < E; ++e) {
             p[e] = exp2_of((t[e] - base_of(m)) * a.c);
             s += p[e];
         }
@@ -147,17 +153,17 @@ struct Team {
         s += exp2_of((rest - base_of(m)) * a.c);
         if (a.error != nullptr && bad) atomicOr(a.error, TCC_DEVERR_FEATURE_INDEX);
         if constexpr (TEAM > kWave) {  // from the first wave, which holds the entries, to the others
-            if (threadIdx.x == 0) lds.one[row] = make_float2(m, s);
+            if (threadIdx.x == 0) lds.one[odd] = make_float2(m, s);
             __syncthreads();
-            m = lds.one[row].x;
-            s = lds.one[row].y;
-            row ^= 1;
+            m = lds.one[odd].x;
+            s = lds.one[odd].y;
+            odd ^= 1;
         }
         top = m;
         sum = s;
         const float per = 1.0f / s;
 #pragma unroll
-        for (int e = 0; e < kEntries<TEAM>; ++e) p[e] *= per;
+        for (int e = 0; e < E; ++e) p[e] *= per;
         pRest = exp2_of((rest - base_of(m)) * a.c) * per;
         return m != kNone;
     }
@@ -170,7 +176,7 @@ struct Team {
         team_sync<TEAM>();
         bool again = false;
 #pragma unroll
-        for (int e = 0; e < kEntries<TEAM>; ++e) {
+        for (int e = 0; e < E; ++e) {
             if (!mine(e, first)) continue;
             const std::uint32_t at = static_cast<std::uint32_t>(id[e]) - first, bit = 1u << (at & 31);
             again |= (atomicOr(&bits[at / 32], bit) & bit) != 0;
@@ -222,56 +228,90 @@ struct Team {
     }
 };
 
-template <typename T, int V, int TEAM, bool REST>
+// A batch of a team: kBatch vectors a lane, from element `base` of the row on.
+template <typename T, int V, int TEAM>
+struct Batch {
+    static constexpr std::uint32_t stride = TEAM * kBatch * V;
+    static constexpr bool whole = TEAM <= 16;  // rows of these teams are one batch
+    vec_t<T, V> x[kBatch];
+
+    static __device__ __forceinline__ Place<V> place(std::uint32_t base, int u, std::uint32_t lane, std::uint32_t C) {
+        return Place<V>(base / V + u * TEAM + lane, C);
+    }
+    // Whether any lane has a vector u.
+    static __device__ __forceinline__ bool any(std::uint32_t base, int u, std::uint32_t C) {
+        return base + static_cast<std::uint32_t>(u * TEAM * V) < C;
+    }
+    __device__ __forceinline__ void load(const T* z, std::uint32_t base, std::uint32_t lane, std::uint32_t C) {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            if (!any(base, u, C)) break;
+            const Place<V> at = place(base, u, lane, C);
+            if (at.any()) x[u] = load_global<any_vec_t<T, V>>(z + at.at);
+        }
+    }
+    __device__ __forceinline__ vec_t<float, V> values(int u) const { return __builtin_convertvector(x[u], vec_t<float, V>); }
+};
+
+template <typename T, int V, int TEAM, int E, bool REST>
 __global__ void __launch_bounds__(kThreads) loss_kernel(Args a) {
     using F = vec_t<float, V>;
+    using B = Batch<T, V, TEAM>;
+    static_assert(kWindow<TEAM> % B::stride == 0 || B::whole);
     __shared__ Shared<TEAM> lds;
-    Team<TEAM> team(lds, a);
+    Team<TEAM, E> team(lds, a);
     double lossSum = 0.0, weightSum = 0.0;
     const std::uint64_t step = static_cast<std::uint64_t>(gridDim.x) * kTeams<TEAM>;
-    for (std::uint64_t r = static_cast<std::uint64_t>(blockIdx.x) * kTeams<TEAM> + threadIdx.x / TEAM; r < a.n; r += step) {
-        const float w = a.weight == nullptr ? 1.0f : a.weight[r];
+    std::uint64_t r = static_cast<std::uint64_t>(blockIdx.x) * kTeams<TEAM> + threadIdx.x / TEAM;
+    float w = weight_of(a, r);
+    while (r < a.n) {
+        const float next = weight_of(a, r + step);
         weightSum += w;
         float loss = 0.0f;
         float4 stats = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (w != 0.0f && team.load(r)) {
-            const T* z = static_cast<const T*>(a.z) + r * a.ldz;
+        const T* z = static_cast<const T*>(a.z) + r * a.ldz;
+        B batch;
+        if (w != 0.0f) batch.load(z, 0, team.lane, a.C);
+        if (w != 0.0f && team.load(r, z)) {
             Share v, firsts;  // of the stream, and of the ids that are not in it
-            for (std::uint32_t first = 0; first < a.C; first += kWindow<TEAM>) {
-                if (REST) team.mark(first);
-                const std::uint32_t end = min(a.C - first, kWindow<TEAM>) + first;
-                for (std::uint32_t j = first / V + team.lane; static_cast<std::uint64_t>(j) * V < end; j += TEAM * kBatch) {
-                    F x[kBatch];
-                    float m = kNone;
+            for (std::uint32_t base = 0; base < a.C; base += B::stride) {
+                const std::uint32_t first = base & ~(kWindow<TEAM> - 1);
+                if (REST && first == base) {
+                    team.mark(first);
 #pragma unroll
-                    for (int u = 0; u < kBatch; ++u) {
-                        const Place<V> at(j + u * TEAM, a.C);
-                        const bool here = at.any() && static_cast<std::uint64_t>(j + u * TEAM) * V < end;
-                        x[u] = here ? load_any<T, V>(z + at.at) : F(kNone);
-                        std::uint32_t out = here ? (1u << at.skip) - 1 : 0;
-                        if (REST && here) out |= team.template marked<V>(at.at + at.skip - first) << at.skip;
-                        if (out != 0) {
-#pragma unroll
-                            for (int q = 0; q < V; ++q) x[u][q] = (out >> q) & 1 ? kNone : x[u][q];
-                        }
-#pragma unroll
-                        for (int q = 0; q < V; ++q) m = fmaxf(m, x[u][q]);
-                    }
-                    if (m > v.m) v.scale_to(m, a.c);
-                    const float b = base_of(v.m);
-#pragma unroll
-                    for (int u = 0; u < kBatch; ++u)
-#pragma unroll
-                        for (int q = 0; q < V; ++q) v.s += exp2_of((x[u][q] - b) * a.c);
-                }
-                if (REST) {
-#pragma unroll
-                    for (int e = 0; e < kEntries<TEAM>; ++e) {
+                    for (int e = 0; e < E; ++e) {
                         float unused;
-                        if (team.mine(e, first) && team.leads(e, r, unused))
-                            firsts = firsts.with({static_cast<float>(z[team.id[e]]), 1.0f}, a.c);
+                        if (team.mine(e, first) && team.leads(e, r, unused)) firsts = firsts.with({team.z[e], 1.0f}, a.c);
                     }
                 }
+                B after;
+                if constexpr (!B::whole) after.load(z, base + B::stride, team.lane, a.C);
+                F x[kBatch];
+                float m = kNone;
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u) {
+                    if (!B::any(base, u, a.C)) break;
+                    const Place<V> at = B::place(base, u, team.lane, a.C);
+                    x[u] = batch.values(u);
+                    std::uint32_t out = (1u << at.skip) - 1;
+                    if (REST && at.any()) out |= team.template marked<V>(at.at + at.skip - first) << at.skip;
+                    if (out != 0) {
+#pragma unroll
+                        for (int q = 0; q < V; ++q) x[u][q] = (out >> q) & 1 ? kNone : x[u][q];
+                    }
+#pragma unroll
+                    for (int q = 0; q < V; ++q) m = fmaxf(m, x[u][q]);
+                }
+                if (m > v.m) v.scale_to(m, a.c);
+                const float b = base_of(v.m);
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u) {
+                    if (!B::any(base, u, a.C)) break;
+#pragma unroll
+                    for (int q = 0; q < V; ++q) v.s += exp2_of((x[u][q] - b) * a.c);
+                }
+                if constexpr (B::whole) break;
+                batch = after;
             }
             const Share others = team.join(v);
             const Share all = REST ? others.with(team.join(firsts), a.c) : others;
@@ -279,12 +319,12 @@ __global__ void __launch_bounds__(kThreads) loss_kernel(Args a) {
             const float b = base_of(all.m), tb = base_of(team.top), sums = logAll.over(logTop);
             float sum = 0.0f;
 #pragma unroll
-            for (int e = 0; e < kEntries<TEAM>; ++e) {
+            for (int e = 0; e < E; ++e) {
                 if (team.id[e] < 0 || team.p[e] == 0.0f) continue;
-                const float apart = (team.t[e] - tb) * a.c - (static_cast<float>(z[team.id[e]]) - b) * a.c;
+                const float apart = (team.t[e] - tb) * a.c - (team.z[e] - b) * a.c;
                 sum += team.p[e] * (apart + sums);
             }
-            sum = wave_join<Team<TEAM>::inWave>(sum, Add());
+            sum = wave_join<Team<TEAM, E>::inWave>(sum, Add());
             if (REST && team.pRest != 0.0f) {
                 const float apart = (team.rest - tb) * a.c - (base_of(others.m) - b) * a.c;
                 sum += team.pRest * (apart + (sums - Log2(others.s).over(Log2(1.0f))));
@@ -297,6 +337,8 @@ __global__ void __launch_bounds__(kThreads) loss_kernel(Args a) {
             if (a.loss != nullptr) a.loss[r] = loss;
             lossSum += loss;
         }
+        w = next;
+        r += step;
     }
     if (a.part == nullptr) return;
     // the first lanes' sums, in the order of the teams
@@ -341,11 +383,12 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const double2* part, std
     if (total != nullptr) *total = static_cast<float>(w);
 }
 
-template <typename T, int V, int TEAM, bool REST>
+template <typename T, int V, int TEAM, int E, bool REST>
 __global__ void __launch_bounds__(kThreads) grad_kernel(Args a) {
     using F = vec_t<float, V>;
+    using B = Batch<T, V, TEAM>;
     __shared__ Shared<TEAM> lds;
-    Team<TEAM> team(lds, a);
+    Team<TEAM, E> team(lds, a);
     float each = a.T;
     if (a.reduction == TCC_REDUCE_MEAN) {
         const float count = a.total == nullptr ? static_cast<float>(a.n) : *a.total;
@@ -353,85 +396,98 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(Args a) {
     }
     if (a.reduction != TCC_REDUCE_NONE) each *= *a.dLoss;
     const std::uint64_t step = static_cast<std::uint64_t>(gridDim.x) * kTeams<TEAM>;
-    for (std::uint64_t r = static_cast<std::uint64_t>(blockIdx.x) * kTeams<TEAM> + threadIdx.x / TEAM; r < a.n; r += step) {
-        const float w = a.weight == nullptr ? 1.0f : a.weight[r];
+    std::uint64_t r = static_cast<std::uint64_t>(blockIdx.x) * kTeams<TEAM> + threadIdx.x / TEAM;
+    float w = weight_of(a, r);
+    while (r < a.n) {
+        const float next = weight_of(a, r + step);
         const T* z = static_cast<const T*>(a.z) + r * a.ldz;
         T* dz = static_cast<T*>(a.dz) + r * a.ldd;
-        const bool target = w != 0.0f && team.load(r);
+        B batch;
+        if (w != 0.0f) batch.load(z, 0, team.lane, a.C);
         const float4 stats = a.stats[r];
-        float g = each * w, base = stats.x, factor;
+        float g = each * w;
         if (a.reduction == TCC_REDUCE_NONE) g *= a.dLoss[r];
+        const bool target = w != 0.0f && team.load(r, z);
+        float base2 = stats.x, factor;  // of the others: factor 2^((z - base2) c)
         if (REST) {
             const float left = exp2_of((stats.z - stats.x) * a.c) * stats.w / stats.y - team.pRest;
-            base = stats.z;
+            base2 = stats.z;
             factor = stats.w == 0.0f ? 0.0f : g * left / stats.w;
         } else {
             factor = g / stats.y;
         }
-        for (std::uint32_t first = 0; first < a.C; first += kWindow<TEAM>) {
-            if (target) team.mark(first);
-            const std::uint32_t end = min(a.C - first, kWindow<TEAM>) + first;
-            for (std::uint32_t j = first / V + team.lane; static_cast<std::uint64_t>(j) * V < end; j += TEAM * kBatch) {
-                F x[kBatch];
+        for (std::uint32_t base = 0; base < a.C; base += B::stride) {
+            const std::uint32_t first = base & ~(kWindow<TEAM> - 1);
+            if (target && first == base) {
+                team.mark(first);
 #pragma unroll
-                for (int u = 0; u < kBatch; ++u) {
-                    const Place<V> at(j + u * TEAM, a.C);
-                    const bool here = target && at.any() && static_cast<std::uint64_t>(j + u * TEAM) * V < end;
-                    x[u] = here ? load_any<T, V>(z + at.at) : F(0.0f);
-                }
-#pragma unroll
-                for (int u = 0; u < kBatch; ++u) {
-                    const Place<V> at(j + u * TEAM, a.C);
-                    if (!at.any() || static_cast<std::uint64_t>(j + u * TEAM) * V >= end) continue;
-                    F d(0.0f);
-                    std::uint32_t out = (1u << at.skip) - 1;
-                    if (target) {
-                        out |= team.template marked<V>(at.at + at.skip - first) << at.skip;
-#pragma unroll
-                        for (int q = 0; q < V; ++q) d[q] = factor * exp2_of((x[u][q] - base) * a.c);
-                    }
-                    if (out == 0) {
-                        store_any<T, V>(dz + at.at, d);
-                    } else {
-#pragma unroll
-                        for (int q = 0; q < V; ++q)
-                            if (((out >> q) & 1) == 0) dz[at.at + q] = static_cast<T>(d[q]);
-                    }
+                for (int e = 0; e < E; ++e) {
+                    float p;
+                    if (!team.mine(e, first) || !team.leads(e, r, p)) continue;
+                    const float q = exp2_of((team.z[e] - stats.x) * a.c) / stats.y;
+                    dz[team.id[e]] = static_cast<T>(g * (q - p));
                 }
             }
-            if (!target) continue;
-#pragma unroll
-            for (int e = 0; e < kEntries<TEAM>; ++e) {
-                float p;
-                if (!team.mine(e, first) || !team.leads(e, r, p)) continue;
-                const float q = exp2_of((static_cast<float>(z[team.id[e]]) - stats.x) * a.c) / stats.y;
-                dz[team.id[e]] = static_cast<T>(g * (q - p));
+            B after;
+            if constexpr (!B::whole) {
+                if (target) after.load(z, base + B::stride, team.lane, a.C);
             }
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                if (!B::any(base, u, a.C)) break;
+                const Place<V> at = B::place(base, u, team.lane, a.C);
+                if (!at.any()) continue;
+                F d(0.0f);
+                std::uint32_t out = (1u << at.skip) - 1;
+                if (target) {
+                    const F x = batch.values(u);
+                    out |= team.template marked<V>(at.at + at.skip - first) << at.skip;
+#pragma unroll
+                    for (int q = 0; q < V; ++q) d[q] = factor * exp2_of((x[q] - base2) * a.c);
+                }
+                if (out == 0) {
+                    store_any<T, V>(dz + at.at, d);
+                } else {
+#pragma unroll
+                    for (int q = 0; q < V; ++q)
+                        if (((out >> q) & 1) == 0) dz[at.at + q] = static_cast<T>(d[q]);
+                }
+            }
+            if constexpr (B::whole) break;
+            batch = after;
         }
+        w = next;
+        r += step;
     }
 }
 
 // ---------------------------------------------------------------- launches
 
-// The team for rows of C classes and K entries; f is called with <V, TEAM>.
+// The team for rows of C classes and K entries; f is called with <V, TEAM, E>.
 // A team's lanes take one batch of a row where it can be, and a wave up to
-// 4,096 classes; they hold K / 4 lanes at least.
+// 4,096 classes; they have room for the entries.
 template <typename T, typename F>
 void with_team(std::uint32_t C, std::uint32_t K, F f) {
     constexpr int V = kVec<T>;
     if (C < V) {
-        if (K <= 16) return f.template operator()<1, 4>();
-        return f.template operator()<1, 16>();
+        if (K <= 4) return f.template operator()<1, 4, 1>();
+        return f.template operator()<1, 16, 4>();
     }
-    if (C <= 4 * kBatch * V && C <= kWindow<4> && K <= 16) return f.template operator()<V, 4>();
-    if (C <= 16 * kBatch * V && C <= kWindow<16>) return f.template operator()<V, 16>();
-    if (C <= 4096) return f.template operator()<V, 64>();
-    return f.template operator()<V, 256>();
+    if (C <= 4 * kBatch * V && C <= kWindow<4> && K <= 4) return f.template operator()<V, 4, 1>();
+    if (C <= 16 * kBatch * V && C <= kWindow<16>) {
+        if (K <= 16) return f.template operator()<V, 16, 1>();
+        return f.template operator()<V, 16, 4>();
+    }
+    if (C <= 4096) return f.template operator()<V, 64, 1>();
+    return f.template operator()<V, 256, 1>();
 }
 
-// Workgroups for n rows: eight a compute unit at most, each with as many rows.
-std::uint64_t blocks_of(std::uint64_t n, std::uint64_t teams) {
-    return std::min<std::uint64_t>((n + teams - 1) / teams, 8ull * device_cus());
+// A grid of the workgroups that run at once, or those that n rows need.
+template <typename Kernel>
+std::uint64_t launch(Kernel kernel, std::uint32_t& perCu, const Args& a, std::uint64_t teams, hipStream_t st) {
+    const std::uint64_t blocks = std::min<std::uint64_t>((a.n + teams - 1) / teams, resident_blocks(kernel, kThreads, perCu));
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st, a);
+    return blocks;
 }
 
 template <typename T>
@@ -439,23 +495,22 @@ struct Loss {
     const Args& a;
     hipStream_t st;
     std::uint64_t& blocks;
-    template <int V, int TEAM>
+    template <int V, int TEAM, int E>
     void operator()() const {
-        blocks = blocks_of(a.n, kTeams<TEAM>);
-        const dim3 grid(static_cast<unsigned>(blocks));
-        if (a.rest != nullptr) hipLaunchKernelGGL((loss_kernel<T, V, TEAM, true>), grid, dim3(kThreads), 0, st, a);
-        else hipLaunchKernelGGL((loss_kernel<T, V, TEAM, false>), grid, dim3(kThreads), 0, st, a);
+        static std::uint32_t perCu[2];
+        blocks = a.rest != nullptr ? launch(loss_kernel<T, V, TEAM, E, true>, perCu[1], a, kTeams<TEAM>, st)
+                                   : launch(loss_kernel<T, V, TEAM, E, false>, perCu[0], a, kTeams<TEAM>, st);
     }
 };
 template <typename T>
 struct Grad {
     const Args& a;
     hipStream_t st;
-    template <int V, int TEAM>
+    template <int V, int TEAM, int E>
     void operator()() const {
-        const dim3 grid(static_cast<unsigned>(blocks_of(a.n, kTeams<TEAM>)));
-        if (a.rest != nullptr) hipLaunchKernelGGL((grad_kernel<T, V, TEAM, true>), grid, dim3(kThreads), 0, st, a);
-        else hipLaunchKernelGGL((grad_kernel<T, V, TEAM, false>), grid, dim3(kThreads), 0, st, a);
+        static std::uint32_t perCu[2];
+        if (a.rest != nullptr) launch(grad_kernel<T, V, TEAM, E, true>, perCu[1], a, kTeams<TEAM>, st);
+        else launch(grad_kernel<T, V, TEAM, E, false>, perCu[0], a, kTeams<TEAM>, st);
     }
 };
 
