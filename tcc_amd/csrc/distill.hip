@@ -19,7 +19,8 @@
 // confident student leaves them): one bit of a class in LDS says that it is an
 // id, and their logits are taken out of the stream and added afterwards.
 // The gradient's stream leaves out the ids in the same way, and the lanes that
-// hold the entries write there.
+// hold the entries write there; teams that hold a whole row in registers get the
+// entries' gradients from a table of its classes in LDS instead.
 #include <algorithm>
 
 #include "../../include/tcc_spmm_cnic.h"
@@ -94,7 +95,7 @@ struct Team {
 
     // The entries of a row: lane + e TEAM < K.  Only the first wave of a
     // workgroup holds any.
-    std::int64_t id[E];  // -1: no entry
+    std::int32_t id[E];  // -1: no entry
     float t[E], p[E], z[E];  // the teacher's value and probability, the student's logit
     float top, sum, pRest, rest;  // of the teacher's values
     bool twice;  // some id occurs again
@@ -127,18 +128,16 @@ struct Team {
             id[e] = -1;
             t[e] = kNone;
             if (k < a.K) {
-                id[e] = id_at(r, k);
+                const std::int64_t i = id_at(r, k);
+                id[e] = is_class(i) ? static_cast<std::int32_t>(i) : -1;
+                bad |= id[e] < 0 && i != -1;
                 t[e] = value_at(r, k);
             }
         }
         rest = a.rest == nullptr ? kNone : a.rest[r];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            if (!is_class(id[e])) {
-                bad |= id[e] != -1;
-                id[e] = -1;
-                t[e] = kNone;
-            }
+            if (id[e] < 0) t[e] = kNone;
             z[e] = id[e] < 0 ? kNone : static_cast<float>(row[id[e]]);
             m = fmaxf(m, bound(t[e]));
         }
@@ -161,7 +160,7 @@ struct Team {
         }
         top = m;
         sum = s;
-        const float per = 1.0f / s;
+        const float per = inverse_of(s);
 #pragma unroll
         for (int e = 0; e < E; ++e) p[e] *= per;
         pRest = exp2_of((rest - base_of(m)) * a.c) * per;
@@ -196,7 +195,7 @@ struct Team {
         for (std::uint32_t o = 0; o < a.K; ++o) {
             if (id_at(r, o) != id[e]) continue;
             if (o < k) return false;
-            all += exp2_of((value_at(r, o) - base_of(top)) * a.c) / sum;
+            all += exp2_of((value_at(r, o) - base_of(top)) * a.c) * inverse_of(sum);
         }
         return true;
     }
@@ -227,6 +226,9 @@ struct Team {
         return v;
     }
 };
+
+// A NaN that no operation gives: a class that no entry has.
+constexpr std::uint32_t kNoEntry = 0x7FD00001u;
 
 // A batch of a team: kBatch vectors a lane, from element `base` of the row on.
 template <typename T, int V, int TEAM>
@@ -388,6 +390,7 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(Args a) {
     using F = vec_t<float, V>;
     using B = Batch<T, V, TEAM>;
     __shared__ Shared<TEAM> lds;
+    __shared__ __attribute__((aligned(16))) float table[B::whole ? kTeams<TEAM> : 1][B::whole ? B::stride : V];
     Team<TEAM, E> team(lds, a);
     float each = a.T;
     if (a.reduction == TCC_REDUCE_MEAN) {
@@ -408,53 +411,92 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(Args a) {
         float g = each * w;
         if (a.reduction == TCC_REDUCE_NONE) g *= a.dLoss[r];
         const bool target = w != 0.0f && team.load(r, z);
+        const float perAll = inverse_of(stats.y);
         float base2 = stats.x, factor;  // of the others: factor 2^((z - base2) c)
         if (REST) {
-            const float left = exp2_of((stats.z - stats.x) * a.c) * stats.w / stats.y - team.pRest;
+            const float left = exp2_of((stats.z - stats.x) * a.c) * stats.w * perAll - team.pRest;
             base2 = stats.z;
-            factor = stats.w == 0.0f ? 0.0f : g * left / stats.w;
+            factor = stats.w == 0.0f ? 0.0f : g * left * inverse_of(stats.w);
         } else {
-            factor = g / stats.y;
+            factor = g * perAll;
         }
-        for (std::uint32_t base = 0; base < a.C; base += B::stride) {
-            const std::uint32_t first = base & ~(kWindow<TEAM> - 1);
-            if (target && first == base) {
-                team.mark(first);
+        const auto entry = [&](float x, float p) { return g * (exp2_of((x - stats.x) * a.c) * perAll - p); };
+        if constexpr (B::whole) {
+            // the entries' gradients by their classes, so that every vector is stored once
+            float* mine = table[threadIdx.x / TEAM];
+            if (target) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    float p;
-                    if (!team.mine(e, first) || !team.leads(e, r, p)) continue;
-                    const float q = exp2_of((team.z[e] - stats.x) * a.c) / stats.y;
-                    dz[team.id[e]] = static_cast<T>(g * (q - p));
+                for (int u = 0; u < kBatch; ++u)
+                    if (B::any(0, u, a.C))
+                        *reinterpret_cast<F*>(mine + (u * TEAM + team.lane) * V) = F(__uint_as_float(kNoEntry));
+                team_sync<TEAM>();
+                bool again = false;
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (team.id[e] >= 0)
+                        again |= __float_as_uint(atomicExch(mine + team.id[e], entry(team.z[e], team.p[e]))) != kNoEntry;
+                team.twice = __ballot(again) != 0;
+                team_sync<TEAM>();
+                if (team.twice) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        float p;
+                        if (team.id[e] >= 0 && team.leads(e, r, p)) mine[team.id[e]] = entry(team.z[e], p);
+                    }
+                    team_sync<TEAM>();
                 }
-            }
-            B after;
-            if constexpr (!B::whole) {
-                if (target) after.load(z, base + B::stride, team.lane, a.C);
             }
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) {
-                if (!B::any(base, u, a.C)) break;
-                const Place<V> at = B::place(base, u, team.lane, a.C);
+                if (!B::any(0, u, a.C)) break;
+                const Place<V> at = B::place(0, u, team.lane, a.C);
                 if (!at.any()) continue;
                 F d(0.0f);
-                std::uint32_t out = (1u << at.skip) - 1;
                 if (target) {
-                    const F x = batch.values(u);
-                    out |= team.template marked<V>(at.at + at.skip - first) << at.skip;
-#pragma unroll
-                    for (int q = 0; q < V; ++q) d[q] = factor * exp2_of((x[q] - base2) * a.c);
-                }
-                if (out == 0) {
-                    store_any<T, V>(dz + at.at, d);
-                } else {
+                    const F x = batch.values(u), known = *reinterpret_cast<const any_vec_t<float, V>*>(mine + at.at);
 #pragma unroll
                     for (int q = 0; q < V; ++q)
-                        if (((out >> q) & 1) == 0) dz[at.at + q] = static_cast<T>(d[q]);
+                        d[q] = __float_as_uint(known[q]) == kNoEntry ? factor * exp2_of((x[q] - base2) * a.c) : known[q];
                 }
+                store_any<T, V>(dz + at.at, d);
             }
-            if constexpr (B::whole) break;
-            batch = after;
+        } else {
+            for (std::uint32_t base = 0; base < a.C; base += B::stride) {
+                const std::uint32_t first = base & ~(kWindow<TEAM> - 1);
+                if (target && first == base) {
+                    team.mark(first);
+    #pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        float p;
+                        if (!team.mine(e, first) || !team.leads(e, r, p)) continue;
+                        dz[team.id[e]] = static_cast<T>(entry(team.z[e], p));
+                    }
+                }
+                B after;
+                if (target) after.load(z, base + B::stride, team.lane, a.C);
+    #pragma unroll
+                for (int u = 0; u < kBatch; ++u) {
+                    if (!B::any(base, u, a.C)) break;
+                    const Place<V> at = B::place(base, u, team.lane, a.C);
+                    if (!at.any()) continue;
+                    F d(0.0f);
+                    std::uint32_t out = (1u << at.skip) - 1;
+                    if (target) {
+                        const F x = batch.values(u);
+                        out |= team.template marked<V>(at.at + at.skip - first) << at.skip;
+    #pragma unroll
+                        for (int q = 0; q < V; ++q) d[q] = factor * exp2_of((x[q] - base2) * a.c);
+                    }
+                    if (out == 0) {
+                        store_any<T, V>(dz + at.at, d);
+                    } else {
+    #pragma unroll
+                        for (int q = 0; q < V; ++q)
+                            if (((out >> q) & 1) == 0) dz[at.at + q] = static_cast<T>(d[q]);
+                    }
+                }
+                batch = after;
+            }
         }
         w = next;
         r += step;

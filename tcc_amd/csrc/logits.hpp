@@ -10,6 +10,7 @@ constexpr float kNone = -__builtin_huge_valf();  // the logit of nothing
 
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log2_of(float x) { return __builtin_amdgcn_logf(x); }
+__device__ __forceinline__ float inverse_of(float x) { return __builtin_amdgcn_rcpf(x); }
 // log2(x) as a whole number and a fraction of [-1, 0): differences of two keep the
 // digits that the logarithm of a large sum rounds away (v_log_f32 does so to one
 // side, which the mean of many rows does not even out).
@@ -41,10 +42,11 @@ struct Share {
 template <int V>
 struct Place {
     std::uint32_t at, skip;  // first element, and how many of them are another vector's (V: all)
+    // (a row has fewer than 2^31 elements, and vectors a batch past its end)
     __device__ __forceinline__ Place(std::uint32_t vector, std::uint32_t C) {
-        const std::uint64_t c = static_cast<std::uint64_t>(vector) * V;
-        at = static_cast<std::uint32_t>(min<std::uint64_t>(c, C - V));
-        skip = static_cast<std::uint32_t>(min<std::uint64_t>(c - at, V));
+        const std::uint32_t c = vector * V, last = C - V;
+        at = c < last ? c : last;
+        skip = c - at < V ? c - at : V;
     }
     __device__ __forceinline__ bool any() const { return skip < V; }
 };
