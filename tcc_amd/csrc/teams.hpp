@@ -6,6 +6,38 @@
 
 namespace tcc {
 
+// v of the lane whose number differs in bit D (16 or 32).
+template <int D>
+__device__ __forceinline__ std::uint32_t swapped(std::uint32_t v) {
+    static_assert(D == 16 || D == 32);
+    if constexpr (D == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return (__lane_id() & 16) ? r[0] : r[1];
+    } else {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return (__lane_id() & 32) ? r[0] : r[1];
+    }
+}
+
+// v of the lane whose number differs in bit D, whatever its neighbours hold.
+template <int D>
+__device__ __forceinline__ std::uint32_t other(std::uint32_t v) {
+    const int i = static_cast<int>(v);
+    if constexpr (D == 1) return __builtin_amdgcn_update_dpp(i, i, 0xB1, 0xF, 0xF, false);  // quad_perm [1,0,3,2]
+    if constexpr (D == 2) return __builtin_amdgcn_update_dpp(i, i, 0x4E, 0xF, 0xF, false);  // quad_perm [2,3,0,1]
+    if constexpr (D == 4) {  // row_half_mirror, then quad_perm [3,2,1,0]: 7 - i, then ^ 3
+        const int h = __builtin_amdgcn_update_dpp(i, i, 0x141, 0xF, 0xF, false);
+        return __builtin_amdgcn_update_dpp(h, h, 0x1B, 0xF, 0xF, false);
+    }
+    if constexpr (D == 8) return __builtin_amdgcn_update_dpp(i, i, 0x128, 0xF, 0xF, false);  // row_ror:8
+    if constexpr (D >= 16) return swapped<D>(v);
+}
+template <int D>
+__device__ __forceinline__ std::uint64_t other(std::uint64_t v) {
+    const std::uint64_t lo = other<D>(static_cast<std::uint32_t>(v)), hi = other<D>(static_cast<std::uint32_t>(v >> 32));
+    return hi << 32 | lo;
+}
+
 // v of the lane at distance D (1 to 32, a power of two) by exclusive or,
 // provided that v is already the same within aligned groups of D lanes: lanes
 // are mirrored then instead of exchanged, which costs one instruction without
@@ -18,7 +50,7 @@ __device__ __forceinline__ std::uint32_t across(std::uint32_t v) {
     if constexpr (D == 2) return __builtin_amdgcn_update_dpp(i, i, 0x4E, 0xF, 0xF, false);   // quad_perm [2,3,0,1]
     if constexpr (D == 4) return __builtin_amdgcn_update_dpp(i, i, 0x141, 0xF, 0xF, false);  // row_half_mirror
     if constexpr (D == 8) return __builtin_amdgcn_update_dpp(i, i, 0x140, 0xF, 0xF, false);  // row_mirror
-    if constexpr (D >= 16) return static_cast<std::uint32_t>(__shfl_xor(i, D, kWave));
+    if constexpr (D >= 16) return swapped<D>(v);
 }
 template <int D>
 __device__ __forceinline__ float across(float v) { return __uint_as_float(across<D>(__float_as_uint(v))); }
@@ -41,6 +73,9 @@ __device__ __forceinline__ V wave_join(V v, F f) {
 struct Add {
     template <typename V>
     __device__ __forceinline__ V operator()(V a, V b) const { return a + b; }
+};
+struct Smaller {
+    __device__ __forceinline__ float operator()(float a, float b) const { return fminf(a, b); }
 };
 struct Larger {
     __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }

@@ -57,31 +57,23 @@ __device__ __forceinline__ Key key_of(float v, std::uint32_t index) {
 }
 __device__ __forceinline__ std::uint32_t index_of(Key k) { return ~static_cast<std::uint32_t>(k); }
 
-template <typename K>
-__device__ __forceinline__ K pair_step(K v, int d, bool larger) {
-    const K o = __shfl_xor(v, d, kWave);
-    return (v > o) == larger ? v : o;
-}
-// Sorted over the lanes, a bitonic network: the larger first if `down`.
-template <typename K>
-__device__ __forceinline__ K wave_sort(K v, bool down) {
+// The steps of a bitonic network from distance D on, in runs of SIZE lanes that
+// alternate in direction: the larger first in the first run if DOWN.
+template <int SIZE, bool DOWN, int D, typename K>
+__device__ __forceinline__ K wave_steps(K v) {
     const unsigned l = lane_id();
-#pragma unroll
-    for (int size = 2; size <= kWave; size <<= 1)
-#pragma unroll
-        for (int d = size / 2; d > 0; d >>= 1) {
-            const bool first = (l & d) == 0, forward = size == kWave || (l & size) == 0;
-            v = pair_step(v, d, (first == forward) == down);
-        }
-    return v;
+    const K o = other<D>(v);
+    const bool first = (l & D) == 0, forward = SIZE == kWave || (l & SIZE) == 0;
+    v = (v > o) == ((first == forward) == DOWN) ? v : o;
+    if constexpr (D > 1) return wave_steps<SIZE, DOWN, D / 2>(v);
+    else return v;
 }
-// A bitonic sequence sorted down.
-template <typename K>
-__device__ __forceinline__ K wave_merge_down(K v) {
-    const unsigned l = lane_id();
-#pragma unroll
-    for (int d = kWave / 2; d > 0; d >>= 1) v = pair_step(v, d, (l & d) == 0);
-    return v;
+// Sorted over the lanes.
+template <bool DOWN, int SIZE = 2, typename K>
+__device__ __forceinline__ K wave_sort(K v) {
+    v = wave_steps<SIZE, DOWN, SIZE / 2>(v);
+    if constexpr (SIZE < kWave) return wave_sort<DOWN, 2 * SIZE>(v);
+    else return v;
 }
 
 struct Buffer {
@@ -105,7 +97,7 @@ struct Top {
     // Takes in a list that is sorted up.
     __device__ __forceinline__ void take(Key up) {
         const Key low = list > up ? up : list;
-        list = wave_merge_down(list > up ? list : up);
+        list = wave_steps<kWave, true, kWave / 2>(list > up ? list : up);
         drop(low);
         if (lane_id() >= a.K) {
             drop(list);
@@ -124,7 +116,7 @@ struct Top {
         if (count == 0) return;
         sync();
         const Key mine = lane_id() < count ? buffer.k[lane_id()] : 0;
-        take(wave_sort(mine, false));
+        take(wave_sort<false>(mine));
         count = 0;
     }
     __device__ __forceinline__ void sync() const {
@@ -138,12 +130,38 @@ struct Top {
         count += __popcll(all);
         if (count < kWave) return;
         sync();
-        take(wave_sort(buffer.k[lane_id()], false));
+        take(wave_sort<false>(buffer.k[lane_id()]));
         const Key left = buffer.k[kWave + lane_id()];
         sync();
         buffer.k[lane_id()] = left;
         count -= kWave;
         sync();
+    }
+};
+
+// Element b of N (a power of two).
+template <int N, typename A>
+__device__ __forceinline__ float pick(const A& v, std::uint32_t b) {
+    float s[N];
+#pragma unroll
+    for (int q = 0; q < N; ++q) s[q] = v[q];
+#pragma unroll
+    for (int d = 1; d < N; d <<= 1)
+#pragma unroll
+        for (int q = 0; q < N; q += 2 * d) s[q] = b & d ? s[q + d] : s[q];
+    return s[0];
+}
+
+// The vectors first + lane, and those step, 2 step, ... after them, of a row.
+template <typename T, int V>
+struct Ahead {
+    vec_t<T, V> x[kBatch];
+    __device__ __forceinline__ void load(const T* z, std::uint32_t first, std::uint32_t step, std::uint32_t C) {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const Place<V> at(first + lane_id() + u * step, C);
+            if (at.any()) x[u] = load_as<T, V>(z + at.at);
+        }
     }
 };
 
@@ -153,45 +171,58 @@ __device__ __forceinline__ void scan(Top& top, const T* z, std::uint32_t first, 
     using F = vec_t<float, V>;
     const Args& a = top.a;
     bool begun = false;
-    for (std::uint64_t j = first; j * V < a.C; j += static_cast<std::uint64_t>(step) * kBatch) {  // of the wave's first lane
+    Ahead<T, V> ahead;
+    ahead.load(z, first, step, a.C);
+    for (std::uint32_t j = first; j * V < a.C; j += step * kBatch) {  // of the wave's first lane
         F x[kBatch];
+        float most[kBatch];  // of a vector; a NaN where it has one
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-            const Place<V> at(static_cast<std::uint32_t>(j + lane_id() + u * step), a.C);
-            x[u] = at.any() ? load_any<T, V>(z + at.at) : F(kNone);
+            const Place<V> at(j + lane_id() + u * step, a.C);
+            x[u] = __builtin_convertvector(ahead.x[u], F);
+            if (at.skip != 0) {
+#pragma unroll
+                for (std::uint32_t q = 0; q < V; ++q) x[u][q] = q < at.skip ? kNone : x[u][q];
+            }
+            most[u] = x[u][0];
+#pragma unroll
+            for (int q = 1; q < V; ++q) most[u] = __builtin_elementwise_maximum(most[u], x[u][q]);
         }
+        ahead.load(z, j + step * kBatch, step, a.C);
         if (!begun) {  // a first bound
             begun = true;
-            std::uint32_t own = 0;
+            float own = kNone;
 #pragma unroll
-            for (int u = 0; u < kBatch; ++u) {
-                const Place<V> at(static_cast<std::uint32_t>(j + lane_id() + u * step), a.C);
-#pragma unroll
-                for (std::uint32_t q = 0; q < V; ++q) own = max(own, q >= at.skip ? order_of(x[u][q]) : 0u);
-            }
-            const std::uint32_t last = static_cast<std::uint32_t>(__shfl(static_cast<int>(wave_sort(own, true)), a.K - 1, kWave));
-            if (last != 0) top.raise(last - 1);  // itself may be one of the K
+            for (int u = 0; u < kBatch; ++u) own = __builtin_elementwise_maximum(own, most[u]);
+            const std::uint32_t last =
+                static_cast<std::uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(wave_sort<true>(order_of(own))), a.K - 1));
+            top.raise(last - 1);  // itself may be one of the K
         }
         float m = kNone;
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-            const Place<V> at(static_cast<std::uint32_t>(j + lane_id() + u * step), a.C);
             // larger than the bound at the start of this vector: elements equal to a
             // bound from among these may come before it in the row
             const float bound = top.bound;
-            std::uint32_t larger = 0;
+            if (__ballot(!(most[u] <= bound)) != 0) {
+                const Place<V> at(j + lane_id() + u * step, a.C);
+                std::uint32_t larger = 0;
 #pragma unroll
-            for (std::uint32_t q = 0; q < V; ++q) larger |= (q >= at.skip && !(x[u][q] <= bound) ? 1u : 0u) << q;
-            if (__ballot(larger != 0) != 0) {
+                for (std::uint32_t q = 0; q < V; ++q) larger |= (q >= at.skip && !(x[u][q] <= bound) ? 1u : 0u) << q;
+                std::uint32_t left = larger;
+                while (__ballot(left != 0) != 0) {
+                    const std::uint32_t q = left != 0 ? __builtin_ctz(left) : 0u;
+                    top.push(left != 0, pick<V>(x[u], q), at.at + q);
+                    left &= left - 1;
+                }
+                most[u] = kNone;
 #pragma unroll
-                for (std::uint32_t q = 0; q < V; ++q) top.push((larger >> q) & 1, x[u][q], at.at + q);
+                for (int q = 0; q < V; ++q) {
+                    x[u][q] = (larger >> q) & 1 ? kNone : x[u][q];
+                    most[u] = fmaxf(most[u], x[u][q]);
+                }
             }
-            if (at.skip != 0) larger |= (1u << at.skip) - 1;
-#pragma unroll
-            for (int q = 0; q < V; ++q) {
-                x[u][q] = (larger >> q) & 1 ? kNone : x[u][q];
-                m = fmaxf(m, x[u][q]);
-            }
+            m = fmaxf(m, most[u]);
         }
         if (m > top.rest.m) top.rest.scale_to(m, a.c);
         const float b = base_of(top.rest.m);
@@ -264,16 +295,177 @@ __global__ void __launch_bounds__(kThreads) block_kernel(Args a) {
     }
 }
 
+// ---------------------------------------------------------------- rows in registers
+
+// How many lanes of a team have a larger v.
+template <int TEAM, int D = 1>
+__device__ __forceinline__ std::uint32_t larger_lanes(float v) {
+    static_assert(TEAM == 4 || TEAM == 16);
+    constexpr int turn = TEAM == 16 ? 0x120 + D : D == 1 ? 0x39 : D == 2 ? 0x4E : 0x93;  // row_ror:D, quad_perm turned by D
+    const int i = static_cast<int>(__float_as_uint(v));
+    const float o = __uint_as_float(static_cast<std::uint32_t>(__builtin_amdgcn_update_dpp(i, i, turn, 0xF, 0xF, false)));
+    const std::uint32_t one = o > v ? 1u : 0u;
+    if constexpr (D + 1 < TEAM) return one + larger_lanes<TEAM, D + 1>(v);
+    else return one;
+}
+
+// The K-th largest of a team's v (of K <= TEAM), in all its lanes.
+template <int TEAM>
+__device__ __forceinline__ float kth_largest(float v, std::uint32_t K) {
+    if constexpr (TEAM == kWave) {
+        return value_of(static_cast<std::uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(wave_sort<true>(order_of(v))), K - 1)));
+    } else {
+        return wave_join<TEAM>(larger_lanes<TEAM>(v) < K ? v : -kNone, Smaller());
+    }
+}
+
+// The sum of v over the lanes of a team up to this one.
+template <int TEAM>
+__device__ __forceinline__ std::uint32_t team_scan(std::uint32_t x) {
+    int v = static_cast<int>(x);
+    if constexpr (TEAM == 4) {  // a row of lanes has four teams
+        const unsigned l = lane_id() % 4;
+        const int one = __builtin_amdgcn_update_dpp(v, v, 0x90, 0xF, 0xF, false);  // quad_perm [0,0,1,2]
+        v += l >= 1 ? one : 0;
+        const int two = __builtin_amdgcn_update_dpp(v, v, 0x44, 0xF, 0xF, false);  // quad_perm [0,1,0,1]
+        v += l >= 2 ? two : 0;
+    } else {
+        v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);  // row_shr:1
+        v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+        v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+        v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    }
+    if constexpr (TEAM == kWave) {
+        v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+        v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
+    }
+    return static_cast<std::uint32_t>(v);
+}
+
+// A team holds a row in registers, E vectors of V a lane.  The K-th largest of its
+// lanes' maxima is one that K elements reach; what reaches it, hardly more than K
+// where these are few beside the lanes, goes to LDS, and each of those counts the
+// larger ones among them, which is its place.
+template <typename T, int V, int E, int TEAM>
+__global__ void __launch_bounds__(kThreads) registers_kernel(Args a) {
+    constexpr int teams = kThreads / TEAM, N = E * V;
+    __shared__ Key found[teams][TEAM * N];
+    Key* mine = found[threadIdx.x / TEAM];
+    const std::uint32_t lane = threadIdx.x % TEAM;
+    std::uint32_t valid = 0, at[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const Place<V> p(lane + e * TEAM, a.C);
+        at[e] = p.at;
+        valid |= (((1u << V) - 1) & ~((1u << p.skip) - 1)) << (e * V);
+    }
+    const std::uint64_t step = static_cast<std::uint64_t>(gridDim.x) * teams;
+    std::uint64_t r = static_cast<std::uint64_t>(blockIdx.x) * teams + threadIdx.x / TEAM;
+    vec_t<T, V> ahead[E];
+    const auto load = [&](std::uint64_t row) {
+        const T* z = static_cast<const T*>(a.z) + row * a.ldz;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+            if (row < a.n && (valid >> (e * V) & ((1u << V) - 1)) != 0) ahead[e] = load_as<T, V>(z + at[e]);
+    };
+    load(r);
+    for (; r < a.n; r += step) {
+        const T* z = static_cast<const T*>(a.z) + r * a.ldz;
+        float v[N];
+        float most = kNone;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            v[i] = (valid >> i) & 1 ? static_cast<float>(ahead[i / V][i % V]) : kNone;
+            most = fmaxf(most, v[i]);
+        }
+        load(r + step);
+        const float bound = a.K <= TEAM ? kth_largest<TEAM>(most, a.K) : kNone;
+        std::uint32_t reach = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) reach |= (v[i] < bound ? 0u : 1u) << i;
+        reach &= valid;
+        const std::uint32_t own = __popc(reach);
+        std::uint32_t to = team_scan<TEAM>(own);
+        const std::uint32_t all = static_cast<std::uint32_t>(__shfl(static_cast<int>(to), TEAM - 1, TEAM));
+        to -= own;
+        while (reach != 0) {
+            const std::uint32_t i = __builtin_ctz(reach);
+            std::uint32_t first = at[0];
+#pragma unroll
+            for (int e = 1; e < E; ++e) first = i >= static_cast<std::uint32_t>(e * V) ? at[e] - e * V : first;
+            mine[to++] = key_of(pick<N>(v, i), first + i);
+            reach &= reach - 1;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        Share rest;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            v[i] = v[i] < bound ? v[i] : kNone;
+            rest.m = fmaxf(rest.m, v[i]);
+        }
+        const float b = base_of(rest.m);
+#pragma unroll
+        for (int i = 0; i < N; ++i) rest.s += exp2_of((v[i] - b) * a.c);
+        for (std::uint32_t i = lane; i < all; i += TEAM) {
+            const Key k = mine[i];
+            std::uint32_t place = 0;
+            for (std::uint32_t o = 0; o < all; ++o) place += mine[o] > k ? 1u : 0u;
+            if (place < a.K) {
+                const std::uint32_t c = index_of(k);
+                static_cast<T*>(a.values)[r * a.ldv + place] = z[c];
+                a.ids[r * a.ldi + place] = static_cast<std::int32_t>(c);
+            } else {
+                rest = rest.with({value_of(static_cast<std::uint32_t>(k >> 32)), 1.0f}, a.c);
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (a.rest == nullptr) continue;
+        const float top = wave_join<TEAM>(rest.m, Larger());
+        rest.scale_to(top, a.c);
+        const float sum = wave_join<TEAM>(rest.s, Add());
+        if (lane == 0) a.rest[r] = top == -kNone ? top : base_of(top) + a.T * kLn2 * log2_of(sum);
+    }
+}
+
 // ---------------------------------------------------------------- launches
 
+template <typename Kernel>
+void launch_all(Kernel kernel, const Args& a, std::uint64_t rows, std::uint64_t most, hipStream_t st) {
+    const std::uint64_t blocks = std::min<std::uint64_t>((a.n + rows - 1) / rows, most);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, st, a);
+}
+template <typename T, int V, int E, int TEAM>
+void in_registers(const Args& a, hipStream_t st) {
+    static std::uint32_t perCu;
+    const auto kernel = registers_kernel<T, V, E, TEAM>;
+    launch_all(kernel, a, kThreads / TEAM, resident_blocks(kernel, kThreads, perCu), st);
+}
+
+// Rows of up to 1,024 classes are held in registers: by 4 lanes of a wave where
+// one vector a lane is enough, by 16 up to 16 elements a lane if they make a bound
+// for K, else by a wave.  Longer ones are streamed.
 template <typename T>
 void launch(const Args& a, hipStream_t st) {
-    const bool wave = a.C <= kWaveClasses;
-    const std::uint64_t blocks = std::min<std::uint64_t>(wave ? (a.n + kWaves - 1) / kWaves : a.n, 1u << 20);
-    const dim3 grid(static_cast<unsigned>(blocks));
-    if (a.C < kVec<T>) hipLaunchKernelGGL((wave_kernel<T, 1>), grid, dim3(kThreads), 0, st, a);
-    else if (wave) hipLaunchKernelGGL((wave_kernel<T, kVec<T>>), grid, dim3(kThreads), 0, st, a);
-    else hipLaunchKernelGGL((block_kernel<T, kVec<T>>), grid, dim3(kThreads), 0, st, a);
+    constexpr int V = kVec<T>;
+    const std::uint32_t C = a.C;
+    if (C < V) return in_registers<T, 1, 2, 4>(a, st);
+    if (C <= 4 * V) return in_registers<T, V, 1, 4>(a, st);
+    if (a.K <= 16 || C <= 64) {
+        if (C <= 16 * V) return in_registers<T, V, 1, 16>(a, st);
+        if (C <= 32 * V) return in_registers<T, V, 2, 16>(a, st);
+        if constexpr (V == 4) {
+            if (C <= 64 * V) return in_registers<T, V, 4, 16>(a, st);
+        }
+    }
+    if (C <= 64 * V) return in_registers<T, V, 1, 64>(a, st);
+    if (C <= 128 * V) return in_registers<T, V, 2, 64>(a, st);
+    if constexpr (V == 4) {
+        if (C <= 256 * V) return in_registers<T, V, 4, 64>(a, st);
+    }
+    if (C <= kWaveClasses) return launch_all(wave_kernel<T, V>, a, kWaves, 1u << 20, st);
+    launch_all(block_kernel<T, V>, a, 1, 1u << 20, st);
 }
 
 }  // namespace
