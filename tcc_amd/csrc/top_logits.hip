@@ -76,6 +76,12 @@ __device__ __forceinline__ K wave_sort(K v) {
     else return v;
 }
 
+// A wave's LDS operations run in order; the compiler keeps them so across this.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 struct Buffer {
     Key k[2 * kWave];
 };
@@ -114,14 +120,10 @@ struct Top {
 
     __device__ __forceinline__ void flush() {
         if (count == 0) return;
-        sync();
+        wave_sync();
         const Key mine = lane_id() < count ? buffer.k[lane_id()] : 0;
         take(wave_sort<false>(mine));
         count = 0;
-    }
-    __device__ __forceinline__ void sync() const {
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
     }
     __device__ __forceinline__ void push(bool mine, float v, std::uint32_t index) {
         const std::uint64_t all = __ballot(mine);
@@ -129,13 +131,13 @@ struct Top {
         if (mine) buffer.k[count + __popcll(all & lanemask_lt())] = key_of(v, index);
         count += __popcll(all);
         if (count < kWave) return;
-        sync();
+        wave_sync();
         take(wave_sort<false>(buffer.k[lane_id()]));
         const Key left = buffer.k[kWave + lane_id()];
-        sync();
+        wave_sync();
         buffer.k[lane_id()] = left;
         count -= kWave;
-        sync();
+        wave_sync();
     }
 };
 
@@ -297,25 +299,47 @@ __global__ void __launch_bounds__(kThreads) block_kernel(Args a) {
 
 // ---------------------------------------------------------------- rows in registers
 
-// How many lanes of a team have a larger v.
-template <int TEAM, int D = 1>
-__device__ __forceinline__ std::uint32_t larger_lanes(float v) {
+// How many of the P values of the other lanes of a team, D and more lanes on, are
+// larger than v.
+template <int TEAM, int P, int D = 1>
+__device__ __forceinline__ std::uint32_t larger_elsewhere(float v, const float (&t)[P]) {
     static_assert(TEAM == 4 || TEAM == 16);
     constexpr int turn = TEAM == 16 ? 0x120 + D : D == 1 ? 0x39 : D == 2 ? 0x4E : 0x93;  // row_ror:D, quad_perm turned by D
-    const int i = static_cast<int>(__float_as_uint(v));
-    const float o = __uint_as_float(static_cast<std::uint32_t>(__builtin_amdgcn_update_dpp(i, i, turn, 0xF, 0xF, false)));
-    const std::uint32_t one = o > v ? 1u : 0u;
-    if constexpr (D + 1 < TEAM) return one + larger_lanes<TEAM, D + 1>(v);
-    else return one;
+    std::uint32_t n = 0;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        const int i = static_cast<int>(__float_as_uint(t[p]));
+        const float o = __uint_as_float(static_cast<std::uint32_t>(__builtin_amdgcn_update_dpp(i, i, turn, 0xF, 0xF, false)));
+        n += o > v ? 1u : 0u;
+    }
+    if constexpr (D + 1 < TEAM) return n + larger_elsewhere<TEAM, P, D + 1>(v, t);
+    else return n;
 }
 
-// The K-th largest of a team's v (of K <= TEAM), in all its lanes.
-template <int TEAM>
-__device__ __forceinline__ float kth_largest(float v, std::uint32_t K) {
+// A value that K elements of a team reach at least (-inf where none is known), in
+// all its lanes: the K-th largest of the lanes' maxima, or, of 4 lanes, that of
+// their four largest each.
+template <int TEAM, int N>
+__device__ __forceinline__ float reached(const float (&v)[N], std::uint32_t K) {
+    constexpr int P = TEAM == 4 ? 4 : 1;
+    if (K > TEAM * P) return kNone;
+    float t[P];  // sorted down
+#pragma unroll
+    for (int p = 0; p < P; ++p) t[p] = kNone;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+#pragma unroll
+        for (int p = P - 1; p > 0; --p) t[p] = __builtin_amdgcn_fmed3f(t[p - 1], t[p], v[i]);
+        t[0] = fmaxf(t[0], v[i]);
+    }
     if constexpr (TEAM == kWave) {
-        return value_of(static_cast<std::uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(wave_sort<true>(order_of(v))), K - 1)));
+        return value_of(static_cast<std::uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(wave_sort<true>(order_of(t[0]))), K - 1)));
     } else {
-        return wave_join<TEAM>(larger_lanes<TEAM>(v) < K ? v : -kNone, Smaller());
+        float least = -kNone;
+#pragma unroll
+        for (int p = 0; p < P; ++p)  // (p of the lane's own are before it, or equal)
+            least = larger_elsewhere<TEAM>(t[p], t) + p < K ? t[p] : least;
+        return wave_join<TEAM>(least, Smaller());
     }
 }
 
@@ -342,85 +366,141 @@ __device__ __forceinline__ std::uint32_t team_scan(std::uint32_t x) {
     return static_cast<std::uint32_t>(v);
 }
 
-// A team holds a row in registers, E vectors of V a lane.  The K-th largest of its
-// lanes' maxima is one that K elements reach; what reaches it, hardly more than K
-// where these are few beside the lanes, goes to LDS, and each of those counts the
-// larger ones among them, which is its place.
+// Keys of a team that have room in LDS, a multiple of 4.
+template <int TEAM>
+constexpr std::uint32_t kRoom = TEAM == 4 ? 32 : TEAM == 16 ? 64 : 256;
+
+__device__ __forceinline__ Key larger_key(Key a, Key b) { return a > b ? a : b; }
+// The largest key of a team.
+template <int TEAM, int D = 1>
+__device__ __forceinline__ Key team_top(Key k) {
+    if constexpr (D < TEAM) return team_top<TEAM, 2 * D>(larger_key(k, other<D>(k)));
+    else return k;
+}
+
+// A team holds a row in registers, E vectors of V a lane.  What reaches a value
+// that K elements reach, hardly more than K of them where these are few beside
+// the row, goes to LDS, and each of those counts the larger ones among them, which
+// is its place.  Rows with more of them than there is room for (equal ones, or
+// mostly -inf) have their K taken one after the other.
 template <typename T, int V, int E, int TEAM>
 __global__ void __launch_bounds__(kThreads) registers_kernel(Args a) {
     constexpr int teams = kThreads / TEAM, N = E * V;
-    __shared__ Key found[teams][TEAM * N];
+    constexpr std::uint32_t room = kRoom<TEAM>;
+    __shared__ __attribute__((aligned(16))) Key found[teams][room];
     Key* mine = found[threadIdx.x / TEAM];
     const std::uint32_t lane = threadIdx.x % TEAM;
-    std::uint32_t valid = 0, at[E];
+    const auto place = [&](int e) { return Place<V>(lane + e * TEAM, a.C); };
+    // whether some lanes of the team have a vector e, and whether all have a whole one
+    const auto some = [&](int e) { return static_cast<std::uint32_t>(e * TEAM * V) < a.C; };
+    const auto whole = [&](int e) { return static_cast<std::uint32_t>((e + 1) * TEAM * V) <= a.C; };
+    std::uint32_t valid = 0;  // element i is bit N - 1 - i
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        const Place<V> p(lane + e * TEAM, a.C);
-        at[e] = p.at;
-        valid |= (((1u << V) - 1) & ~((1u << p.skip) - 1)) << (e * V);
+        const std::uint32_t skip = place(e).skip;
+#pragma unroll
+        for (std::uint32_t q = 0; q < V; ++q) valid += valid + (q >= skip ? 1u : 0u);
     }
     const std::uint64_t step = static_cast<std::uint64_t>(gridDim.x) * teams;
     std::uint64_t r = static_cast<std::uint64_t>(blockIdx.x) * teams + threadIdx.x / TEAM;
     vec_t<T, V> ahead[E];
     const auto load = [&](std::uint64_t row) {
+        if (row >= a.n) return;
         const T* z = static_cast<const T*>(a.z) + row * a.ldz;
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (row < a.n && (valid >> (e * V) & ((1u << V) - 1)) != 0) ahead[e] = load_as<T, V>(z + at[e]);
+        for (int e = 0; e < E; ++e) {
+            if (!some(e)) break;
+            const Place<V> at = place(e);
+            if (at.any()) ahead[e] = load_as<T, V>(z + at.at);
+        }
     };
     load(r);
     for (; r < a.n; r += step) {
         const T* z = static_cast<const T*>(a.z) + r * a.ldz;
+        T* values = static_cast<T*>(a.values) + r * a.ldv;
+        std::int32_t* ids = a.ids + r * a.ldi;
         float v[N];
-        float most = kNone;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            v[i] = (valid >> i) & 1 ? static_cast<float>(ahead[i / V][i % V]) : kNone;
-            most = fmaxf(most, v[i]);
+        for (int e = 0; e < E; ++e) {
+#pragma unroll
+            for (int q = 0; q < V; ++q) v[e * V + q] = kNone;
+            if (!some(e)) continue;
+            const std::uint32_t skip = whole(e) ? 0 : place(e).skip;
+#pragma unroll
+            for (std::uint32_t q = 0; q < V; ++q) v[e * V + q] = q >= skip ? static_cast<float>(ahead[e][q]) : kNone;
         }
         load(r + step);
-        const float bound = a.K <= TEAM ? kth_largest<TEAM>(most, a.K) : kNone;
+        const float bound = reached<TEAM>(v, a.K);
         std::uint32_t reach = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i) reach |= (v[i] < bound ? 0u : 1u) << i;
+        for (int i = 0; i < N; ++i) reach += reach + (v[i] < bound ? 0u : 1u);
         reach &= valid;
         const std::uint32_t own = __popc(reach);
         std::uint32_t to = team_scan<TEAM>(own);
         const std::uint32_t all = static_cast<std::uint32_t>(__shfl(static_cast<int>(to), TEAM - 1, TEAM));
-        to -= own;
-        while (reach != 0) {
-            const std::uint32_t i = __builtin_ctz(reach);
-            std::uint32_t first = at[0];
-#pragma unroll
-            for (int e = 1; e < E; ++e) first = i >= static_cast<std::uint32_t>(e * V) ? at[e] - e * V : first;
-            mine[to++] = key_of(pick<N>(v, i), first + i);
-            reach &= reach - 1;
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        const auto index = [&](std::uint32_t i) { return Place<V>(lane + i / V * TEAM, a.C).at + i % V; };
         Share rest;
+        if (all <= room) {
+            // their classes first: a register chosen at run time costs two instructions
+            // for each that there is, and the row's lines are near
+            auto* classes = reinterpret_cast<std::uint32_t*>(mine);
+            for (to -= own; reach != 0; reach &= reach - 1) classes[2 * to++] = index(N - 1 - __builtin_ctz(reach));
+            wave_sync();
+#pragma unroll 4
+            for (std::uint32_t i = lane; i < all; i += TEAM) {
+                const std::uint32_t c = classes[2 * i];
+                mine[i] = key_of(static_cast<float>(z[c]), c);
+            }
+            if (lane < 3 && all + lane < room) mine[all + lane] = 0;  // for the reads of four
+            wave_sync();
+        } else {  // from memory again: the keys of all elements need more registers than all else
+            Key last = ~Key(0);
+            for (std::uint32_t k = 0; k < a.K; ++k) {
+                Key best = 0;
+#pragma unroll 4
+                for (std::uint32_t c = lane; c < a.C; c += TEAM) {
+                    const Key key = key_of(static_cast<float>(z[c]), c);
+                    best = key < last ? larger_key(best, key) : best;
+                }
+                last = team_top<TEAM>(best);
+                if (lane == 0) {
+                    values[k] = z[index_of(last)];
+                    ids[k] = static_cast<std::int32_t>(index_of(last));
+                }
+            }
+#pragma unroll 1
+            for (std::uint32_t c = lane; c < a.C; c += TEAM) {
+                const float x = static_cast<float>(z[c]);
+                if (key_of(x, c) < last) rest = rest.with({x, 1.0f}, a.c);
+            }
+        }
+        const float below = all <= room ? bound : kNone;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            v[i] = v[i] < bound ? v[i] : kNone;
+            v[i] = v[i] < below ? v[i] : kNone;
             rest.m = fmaxf(rest.m, v[i]);
         }
         const float b = base_of(rest.m);
 #pragma unroll
         for (int i = 0; i < N; ++i) rest.s += exp2_of((v[i] - b) * a.c);
-        for (std::uint32_t i = lane; i < all; i += TEAM) {
-            const Key k = mine[i];
-            std::uint32_t place = 0;
-            for (std::uint32_t o = 0; o < all; ++o) place += mine[o] > k ? 1u : 0u;
-            if (place < a.K) {
-                const std::uint32_t c = index_of(k);
-                static_cast<T*>(a.values)[r * a.ldv + place] = z[c];
-                a.ids[r * a.ldi + place] = static_cast<std::int32_t>(c);
-            } else {
-                rest = rest.with({value_of(static_cast<std::uint32_t>(k >> 32)), 1.0f}, a.c);
+        if (all <= room) {
+            for (std::uint32_t i = lane; i < all; i += TEAM) {
+                const Key k = mine[i];
+                std::uint32_t at = 0;
+                for (std::uint32_t o = 0; o < all; o += 4) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) at += mine[o + q] > k ? 1u : 0u;
+                }
+                if (at < a.K) {
+                    const std::uint32_t c = index_of(k);
+                    values[at] = z[c];
+                    ids[at] = static_cast<std::int32_t>(c);
+                } else {
+                    rest = rest.with({value_of(static_cast<std::uint32_t>(k >> 32)), 1.0f}, a.c);
+                }
             }
+            wave_sync();
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
         if (a.rest == nullptr) continue;
         const float top = wave_join<TEAM>(rest.m, Larger());
         rest.scale_to(top, a.c);
@@ -443,22 +523,22 @@ void in_registers(const Args& a, hipStream_t st) {
     launch_all(kernel, a, kThreads / TEAM, resident_blocks(kernel, kThreads, perCu), st);
 }
 
-// Rows of up to 1,024 classes are held in registers: by 4 lanes of a wave where
-// one vector a lane is enough, by 16 up to 16 elements a lane if they make a bound
-// for K, else by a wave.  Longer ones are streamed.
+// Rows of up to 1,024 classes are held in registers: by 4 lanes of a wave with up to
+// 32 elements each where K allows their bound, by 16 with up to 16, else by a wave.
+// Longer ones are streamed.
 template <typename T>
 void launch(const Args& a, hipStream_t st) {
     constexpr int V = kVec<T>;
     const std::uint32_t C = a.C;
-    if (C < V) return in_registers<T, 1, 2, 4>(a, st);
+    if (C < V) return in_registers<T, 1, 8, 4>(a, st);
     if (C <= 4 * V) return in_registers<T, V, 1, 4>(a, st);
-    if (a.K <= 16 || C <= 64) {
-        if (C <= 16 * V) return in_registers<T, V, 1, 16>(a, st);
-        if (C <= 32 * V) return in_registers<T, V, 2, 16>(a, st);
-        if constexpr (V == 4) {
-            if (C <= 64 * V) return in_registers<T, V, 4, 16>(a, st);
-        }
+    if (a.K <= 16) {
+        if (C <= 8 * V) return in_registers<T, V, 2, 4>(a, st);
+        if (C <= 64) return in_registers<T, V, 16 / V, 4>(a, st);
+        if (C <= 128) return in_registers<T, V, 32 / V, 4>(a, st);
+        if (C <= 256) return in_registers<T, V, 16 / V, 16>(a, st);
     }
+    if (C <= 64) return in_registers<T, V, 8 / V, 16>(a, st);
     if (C <= 64 * V) return in_registers<T, V, 1, 64>(a, st);
     if (C <= 128 * V) return in_registers<T, V, 2, 64>(a, st);
     if constexpr (V == 4) {
