@@ -4,15 +4,16 @@
 //   ids: the K largest, the lowest index first among equals, NaN above all
 //   rest = T log(sum of exp(z_j / T) over the other classes)
 //
-// A row is read once.  A wave keeps the K largest so far sorted over its lanes,
-// as 64-bit keys (the value's order, then the index's), and sends what is larger
-// than the last of them into a buffer in LDS; 64 of these at a time are sorted
-// and merged (the larger of each pair of a descending and an ascending list are
-// the 64 largest of both).  What is not larger, and what a merge drops, goes to
-// the sum of the rest, so that nothing is read or subtracted again.  The first
-// bound is the K-th largest of the lanes' own maxima, which no more than K of
-// the row's elements need exceed.  Rows of up to 4,096 classes have a wave each,
-// longer ones a workgroup whose waves' lists are merged.
+// A row is read once from memory.  From what the lanes have at first comes a bound
+// that K elements reach; those that reach it, hardly more than K of a short row and
+// a few hundred of a long one, go to LDS as 64-bit keys (the value's order, then the
+// index's), and each counts the larger ones, which is its place.  What does not
+// reach the bound, and what K others beat, is summed for the rest: nothing is
+// subtracted from a sum of all.  Rows of up to 1,024 classes are held in registers
+// by 4, 16 or 64 lanes; longer ones are streamed, by a wave up to 4,096 classes, by
+// a workgroup above.  Rows with more at the bound than there is room for (sorted
+// upwards, or many equal) go another way: the short ones take their K one after the
+// other, the long ones by a second kernel that keeps sorted lists.
 #include <algorithm>
 
 #include "../../include/tcc_swtcf.h"
@@ -82,6 +83,196 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_wave_barrier();
 }
 
+// The vectors first + lane, and those step, 2 step, ... after them, of a row.
+template <typename T, int V>
+struct Ahead {
+    vec_t<T, V> x[kBatch];
+    __device__ __forceinline__ void load(const T* z, std::uint32_t first, std::uint32_t step, std::uint32_t C) {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const Place<V> at(first + lane_id() + u * step, C);
+            if (at.any()) x[u] = load_as<T, V>(z + at.at);
+        }
+    }
+};
+
+// A batch of a wave as floats, what is no element of it as -inf, and the largest of
+// each vector, a NaN where it has one.
+template <typename T, int V>
+struct Elements {
+    vec_t<float, V> x[kBatch];
+    float most[kBatch];
+    __device__ __forceinline__ Elements(const Ahead<T, V>& raw, std::uint32_t first, std::uint32_t step, std::uint32_t C) {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const Place<V> at(first + lane_id() + u * step, C);
+            x[u] = __builtin_convertvector(raw.x[u], vec_t<float, V>);
+            if (at.skip != 0) {
+#pragma unroll
+                for (std::uint32_t q = 0; q < V; ++q) x[u][q] = q < at.skip ? kNone : x[u][q];
+            }
+            most[u] = x[u][0];
+#pragma unroll
+            for (int q = 1; q < V; ++q) most[u] = __builtin_elementwise_maximum(most[u], x[u][q]);
+        }
+    }
+    // The K-th largest of the lanes' maxima, in the order of unsigned integers.
+    __device__ __forceinline__ std::uint32_t reached(std::uint32_t K) const {
+        float own = kNone;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) own = __builtin_elementwise_maximum(own, most[u]);
+        return static_cast<std::uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(wave_sort<true>(order_of(own))), K - 1));
+    }
+    // Takes the elements of `out` from vector u.
+    __device__ __forceinline__ void leave(int u, std::uint32_t out) {
+        most[u] = kNone;
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+            x[u][q] = (out >> q) & 1 ? kNone : x[u][q];
+            most[u] = fmaxf(most[u], x[u][q]);
+        }
+    }
+    __device__ __forceinline__ void add_to(Share& rest, float c) const {
+        float m = kNone;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) m = fmaxf(m, most[u]);
+        if (m > rest.m) rest.scale_to(m, c);
+        const float b = base_of(rest.m);
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+            for (int q = 0; q < V; ++q) rest.s += exp2_of((x[u][q] - b) * c);
+    }
+};
+
+__device__ __forceinline__ Share wave_join_share(Share v, float c) {
+    const float m = wave_join<kWave>(v.m, Larger());
+    v.scale_to(m, c);
+    v.s = wave_join<kWave>(v.s, Add());
+    return v;
+}
+__device__ __forceinline__ float as_logit(const Args& a, Share rest) {
+    return rest.m == -kNone ? rest.m : base_of(rest.m) + a.T * kLn2 * log2_of(rest.s);
+}
+
+// ---------------------------------------------------------------- streamed rows
+
+constexpr std::uint32_t kFound = 256;      // classes of a wave that have room in LDS
+constexpr std::int32_t kToSort = -1;       // the first id of a row that had more
+static_assert(kMostTop <= kWave);
+
+// A row is read once by a wave, or by the four of a workgroup.  The first batch
+// gives a bound that K of its elements reach: the least of the waves' K-th (or
+// K/4-th) largest lane maxima.  The classes that reach it, a few hundred of 50,000,
+// go to LDS, and each counts the larger ones among them, which is its place.
+template <typename T, int V, int WAVES>
+__global__ void __launch_bounds__(kThreads) stream_kernel(Args a) {
+    static_assert(WAVES == 1 || WAVES == kWaves);
+    constexpr std::uint32_t teams = kWaves / WAVES, lanes = WAVES * kWave, step = lanes;
+    __shared__ std::uint32_t classes[kWaves][kFound], counts[kWaves];
+    __shared__ __attribute__((aligned(16))) Key keys[teams][WAVES * kFound + 4];
+    __shared__ float bounds[kWaves];
+    __shared__ float2 rests[kWaves];
+    const std::uint32_t w = uniform(threadIdx.x / kWave), team = WAVES == 1 ? w : 0, first = WAVES == 1 ? 0 : w * kWave;
+    const auto sync = [] {
+        if constexpr (WAVES == 1) wave_sync();
+        else __syncthreads();
+    };
+    const std::uint64_t rows = static_cast<std::uint64_t>(gridDim.x) * teams;
+    for (std::uint64_t r = static_cast<std::uint64_t>(blockIdx.x) * teams + team; r < a.n; r += rows) {
+        const T* z = static_cast<const T*>(a.z) + r * a.ldz;
+        Share rest;
+        std::uint32_t count = 0;
+        float bound = 0.0f;
+        bool begun = false;
+        Ahead<T, V> ahead;
+        ahead.load(z, first, step, a.C);
+        for (std::uint32_t j = first; j * V < a.C; j += step * kBatch) {  // of the wave's first lane
+            Elements<T, V> e(ahead, j, step, a.C);
+            ahead.load(z, j + step * kBatch, step, a.C);
+            if (!begun) {
+                begun = true;
+                bound = value_of(e.reached((a.K + WAVES - 1) / WAVES));
+                if constexpr (WAVES > 1) {
+                    if (lane_id() == 0) bounds[w] = bound;
+                    __syncthreads();
+                    bound = wave_join<WAVES>(bounds[lane_id() % WAVES], Smaller());
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                if (__ballot(!(e.most[u] < bound)) == 0) continue;
+                const Place<V> at(j + lane_id() + u * step, a.C);
+                std::uint32_t out = 0;
+#pragma unroll
+                for (std::uint32_t q = 0; q < V; ++q) out |= (q >= at.skip && !(e.x[u][q] < bound) ? 1u : 0u) << q;
+                std::uint32_t left = out;
+                for (std::uint64_t more; (more = __ballot(left != 0)) != 0; left &= left - 1) {
+                    const std::uint32_t to = count + __popcll(more & lanemask_lt());
+                    if (left != 0 && to < kFound) classes[w][to] = at.at + __builtin_ctz(left);
+                    count += __popcll(more);
+                }
+                e.leave(u, out);
+            }
+            e.add_to(rest, a.c);
+        }
+        std::uint32_t before = 0, all = count, most = count;
+        if constexpr (WAVES > 1) {
+            if (lane_id() == 0) counts[w] = count;
+            __syncthreads();
+            all = most = 0;
+#pragma unroll
+            for (std::uint32_t o = 0; o < WAVES; ++o) {
+                const std::uint32_t n = counts[o];
+                before += o < w ? n : 0;
+                all += n;
+                most = max(most, n);
+            }
+        }
+        const std::uint32_t lane = WAVES == 1 ? lane_id() : threadIdx.x;
+        if (most > kFound) {
+            if (lane == 0) a.ids[r * a.ldi] = kToSort;
+            continue;
+        }
+        wave_sync();
+        Key* mine = keys[team];
+#pragma unroll 4
+        for (std::uint32_t i = lane_id(); i < count; i += kWave) {
+            const std::uint32_t c = classes[w][i];
+            mine[before + i] = key_of(static_cast<float>(z[c]), c);
+        }
+        if (lane < 3) mine[all + lane] = 0;  // for the reads of four
+        sync();
+        for (std::uint32_t i = lane; i < all; i += lanes) {
+            const Key k = mine[i];
+            std::uint32_t at = 0;
+            for (std::uint32_t o = 0; o < all; o += 4) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) at += mine[o + q] > k ? 1u : 0u;
+            }
+            if (at < a.K) {
+                const std::uint32_t c = index_of(k);
+                static_cast<T*>(a.values)[r * a.ldv + at] = z[c];
+                a.ids[r * a.ldi + at] = static_cast<std::int32_t>(c);
+            } else {
+                rest = rest.with({value_of(static_cast<std::uint32_t>(k >> 32)), 1.0f}, a.c);
+            }
+        }
+        rest = wave_join_share(rest, a.c);
+        if constexpr (WAVES > 1) {
+            if (lane_id() == 0) rests[w] = make_float2(rest.m, rest.s);
+            __syncthreads();
+            if (w == 0)
+                for (int o = 1; o < WAVES; ++o) rest = rest.with({rests[o].x, rests[o].y}, a.c);
+        } else {
+            wave_sync();
+        }
+        if (a.rest != nullptr && lane == 0) a.rest[r] = as_logit(a, rest);
+    }
+}
+
+// ---------------------------------------------------------------- rows by sorted lists
+
 struct Buffer {
     Key k[2 * kWave];
 };
@@ -141,106 +332,36 @@ struct Top {
     }
 };
 
-// Element b of N (a power of two).
-template <int N, typename A>
-__device__ __forceinline__ float pick(const A& v, std::uint32_t b) {
-    float s[N];
-#pragma unroll
-    for (int q = 0; q < N; ++q) s[q] = v[q];
-#pragma unroll
-    for (int d = 1; d < N; d <<= 1)
-#pragma unroll
-        for (int q = 0; q < N; q += 2 * d) s[q] = b & d ? s[q + d] : s[q];
-    return s[0];
-}
-
-// The vectors first + lane, and those step, 2 step, ... after them, of a row.
-template <typename T, int V>
-struct Ahead {
-    vec_t<T, V> x[kBatch];
-    __device__ __forceinline__ void load(const T* z, std::uint32_t first, std::uint32_t step, std::uint32_t C) {
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-            const Place<V> at(first + lane_id() + u * step, C);
-            if (at.any()) x[u] = load_as<T, V>(z + at.at);
-        }
-    }
-};
-
 // The elements of vectors first, first + step, ... of a row.
 template <typename T, int V>
 __device__ __forceinline__ void scan(Top& top, const T* z, std::uint32_t first, std::uint32_t step) {
-    using F = vec_t<float, V>;
     const Args& a = top.a;
     bool begun = false;
-    Ahead<T, V> ahead;
-    ahead.load(z, first, step, a.C);
     for (std::uint32_t j = first; j * V < a.C; j += step * kBatch) {  // of the wave's first lane
-        F x[kBatch];
-        float most[kBatch];  // of a vector; a NaN where it has one
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) {
-            const Place<V> at(j + lane_id() + u * step, a.C);
-            x[u] = __builtin_convertvector(ahead.x[u], F);
-            if (at.skip != 0) {
-#pragma unroll
-                for (std::uint32_t q = 0; q < V; ++q) x[u][q] = q < at.skip ? kNone : x[u][q];
-            }
-            most[u] = x[u][0];
-#pragma unroll
-            for (int q = 1; q < V; ++q) most[u] = __builtin_elementwise_maximum(most[u], x[u][q]);
-        }
-        ahead.load(z, j + step * kBatch, step, a.C);
-        if (!begun) {  // a first bound
-            begun = true;
-            float own = kNone;
-#pragma unroll
-            for (int u = 0; u < kBatch; ++u) own = __builtin_elementwise_maximum(own, most[u]);
-            const std::uint32_t last =
-                static_cast<std::uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(wave_sort<true>(order_of(own))), a.K - 1));
-            top.raise(last - 1);  // itself may be one of the K
-        }
-        float m = kNone;
+        Ahead<T, V> raw;
+        raw.load(z, j, step, a.C);
+        Elements<T, V> e(raw, j, step, a.C);
+        if (!begun) top.raise(e.reached(a.K) - 1);  // itself may be one of the K
+        begun = true;
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
             // larger than the bound at the start of this vector: elements equal to a
             // bound from among these may come before it in the row
             const float bound = top.bound;
-            if (__ballot(!(most[u] <= bound)) != 0) {
-                const Place<V> at(j + lane_id() + u * step, a.C);
-                std::uint32_t larger = 0;
+            if (__ballot(!(e.most[u] <= bound)) == 0) continue;
+            const Place<V> at(j + lane_id() + u * step, a.C);
+            std::uint32_t out = 0;
 #pragma unroll
-                for (std::uint32_t q = 0; q < V; ++q) larger |= (q >= at.skip && !(x[u][q] <= bound) ? 1u : 0u) << q;
-                std::uint32_t left = larger;
-                while (__ballot(left != 0) != 0) {
-                    const std::uint32_t q = left != 0 ? __builtin_ctz(left) : 0u;
-                    top.push(left != 0, pick<V>(x[u], q), at.at + q);
-                    left &= left - 1;
-                }
-                most[u] = kNone;
-#pragma unroll
-                for (int q = 0; q < V; ++q) {
-                    x[u][q] = (larger >> q) & 1 ? kNone : x[u][q];
-                    most[u] = fmaxf(most[u], x[u][q]);
-                }
+            for (std::uint32_t q = 0; q < V; ++q) out |= (q >= at.skip && !(e.x[u][q] <= bound) ? 1u : 0u) << q;
+            for (std::uint32_t left = out; __ballot(left != 0) != 0; left &= left - 1) {
+                const std::uint32_t q = left != 0 ? __builtin_ctz(left) : 0u;
+                top.push(left != 0, left != 0 ? static_cast<float>(z[at.at + q]) : 0.0f, at.at + q);
             }
-            m = fmaxf(m, most[u]);
+            e.leave(u, out);
         }
-        if (m > top.rest.m) top.rest.scale_to(m, a.c);
-        const float b = base_of(top.rest.m);
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u)
-#pragma unroll
-            for (int q = 0; q < V; ++q) top.rest.s += exp2_of((x[u][q] - b) * a.c);
+        e.add_to(top.rest, a.c);
     }
     top.flush();
-}
-
-__device__ __forceinline__ Share wave_join_share(Share v, float c) {
-    const float m = wave_join<kWave>(v.m, Larger());
-    v.scale_to(m, c);
-    v.s = wave_join<kWave>(v.s, Add());
-    return v;
 }
 
 // By the wave that has the row's list and, in any lane, the sum of its rest.
@@ -253,16 +374,17 @@ __device__ __forceinline__ void write(const Top& top, const T* z, std::uint64_t 
         static_cast<T*>(a.values)[r * a.ldv + l] = z[i];
         a.ids[r * a.ldi + l] = static_cast<std::int32_t>(i);
     }
-    if (a.rest != nullptr && l == 0) a.rest[r] = rest.m == -kNone ? rest.m : base_of(rest.m) + a.T * kLn2 * log2_of(rest.s);
+    if (a.rest != nullptr && l == 0) a.rest[r] = as_logit(a, rest);
 }
 
-// A row a wave.
+// The rows that stream_kernel marked, a wave each.
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) wave_kernel(Args a) {
     __shared__ Buffer buffers[kWaves];
     const std::uint32_t w = uniform(threadIdx.x / kWave);
     const std::uint64_t step = static_cast<std::uint64_t>(gridDim.x) * kWaves;
     for (std::uint64_t r = static_cast<std::uint64_t>(blockIdx.x) * kWaves + w; r < a.n; r += step) {
+        if (a.ids[r * a.ldi] != kToSort) continue;
         const T* z = static_cast<const T*>(a.z) + r * a.ldz;
         Top top(a, buffers[w]);
         scan<T, V>(top, z, 0, kWave);
@@ -270,7 +392,7 @@ __global__ void __launch_bounds__(kThreads) wave_kernel(Args a) {
     }
 }
 
-// A row a workgroup: its waves take the vectors in turn.
+// The same, a workgroup each, whose waves take the vectors in turn.
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) block_kernel(Args a) {
     __shared__ Buffer buffers[kWaves];
@@ -278,6 +400,7 @@ __global__ void __launch_bounds__(kThreads) block_kernel(Args a) {
     __shared__ float2 rests[kWaves];
     const std::uint32_t w = uniform(threadIdx.x / kWave);
     for (std::uint64_t r = blockIdx.x; r < a.n; r += gridDim.x) {
+        if (a.ids[r * a.ldi] != kToSort) continue;
         const T* z = static_cast<const T*>(a.z) + r * a.ldz;
         Top top(a, buffers[w]);
         scan<T, V>(top, z, w * kWave, kThreads);
@@ -505,7 +628,7 @@ __global__ void __launch_bounds__(kThreads) registers_kernel(Args a) {
         const float top = wave_join<TEAM>(rest.m, Larger());
         rest.scale_to(top, a.c);
         const float sum = wave_join<TEAM>(rest.s, Add());
-        if (lane == 0) a.rest[r] = top == -kNone ? top : base_of(top) + a.T * kLn2 * log2_of(sum);
+        if (lane == 0) a.rest[r] = as_logit(a, {top, sum});
     }
 }
 
@@ -544,8 +667,13 @@ void launch(const Args& a, hipStream_t st) {
     if constexpr (V == 4) {
         if (C <= 256 * V) return in_registers<T, V, 4, 64>(a, st);
     }
-    if (C <= kWaveClasses) return launch_all(wave_kernel<T, V>, a, kWaves, 1u << 20, st);
-    launch_all(block_kernel<T, V>, a, 1, 1u << 20, st);
+    if (C <= kWaveClasses) {
+        launch_all(stream_kernel<T, V, 1>, a, kWaves, 1u << 20, st);
+        launch_all(wave_kernel<T, V>, a, kWaves, 2048, st);
+    } else {
+        launch_all(stream_kernel<T, V, kWaves>, a, 1, 1u << 20, st);
+        launch_all(block_kernel<T, V>, a, 1, 2048, st);
+    }
 }
 
 }  // namespace
