@@ -83,54 +83,82 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// The vectors first + lane, and those step, 2 step, ... after them, of a row.
+// A batch of a wave: its lanes' vectors first + lane, and those step, 2 step, ...
+// after them, of a row.
+template <int V>
+struct Range {
+    std::uint32_t first, step, C;
+    // Whether all of its vectors are whole ones, for the whole wave.
+    __device__ __forceinline__ bool inside() const { return (first + kWave + (kBatch - 1) * step) * V <= C; }
+    __device__ __forceinline__ Place<V> place(int u) const { return Place<V>(first + lane_id() + u * step, C); }
+    // The first element of vector u.
+    __device__ __forceinline__ std::uint32_t at(int u) const { return inside() ? (first + lane_id() + u * step) * V : place(u).at; }
+};
+
 template <typename T, int V>
 struct Ahead {
     vec_t<T, V> x[kBatch];
-    __device__ __forceinline__ void load(const T* z, std::uint32_t first, std::uint32_t step, std::uint32_t C) {
+    __device__ __forceinline__ void load(const T* z, Range<V> r) {
+        if (r.inside()) {
+            z += (r.first + lane_id()) * V;
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) x[u] = load_as<T, V>(z + u * r.step * V);
+            return;
+        }
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-            const Place<V> at(first + lane_id() + u * step, C);
+            const Place<V> at = r.place(u);
             if (at.any()) x[u] = load_as<T, V>(z + at.at);
         }
     }
 };
 
-// A batch of a wave as floats, what is no element of it as -inf, and the largest of
-// each vector, a NaN where it has one.
+// Its elements as floats, what is no element of it as -inf, and the largest of each
+// vector, a NaN where it has one.
 template <typename T, int V>
 struct Elements {
     vec_t<float, V> x[kBatch];
     float most[kBatch];
-    __device__ __forceinline__ Elements(const Ahead<T, V>& raw, std::uint32_t first, std::uint32_t step, std::uint32_t C) {
+    __device__ __forceinline__ Elements(const Ahead<T, V>& raw, Range<V> r) {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) x[u] = __builtin_convertvector(raw.x[u], vec_t<float, V>);
+        if (!r.inside()) {
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                const std::uint32_t skip = r.place(u).skip;
+#pragma unroll
+                for (std::uint32_t q = 0; q < V; ++q) x[u][q] = q < skip ? kNone : x[u][q];
+            }
+        }
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-            const Place<V> at(first + lane_id() + u * step, C);
-            x[u] = __builtin_convertvector(raw.x[u], vec_t<float, V>);
-            if (at.skip != 0) {
-#pragma unroll
-                for (std::uint32_t q = 0; q < V; ++q) x[u][q] = q < at.skip ? kNone : x[u][q];
-            }
             most[u] = x[u][0];
 #pragma unroll
             for (int q = 1; q < V; ++q) most[u] = __builtin_elementwise_maximum(most[u], x[u][q]);
         }
     }
-    // The K-th largest of the lanes' maxima, in the order of unsigned integers.
-    __device__ __forceinline__ std::uint32_t reached(std::uint32_t K) const {
-        float own = kNone;
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) own = __builtin_elementwise_maximum(own, most[u]);
-        return static_cast<std::uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(wave_sort<true>(order_of(own))), K - 1));
-    }
-    // Takes the elements of `out` from vector u.
-    __device__ __forceinline__ void leave(int u, std::uint32_t out) {
-        most[u] = kNone;
+    // Takes what is not below (ABOVE: not up to) the bound from vector u, and says
+    // what that is: element q is bit V - 1 - q.
+    template <bool ABOVE>
+    __device__ __forceinline__ std::uint32_t leave(int u, float bound, Range<V> r) {
+        std::uint32_t out = 0;
 #pragma unroll
         for (int q = 0; q < V; ++q) {
-            x[u][q] = (out >> q) & 1 ? kNone : x[u][q];
-            most[u] = fmaxf(most[u], x[u][q]);
+            const bool goes = ABOVE ? !(x[u][q] <= bound) : !(x[u][q] < bound);
+            out += out + (goes ? 1u : 0u);
+            x[u][q] = goes ? kNone : x[u][q];
         }
+        most[u] = x[u][0];
+#pragma unroll
+        for (int q = 1; q < V; ++q) most[u] = fmaxf(most[u], x[u][q]);
+        if (!r.inside()) out &= (1u << (V - r.place(u).skip)) - 1;
+        return out;
+    }
+    // The larger of `own` and its elements of this lane.
+    __device__ __forceinline__ float largest(float own) const {
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) own = __builtin_elementwise_maximum(own, most[u]);
+        return own;
     }
     __device__ __forceinline__ void add_to(Share& rest, float c) const {
         float m = kNone;
@@ -151,104 +179,114 @@ __device__ __forceinline__ Share wave_join_share(Share v, float c) {
     v.s = wave_join<kWave>(v.s, Add());
     return v;
 }
+// The K-th largest of the lanes' v, in the order of unsigned integers.
+__device__ __forceinline__ std::uint32_t kth_lane(float v, std::uint32_t K) {
+    return static_cast<std::uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(wave_sort<true>(order_of(v))), K - 1));
+}
 __device__ __forceinline__ float as_logit(const Args& a, Share rest) {
     return rest.m == -kNone ? rest.m : base_of(rest.m) + a.T * kLn2 * log2_of(rest.s);
 }
 
 // ---------------------------------------------------------------- streamed rows
 
-constexpr std::uint32_t kFound = 256;      // classes of a wave that have room in LDS
+constexpr std::uint32_t kFound = 512;      // classes of a wave that have room in LDS
 constexpr std::int32_t kToSort = -1;       // the first id of a row that had more
 static_assert(kMostTop <= kWave);
 
-// A row is read once by a wave, or by the four of a workgroup.  The first batch
-// gives a bound that K of its elements reach: the least of the waves' K-th (or
-// K/4-th) largest lane maxima.  The classes that reach it, a few hundred of 50,000,
-// go to LDS, and each counts the larger ones among them, which is its place.
+// A row is read once by a wave, or by the four of a workgroup.  K elements at least
+// reach the K-th largest of the lanes' maxima so far (of four waves: the least of
+// their K/4-th); one wave raises that bound as it goes, four agree on one after the
+// first batch and on another at the end.  The classes that reach it, a few hundred
+// of 50,000, go to LDS; of these, those that reach the last bound each count the
+// larger ones among them, which is their place.
 template <typename T, int V, int WAVES>
-__global__ void __launch_bounds__(kThreads) stream_kernel(Args a) {
+__global__ void __launch_bounds__(kThreads, 5) stream_kernel(Args a) {
     static_assert(WAVES == 1 || WAVES == kWaves);
-    constexpr std::uint32_t teams = kWaves / WAVES, lanes = WAVES * kWave, step = lanes;
-    __shared__ std::uint32_t classes[kWaves][kFound], counts[kWaves];
-    __shared__ __attribute__((aligned(16))) Key keys[teams][WAVES * kFound + 4];
-    __shared__ float bounds[kWaves];
+    constexpr std::uint32_t teams = kWaves / WAVES, step = WAVES * kWave;
+    __shared__ std::uint32_t classes[kWaves][kFound], counts[kWaves], kept[kWaves];
+    __shared__ __attribute__((aligned(16))) Key keys[kWaves][kFound + 4];
+    __shared__ float bounds[2][kWaves];
     __shared__ float2 rests[kWaves];
-    const std::uint32_t w = uniform(threadIdx.x / kWave), team = WAVES == 1 ? w : 0, first = WAVES == 1 ? 0 : w * kWave;
-    const auto sync = [] {
-        if constexpr (WAVES == 1) wave_sync();
-        else __syncthreads();
+    const std::uint32_t w = uniform(threadIdx.x / kWave), first = WAVES == 1 ? 0 : w * kWave;
+    // the least of the waves' bounds; the whole workgroup
+    const auto agreed = [&](int turn, float bound) {
+        if (lane_id() == 0) bounds[turn][w] = bound;
+        __syncthreads();
+        return wave_join<WAVES>(bounds[turn][lane_id() % WAVES], Smaller());
     };
     const std::uint64_t rows = static_cast<std::uint64_t>(gridDim.x) * teams;
-    for (std::uint64_t r = static_cast<std::uint64_t>(blockIdx.x) * teams + team; r < a.n; r += rows) {
+    for (std::uint64_t r = static_cast<std::uint64_t>(blockIdx.x) * teams + (WAVES == 1 ? w : 0); r < a.n; r += rows) {
         const T* z = static_cast<const T*>(a.z) + r * a.ldz;
+        const std::uint32_t K = (a.K + WAVES - 1) / WAVES;
         Share rest;
-        std::uint32_t count = 0;
-        float bound = 0.0f;
-        bool begun = false;
+        std::uint32_t count = 0, batch = 0;
+        float bound = 0.0f, own = kNone;
         Ahead<T, V> ahead;
-        ahead.load(z, first, step, a.C);
-        for (std::uint32_t j = first; j * V < a.C; j += step * kBatch) {  // of the wave's first lane
-            Elements<T, V> e(ahead, j, step, a.C);
-            ahead.load(z, j + step * kBatch, step, a.C);
-            if (!begun) {
-                begun = true;
-                bound = value_of(e.reached((a.K + WAVES - 1) / WAVES));
-                if constexpr (WAVES > 1) {
-                    if (lane_id() == 0) bounds[w] = bound;
-                    __syncthreads();
-                    bound = wave_join<WAVES>(bounds[lane_id() % WAVES], Smaller());
-                }
+        Range<V> range{first, step, a.C};
+        ahead.load(z, range);
+        for (; range.first * V < a.C; range.first += step * kBatch, ++batch) {  // of the wave's first lane
+            Elements<T, V> e(ahead, range);
+            ahead.load(z, {range.first + step * kBatch, step, a.C});
+            own = e.largest(own);
+            if constexpr (WAVES > 1) {
+                if (batch == 0) bound = agreed(0, value_of(kth_lane(own, K)));
+            } else {
+                if (batch < 4 || batch % 4 == 0) bound = value_of(kth_lane(own, K));
             }
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) {
                 if (__ballot(!(e.most[u] < bound)) == 0) continue;
-                const Place<V> at(j + lane_id() + u * step, a.C);
-                std::uint32_t out = 0;
-#pragma unroll
-                for (std::uint32_t q = 0; q < V; ++q) out |= (q >= at.skip && !(e.x[u][q] < bound) ? 1u : 0u) << q;
-                std::uint32_t left = out;
+                std::uint32_t left = e.template leave<false>(u, bound, range);
+                const std::uint32_t last = range.at(u) + V - 1;
                 for (std::uint64_t more; (more = __ballot(left != 0)) != 0; left &= left - 1) {
                     const std::uint32_t to = count + __popcll(more & lanemask_lt());
-                    if (left != 0 && to < kFound) classes[w][to] = at.at + __builtin_ctz(left);
+                    if (left != 0 && to < kFound) classes[w][to] = last - __builtin_ctz(left);
                     count += __popcll(more);
                 }
-                e.leave(u, out);
             }
             e.add_to(rest, a.c);
         }
-        std::uint32_t before = 0, all = count, most = count;
+        bound = value_of(kth_lane(own, K));
+        bool fits = count <= kFound;
         if constexpr (WAVES > 1) {
             if (lane_id() == 0) counts[w] = count;
-            __syncthreads();
-            all = most = 0;
+            bound = agreed(1, bound);
 #pragma unroll
-            for (std::uint32_t o = 0; o < WAVES; ++o) {
-                const std::uint32_t n = counts[o];
-                before += o < w ? n : 0;
-                all += n;
-                most = max(most, n);
-            }
+            for (int o = 0; o < WAVES; ++o) fits &= counts[o] <= kFound;
         }
-        const std::uint32_t lane = WAVES == 1 ? lane_id() : threadIdx.x;
-        if (most > kFound) {
-            if (lane == 0) a.ids[r * a.ldi] = kToSort;
+        if (!fits) {
+            if (lane_id() == 0 && (WAVES == 1 || w == 0)) a.ids[r * a.ldi] = kToSort;
             continue;
         }
         wave_sync();
-        Key* mine = keys[team];
-#pragma unroll 4
-        for (std::uint32_t i = lane_id(); i < count; i += kWave) {
-            const std::uint32_t c = classes[w][i];
-            mine[before + i] = key_of(static_cast<float>(z[c]), c);
+        std::uint32_t all = 0;
+        for (std::uint32_t i = lane_id(); i - lane_id() < count; i += kWave) {
+            const std::uint32_t c = i < count ? classes[w][i] : 0u;
+            const float x = static_cast<float>(z[c]);
+            const bool keeps = i < count && !(x < bound);
+            const std::uint64_t those = __ballot(keeps);
+            if (keeps) keys[w][all + __popcll(those & lanemask_lt())] = key_of(x, c);
+            else if (i < count) rest = rest.with({x, 1.0f}, a.c);
+            all += __popcll(those);
         }
-        if (lane < 3) mine[all + lane] = 0;  // for the reads of four
-        sync();
-        for (std::uint32_t i = lane; i < all; i += lanes) {
-            const Key k = mine[i];
+        if (lane_id() < 3) keys[w][all + lane_id()] = 0;  // for the reads of four
+        if constexpr (WAVES > 1) {
+            if (lane_id() == 0) kept[w] = all;
+            __syncthreads();
+        } else {
+            wave_sync();
+        }
+        for (std::uint32_t i = lane_id(); i < all; i += kWave) {
+            const Key k = keys[w][i];
             std::uint32_t at = 0;
-            for (std::uint32_t o = 0; o < all; o += 4) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q) at += mine[o + q] > k ? 1u : 0u;
+            for (int t = 0; t < WAVES; ++t) {
+                const Key* others = keys[WAVES == 1 ? w : t];
+                const std::uint32_t n = WAVES == 1 ? all : kept[t];
+                for (std::uint32_t o = 0; o < n; o += 4) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) at += others[o + q] > k ? 1u : 0u;
+                }
             }
             if (at < a.K) {
                 const std::uint32_t c = index_of(k);
@@ -267,7 +305,7 @@ __global__ void __launch_bounds__(kThreads) stream_kernel(Args a) {
         } else {
             wave_sync();
         }
-        if (a.rest != nullptr && lane == 0) a.rest[r] = as_logit(a, rest);
+        if (a.rest != nullptr && lane_id() == 0 && (WAVES == 1 || w == 0)) a.rest[r] = as_logit(a, rest);
     }
 }
 
@@ -337,11 +375,11 @@ template <typename T, int V>
 __device__ __forceinline__ void scan(Top& top, const T* z, std::uint32_t first, std::uint32_t step) {
     const Args& a = top.a;
     bool begun = false;
-    for (std::uint32_t j = first; j * V < a.C; j += step * kBatch) {  // of the wave's first lane
+    for (Range<V> range{first, step, a.C}; range.first * V < a.C; range.first += step * kBatch) {
         Ahead<T, V> raw;
-        raw.load(z, j, step, a.C);
-        Elements<T, V> e(raw, j, step, a.C);
-        if (!begun) top.raise(e.reached(a.K) - 1);  // itself may be one of the K
+        raw.load(z, range);
+        Elements<T, V> e(raw, range);
+        if (!begun) top.raise(kth_lane(e.largest(kNone), a.K) - 1);  // itself may be one of the K
         begun = true;
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
@@ -349,15 +387,11 @@ __device__ __forceinline__ void scan(Top& top, const T* z, std::uint32_t first, 
             // bound from among these may come before it in the row
             const float bound = top.bound;
             if (__ballot(!(e.most[u] <= bound)) == 0) continue;
-            const Place<V> at(j + lane_id() + u * step, a.C);
-            std::uint32_t out = 0;
-#pragma unroll
-            for (std::uint32_t q = 0; q < V; ++q) out |= (q >= at.skip && !(e.x[u][q] <= bound) ? 1u : 0u) << q;
-            for (std::uint32_t left = out; __ballot(left != 0) != 0; left &= left - 1) {
-                const std::uint32_t q = left != 0 ? __builtin_ctz(left) : 0u;
-                top.push(left != 0, left != 0 ? static_cast<float>(z[at.at + q]) : 0.0f, at.at + q);
+            const std::uint32_t last = range.at(u) + V - 1;
+            for (std::uint32_t left = e.template leave<true>(u, bound, range); __ballot(left != 0) != 0; left &= left - 1) {
+                const std::uint32_t c = left != 0 ? last - __builtin_ctz(left) : 0u;
+                top.push(left != 0, static_cast<float>(z[c]), c);
             }
-            e.leave(u, out);
         }
         e.add_to(top.rest, a.c);
     }
@@ -456,7 +490,7 @@ __device__ __forceinline__ float reached(const float (&v)[N], std::uint32_t K) {
         t[0] = fmaxf(t[0], v[i]);
     }
     if constexpr (TEAM == kWave) {
-        return value_of(static_cast<std::uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(wave_sort<true>(order_of(t[0]))), K - 1)));
+        return value_of(kth_lane(t[0], K));
     } else {
         float least = -kNone;
 #pragma unroll
@@ -667,7 +701,10 @@ void launch(const Args& a, hipStream_t st) {
     if constexpr (V == 4) {
         if (C <= 256 * V) return in_registers<T, V, 4, 64>(a, st);
     }
-    if (C <= kWaveClasses) {
+    // A wave a row where there are three for each SIMD (4,096 x 50,000 bf16, K = 32: 100 us
+    // instead of 112 with a workgroup a row, of which an uneven number are left at the
+    // end) and K leaves its bound room; a workgroup else.
+    if (C <= kWaveClasses || (a.K <= 32 && a.n >= 12ull * device_cus())) {
         launch_all(stream_kernel<T, V, 1>, a, kWaves, 1u << 20, st);
         launch_all(wave_kernel<T, V>, a, kWaves, 2048, st);
     } else {
