@@ -69,7 +69,7 @@ template <int TEAM>
 constexpr std::uint32_t kWindow = TEAM == 4 ? 128 : TEAM == 16 ? 512 : TEAM == 64 ? 4096 : 1u << 17;
 
 __device__ __forceinline__ float weight_of(const Args& a, std::uint64_t r) {
-    return a.weight == nullptr ? 1.0f : r < a.n ? a.weight[r] : 0.0f;
+    return r >= a.n ? 0.0f : a.weight == nullptr ? 1.0f : a.weight[r];
 }
 
 // LDS of the workgroup.
@@ -116,28 +116,38 @@ struct Team {
     // The maximum of a NaN is an infinity, so that its differences are NaN.
     static __device__ __forceinline__ float bound(float v) { return v != v ? -kNone : v; }
 
-    // Loads the entries of row r, with logits at `row`, and the teacher's
-    // probabilities; false where the row has no target.
-    template <typename T>
-    __device__ __forceinline__ bool load(std::uint64_t r, const T* row) {
-        float m = kNone;
-        bool bad = false;
+    // The entries of row r, as memory holds them.
+    __device__ __forceinline__ void fetch(std::uint64_t r) {
+        bad = false;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const std::uint32_t k = lane + e * TEAM;
-            id[e] = -1;
-            t[e] = kNone;
+            nextId[e] = -1;
+            nextT[e] = kNone;
             if (k < a.K) {
                 const std::int64_t i = id_at(r, k);
-                id[e] = is_class(i) ? static_cast<std::int32_t>(i) : -1;
-                bad |= id[e] < 0 && i != -1;
-                t[e] = value_at(r, k);
+                nextId[e] = is_class(i) ? static_cast<std::int32_t>(i) : -1;
+                bad |= nextId[e] < 0 && i != -1;
+                nextT[e] = value_at(r, k);
             }
         }
-        rest = a.rest == nullptr ? kNone : a.rest[r];
+        nextRest = a.rest == nullptr ? kNone : a.rest[r];
+    }
+    std::int32_t nextId[E];
+    float nextT[E], nextRest;
+    bool bad;
+
+    // The fetched row, its logits at `row`, and the teacher's probabilities; false
+    // where it has no target.
+    template <typename T>
+    __device__ __forceinline__ bool load(const T* row) {
+        float m = kNone;
+        rest = nextRest;
+        if (a.error != nullptr && bad) atomicOr(a.error, TCC_DEVERR_FEATURE_INDEX);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            if (id[e] < 0) t[e] = kNone;
+            id[e] = nextId[e];
+            t[e] = id[e] < 0 ? kNone : nextT[e];
             z[e] = id[e] < 0 ? kNone : static_cast<float>(row[id[e]]);
             m = fmaxf(m, bound(t[e]));
         }
@@ -150,7 +160,6 @@ struct Team {
         }
         s = wave_join<inWave>(s, Add());
         s += exp2_of((rest - base_of(m)) * a.c);
-        if (a.error != nullptr && bad) atomicOr(a.error, TCC_DEVERR_FEATURE_INDEX);
         if constexpr (TEAM > kWave) {  // from the first wave, which holds the entries, to the others
             if (threadIdx.x == 0) lds.one[odd] = make_float2(m, s);
             __syncthreads();
@@ -255,6 +264,59 @@ struct Batch {
     __device__ __forceinline__ vec_t<float, V> values(int u) const { return __builtin_convertvector(x[u], vec_t<float, V>); }
 };
 
+// A row that a team begins, and the next one where it holds whole rows: their
+// logits and entries are on their way while this one is computed (the gradient of
+// 2.45M x 100 fp32 rows: 420 us instead of 556), and the entries' logits
+// come from `row` in LDS instead of memory.
+template <typename T, int V, int TEAM, int E>
+struct Front {
+    using B = Batch<T, V, TEAM>;
+    const Args& a;
+    Team<TEAM, E>& team;
+    std::uint64_t r, step;
+    float w, nextW;
+    B batch, after;
+
+    __device__ __forceinline__ Front(const Args& args, Team<TEAM, E>& t) : a(args), team(t) {
+        step = static_cast<std::uint64_t>(gridDim.x) * kTeams<TEAM>;
+        r = static_cast<std::uint64_t>(blockIdx.x) * kTeams<TEAM> + threadIdx.x / TEAM;
+        nextW = weight_of(a, r);
+        if constexpr (B::whole) load(after, r, nextW);
+    }
+    __device__ __forceinline__ void load(B& to, std::uint64_t row, float weight) {
+        if (weight == 0.0f) return;
+        to.load(logits(row), 0, team.lane, a.C);
+        team.fetch(row);
+    }
+    __device__ __forceinline__ const T* logits(std::uint64_t row) const { return static_cast<const T*>(a.z) + row * a.ldz; }
+
+    // Takes up row r; true where it has a target.
+    __device__ __forceinline__ bool begin(float* row) {
+        w = nextW;
+        nextW = weight_of(a, r + step);
+        bool target = w != 0.0f;
+        if constexpr (B::whole) {
+            batch = after;
+            if (target) {
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u) {
+                    if (!B::any(0, u, a.C)) break;
+                    const Place<V> at = B::place(0, u, team.lane, a.C);
+                    if (at.any()) *reinterpret_cast<any_vec_t<float, V>*>(row + at.at) = batch.values(u);
+                }
+                team_sync<TEAM>();
+                target = team.load(row);
+                team_sync<TEAM>();
+            }
+            load(after, r + step, nextW);
+        } else {
+            load(batch, r, w);
+            target = target && team.load(logits(r));
+        }
+        return target;
+    }
+};
+
 template <typename T, int V, int TEAM, int E, bool REST>
 __global__ void __launch_bounds__(kThreads) loss_kernel(Args a) {
     using F = vec_t<float, V>;
@@ -263,18 +325,17 @@ __global__ void __launch_bounds__(kThreads) loss_kernel(Args a) {
     __shared__ Shared<TEAM> lds;
     Team<TEAM, E> team(lds, a);
     double lossSum = 0.0, weightSum = 0.0;
-    const std::uint64_t step = static_cast<std::uint64_t>(gridDim.x) * kTeams<TEAM>;
-    std::uint64_t r = static_cast<std::uint64_t>(blockIdx.x) * kTeams<TEAM> + threadIdx.x / TEAM;
-    float w = weight_of(a, r);
-    while (r < a.n) {
-        const float next = weight_of(a, r + step);
+    __shared__ __attribute__((aligned(16))) float table[B::whole ? kTeams<TEAM> : 1][B::whole ? B::stride : V];
+    for (Front<T, V, TEAM, E> front(a, team); front.r < a.n; front.r += front.step) {
+        const std::uint64_t r = front.r;
+        const bool target = front.begin(B::whole ? table[threadIdx.x / TEAM] : nullptr);
+        const T* z = front.logits(r);
+        const float w = front.w;
+        B& batch = front.batch;
         weightSum += w;
         float loss = 0.0f;
         float4 stats = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const T* z = static_cast<const T*>(a.z) + r * a.ldz;
-        B batch;
-        if (w != 0.0f) batch.load(z, 0, team.lane, a.C);
-        if (w != 0.0f && team.load(r, z)) {
+        if (target) {
             Share v, firsts;  // of the stream, and of the ids that are not in it
             for (std::uint32_t base = 0; base < a.C; base += B::stride) {
                 const std::uint32_t first = base & ~(kWindow<TEAM> - 1);
@@ -339,8 +400,6 @@ __global__ void __launch_bounds__(kThreads) loss_kernel(Args a) {
             if (a.loss != nullptr) a.loss[r] = loss;
             lossSum += loss;
         }
-        w = next;
-        r += step;
     }
     if (a.part == nullptr) return;
     // the first lanes' sums, in the order of the teams
@@ -398,19 +457,16 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(Args a) {
         each = count == 0.0f ? 0.0f : a.T / count;
     }
     if (a.reduction != TCC_REDUCE_NONE) each *= *a.dLoss;
-    const std::uint64_t step = static_cast<std::uint64_t>(gridDim.x) * kTeams<TEAM>;
-    std::uint64_t r = static_cast<std::uint64_t>(blockIdx.x) * kTeams<TEAM> + threadIdx.x / TEAM;
-    float w = weight_of(a, r);
-    while (r < a.n) {
-        const float next = weight_of(a, r + step);
-        const T* z = static_cast<const T*>(a.z) + r * a.ldz;
-        T* dz = static_cast<T*>(a.dz) + r * a.ldd;
-        B batch;
-        if (w != 0.0f) batch.load(z, 0, team.lane, a.C);
+    for (Front<T, V, TEAM, E> front(a, team); front.r < a.n; front.r += front.step) {
+        const std::uint64_t r = front.r;
         const float4 stats = a.stats[r];
-        float g = each * w;
+        float g = each;
         if (a.reduction == TCC_REDUCE_NONE) g *= a.dLoss[r];
-        const bool target = w != 0.0f && team.load(r, z);
+        const bool target = front.begin(B::whole ? table[threadIdx.x / TEAM] : nullptr);
+        g *= front.w;
+        const T* z = front.logits(r);
+        T* dz = static_cast<T*>(a.dz) + r * a.ldd;
+        B& batch = front.batch;
         const float perAll = inverse_of(stats.y);
         float base2 = stats.x, factor;  // of the others: factor 2^((z - base2) c)
         if (REST) {
@@ -465,7 +521,7 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(Args a) {
                 const std::uint32_t first = base & ~(kWindow<TEAM> - 1);
                 if (target && first == base) {
                     team.mark(first);
-    #pragma unroll
+#pragma unroll
                     for (int e = 0; e < E; ++e) {
                         float p;
                         if (!team.mine(e, first) || !team.leads(e, r, p)) continue;
@@ -474,7 +530,7 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(Args a) {
                 }
                 B after;
                 if (target) after.load(z, base + B::stride, team.lane, a.C);
-    #pragma unroll
+#pragma unroll
                 for (int u = 0; u < kBatch; ++u) {
                     if (!B::any(base, u, a.C)) break;
                     const Place<V> at = B::place(base, u, team.lane, a.C);
@@ -484,13 +540,13 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(Args a) {
                     if (target) {
                         const F x = batch.values(u);
                         out |= team.template marked<V>(at.at + at.skip - first) << at.skip;
-    #pragma unroll
+#pragma unroll
                         for (int q = 0; q < V; ++q) d[q] = factor * exp2_of((x[q] - base2) * a.c);
                     }
                     if (out == 0) {
                         store_any<T, V>(dz + at.at, d);
                     } else {
-    #pragma unroll
+#pragma unroll
                         for (int q = 0; q < V; ++q)
                             if (((out >> q) & 1) == 0) dz[at.at + q] = static_cast<T>(d[q]);
                     }
@@ -498,8 +554,6 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(Args a) {
                 batch = after;
             }
         }
-        w = next;
-        r += step;
     }
 }
 
