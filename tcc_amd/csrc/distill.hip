@@ -22,6 +22,7 @@
 // hold the entries write there; teams that hold a whole row in registers get the
 // entries' gradients from a table of its classes in LDS instead.
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/tcc_spmm_cnic.h"
 #include "../../include/tcc_swtcf.h"
@@ -208,7 +209,12 @@ struct Team {
         }
         return true;
     }
-    // Bits of the N classes from `at` (of this window) on.
+    // Bits of the N classes from `at` (of this window) on; marked_here: of a
+    // multiple of N.
+    template <int N>
+    __device__ __forceinline__ std::uint32_t marked_here(std::uint32_t at) const {
+        return bits[at / 32] >> (at & 31) & ((1u << N) - 1);
+    }
     template <int N>
     __device__ __forceinline__ std::uint32_t marked(std::uint32_t at) const {
         const std::uint32_t s = at & 31;
@@ -249,16 +255,24 @@ struct Batch {
     static __device__ __forceinline__ Place<V> place(std::uint32_t base, int u, std::uint32_t lane, std::uint32_t C) {
         return Place<V>(base / V + u * TEAM + lane, C);
     }
+    // Whether every lane has all of its vectors, whole ones.
+    static __device__ __forceinline__ bool inside(std::uint32_t base, std::uint32_t C) { return base + stride <= C; }
     // Whether any lane has a vector u.
     static __device__ __forceinline__ bool any(std::uint32_t base, int u, std::uint32_t C) {
         return base + static_cast<std::uint32_t>(u * TEAM * V) < C;
     }
     __device__ __forceinline__ void load(const T* z, std::uint32_t base, std::uint32_t lane, std::uint32_t C) {
+        if (!whole && inside(base, C)) {
+            z += base + lane * V;
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) x[u] = load_as<T, V>(z + u * TEAM * V);
+            return;
+        }
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
             if (!any(base, u, C)) break;
             const Place<V> at = place(base, u, lane, C);
-            if (at.any()) x[u] = load_global<any_vec_t<T, V>>(z + at.at);
+            if (at.any()) x[u] = load_as<T, V>(z + at.at);
         }
     }
     __device__ __forceinline__ vec_t<float, V> values(int u) const { return __builtin_convertvector(x[u], vec_t<float, V>); }
@@ -349,30 +363,39 @@ __global__ void __launch_bounds__(kThreads) loss_kernel(Args a) {
                 }
                 B after;
                 if constexpr (!B::whole) after.load(z, base + B::stride, team.lane, a.C);
-                F x[kBatch];
-                float m = kNone;
+                const auto add = [&](auto inside) {
+                    F x[kBatch];
+                    float m = kNone;
 #pragma unroll
-                for (int u = 0; u < kBatch; ++u) {
-                    if (!B::any(base, u, a.C)) break;
-                    const Place<V> at = B::place(base, u, team.lane, a.C);
-                    x[u] = batch.values(u);
-                    std::uint32_t out = (1u << at.skip) - 1;
-                    if (REST && at.any()) out |= team.template marked<V>(at.at + at.skip - first) << at.skip;
-                    if (out != 0) {
+                    for (int u = 0; u < kBatch; ++u) {
+                        if (!inside && !B::any(base, u, a.C)) break;
+                        x[u] = batch.values(u);
+                        std::uint32_t out = 0;
+                        if constexpr (inside) {
+                            if (REST) out = team.template marked_here<V>(base + (u * TEAM + team.lane) * V - first);
+                        } else {
+                            const Place<V> at = B::place(base, u, team.lane, a.C);
+                            out = (1u << at.skip) - 1;
+                            if (REST && at.any()) out |= team.template marked<V>(at.at + at.skip - first) << at.skip;
+                        }
+                        if (out != 0) {
 #pragma unroll
-                        for (int q = 0; q < V; ++q) x[u][q] = (out >> q) & 1 ? kNone : x[u][q];
+                            for (int q = 0; q < V; ++q) x[u][q] = (out >> q) & 1 ? kNone : x[u][q];
+                        }
+#pragma unroll
+                        for (int q = 0; q < V; ++q) m = fmaxf(m, x[u][q]);
                     }
+                    if (m > v.m) v.scale_to(m, a.c);
+                    const float b = base_of(v.m);
 #pragma unroll
-                    for (int q = 0; q < V; ++q) m = fmaxf(m, x[u][q]);
-                }
-                if (m > v.m) v.scale_to(m, a.c);
-                const float b = base_of(v.m);
+                    for (int u = 0; u < kBatch; ++u) {
+                        if (!inside && !B::any(base, u, a.C)) break;
 #pragma unroll
-                for (int u = 0; u < kBatch; ++u) {
-                    if (!B::any(base, u, a.C)) break;
-#pragma unroll
-                    for (int q = 0; q < V; ++q) v.s += exp2_of((x[u][q] - b) * a.c);
-                }
+                        for (int q = 0; q < V; ++q) v.s += exp2_of((x[u][q] - b) * a.c);
+                    }
+                };
+                if (!B::whole && B::inside(base, a.C)) add(std::true_type());
+                else add(std::false_type());
                 if constexpr (B::whole) break;
                 batch = after;
             }
@@ -530,27 +553,37 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(Args a) {
                 }
                 B after;
                 if (target) after.load(z, base + B::stride, team.lane, a.C);
+                const auto give = [&](auto inside) {
 #pragma unroll
-                for (int u = 0; u < kBatch; ++u) {
-                    if (!B::any(base, u, a.C)) break;
-                    const Place<V> at = B::place(base, u, team.lane, a.C);
-                    if (!at.any()) continue;
-                    F d(0.0f);
-                    std::uint32_t out = (1u << at.skip) - 1;
-                    if (target) {
-                        const F x = batch.values(u);
-                        out |= team.template marked<V>(at.at + at.skip - first) << at.skip;
+                    for (int u = 0; u < kBatch; ++u) {
+                        if (!inside && !B::any(base, u, a.C)) break;
+                        Place<V> at(0, V);
+                        if constexpr (inside) {
+                            at.at = base + (u * TEAM + team.lane) * V;
+                        } else {
+                            at = B::place(base, u, team.lane, a.C);
+                            if (!at.any()) continue;
+                        }
+                        F d(0.0f);
+                        std::uint32_t out = inside ? 0 : (1u << at.skip) - 1;
+                        if (target) {
+                            const F x = batch.values(u);
+                            out |= inside ? team.template marked_here<V>(at.at - first)
+                                          : team.template marked<V>(at.at + at.skip - first) << at.skip;
 #pragma unroll
-                        for (int q = 0; q < V; ++q) d[q] = factor * exp2_of((x[q] - base2) * a.c);
+                            for (int q = 0; q < V; ++q) d[q] = factor * exp2_of((x[q] - base2) * a.c);
+                        }
+                        if (out == 0) {
+                            store_any<T, V>(dz + at.at, d);
+                        } else {
+#pragma unroll
+                            for (int q = 0; q < V; ++q)
+                                if (((out >> q) & 1) == 0) dz[at.at + q] = static_cast<T>(d[q]);
+                        }
                     }
-                    if (out == 0) {
-                        store_any<T, V>(dz + at.at, d);
-                    } else {
-#pragma unroll
-                        for (int q = 0; q < V; ++q)
-                            if (((out >> q) & 1) == 0) dz[at.at + q] = static_cast<T>(d[q]);
-                    }
-                }
+                };
+                if (B::inside(base, a.C)) give(std::true_type());
+                else give(std::false_type());
                 batch = after;
             }
         }
