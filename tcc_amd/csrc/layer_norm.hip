@@ -382,7 +382,9 @@ struct Forward {
 
 // The gradient's workgroups are as many as run at once, with equal shares of the
 // rows: 1,795 us instead of 1,834 for 2.45M x 256 fp32 rows.
-constexpr std::uint64_t kMostBlocks = 8;  // a compute unit, of 256 threads: the workspace is for these
+// The most of them, for which the workspace is: no compute unit runs more of their
+// size and registers at once.
+std::uint64_t most_blocks(std::uint32_t C) { return (C <= 1024 ? 8ull : C <= 4096 ? 4ull : 1ull) * device_cus(); }
 template <typename T>
 struct Backward {
     const Args& a;
@@ -393,7 +395,7 @@ struct Backward {
         static std::uint32_t perCu;
         const auto kernel = grad_kernel<T, V, E, TEAM, ONCE>;
         blocks = std::min<std::uint64_t>({(a.N + kTeams<TEAM> - 1) / kTeams<TEAM>, resident_blocks(kernel, kThreads<TEAM>, perCu),
-                                          kMostBlocks * device_cus()});
+                                          most_blocks(a.C)});
         hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads<TEAM>), 0, st, a);
     }
     template <int V, int E, int TEAM>
@@ -468,7 +470,7 @@ extern "C" size_t tcc_layer_norm_grad_workspace_bytes(const tcc_layer_norm_shape
     using namespace tcc;
     if (check_shape(s) != TCC_OK) return 0;
     // the most workgroups of any team, which has one row or more
-    return std::min<std::uint64_t>(s->N, kMostBlocks * device_cus()) * 2 * s->C * sizeof(float);
+    return std::min<std::uint64_t>(s->N, most_blocks(s->C)) * 2 * s->C * sizeof(float);
 }
 
 extern "C" int tcc_layer_norm_grad(const tcc_layer_norm_shape* s, const void* dY, uint64_t lddy, const void* h,

@@ -113,6 +113,10 @@ struct Ahead {
     }
 };
 
+// How many elements a bound is good for that K are wanted of: each of them is
+// compared with all.
+__device__ __forceinline__ std::uint32_t enough(std::uint32_t K) { return K + K / 2 + 8; }
+
 // Its elements as floats, what is no element of it as -inf, and the largest of each
 // vector, a NaN where it has one.
 template <typename T, int V>
@@ -136,6 +140,29 @@ struct Elements {
 #pragma unroll
             for (int q = 1; q < V; ++q) most[u] = __builtin_elementwise_maximum(most[u], x[u][q]);
         }
+    }
+    // How many of the wave's elements reach b, which is above -inf.
+    __device__ __forceinline__ std::uint32_t reaching(float b) const {
+        std::uint32_t n = 0;
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+            for (int q = 0; q < V; ++q) n += __popcll(__ballot(!(x[u][q] < b)));
+        return n;
+    }
+    // As `halved` of rows in registers.
+    __device__ __forceinline__ float halved(float bound, std::uint32_t K) const {
+        std::uint32_t lo = order_of(bound), hi = uniform(order_of(wave_join<kWave>(largest(kNone), Larger()))) + 1;
+        while (hi - lo > 1) {
+            const std::uint32_t mid = lo + (hi - lo) / 2, n = reaching(value_of(mid));
+            if (n < K) {
+                hi = mid;
+            } else {
+                lo = mid;
+                if (n <= enough(K)) break;
+            }
+        }
+        return value_of(lo);
     }
     // Takes what is not below (ABOVE: not up to) the bound from vector u, and says
     // what that is: element q is bit V - 1 - q.
@@ -231,7 +258,11 @@ __global__ void __launch_bounds__(kThreads, 5) stream_kernel(Args a) {
             if constexpr (WAVES > 1) {
                 if (batch == 0) bound = agreed(0, value_of(kth_lane(own, K)));
             } else {
-                if (batch < 4 || batch % 4 == 0) bound = value_of(kth_lane(own, K));
+                if (K > 32) {  // the lanes' maxima are few for it: 2.5 times as many would reach the least of 64
+                    if (batch == 0) bound = e.halved(value_of(kth_lane(own, K)), K);
+                } else if (batch < 4 || batch % 4 == 0) {
+                    bound = value_of(kth_lane(own, K));
+                }
             }
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) {
@@ -246,7 +277,7 @@ __global__ void __launch_bounds__(kThreads, 5) stream_kernel(Args a) {
             }
             e.add_to(rest, a.c);
         }
-        bound = value_of(kth_lane(own, K));
+        bound = fmaxf(bound, value_of(kth_lane(own, K)));
         bool fits = count <= kFound;
         if constexpr (WAVES > 1) {
             if (lane_id() == 0) counts[w] = count;
@@ -525,7 +556,32 @@ __device__ __forceinline__ std::uint32_t team_scan(std::uint32_t x) {
 
 // Keys of a team that have room in LDS, a multiple of 4.
 template <int TEAM>
-constexpr std::uint32_t kRoom = TEAM == 4 ? 32 : TEAM == 16 ? 64 : 256;
+constexpr std::uint32_t kRoom = TEAM == 4 ? 32 : TEAM == 16 ? 128 : 256;
+
+// A bound that at least K elements reach and at most `most`, or the K-th largest,
+// from one that more reach: by halves of the range up to the team's largest.
+template <int TEAM, int N>
+__device__ __forceinline__ float halved(const float (&v)[N], float bound, std::uint32_t K, std::uint32_t most) {
+    float top = kNone;
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = fmaxf(top, v[i]);
+    std::uint32_t lo = order_of(bound), hi = order_of(wave_join<TEAM>(top, Larger())) + 1;
+    while (hi - lo > 1) {
+        const std::uint32_t mid = lo + (hi - lo) / 2;
+        const float b = value_of(mid);
+        std::uint32_t n = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) n += v[i] < b ? 0u : 1u;
+        n = wave_join<TEAM>(n, Add());
+        if (n < K) {
+            hi = mid;
+        } else {
+            lo = mid;
+            if (n <= most) break;
+        }
+    }
+    return value_of(lo);
+}
 
 __device__ __forceinline__ Key larger_key(Key a, Key b) { return a > b ? a : b; }
 // The largest key of a team.
@@ -587,14 +643,19 @@ __global__ void __launch_bounds__(kThreads) registers_kernel(Args a) {
             for (std::uint32_t q = 0; q < V; ++q) v[e * V + q] = q >= skip ? static_cast<float>(ahead[e][q]) : kNone;
         }
         load(r + step);
-        const float bound = reached<TEAM>(v, a.K);
-        std::uint32_t reach = 0;
+        float bound = reached<TEAM>(v, a.K);
+        std::uint32_t reach, own, to, all;
+        for (bool again = false;; again = true) {
+            reach = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i) reach += reach + (v[i] < bound ? 0u : 1u);
-        reach &= valid;
-        const std::uint32_t own = __popc(reach);
-        std::uint32_t to = team_scan<TEAM>(own);
-        const std::uint32_t all = static_cast<std::uint32_t>(__shfl(static_cast<int>(to), TEAM - 1, TEAM));
+            for (int i = 0; i < N; ++i) reach += reach + (v[i] < bound ? 0u : 1u);
+            reach &= valid;
+            own = __popc(reach);
+            to = team_scan<TEAM>(own);
+            all = static_cast<std::uint32_t>(__shfl(static_cast<int>(to), TEAM - 1, TEAM));
+            if (again || all <= min(room, enough(a.K))) break;
+            bound = halved<TEAM>(v, bound, a.K, min(room, enough(a.K)));
+        }
         const auto index = [&](std::uint32_t i) { return Place<V>(lane + i / V * TEAM, a.C).at + i % V; };
         Share rest;
         if (all <= room) {
@@ -681,8 +742,8 @@ void in_registers(const Args& a, hipStream_t st) {
 }
 
 // Rows of up to 1,024 classes are held in registers: by 4 lanes of a wave with up to
-// 32 elements each where K allows their bound, by 16 with up to 16, else by a wave.
-// Longer ones are streamed.
+// 32 elements each where these have room for K, by 16 with as many, by a wave with
+// 16.  Longer ones are streamed.
 template <typename T>
 void launch(const Args& a, hipStream_t st) {
     constexpr int V = kVec<T>;
@@ -693,14 +754,11 @@ void launch(const Args& a, hipStream_t st) {
         if (C <= 8 * V) return in_registers<T, V, 2, 4>(a, st);
         if (C <= 64) return in_registers<T, V, 16 / V, 4>(a, st);
         if (C <= 128) return in_registers<T, V, 32 / V, 4>(a, st);
-        if (C <= 256) return in_registers<T, V, 16 / V, 16>(a, st);
     }
-    if (C <= 64) return in_registers<T, V, 8 / V, 16>(a, st);
-    if (C <= 64 * V) return in_registers<T, V, 1, 64>(a, st);
-    if (C <= 128 * V) return in_registers<T, V, 2, 64>(a, st);
-    if constexpr (V == 4) {
-        if (C <= 256 * V) return in_registers<T, V, 4, 64>(a, st);
-    }
+    if (C <= 128) return in_registers<T, V, 8 / V, 16>(a, st);
+    if (C <= 256) return in_registers<T, V, 16 / V, 16>(a, st);
+    if (C <= 512) return in_registers<T, V, 32 / V, 16>(a, st);
+    if (C <= 1024) return in_registers<T, V, 16 / V, 64>(a, st);
     // A wave a row where there are three for each SIMD (4,096 x 50,000 bf16, K = 32: 100 us
     // instead of 112 with a workgroup a row, of which an uneven number are left at the
     // end) and K leaves its bound room; a workgroup else.
