@@ -246,10 +246,10 @@ struct Team {
 constexpr std::uint32_t kNoEntry = 0x7FD00001u;
 
 // A batch of a team: kBatch vectors a lane, from element `base` of the row on.
-template <typename T, int V, int TEAM>
+template <typename T, int V, int TEAM, bool WHOLE>
 struct Batch {
     static constexpr std::uint32_t stride = TEAM * kBatch * V;
-    static constexpr bool whole = TEAM <= 16;  // rows of these teams are one batch
+    static constexpr bool whole = WHOLE;  // rows are one batch
     vec_t<T, V> x[kBatch];
 
     static __device__ __forceinline__ Place<V> place(std::uint32_t base, int u, std::uint32_t lane, std::uint32_t C) {
@@ -282,9 +282,9 @@ struct Batch {
 // logits and entries are on their way while this one is computed (the gradient of
 // 2.45M x 100 fp32 rows: 420 us instead of 556), and the entries' logits
 // come from `row` in LDS instead of memory.
-template <typename T, int V, int TEAM, int E>
+template <typename T, int V, int TEAM, int E, bool WHOLE>
 struct Front {
-    using B = Batch<T, V, TEAM>;
+    using B = Batch<T, V, TEAM, WHOLE>;
     const Args& a;
     Team<TEAM, E>& team;
     std::uint64_t r, step;
@@ -331,16 +331,16 @@ struct Front {
     }
 };
 
-template <typename T, int V, int TEAM, int E, bool REST>
+template <typename T, int V, int TEAM, int E, bool WHOLE, bool REST>
 __global__ void __launch_bounds__(kThreads) loss_kernel(Args a) {
     using F = vec_t<float, V>;
-    using B = Batch<T, V, TEAM>;
+    using B = Batch<T, V, TEAM, WHOLE>;
     static_assert(kWindow<TEAM> % B::stride == 0 || B::whole);
     __shared__ Shared<TEAM> lds;
     Team<TEAM, E> team(lds, a);
     double lossSum = 0.0, weightSum = 0.0;
     __shared__ __attribute__((aligned(16))) float table[B::whole ? kTeams<TEAM> : 1][B::whole ? B::stride : V];
-    for (Front<T, V, TEAM, E> front(a, team); front.r < a.n; front.r += front.step) {
+    for (Front<T, V, TEAM, E, WHOLE> front(a, team); front.r < a.n; front.r += front.step) {
         const std::uint64_t r = front.r;
         const bool target = front.begin(B::whole ? table[threadIdx.x / TEAM] : nullptr);
         const T* z = front.logits(r);
@@ -467,10 +467,10 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const double2* part, std
     if (total != nullptr) *total = static_cast<float>(w);
 }
 
-template <typename T, int V, int TEAM, int E, bool REST>
+template <typename T, int V, int TEAM, int E, bool WHOLE, bool REST>
 __global__ void __launch_bounds__(kThreads) grad_kernel(Args a) {
     using F = vec_t<float, V>;
-    using B = Batch<T, V, TEAM>;
+    using B = Batch<T, V, TEAM, WHOLE>;
     __shared__ Shared<TEAM> lds;
     __shared__ __attribute__((aligned(16))) float table[B::whole ? kTeams<TEAM> : 1][B::whole ? B::stride : V];
     Team<TEAM, E> team(lds, a);
@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(Args a) {
         each = count == 0.0f ? 0.0f : a.T / count;
     }
     if (a.reduction != TCC_REDUCE_NONE) each *= *a.dLoss;
-    for (Front<T, V, TEAM, E> front(a, team); front.r < a.n; front.r += front.step) {
+    for (Front<T, V, TEAM, E, WHOLE> front(a, team); front.r < a.n; front.r += front.step) {
         const std::uint64_t r = front.r;
         const float4 stats = a.stats[r];
         float g = each;
@@ -592,23 +592,24 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(Args a) {
 
 // ---------------------------------------------------------------- launches
 
-// The team for rows of C classes and K entries; f is called with <V, TEAM, E>.
-// A team's lanes take one batch of a row where it can be, and a wave up to
-// 4,096 classes; they have room for the entries.
+// The team for rows of C classes and K entries; f is called with <V, TEAM, E,
+// WHOLE>.  A team takes whole rows where its lanes' batch holds them; a wave longer
+// ones up to 4,096 classes, a workgroup above.
 template <typename T, typename F>
 void with_team(std::uint32_t C, std::uint32_t K, F f) {
     constexpr int V = kVec<T>;
     if (C < V) {
-        if (K <= 4) return f.template operator()<1, 4, 1>();
-        return f.template operator()<1, 16, 4>();
+        if (K <= 4) return f.template operator()<1, 4, 1, true>();
+        return f.template operator()<1, 16, 4, true>();
     }
-    if (C <= 4 * kBatch * V && C <= kWindow<4> && K <= 4) return f.template operator()<V, 4, 1>();
-    if (C <= 16 * kBatch * V && C <= kWindow<16>) {
-        if (K <= 16) return f.template operator()<V, 16, 1>();
-        return f.template operator()<V, 16, 4>();
+    if (C <= 4 * kBatch * V && K <= 4) return f.template operator()<V, 4, 1, true>();
+    if (C <= 16 * kBatch * V) {
+        if (K <= 16) return f.template operator()<V, 16, 1, true>();
+        return f.template operator()<V, 16, 4, true>();
     }
-    if (C <= 4096) return f.template operator()<V, 64, 1>();
-    return f.template operator()<V, 256, 1>();
+    if (C <= 64 * kBatch * V) return f.template operator()<V, 64, 1, true>();
+    if (C <= 4096) return f.template operator()<V, 64, 1, false>();
+    return f.template operator()<V, 256, 1, false>();
 }
 
 // A grid of the workgroups that run at once, or those that n rows need.
@@ -624,22 +625,22 @@ struct Loss {
     const Args& a;
     hipStream_t st;
     std::uint64_t& blocks;
-    template <int V, int TEAM, int E>
+    template <int V, int TEAM, int E, bool WHOLE>
     void operator()() const {
         static std::uint32_t perCu[2];
-        blocks = a.rest != nullptr ? launch(loss_kernel<T, V, TEAM, E, true>, perCu[1], a, kTeams<TEAM>, st)
-                                   : launch(loss_kernel<T, V, TEAM, E, false>, perCu[0], a, kTeams<TEAM>, st);
+        blocks = a.rest != nullptr ? launch(loss_kernel<T, V, TEAM, E, WHOLE, true>, perCu[1], a, kTeams<TEAM>, st)
+                                   : launch(loss_kernel<T, V, TEAM, E, WHOLE, false>, perCu[0], a, kTeams<TEAM>, st);
     }
 };
 template <typename T>
 struct Grad {
     const Args& a;
     hipStream_t st;
-    template <int V, int TEAM, int E>
+    template <int V, int TEAM, int E, bool WHOLE>
     void operator()() const {
         static std::uint32_t perCu[2];
-        if (a.rest != nullptr) launch(grad_kernel<T, V, TEAM, E, true>, perCu[1], a, kTeams<TEAM>, st);
-        else launch(grad_kernel<T, V, TEAM, E, false>, perCu[0], a, kTeams<TEAM>, st);
+        if (a.rest != nullptr) launch(grad_kernel<T, V, TEAM, E, WHOLE, true>, perCu[1], a, kTeams<TEAM>, st);
+        else launch(grad_kernel<T, V, TEAM, E, WHOLE, false>, perCu[0], a, kTeams<TEAM>, st);
     }
 };
 

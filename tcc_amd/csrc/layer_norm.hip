@@ -14,7 +14,7 @@
 // does not divide into them is moved back to end with it; what it shares with
 // the one before counts once in every sum, and is written twice with the same
 // value).  Teams are as small as 16 elements a lane allow, which saves
-// reductions, at least four lanes, at most the 1,024 threads of a workgroup.
+// reductions: four lanes of a wave to the 1,024 threads of a workgroup.
 // A lane adds its elements in pairs, and the lanes' sums are added in 64 bits: the
 // mean comes out rounded once for most rows.  The variance is the mean square of
 // the differences from that, less the square of their mean, which is what rows
@@ -344,6 +344,7 @@ void with_team(std::uint32_t C, F f) {
     const auto fits = [&](std::uint64_t v, std::uint64_t e, std::uint64_t team) { return C <= team * e * v; };
     if (C < V) return f.template operator()<1, 2, 4>();
     if (fits(V, 1, 4)) return f.template operator()<V, 1, 4>();
+    if (fits(V, 1, 8)) return f.template operator()<V, 1, 8>();
     if (fits(V, 1, 16)) return f.template operator()<V, 1, 16>();
     if (fits(V, 2, 16)) return f.template operator()<V, 2, 16>();
     if constexpr (V == 4) {
@@ -356,6 +357,7 @@ void with_team(std::uint32_t C, F f) {
     if (fits(4, 4, 64)) return f.template operator()<V, 16 / V, 64>();
     if (fits(4, 2, 256)) return f.template operator()<V, 8 / V, 256>();
     if (fits(4, 4, 256)) return f.template operator()<V, 16 / V, 256>();
+    if (fits(4, 4, 512)) return f.template operator()<V, 16 / V, 512>();
     return f.template operator()<V, 16 / V, 1024>();
 }
 
@@ -384,7 +386,7 @@ struct Forward {
 // rows: 1,795 us instead of 1,834 for 2.45M x 256 fp32 rows.
 // The most of them, for which the workspace is: no compute unit runs more of their
 // size and registers at once.
-std::uint64_t most_blocks(std::uint32_t C) { return (C <= 1024 ? 8ull : C <= 4096 ? 4ull : 1ull) * device_cus(); }
+std::uint64_t most_blocks(std::uint32_t C) { return (C <= 1024 ? 8ull : C <= 4096 ? 4ull : C <= 8192 ? 2ull : 1ull) * device_cus(); }
 template <typename T>
 struct Backward {
     const Args& a;
