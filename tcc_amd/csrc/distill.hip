@@ -9,7 +9,7 @@
 //   dz_j = g w T (q_j - p_k)            for j = id_k
 //          g w T (q_j - p_r q_j / q_r)  for the others (p_r = 0 without r)
 //
-// A team of lanes takes a row: 4, 16 or 64 of a wave, or a workgroup of 256.
+// A team of lanes takes a row: 4, 16, 32 or 64 of a wave, or a workgroup of 256.
 // Each lane keeps the maximum of what it read and the sum of
 // exp((z - maximum) / T), rescaled when the maximum rises, so that a row is
 // read once.  Everything is in base 2 with one factor log2(e) / T, rounded
@@ -67,7 +67,7 @@ constexpr int kTeams = kThreads / TEAM;
 
 // Classes whose bits a team holds at once, a multiple of 32.
 template <int TEAM>
-constexpr std::uint32_t kWindow = TEAM == 4 ? 128 : TEAM == 16 ? 512 : TEAM == 64 ? 4096 : 1u << 17;
+constexpr std::uint32_t kWindow = TEAM == 4 ? 128 : TEAM == 16 ? 512 : TEAM == 32 ? 1024 : TEAM == 64 ? 4096 : 1u << 17;
 
 __device__ __forceinline__ float weight_of(const Args& a, std::uint64_t r) {
     return r >= a.n ? 0.0f : a.weight == nullptr ? 1.0f : a.weight[r];
@@ -605,7 +605,12 @@ void with_team(std::uint32_t C, std::uint32_t K, F f) {
     if (C <= 4 * kBatch * V && K <= 4) return f.template operator()<V, 4, 1, true>();
     if (C <= 16 * kBatch * V) {
         if (K <= 16) return f.template operator()<V, 16, 1, true>();
+        if (K <= 32) return f.template operator()<V, 16, 2, true>();
         return f.template operator()<V, 16, 4, true>();
+    }
+    if (C <= 32 * kBatch * V) {
+        if (K <= 32) return f.template operator()<V, 32, 1, true>();
+        return f.template operator()<V, 32, 2, true>();
     }
     if (C <= 64 * kBatch * V) return f.template operator()<V, 64, 1, true>();
     if (C <= 4096) return f.template operator()<V, 64, 1, false>();

@@ -357,7 +357,10 @@ void with_team(std::uint32_t C, F f) {
     if (fits(4, 4, 64)) return f.template operator()<V, 16 / V, 64>();
     if (fits(4, 2, 256)) return f.template operator()<V, 8 / V, 256>();
     if (fits(4, 4, 256)) return f.template operator()<V, 16 / V, 256>();
-    if (fits(4, 4, 512)) return f.template operator()<V, 16 / V, 512>();
+    if (fits(4, 4, 512)) {  // the gradient has registers for two waves of 16 elements a lane on a SIMD, no more
+        if constexpr (F::forward) return f.template operator()<V, 16 / V, 512>();
+        else return f.template operator()<V, 8 / V, 1024>();
+    }
     return f.template operator()<V, 16 / V, 1024>();
 }
 
@@ -369,6 +372,7 @@ bool once(const Args& a) { return a.N * a.C * sizeof(T) > kCacheBytes; }
 
 template <typename T>
 struct Forward {
+    static constexpr bool forward = true;
     const Args& a;
     hipStream_t st;
     template <int V, int E, int TEAM>
@@ -386,9 +390,10 @@ struct Forward {
 // rows: 1,795 us instead of 1,834 for 2.45M x 256 fp32 rows.
 // The most of them, for which the workspace is: no compute unit runs more of their
 // size and registers at once.
-std::uint64_t most_blocks(std::uint32_t C) { return (C <= 1024 ? 8ull : C <= 4096 ? 4ull : C <= 8192 ? 2ull : 1ull) * device_cus(); }
+std::uint64_t most_blocks(std::uint32_t C) { return (C <= 1024 ? 8ull : C <= 4096 ? 4ull : 1ull) * device_cus(); }
 template <typename T>
 struct Backward {
+    static constexpr bool forward = false;
     const Args& a;
     hipStream_t st;
     std::uint64_t& blocks;
