@@ -661,7 +661,8 @@ __global__ void __launch_bounds__(kThreads) registers_kernel(Args a) {
         if (all <= room) {
             // their classes first: a register chosen at run time costs two instructions
             // for each that there is, and the row's lines are near
-            auto* classes = reinterpret_cast<std::uint32_t*>(mine);
+            using Class = std::uint32_t __attribute__((may_alias));
+            auto* classes = reinterpret_cast<Class*>(mine);
             for (to -= own; reach != 0; reach &= reach - 1) classes[2 * to++] = index(N - 1 - __builtin_ctz(reach));
             wave_sync();
 #pragma unroll 4
