@@ -21,8 +21,8 @@
 // far from zero have lost.
 //
 // The gradient's teams walk the rows in equal steps and keep the sums of dz and
-// dz xh of their channels in registers; a workgroup adds its teams' in LDS and
-// writes one row, and a second kernel adds the rows in 64 bits.
+// dz xh of their channels in registers, in up to four runs; a workgroup adds its
+// teams' in LDS in 64 bits and writes a row a run, and a second kernel adds those.
 #include <algorithm>
 
 #include "../../include/tcc_swtcf.h"
@@ -39,9 +39,11 @@ constexpr std::uint32_t kMaxChannels = 16384;
 struct Args {
     const void *x, *residual, *dy, *dSum, *weight, *bias;
     void *out, *sum;  // y or dx, h
-    float *mean, *rstd, *part;  // part: [workgroups][2][C], dBias and dWeight
+    float *mean, *rstd;
+    float* part;  // [runs][workgroups][2][C], dBias and dWeight
+    std::uint64_t runRows;  // rows of a team in each of its runs
     std::uint64_t N, ldx, ldr, lddy, ldds, ldo, lds;
-    std::uint32_t C, paramType, act;
+    std::uint32_t C, paramType, act, runs;
     float eps;
 };
 
@@ -233,81 +235,86 @@ __global__ void __launch_bounds__(kThreads<TEAM>) grad_kernel(Args a) {
         rstd = a.rstd[row];
     };
     if constexpr (kAhead<T, V, E, TEAM>) load(r);
-    for (; r < a.N; r += step) {
-        if constexpr (!kAhead<T, V, E, TEAM>) load(r);
-        F xh[E], dz[E];
+    for (std::uint32_t run = 0; run < a.runs; ++run) {
+        for (std::uint64_t i = 0; i < a.runRows && r < a.N; ++i, r += step) {
+            if constexpr (!kAhead<T, V, E, TEAM>) load(r);
+            F xh[E], dz[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            xh[e] = x[e];
-            dz[e] = dy[e];
-        }
-        const float m = mean, rs = rstd;
-        if constexpr (kAhead<T, V, E, TEAM>) load(r + step);
-        float s1 = 0.0f, s2 = 0.0f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            if (!cols.any(e)) continue;
-            F z;
-#pragma unroll
-            for (int q = 0; q < V; ++q) {
-                xh[e][q] = normalise(xh[e][q], m, rs);
-                z[q] = affine(xh[e][q], w[e][q], b[e][q]);
+            for (int e = 0; e < E; ++e) {
+                xh[e] = x[e];
+                dz[e] = dy[e];
             }
-            dz[e] = through_by<kFine<T>, V>(a.act, dz[e], z);
-            const F d = cols.own(e, dz[e]);
-            db[e] += d;
+            const float m = mean, rs = rstd;
+            if constexpr (kAhead<T, V, E, TEAM>) load(r + step);
+            float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
-            for (int q = 0; q < V; ++q) {
-                const float dx = d[q] * xh[e][q];
-                dw[e][q] += dx;
-                s1 = fmaf(d[q], w[e][q], s1);
-                s2 = fmaf(dx, w[e][q], s2);
-            }
-        }
-        const float2 both = sum(s1, s2);
-        const float m1 = both.x * perC, m2 = both.y * perC;
-        T* out = static_cast<T*>(a.out) + r * a.ldo;
-        const T* add = static_cast<const T*>(a.dSum) + r * a.ldds;
+            for (int e = 0; e < E; ++e) {
+                if (!cols.any(e)) continue;
+                F z;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            if (!cols.any(e)) continue;
-            F v;
-#pragma unroll
-            for (int q = 0; q < V; ++q) v[q] = rs * (fmaf(dz[e][q], w[e][q], -m1) - xh[e][q] * m2);
-            if (a.dSum != nullptr) v += load_any<T, V, ONCE>(add + cols.c[e]);
-            store_any<T, V, ONCE>(out + cols.c[e], v);
-        }
-    }
-    if (a.part == nullptr) return;
-    // the workgroup's sums: its teams', one after the other
-    float* to = a.part + static_cast<std::uint64_t>(blockIdx.x) * 2 * a.C;
-    if constexpr (kTeams<TEAM> == 1) {
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-#pragma unroll
-            for (int q = 0; q < V; ++q)
-                if (static_cast<std::uint32_t>(q) >= cols.skip[e]) {
-                    to[cols.c[e] + q] = db[e][q];
-                    to[a.C + cols.c[e] + q] = dw[e][q];
+                for (int q = 0; q < V; ++q) {
+                    xh[e][q] = normalise(xh[e][q], m, rs);
+                    z[q] = affine(xh[e][q], w[e][q], b[e][q]);
                 }
-    } else {
-        __shared__ float total[2][TEAM * E * V];
-        for (int k = 0; k < kTeams<TEAM>; ++k) {
-            if (threadIdx.x / TEAM == k) {
+                dz[e] = through_by<kFine<T>, V>(a.act, dz[e], z);
+                const F d = cols.own(e, dz[e]);
+                db[e] += d;
 #pragma unroll
-                for (int e = 0; e < E; ++e)
-#pragma unroll
-                    for (int q = 0; q < V; ++q)
-                        if (static_cast<std::uint32_t>(q) >= cols.skip[e]) {
-                            const std::uint32_t c = cols.c[e] + q;
-                            total[0][c] = k == 0 ? db[e][q] : total[0][c] + db[e][q];
-                            total[1][c] = k == 0 ? dw[e][q] : total[1][c] + dw[e][q];
-                        }
+                for (int q = 0; q < V; ++q) {
+                    const float dx = d[q] * xh[e][q];
+                    dw[e][q] += dx;
+                    s1 = fmaf(d[q], w[e][q], s1);
+                    s2 = fmaf(dx, w[e][q], s2);
+                }
             }
+            const float2 both = sum(s1, s2);
+            const float m1 = both.x * perC, m2 = both.y * perC;
+            T* out = static_cast<T*>(a.out) + r * a.ldo;
+            const T* add = static_cast<const T*>(a.dSum) + r * a.ldds;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                if (!cols.any(e)) continue;
+                F v;
+#pragma unroll
+                for (int q = 0; q < V; ++q) v[q] = rs * (fmaf(dz[e][q], w[e][q], -m1) - xh[e][q] * m2);
+                if (a.dSum != nullptr) v += load_any<T, V, ONCE>(add + cols.c[e]);
+                store_any<T, V, ONCE>(out + cols.c[e], v);
+            }
+        }
+        if (a.part == nullptr) continue;
+        // the workgroup's sums of the run: its teams', one after the other
+        float* to = a.part + (static_cast<std::uint64_t>(run) * gridDim.x + blockIdx.x) * 2 * a.C;
+        if constexpr (kTeams<TEAM> == 1) {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+#pragma unroll
+                for (int q = 0; q < V; ++q)
+                    if (static_cast<std::uint32_t>(q) >= cols.skip[e]) {
+                        to[cols.c[e] + q] = db[e][q];
+                        to[a.C + cols.c[e] + q] = dw[e][q];
+                    }
+        } else {
+            __shared__ double total[2][TEAM * E * V];
+            for (int k = 0; k < kTeams<TEAM>; ++k) {
+                if (threadIdx.x / TEAM == k) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e)
+#pragma unroll
+                        for (int q = 0; q < V; ++q)
+                            if (static_cast<std::uint32_t>(q) >= cols.skip[e]) {
+                                const std::uint32_t c = cols.c[e] + q;
+                                total[0][c] = db[e][q] + (k == 0 ? 0.0 : total[0][c]);
+                                total[1][c] = dw[e][q] + (k == 0 ? 0.0 : total[1][c]);
+                            }
+                }
+                __syncthreads();
+            }
+            for (std::uint32_t i = threadIdx.x; i < 2 * a.C; i += kThreads<TEAM>)
+                to[i] = static_cast<float>(i < a.C ? total[0][i] : total[1][i - a.C]);
             __syncthreads();
         }
-        for (std::uint32_t i = threadIdx.x; i < 2 * a.C; i += kThreads<TEAM>)
-            to[i] = i < a.C ? total[0][i] : total[1][i - a.C];
+#pragma unroll
+        for (int e = 0; e < E; ++e) dw[e] = db[e] = F(0.0f);
     }
 }
 
@@ -388,6 +395,13 @@ struct Forward {
 
 // The gradient's workgroups are as many as run at once, with equal shares of the
 // rows: 1,795 us instead of 1,834 for 2.45M x 256 fp32 rows.
+// A team sums a run of its rows in 32 bits, a workgroup its teams' in 64, and the
+// parameters' kernel the runs': sums of the 200 rows that a team has of 2.45M x 256
+// had twice the rounding error of 50 each, and cost 20 us less of 1,800.
+constexpr std::uint64_t kMostRuns = 4;
+template <int TEAM>
+constexpr std::uint64_t kRun = kTeams<TEAM> == 1 ? 96 : 48;
+
 // The most of them, for which the workspace is: no compute unit runs more of their
 // size and registers at once.
 std::uint64_t most_blocks(std::uint32_t C) { return (C <= 1024 ? 8ull : C <= 4096 ? 4ull : 1ull) * device_cus(); }
@@ -396,14 +410,19 @@ struct Backward {
     static constexpr bool forward = false;
     const Args& a;
     hipStream_t st;
-    std::uint64_t& blocks;
+    std::uint64_t& parts;
     template <int V, int E, int TEAM, bool ONCE>
     void launch() const {
         static std::uint32_t perCu;
         const auto kernel = grad_kernel<T, V, E, TEAM, ONCE>;
-        blocks = std::min<std::uint64_t>({(a.N + kTeams<TEAM> - 1) / kTeams<TEAM>, resident_blocks(kernel, kThreads<TEAM>, perCu),
-                                          most_blocks(a.C)});
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads<TEAM>), 0, st, a);
+        const std::uint64_t blocks = std::min<std::uint64_t>(
+            {(a.N + kTeams<TEAM> - 1) / kTeams<TEAM>, resident_blocks(kernel, kThreads<TEAM>, perCu), most_blocks(a.C)});
+        Args k = a;
+        const std::uint64_t rows = (a.N + blocks * kTeams<TEAM> - 1) / (blocks * kTeams<TEAM>);
+        k.runs = a.part == nullptr ? 1u : static_cast<std::uint32_t>(std::clamp<std::uint64_t>(rows / kRun<TEAM>, 1, kMostRuns));
+        k.runRows = (rows + k.runs - 1) / k.runs;
+        parts = blocks * k.runs;
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads<TEAM>), 0, st, k);
     }
     template <int V, int E, int TEAM>
     void operator()() const {
@@ -477,7 +496,7 @@ extern "C" size_t tcc_layer_norm_grad_workspace_bytes(const tcc_layer_norm_shape
     using namespace tcc;
     if (check_shape(s) != TCC_OK) return 0;
     // the most workgroups of any team, which has one row or more
-    return std::min<std::uint64_t>(s->N, most_blocks(s->C)) * 2 * s->C * sizeof(float);
+    return std::min<std::uint64_t>(s->N, most_blocks(s->C)) * kMostRuns * 2 * s->C * sizeof(float);
 }
 
 extern "C" int tcc_layer_norm_grad(const tcc_layer_norm_shape* s, const void* dY, uint64_t lddy, const void* h,
@@ -510,14 +529,14 @@ extern "C" int tcc_layer_norm_grad(const tcc_layer_norm_shape* s, const void* dY
     a.out = dX;
     a.ldo = lddx;
     a.part = params ? static_cast<float*>(workspace) : nullptr;
-    std::uint64_t blocks = 0;
+    std::uint64_t parts = 0;
     if (s->N > 0) {
-        launch_typed<Backward>(s->dtype, a, as_stream(stream), blocks);
+        launch_typed<Backward>(s->dtype, a, as_stream(stream), parts);
         TCC_LAUNCH_CHECK();
     }
     if (params) {
         hipLaunchKernelGGL(params_kernel, dim3(grid_for(2ull * s->C, kParamCols)), dim3(kParamCols * kParamRows), 0,
-                           as_stream(stream), a.part, static_cast<std::uint32_t>(blocks), s->C, dBias, dWeight);
+                           as_stream(stream), a.part, static_cast<std::uint32_t>(parts), s->C, dBias, dWeight);
         TCC_LAUNCH_CHECK();
     }
     return TCC_OK;
