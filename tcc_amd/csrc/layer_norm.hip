@@ -373,7 +373,7 @@ void with_team(std::uint32_t C, F f) {
 
 // Rows past what the caches hold are read and written past their order: 2.45M x
 // 256 fp32 rows with a residual in 1,820 us instead of 1,870, their gradient in
-// 1,795 instead of 1,880.
+// 4% less time than otherwise.
 template <typename T>
 bool once(const Args& a) { return a.N * a.C * sizeof(T) > kCacheBytes; }
 
@@ -394,10 +394,10 @@ struct Forward {
 };
 
 // The gradient's workgroups are as many as run at once, with equal shares of the
-// rows: 1,795 us instead of 1,834 for 2.45M x 256 fp32 rows.
-// A team sums a run of its rows in 32 bits, a workgroup its teams' in 64, and the
-// parameters' kernel the runs': sums of the 200 rows that a team has of 2.45M x 256
-// had twice the rounding error of 50 each, and cost 20 us less of 1,800.
+// rows: 1,838 us for 2.45M x 256 fp32 rows (10.0 GB), 40 less than with three or
+// four times as many.  A team sums a run of its rows in 32 bits, a workgroup its
+// teams' in 64, and the parameters' kernel the runs': with one run of 200 rows
+// dWeight's error was twice that of four of 50, at 35 us less.
 constexpr std::uint64_t kMostRuns = 4;
 template <int TEAM>
 constexpr std::uint64_t kRun = kTeams<TEAM> == 1 ? 96 : 48;

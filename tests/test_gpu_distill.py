@@ -123,6 +123,15 @@ def test_both_passes(gpu, dtype, n, C, K):
     check(z, values, ids.long(), rest, 1.5, None, "none")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,C,K", [(600, 16, 3), (500, 17, 9), (600, 400, 4), (300, 255, 33), (300, 513, 16), (64, 700, 8),
+                                   (64, 1024, 40), (60, 1025, 2), (30, 2500, 64), (40, 8200, 8), (300, 20_000, 4)])
+def test_more_of_every_path(gpu, dtype, n, C, K):
+    z, values, ids, rest, w = inputs(n, C, K, dtype, n + C, spread=6.0)
+    check(z, values, ids, rest, 3.0, w)
+    check(z, values, ids, None, 1.0, None, "none")
+
+
 @pytest.mark.parametrize("value_type", TYPES)
 @pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
 def test_types_of_the_entries(gpu, value_type, reduction):

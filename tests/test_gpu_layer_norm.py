@@ -134,6 +134,45 @@ def test_more_rows_than_teams(gpu, N, C):
                got[3], w, b, "relu", e)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_every_width_of_team(gpu, dtype):
+    """The last channels that a team holds, and the first that the next one does."""
+    from tcc_amd import training
+
+    for C in (4, 5, 8, 12, 17, 31, 32, 36, 65, 95, 128, 129, 192, 193, 255, 257, 383, 385, 511, 513, 767, 769, 1023, 1024, 1025,
+              2047, 2049, 4095, 4096, 8191, 8192, 8193, 16_000):
+        _, x, res, w, b, d, e = inputs(23, C, dtype, C)
+        got = training.layer_norm(x, w, b, residual=res, activation="gelu")
+        check_forward(got, x, res, w, b, 1e-5, "gelu")
+        check_grad(training.layer_norm_grad(d, *got[1:], w, b, d_sum=e, activation="gelu"), d, *got[1:], w, b, "gelu", e)
+
+
+@pytest.mark.parametrize("N,C,dtype,run", [(30_000_000, 6, torch.float32, 144), (1_300_000, 250, torch.float32, 144),
+                                           (2_000_001, 257, torch.bfloat16, 144), (200_000, 4000, torch.bfloat16, 288),
+                                           (70_001, 8192, torch.float32, 288), (60_000, 16_384, torch.float16, 288)])
+def test_parameter_sums_over_many_rows(gpu, N, C, dtype, run):
+    """A team's rows in several runs, each summed in 32 bits: at most `run` rows
+    one after the other, whose sum is off by run u of the terms' sizes, and six
+    roundings of each term; all else is in 64 bits."""
+    from tcc_amd import training
+
+    gen = torch.Generator(device="cuda").manual_seed(N)
+    draw = lambda: torch.empty((N, C), dtype=dtype, device="cuda").normal_(generator=gen)  # noqa: E731
+    x, d = draw(), draw()
+    w, b = torch.ones(C, device="cuda"), torch.zeros(C, device="cuda")
+    _, _, mean, rstd = training.layer_norm(x, w, b)
+    _, dw, db = training.layer_norm_grad(d, x, mean, rstd, w, b)
+    sums = torch.zeros((4, C), dtype=torch.float64, device="cuda")
+    step = 100_000_000 // C
+    for i in range(0, N, step):
+        at = slice(i, i + step)
+        xh = (x[at].double() - mean[at].double()[:, None]) * rstd[at].double()[:, None]
+        terms = d[at].double(), d[at].double() * xh
+        sums += torch.stack([t.sum(0) for v in terms for t in (v, v.abs())])
+    for got, want, size in ((db, sums[0], sums[1]), (dw, sums[2], sums[3])):
+        assert bool(((got.double() - want).abs() <= (run + 6) * 2.0**-24 * size).all())
+
+
 @pytest.mark.parametrize("weight,bias,ptype", [(False, False, torch.float32), (True, False, torch.float32),
                                                (False, True, torch.bfloat16), (True, True, torch.bfloat16),
                                                (True, True, torch.float16)])

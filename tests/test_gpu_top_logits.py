@@ -54,6 +54,25 @@ def test_random_rows(gpu, dtype, n, C, K):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,C,K", [(500, 100, 16), (200, 100, 64), (300, 300, 40), (300, 511, 64), (200, 513, 64), (120, 700, 64),
+                                   (90, 1500, 50), (700, 1025, 3), (40, 3000, 16), (1500, 4100, 8), (300, 8193, 64),
+                                   (30, 40_000, 40)])
+def test_more_of_every_path(gpu, dtype, n, C, K):
+    """Random rows; rows whose elements are nearly all masked; equal ones with
+    a few others."""
+    from tcc_amd import training
+
+    gen = torch.Generator().manual_seed(n + C)
+    z = torch.randn((n, C), generator=gen) * 3
+    z[n // 4:n // 2] = -np.inf
+    z[n // 4:n // 2, torch.randperm(C, generator=gen)[:5]] = torch.randn(5, generator=gen)
+    z[n // 2:3 * n // 4] = 1.0
+    z[n // 2:3 * n // 4, torch.randperm(C, generator=gen)[:9]] = torch.randn(9, generator=gen) + 1
+    z = z.to(dtype).cuda()
+    check(training.top_logits(z, K, temperature=2.0), z, K, 2.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("C", [5, 40, 300, 4000, 9000])
 @pytest.mark.parametrize("levels", [1, 2, 7])
 def test_ties_go_to_the_lowest_class(gpu, dtype, C, levels):
