@@ -153,8 +153,9 @@ int tcc_layer_norm_grad(const tcc_layer_norm_shape* s, const void* dY, uint64_t 
  * among equals, NaN above all; values of the logits' type.  rest [n], unless it
  * is NULL, is one logit that stands for the other classes at this temperature:
  * rest = T log(sum of exp(z_j / T) over them), -inf where there are none.
- * 1 <= K <= C, K <= 64 (TCC_ERR_UNSUPPORTED above), C below 2^31.  Row
- * addresses of the logits need only be aligned to their element. */
+ * 1 <= K <= C, K <= 64 (TCC_ERR_UNSUPPORTED above), C below 2^31, the
+ * temperature between 1e-18 and 1e18.  Row addresses of the logits need only be
+ * aligned to their element. */
 int tcc_top_logits(const void* logits, uint64_t ldz, uint32_t dtype, uint64_t n, uint32_t C, uint32_t K,
                    float temperature, void* values, uint64_t ldv, int32_t* ids, uint64_t ldi, float* rest, void* stream);
 
@@ -164,7 +165,8 @@ int tcc_top_logits(const void* logits, uint64_t ldz, uint32_t dtype, uint64_t n,
 
 /* A distillation of n rows of C logits of `dtype`, each against K entries of a
  * teacher: values of `valueDtype` and ids (classes), int32 or int64 by idBytes 4
- * or 8.  K <= 64, C below 2^31, n below 2^40 (TCC_ERR_UNSUPPORTED above). */
+ * or 8.  K <= 64, C below 2^31, n below 2^40 (TCC_ERR_UNSUPPORTED above), the
+ * temperature between 1e-18 and 1e18. */
 typedef struct tcc_distill_shape {
     uint64_t n;
     uint32_t C, K;

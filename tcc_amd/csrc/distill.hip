@@ -663,8 +663,8 @@ int check_shape(const tcc_distill_shape* s) {
                 "distillation: unknown element type");
     TCC_REQUIRE(s->idBytes == 4 || s->idBytes == 8, TCC_ERR_INVALID_ARGUMENT, "distillation: ids are int32 or int64");
     TCC_REQUIRE(s->reduction <= TCC_REDUCE_SUM, TCC_ERR_INVALID_ARGUMENT, "distillation: unknown reduction");
-    TCC_REQUIRE(s->temperature > 0.0f && s->temperature < 1e18f, TCC_ERR_INVALID_ARGUMENT,
-                "distillation: the temperature is positive");
+    TCC_REQUIRE(s->temperature >= 1e-18f && s->temperature <= 1e18f, TCC_ERR_INVALID_ARGUMENT,
+                "distillation: the temperature lies between 1e-18 and 1e18");
     TCC_REQUIRE(s->K <= kMaxEntries, TCC_ERR_UNSUPPORTED, "distillation: at most 64 entries a row");
     TCC_REQUIRE(s->C <= 0x7FFFFFFFu, TCC_ERR_UNSUPPORTED, "distillation: fewer than 2^31 classes");
     TCC_REQUIRE(s->n < (1ull << 40), TCC_ERR_UNSUPPORTED, "distillation: fewer than 2^40 rows");

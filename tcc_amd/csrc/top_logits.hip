@@ -782,8 +782,8 @@ extern "C" int tcc_top_logits(const void* logits, uint64_t ldz, uint32_t dtype, 
     clear_last_error();
     TCC_REQUIRE(dtype_bytes(dtype) != 0, TCC_ERR_INVALID_ARGUMENT, "top logits: unknown element type");
     TCC_REQUIRE(K >= 1 && K <= C, TCC_ERR_INVALID_ARGUMENT, "top logits: between one and all of a row's classes");
-    TCC_REQUIRE(temperature > 0.0f && temperature < 1e18f, TCC_ERR_INVALID_ARGUMENT,
-                "top logits: the temperature is positive");
+    TCC_REQUIRE(temperature >= 1e-18f && temperature <= 1e18f, TCC_ERR_INVALID_ARGUMENT,
+                "top logits: the temperature lies between 1e-18 and 1e18");
     TCC_REQUIRE(K <= kMostTop, TCC_ERR_UNSUPPORTED, "top logits: at most 64 a row");
     TCC_REQUIRE(C <= 0x7FFFFFFFu, TCC_ERR_UNSUPPORTED, "top logits: fewer than 2^31 classes");
     TCC_REQUIRE(n < (1ull << 40), TCC_ERR_UNSUPPORTED, "top logits: fewer than 2^40 rows");

@@ -411,8 +411,9 @@ std::tuple<Tensor, MaybeTensor, MaybeTensor> layer_norm_grad(const Tensor& dy, c
 
 // ---------------------------------------------------------------- distillation
 
-void temperature_is_positive(double t) {
-    if (!(t > 0 && t < 1e18)) value_error("the temperature is positive (got " + std::to_string(t) + ")");
+void check_temperature(double t) {  // as the kernels have it: its inverse and its square are finite
+    const float f = static_cast<float>(t);
+    if (!(f >= 1e-18f && f <= 1e18f)) value_error("the temperature lies between 1e-18 and 1e18 (got " + std::to_string(t) + ")");
 }
 
 std::tuple<Tensor, Tensor, Tensor> top_logits(const Tensor& logits, std::int64_t k, double temperature) {
@@ -422,7 +423,7 @@ std::tuple<Tensor, Tensor, Tensor> top_logits(const Tensor& logits, std::int64_t
     if (C > 0x7FFFFFFFll) value_error("rows of " + std::to_string(C) + " logits are too long");
     if (k < 1 || k > std::min<std::int64_t>(C, 64))
         value_error("k must be between 1 and the " + std::to_string(C) + " classes, and at most 64 (got " + std::to_string(k) + ")");
-    temperature_is_positive(temperature);
+    check_temperature(temperature);
     on_current_device(logits);
     const Tensor values = empty({n, k}, logits.options()), ids = empty({n, k}, logits.options().dtype(at::kInt));
     const Tensor rest = empty({n}, logits.options().dtype(at::kFloat));
@@ -451,7 +452,7 @@ struct Distill {
             value_error("values " + shape_of(v) + " and ids " + shape_of(i) + " must be 1 to 64 entries for each of the " +
                         std::to_string(n) + " rows");
         if (C > 0x7FFFFFFFll) value_error("rows of " + std::to_string(C) + " logits are too long");
-        temperature_is_positive(temperature);
+        check_temperature(temperature);
         values.emplace(v, "values");
         ids.emplace(i, "ids");
         for (const auto& [t, name, to] : {std::tuple{&r, "rest", &rest}, std::tuple{&w, "weight", &weight}}) {

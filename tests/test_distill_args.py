@@ -73,3 +73,12 @@ def test_distillation_refusals():
     for k in (dict(dl=None), dict(dz=None), dict(ldd=19), dict(w=P), dict(total=P)):
         assert grad(shape(), **k) == INVALID, k
     assert loss(shape(n=0, reduction=0), loss=None) == 0 and grad(shape(n=0)) == 0  # nothing to do
+
+
+def test_temperatures_without_a_finite_inverse_or_square_are_refused():
+    L = lib()
+    for t in (1e-19, 1e-40, 2e18):
+        assert L.tcc_top_logits(P, 20, 0, 10, 20, 4, t, P, 4, P, 4, P, None) == INVALID
+        s = shape(temperature=t)
+        assert L.tcc_distill_loss(ctypes.byref(s), P, 20, P, 4, P, 4, None, None, P, None, P, None, P, 1 << 20, None) == INVALID
+        assert L.tcc_distill_grad(ctypes.byref(s), P, P, 20, P, 4, P, 4, None, None, None, P, P, 20, None) == INVALID

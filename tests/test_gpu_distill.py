@@ -284,6 +284,15 @@ def test_large_logits_lose_nothing(gpu):
     check(z * 30, values * 30, ids, rest, 2.0, w)
 
 
+@pytest.mark.parametrize("T", [1e-18, 1e-4, 1e4, 1e15])
+@pytest.mark.parametrize("C", [9, 150, 700, 6000])
+def test_extreme_temperatures(gpu, C, T):
+    z, values, ids, rest, w = inputs(50, C, 4, torch.float32, C)
+    T = float(np.float32(T))
+    check(z, values, ids, rest, T, w)
+    check(z, values, ids, None, T, w, "none")
+
+
 def test_many_rows(gpu):
     z, values, ids, rest, w = inputs(100_003, 20, 3, torch.float32, 11)
     check(z, values, ids, rest, 2.0, w)

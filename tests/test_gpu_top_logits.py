@@ -142,6 +142,16 @@ def test_no_rows_and_many(gpu):
     check(training.top_logits(z, 3), z, 3, 1.0)
 
 
+@pytest.mark.parametrize("T", [1e-18, 1e-4, 1e4, 1e18])
+@pytest.mark.parametrize("C", [9, 150, 700, 6000])
+def test_extreme_temperatures(gpu, C, T):
+    from tcc_amd import training
+
+    z = torch.randn((50, C), generator=torch.Generator().manual_seed(C)).cuda()
+    T = float(np.float32(T))
+    check(training.top_logits(z, 4, temperature=T), z, 4, T)
+
+
 def test_places_past_32_bits(gpu):
     """4.5e9 logits: the last rows'."""
     from tcc_amd import training
