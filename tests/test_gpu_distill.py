@@ -340,6 +340,38 @@ def test_places_past_32_bits(gpu):
     assert bool(((dz[end].double().cpu() - grad).abs() <= gtol + 2.0**-8 * (grad.abs() + gtol) + 1e-30).all())
 
 
+def test_rows_of_two_billion_classes(gpu):
+    """The longest rows: classes of which none but 70 count, at both ends and on
+    the way, so that every sum is that of 70."""
+    from tcc_amd import training
+
+    C = 2**31 - 9
+    places = torch.cat([torch.arange(20), C // 2 + torch.arange(25), C - 25 + torch.arange(25)]).cuda()
+    near = torch.linspace(-4.0, 4.0, 70).roll(33).to(torch.bfloat16)[None].cuda()
+    z = torch.full((1, C), -200.0, dtype=torch.bfloat16, device="cuda")
+    z[:, places] = near
+    values, ids, rest = training.top_logits(z, 8)
+    want = torch.sort(near, dim=1, descending=True, stable=True)
+    assert torch.equal(values, want.values[:, :8]) and torch.equal(ids[0].long(), places[want.indices[0, :8]])
+    v, i, r = training.top_logits(near, 8)
+    assert float((rest - r).abs()) <= 400 * U * (1 + float(r.abs()))
+    error = torch.zeros(1, dtype=torch.int32, device="cuda")
+    one = torch.ones((), device="cuda")
+    for use in (None, rest):
+        results = []
+        for logits, at in ((z, ids), (near, i)):
+            teacher = 0.5 * values
+            loss, stats, _ = training.distill_loss(logits, teacher, at, rest=use, device_error=error)
+            results.append((loss, training.distill_grad(one, logits, teacher, at, stats, rest=use)))
+        (loss, dz), (loss_near, dz_near) = results
+        assert float((loss - loss_near).abs()) <= 400 * U * (1 + float(loss_near.abs()))
+        step = dz_near.float().abs() * 2 * U_OUT[torch.bfloat16] + 800 * U  # two roundings that may differ
+        assert bool(((dz[:, places].float() - dz_near.float()).abs() <= step).all())
+        dz[:, places] = 0
+        assert float(dz.amax()) < 1e-30 and float(dz.amin()) >= 0
+    assert int(error) == 0
+
+
 def test_replayed_graph_and_other_stream(gpu):
     from tcc_amd import training
 
