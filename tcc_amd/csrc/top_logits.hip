@@ -225,7 +225,9 @@ static_assert(kMostTop <= kWave);
 // their K/4-th); one wave raises that bound as it goes, four agree on one after the
 // first batch and on another at the end.  The classes that reach it, a few hundred
 // of 50,000, go to LDS; of these, those that reach the last bound each count the
-// larger ones among them, which is their place.
+// larger ones among them, which is their place.  4,096 rows of 50,000 bf16 logits
+// with K = 32 take 101 us, with the kernel after it (5 us) that finds no row left to
+// sort: 410 MB at 4.1 TB/s, three instructions an element beside them.
 template <typename T, int V, int WAVES>
 __global__ void __launch_bounds__(kThreads, 5) stream_kernel(Args a) {
     static_assert(WAVES == 1 || WAVES == kWaves);
@@ -442,7 +444,8 @@ __device__ __forceinline__ void write(const Top& top, const T* z, std::uint64_t 
     if (a.rest != nullptr && l == 0) a.rest[r] = as_logit(a, rest);
 }
 
-// The rows that stream_kernel marked, a wave each.
+// The rows that stream_kernel marked, a wave each: 4,096 x 50,000 bf16 rows whose
+// every element beats those before it take 1,800 us.
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads) wave_kernel(Args a) {
     __shared__ Buffer buffers[kWaves];
@@ -557,7 +560,6 @@ __device__ __forceinline__ std::uint32_t team_scan(std::uint32_t x) {
 // Keys of a team that have room in LDS, a multiple of 4.
 template <int TEAM>
 constexpr std::uint32_t kRoom = TEAM == 4 ? 32 : TEAM == 16 ? 128 : 256;
-
 // A bound that at least K elements reach and at most `most`, or the K-th largest,
 // from one that more reach: by halves of the range up to the team's largest.
 template <int TEAM, int N>
@@ -595,7 +597,9 @@ __device__ __forceinline__ Key team_top(Key k) {
 // that K elements reach, hardly more than K of them where these are few beside
 // the row, goes to LDS, and each of those counts the larger ones among them, which
 // is its place.  Rows with more of them than there is room for (equal ones, or
-// mostly -inf) have their K taken one after the other.
+// mostly -inf) have their K taken one after the other.  Vector instructions bound it
+// as much as memory: 2.45M x 100 fp32 rows take 425 us with K = 8 (1.15 GB: 250 at a
+// copy's rate, and 285 of vector instructions), 1,870 if all their elements are equal.
 template <typename T, int V, int E, int TEAM>
 __global__ void __launch_bounds__(kThreads) registers_kernel(Args a) {
     constexpr int teams = kThreads / TEAM, N = E * V;

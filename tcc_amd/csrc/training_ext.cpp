@@ -8,6 +8,8 @@
 // and values that no call takes; tcc_amd._lib.TccError: an error of the
 // library.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
@@ -316,6 +318,22 @@ std::tuple<Tensor, MaybeTensor, MaybeTensor> group_norm_grad(const Tensor& dy, c
                               static_cast<float*>(ptr(dw)), static_cast<float*>(ptr(db)), ws.data_ptr(), need,
                               stream_of(x)));
     return {dx, dw, db};
+}
+
+// ---------------------------------------------------------------- capture
+
+// Whether one of these is a leaf whose gradient a living graph accumulates on the
+// default stream: a captured backward pass would have to wait for that stream,
+// which a capture does not allow.
+bool held_by_default_stream(const std::vector<MaybeTensor>& tensors) {
+    for (const MaybeTensor& t : tensors) {
+        if (!t || !t->requires_grad() || !t->is_leaf()) continue;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        if (node == nullptr) continue;
+        const std::optional<c10::Stream> stream = node->stream();
+        if (stream && stream->id() == 0) return true;
+    }
+    return false;
 }
 
 // ---------------------------------------------------------------- layer norm
@@ -686,6 +704,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("embedding_grad", &embedding_grad);
     m.def("group_norm", &group_norm);
     m.def("group_norm_grad", &group_norm_grad);
+    m.def("held_by_default_stream", &held_by_default_stream);
     m.def("layer_norm", &layer_norm);
     m.def("layer_norm_grad", &layer_norm_grad);
     m.def("top_logits", &top_logits);

@@ -324,6 +324,17 @@ class GroupNormFunction(torch.autograd.Function):
         return dx, dw, db, None, None, None, None, None
 
 
+def _capturable(*leaves) -> None:
+    """Refuses what would end the process: a backward pass, captured into a graph,
+    of leaves that an eager graph made on the default stream still holds."""
+    if torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing():
+        from . import training
+
+        if training.held_by_default_stream(leaves):
+            raise RuntimeError("an output of an earlier eager pass over these parameters is alive, whose gradients belong "
+                               "to the default stream: drop it before the capture, or make it on a side stream")
+
+
 class LayerNormFunction(torch.autograd.Function):
     """act(layer_norm(x)), or (act(layer_norm(h)), h) of h = x + residual
     (tcc_amd.training.layer_norm / layer_norm_grad)."""
@@ -433,6 +444,7 @@ class NodeLayerNorm(torch.nn.Module):
         self.bias = torch.nn.Parameter(torch.zeros(channels, device=device))
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None):
+        _capturable(x, residual, self.weight, self.bias)
         return LayerNormFunction.apply(x, residual, self.weight, self.bias, self.eps, self.activation)
 
 
@@ -486,6 +498,7 @@ class DistillationLoss(torch.nn.Module):
         values, ids, rest = entries
         if any(t is not None and t.requires_grad for t in (values, rest, self.weight)):
             raise ValueError("the teacher's entries and the weights are constants: detach them")
+        _capturable(pred)
         return DistillationFunction.apply(pred, values, ids, rest, self.weight, self.temperature, self.reduction,
                                           self.device_error)
 

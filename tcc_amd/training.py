@@ -106,6 +106,12 @@ def group_norm_grad(d_y: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd
                  _activation(activation), max_rows)
 
 
+def held_by_default_stream(tensors) -> bool:
+    """Whether one of these (None is none) is a leaf whose gradient a living
+    autograd graph accumulates on the default stream."""
+    return _ext.held_by_default_stream(list(tensors))
+
+
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
                residual: torch.Tensor | None = None, eps: float = 1e-5, activation: str = "none",
                stream=None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:

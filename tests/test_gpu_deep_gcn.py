@@ -219,6 +219,36 @@ def test_captured_step(gpu):
             assert torch.equal(p, q)
 
 
+def test_capture_beside_a_living_eager_graph_is_refused(gpu):
+    """Its gradients belong to the default stream, which a capture may not wait
+    for; refused before anything of the backward pass runs."""
+    from tcc_amd import gcn, training
+
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    x = torch.randn((300, 40), generator=gen, device="cuda")
+    teacher = training.top_logits(x * 2, 3)
+    norm, loss_fcn = gcn.NodeLayerNorm(40, "silu"), gcn.DistillationLoss()
+    logits = x.clone().requires_grad_()
+    alive = norm(x), loss_fcn(logits, teacher)
+    assert training.held_by_default_stream([None, norm.weight]) and training.held_by_default_stream([logits])
+    assert not training.held_by_default_stream([None, x])
+    for call in (lambda: norm(x), lambda: loss_fcn(logits, teacher)):
+        with pytest.raises(RuntimeError, match="is alive"), torch.cuda.graph(torch.cuda.CUDAGraph()):
+            x + 1
+            call()
+    with torch.no_grad(), torch.cuda.graph(torch.cuda.CUDAGraph()):
+        norm(x)  # nothing to differentiate
+    del alive
+    assert not training.held_by_default_stream([norm.weight, norm.bias, logits])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = torch.autograd.grad(norm(x), list(norm.parameters()), torch.ones_like(x))
+    graph.replay()
+    torch.cuda.synchronize()
+    for p, q in zip(out, torch.autograd.grad(norm(x), list(norm.parameters()), torch.ones_like(x))):
+        assert torch.equal(p, q)
+
+
 def test_two_streams_at_once(gpu):
     """Calls on two streams share no workspace."""
     from tcc_amd import training
