@@ -593,6 +593,14 @@ __device__ __forceinline__ Key team_top(Key k) {
     else return k;
 }
 
+// Whether a row of N elements a lane goes to LDS too, where what reaches the bound is
+// read again: 7M x 32 fp32 rows take 457 us with it and 618 without (K = 8), 2.45M x
+// 100 bf16 ones 328 and 363.  Larger rows leave too few workgroups room (2.45M x 100
+// fp32 rows 433, and 423 without), and so do fp32 ones of 16 lanes, whose registers
+// suffice for five (800,000 x 200: 230, and 203 without).
+template <typename T, int N, int TEAM>
+constexpr bool kNear = N * sizeof(T) <= 64 && (TEAM != 16 || sizeof(T) == 2);
+
 // A team holds a row in registers, E vectors of V a lane.  What reaches a value
 // that K elements reach, hardly more than K of them where these are few beside
 // the row, goes to LDS, and each of those counts the larger ones among them, which
@@ -601,11 +609,18 @@ __device__ __forceinline__ Key team_top(Key k) {
 // as much as memory: 2.45M x 100 fp32 rows take 425 us with K = 8 (1.15 GB: 250 at a
 // copy's rate, and 285 of vector instructions), 1,870 if all their elements are equal.
 template <typename T, int V, int E, int TEAM>
-__global__ void __launch_bounds__(kThreads) registers_kernel(Args a) {
+__global__ void __launch_bounds__(kThreads, TEAM > 4 && E * V == 16 ? 5 : 1) registers_kernel(Args a) {
     constexpr int teams = kThreads / TEAM, N = E * V;
     constexpr std::uint32_t room = kRoom<TEAM>;
     __shared__ __attribute__((aligned(16))) Key found[teams][room];
+    // the row by the lanes' vectors; 64 bytes more put other teams' into other banks
+    constexpr bool near = kNear<T, N, TEAM>;
+    __shared__ __attribute__((aligned(16))) T rows[near ? teams : 1][near ? TEAM * N + 64 / sizeof(T) : 1];
     Key* mine = found[threadIdx.x / TEAM];
+    T* row = rows[near ? threadIdx.x / TEAM : 0];
+    const std::uint32_t body = a.C / V * V;
+    const auto class_at = [&](std::uint32_t slot) { return slot < body ? slot : slot - body + a.C - V; };
+    const auto slot_of = [&](std::uint32_t c) { return c < body ? c : c + body + V - a.C; };
     const std::uint32_t lane = threadIdx.x % TEAM;
     const auto place = [&](int e) { return Place<V>(lane + e * TEAM, a.C); };
     // whether some lanes of the team have a vector e, and whether all have a whole one
@@ -634,6 +649,10 @@ __global__ void __launch_bounds__(kThreads) registers_kernel(Args a) {
     load(r);
     for (; r < a.n; r += step) {
         const T* z = static_cast<const T*>(a.z) + r * a.ldz;
+        const auto element = [&](std::uint32_t c) {
+            if constexpr (near) return row[slot_of(c)];
+            else return z[c];
+        };
         T* values = static_cast<T*>(a.values) + r * a.ldv;
         std::int32_t* ids = a.ids + r * a.ldi;
         float v[N];
@@ -645,6 +664,7 @@ __global__ void __launch_bounds__(kThreads) registers_kernel(Args a) {
             const std::uint32_t skip = whole(e) ? 0 : place(e).skip;
 #pragma unroll
             for (std::uint32_t q = 0; q < V; ++q) v[e * V + q] = q >= skip ? static_cast<float>(ahead[e][q]) : kNone;
+            if constexpr (near) *reinterpret_cast<vec_t<T, V>*>(row + (lane + e * TEAM) * V) = ahead[e];
         }
         load(r + step);
         float bound = reached<TEAM>(v, a.K);
@@ -660,40 +680,41 @@ __global__ void __launch_bounds__(kThreads) registers_kernel(Args a) {
             if (again || all <= min(room, enough(a.K))) break;
             bound = halved<TEAM>(v, bound, a.K, min(room, enough(a.K)));
         }
-        const auto index = [&](std::uint32_t i) { return Place<V>(lane + i / V * TEAM, a.C).at + i % V; };
+        const auto slot = [&](std::uint32_t i) { return (lane + i / V * TEAM) * V + i % V; };
         Share rest;
         if (all <= room) {
-            // their classes first: a register chosen at run time costs two instructions
-            // for each that there is, and the row's lines are near
-            using Class = std::uint32_t __attribute__((may_alias));
-            auto* classes = reinterpret_cast<Class*>(mine);
-            for (to -= own; reach != 0; reach &= reach - 1) classes[2 * to++] = index(N - 1 - __builtin_ctz(reach));
+            // their places first, then their keys: a register chosen at run time costs
+            // two instructions for each that there is, and the row's lines are near
+            using Slot = std::uint32_t __attribute__((may_alias));
+            auto* slots = reinterpret_cast<Slot*>(mine);
+            for (to -= own; reach != 0; reach &= reach - 1) slots[2 * to++] = slot(N - 1 - __builtin_ctz(reach));
             wave_sync();
 #pragma unroll 4
             for (std::uint32_t i = lane; i < all; i += TEAM) {
-                const std::uint32_t c = classes[2 * i];
-                mine[i] = key_of(static_cast<float>(z[c]), c);
+                const std::uint32_t s = slots[2 * i];
+                mine[i] = key_of(static_cast<float>(near ? row[s] : z[class_at(s)]), class_at(s));
             }
             if (lane < 3 && all + lane < room) mine[all + lane] = 0;  // for the reads of four
             wave_sync();
-        } else {  // from memory again: the keys of all elements need more registers than all else
+        } else {  // read again: the keys of all elements need more registers than all else
+            wave_sync();
             Key last = ~Key(0);
             for (std::uint32_t k = 0; k < a.K; ++k) {
                 Key best = 0;
 #pragma unroll 4
                 for (std::uint32_t c = lane; c < a.C; c += TEAM) {
-                    const Key key = key_of(static_cast<float>(z[c]), c);
+                    const Key key = key_of(static_cast<float>(element(c)), c);
                     best = key < last ? larger_key(best, key) : best;
                 }
                 last = team_top<TEAM>(best);
                 if (lane == 0) {
-                    values[k] = z[index_of(last)];
+                    values[k] = element(index_of(last));
                     ids[k] = static_cast<std::int32_t>(index_of(last));
                 }
             }
 #pragma unroll 1
             for (std::uint32_t c = lane; c < a.C; c += TEAM) {
-                const float x = static_cast<float>(z[c]);
+                const float x = static_cast<float>(element(c));
                 if (key_of(x, c) < last) rest = rest.with({x, 1.0f}, a.c);
             }
         }
@@ -716,14 +737,14 @@ __global__ void __launch_bounds__(kThreads) registers_kernel(Args a) {
                 }
                 if (at < a.K) {
                     const std::uint32_t c = index_of(k);
-                    values[at] = z[c];
+                    values[at] = element(c);
                     ids[at] = static_cast<std::int32_t>(c);
                 } else {
                     rest = rest.with({value_of(static_cast<std::uint32_t>(k >> 32)), 1.0f}, a.c);
                 }
             }
-            wave_sync();
         }
+        wave_sync();
         if (a.rest == nullptr) continue;
         const float top = wave_join<TEAM>(rest.m, Larger());
         rest.scale_to(top, a.c);
