@@ -585,10 +585,34 @@ __device__ __forceinline__ float halved(const float (&v)[N], float bound, std::u
     return value_of(lo);
 }
 
-__device__ __forceinline__ Key larger_key(Key a, Key b) { return a > b ? a : b; }
+// The keys of rows in registers: of 16-bit logits, whose values need the upper 19 bits
+// of their order (fp16's 1 + 8 + 10 as fp32), 32 bits with a class of 10: 7M x 32 bf16
+// rows take 866 us instead of 1,207 (K = 16).
+template <typename T, bool SHORT = sizeof(T) == 2>
+struct RowKey {
+    using type = Key;
+    static __device__ __forceinline__ type of(float v, std::uint32_t c) { return key_of(v, c); }
+    static __device__ __forceinline__ std::uint32_t index(type k) { return index_of(k); }
+    static __device__ __forceinline__ float value(type k) { return value_of(static_cast<std::uint32_t>(k >> 32)); }
+};
+template <typename T>
+struct RowKey<T, true> {
+    using type = std::uint32_t;
+    static __device__ __forceinline__ type of(float v, std::uint32_t c) { return order_of(v) >> 13 << 10 | (1023 - c); }
+    static __device__ __forceinline__ std::uint32_t index(type k) { return 1023 - (k & 1023); }
+    static __device__ __forceinline__ float value(type k) {
+        const std::uint32_t order = k >> 10 << 13;  // its lower bits are 0, or 1 of negative values
+        return value_of(order & 0x80000000u ? order : order | 0x1FFFu);
+    }
+};
+
+template <typename K>
+__device__ __forceinline__ K larger_key(K a, K b) {
+    return a > b ? a : b;
+}
 // The largest key of a team.
-template <int TEAM, int D = 1>
-__device__ __forceinline__ Key team_top(Key k) {
+template <int TEAM, int D = 1, typename K>
+__device__ __forceinline__ K team_top(K k) {
     if constexpr (D < TEAM) return team_top<TEAM, 2 * D>(larger_key(k, other<D>(k)));
     else return k;
 }
@@ -607,11 +631,13 @@ constexpr bool kNear = N * sizeof(T) <= 64 && (TEAM != 16 || sizeof(T) == 2);
 // is its place.  Rows with more of them than there is room for (equal ones, or
 // mostly -inf) have their K taken one after the other.  Vector instructions bound it
 // as much as memory: 2.45M x 100 fp32 rows take 425 us with K = 8 (1.15 GB: 250 at a
-// copy's rate, and 285 of vector instructions), 1,870 if all their elements are equal.
+// copy's rate, and 285 of vector instructions), 1,840 if all their elements are equal.
 template <typename T, int V, int E, int TEAM>
 __global__ void __launch_bounds__(kThreads, TEAM > 4 && E * V == 16 ? 5 : 1) registers_kernel(Args a) {
     constexpr int teams = kThreads / TEAM, N = E * V;
     constexpr std::uint32_t room = kRoom<TEAM>;
+    using Keys = RowKey<T>;
+    using Key = typename Keys::type;
     __shared__ __attribute__((aligned(16))) Key found[teams][room];
     // the row by the lanes' vectors; 64 bytes more put other teams' into other banks
     constexpr bool near = kNear<T, N, TEAM>;
@@ -687,12 +713,13 @@ __global__ void __launch_bounds__(kThreads, TEAM > 4 && E * V == 16 ? 5 : 1) reg
             // two instructions for each that there is, and the row's lines are near
             using Slot = std::uint32_t __attribute__((may_alias));
             auto* slots = reinterpret_cast<Slot*>(mine);
-            for (to -= own; reach != 0; reach &= reach - 1) slots[2 * to++] = slot(N - 1 - __builtin_ctz(reach));
+            constexpr std::uint32_t apart = sizeof(Key) / sizeof(Slot);
+            for (to -= own; reach != 0; reach &= reach - 1) slots[apart * to++] = slot(N - 1 - __builtin_ctz(reach));
             wave_sync();
 #pragma unroll 4
             for (std::uint32_t i = lane; i < all; i += TEAM) {
-                const std::uint32_t s = slots[2 * i];
-                mine[i] = key_of(static_cast<float>(near ? row[s] : z[class_at(s)]), class_at(s));
+                const std::uint32_t s = slots[apart * i];
+                mine[i] = Keys::of(static_cast<float>(near ? row[s] : z[class_at(s)]), class_at(s));
             }
             if (lane < 3 && all + lane < room) mine[all + lane] = 0;  // for the reads of four
             wave_sync();
@@ -703,19 +730,19 @@ __global__ void __launch_bounds__(kThreads, TEAM > 4 && E * V == 16 ? 5 : 1) reg
                 Key best = 0;
 #pragma unroll 4
                 for (std::uint32_t c = lane; c < a.C; c += TEAM) {
-                    const Key key = key_of(static_cast<float>(element(c)), c);
+                    const Key key = Keys::of(static_cast<float>(element(c)), c);
                     best = key < last ? larger_key(best, key) : best;
                 }
                 last = team_top<TEAM>(best);
                 if (lane == 0) {
-                    values[k] = element(index_of(last));
-                    ids[k] = static_cast<std::int32_t>(index_of(last));
+                    values[k] = element(Keys::index(last));
+                    ids[k] = static_cast<std::int32_t>(Keys::index(last));
                 }
             }
 #pragma unroll 1
             for (std::uint32_t c = lane; c < a.C; c += TEAM) {
                 const float x = static_cast<float>(element(c));
-                if (key_of(x, c) < last) rest = rest.with({x, 1.0f}, a.c);
+                if (Keys::of(x, c) < last) rest = rest.with({x, 1.0f}, a.c);
             }
         }
         const float below = all <= room ? bound : kNone;
@@ -736,11 +763,11 @@ __global__ void __launch_bounds__(kThreads, TEAM > 4 && E * V == 16 ? 5 : 1) reg
                     for (int q = 0; q < 4; ++q) at += mine[o + q] > k ? 1u : 0u;
                 }
                 if (at < a.K) {
-                    const std::uint32_t c = index_of(k);
+                    const std::uint32_t c = Keys::index(k);
                     values[at] = element(c);
                     ids[at] = static_cast<std::int32_t>(c);
                 } else {
-                    rest = rest.with({value_of(static_cast<std::uint32_t>(k >> 32)), 1.0f}, a.c);
+                    rest = rest.with({Keys::value(k), 1.0f}, a.c);
                 }
             }
         }
