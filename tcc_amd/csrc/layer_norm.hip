@@ -401,7 +401,7 @@ struct Forward {
 };
 
 // The gradient's workgroups are as many as run at once, with equal shares of the
-// rows: 1,838 us for 2.45M x 256 fp32 rows (10.0 GB), 40 less than with three or
+// rows: 1,829 us for 2.45M x 256 fp32 rows (10.0 GB), 40 less than with three or
 // four times as many.  A team sums a run of its rows in 32 bits, a workgroup its
 // teams' in 64, and the parameters' kernel the runs': with one run of 200 rows
 // dWeight's error was twice that of four of 50, at 35 us less.
