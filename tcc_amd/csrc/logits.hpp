@@ -37,6 +37,27 @@ struct Share {
     }
 };
 
+// The same of a row of any length, held in 64 bits under a reference that the
+// maximum passes by a factor of 2 at most: batches that are summed in 32 bits are
+// added without a rounding of that size each, and a maximum that rises with every
+// one does not scale (and round) the sum every time.
+struct LongShare {
+    float m = kNone, ref = kNone;
+    double s = 0.0;
+    // Takes in logits up to `top`; what is subtracted from them.
+    __device__ __forceinline__ float raise(float top, float c) {
+        m = fmaxf(m, top);
+        if ((m - ref) * c > 1.0f) {
+            s *= exp2_of((ref - base_of(m)) * c);
+            ref = m;
+        }
+        return base_of(ref);
+    }
+    __device__ __forceinline__ Share share(float c) const {
+        return {m, static_cast<float>(s * exp2_of((ref - base_of(m)) * c))};
+    }
+};
+
 // A vector of V of a row's elements; the last one is moved back to end with the
 // row.
 template <int V>
