@@ -53,6 +53,10 @@ struct LongShare {
         }
         return base_of(ref);
     }
+    __device__ __forceinline__ void add(float z, float c) {
+        const float b = raise(z, c);
+        s += exp2_of((z - b) * c);
+    }
     __device__ __forceinline__ Share share(float c) const {
         return {m, static_cast<float>(s * exp2_of((ref - base_of(m)) * c))};
     }

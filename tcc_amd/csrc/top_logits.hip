@@ -8,12 +8,13 @@
 // that K elements reach; those that reach it, hardly more than K of a short row and
 // a few hundred of a long one, go to LDS as 64-bit keys (the value's order, then the
 // index's), and each counts the larger ones, which is its place.  What does not
-// reach the bound, and what K others beat, is summed for the rest: nothing is
-// subtracted from a sum of all.  Rows of up to 1,024 classes are held in registers
-// by 4, 16 or 64 lanes; longer ones are streamed, by a wave up to 4,096 classes, by
-// a workgroup above.  Rows with more at the bound than there is room for (sorted
-// upwards, or many equal) go another way: the short ones take their K one after the
-// other, the long ones by a second kernel that keeps sorted lists.
+// reach the bound, and what K others beat, is summed for the rest, a long row's
+// batches in 64 bits: nothing is subtracted from a sum of all.  Rows of up to 1,024
+// classes are held in registers by 4, 16 or 64 lanes; longer ones are streamed, by a
+// wave up to 4,096 classes, by a workgroup above.  Rows with more at the bound than
+// there is room for (sorted upwards, or many equal) go another way: the short ones
+// take their K one after the other, the long ones by a second kernel that keeps
+// sorted lists.
 #include <algorithm>
 
 #include "../../include/tcc_swtcf.h"
@@ -187,16 +188,16 @@ struct Elements {
         for (int u = 0; u < kBatch; ++u) own = __builtin_elementwise_maximum(own, most[u]);
         return own;
     }
-    __device__ __forceinline__ void add_to(Share& rest, float c) const {
-        float m = kNone;
+    __device__ __forceinline__ void add_to(LongShare& rest, float c) const {
+        float m = kNone, s = 0.0f;
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) m = fmaxf(m, most[u]);
-        if (m > rest.m) rest.scale_to(m, c);
-        const float b = base_of(rest.m);
+        const float b = rest.raise(m, c);
 #pragma unroll
         for (int u = 0; u < kBatch; ++u)
 #pragma unroll
-            for (int q = 0; q < V; ++q) rest.s += exp2_of((x[u][q] - b) * c);
+            for (int q = 0; q < V; ++q) s += exp2_of((x[u][q] - b) * c);
+        rest.s += s;
     }
 };
 
@@ -229,7 +230,7 @@ static_assert(kMostTop <= kWave);
 // with K = 32 take 101 us, with the kernel after it (5 us) that finds no row left to
 // sort: 410 MB at 4.1 TB/s, three instructions an element beside them.
 template <typename T, int V, int WAVES>
-__global__ void __launch_bounds__(kThreads, 5) stream_kernel(Args a) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 6 : 5) stream_kernel(Args a) {
     static_assert(WAVES == 1 || WAVES == kWaves);
     constexpr std::uint32_t teams = kWaves / WAVES, step = WAVES * kWave;
     __shared__ std::uint32_t classes[kWaves][kFound], counts[kWaves], kept[kWaves];
@@ -247,7 +248,7 @@ __global__ void __launch_bounds__(kThreads, 5) stream_kernel(Args a) {
     for (std::uint64_t r = static_cast<std::uint64_t>(blockIdx.x) * teams + (WAVES == 1 ? w : 0); r < a.n; r += rows) {
         const T* z = static_cast<const T*>(a.z) + r * a.ldz;
         const std::uint32_t K = (a.K + WAVES - 1) / WAVES;
-        Share rest;
+        LongShare rest;
         std::uint32_t count = 0, batch = 0;
         float bound = 0.0f, own = kNone;
         Ahead<T, V> ahead;
@@ -299,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, 5) stream_kernel(Args a) {
             const bool keeps = i < count && !(x < bound);
             const std::uint64_t those = __ballot(keeps);
             if (keeps) keys[w][all + __popcll(those & lanemask_lt())] = key_of(x, c);
-            else if (i < count) rest = rest.with({x, 1.0f}, a.c);
+            else if (i < count) rest.add(x, a.c);
             all += __popcll(those);
         }
         if (lane_id() < 3) keys[w][all + lane_id()] = 0;  // for the reads of four
@@ -326,19 +327,19 @@ __global__ void __launch_bounds__(kThreads, 5) stream_kernel(Args a) {
                 static_cast<T*>(a.values)[r * a.ldv + at] = z[c];
                 a.ids[r * a.ldi + at] = static_cast<std::int32_t>(c);
             } else {
-                rest = rest.with({value_of(static_cast<std::uint32_t>(k >> 32)), 1.0f}, a.c);
+                rest.add(value_of(static_cast<std::uint32_t>(k >> 32)), a.c);
             }
         }
-        rest = wave_join_share(rest, a.c);
+        Share sum = wave_join_share(rest.share(a.c), a.c);
         if constexpr (WAVES > 1) {
-            if (lane_id() == 0) rests[w] = make_float2(rest.m, rest.s);
+            if (lane_id() == 0) rests[w] = make_float2(sum.m, sum.s);
             __syncthreads();
             if (w == 0)
-                for (int o = 1; o < WAVES; ++o) rest = rest.with({rests[o].x, rests[o].y}, a.c);
+                for (int o = 1; o < WAVES; ++o) sum = sum.with({rests[o].x, rests[o].y}, a.c);
         } else {
             wave_sync();
         }
-        if (a.rest != nullptr && lane_id() == 0 && (WAVES == 1 || w == 0)) a.rest[r] = as_logit(a, rest);
+        if (a.rest != nullptr && lane_id() == 0 && (WAVES == 1 || w == 0)) a.rest[r] = as_logit(a, sum);
     }
 }
 
@@ -354,13 +355,13 @@ struct Top {
     Buffer& buffer;
     Key list = 0;             // sorted down over the lanes, 0 from K on
     std::uint32_t count = 0;  // waiting in the buffer, fewer than 64 between calls
-    Share rest;
+    LongShare rest;
     float bound;  // what is not larger goes to the rest; NaN: nothing does
 
     __device__ __forceinline__ Top(const Args& args, Buffer& b) : a(args), buffer(b), bound(__builtin_nanf("")) {}
 
     __device__ __forceinline__ void drop(Key k) {
-        if (k != 0) rest = rest.with({value_of(static_cast<std::uint32_t>(k >> 32)), 1.0f}, a.c);
+        if (k != 0) rest.add(value_of(static_cast<std::uint32_t>(k >> 32)), a.c);
     }
     // Takes in a list that is sorted up.
     __device__ __forceinline__ void take(Key up) {
@@ -456,7 +457,7 @@ __global__ void __launch_bounds__(kThreads) wave_kernel(Args a) {
         const T* z = static_cast<const T*>(a.z) + r * a.ldz;
         Top top(a, buffers[w]);
         scan<T, V>(top, z, 0, kWave);
-        write<T>(top, z, r, wave_join_share(top.rest, a.c));
+        write<T>(top, z, r, wave_join_share(top.rest.share(a.c), a.c));
     }
 }
 
@@ -474,13 +475,13 @@ __global__ void __launch_bounds__(kThreads) block_kernel(Args a) {
         scan<T, V>(top, z, w * kWave, kThreads);
         if (w != 0) {
             lists[w][kWave - 1 - lane_id()] = top.list;
-            const Share rest = wave_join_share(top.rest, a.c);
+            const Share rest = wave_join_share(top.rest.share(a.c), a.c);
             if (lane_id() == 0) rests[w] = make_float2(rest.m, rest.s);
         }
         __syncthreads();
         if (w == 0) {
             for (int o = 1; o < kWaves; ++o) top.take(lists[o][lane_id()]);
-            Share rest = wave_join_share(top.rest, a.c);
+            Share rest = wave_join_share(top.rest.share(a.c), a.c);
             for (int o = 1; o < kWaves; ++o) rest = rest.with({rests[o].x, rests[o].y}, a.c);
             write<T>(top, z, r, rest);
         }

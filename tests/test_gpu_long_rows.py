@@ -1,5 +1,5 @@
 """Rows of very many classes: the softmax sums of tcc_amd.training.distill_loss
-keep their digits however long a row is.
+and the rest of top_logits keep their digits however long a row is.
 
 Bounds, with u = 2^-24 and x = (z - m) / T, none of which grows with the row: an
 exponent has four roundings of |x| (the factor log2(e) / T, the difference, the
@@ -101,3 +101,68 @@ def test_loss_of_sorted_logits(gpu, ends):
     rounded again each time."""
     row = torch.linspace(*ends, 1 << 27, device="cuda")
     check_loss(row, [0, 1 << 26, (1 << 27) - 1], 1.0)
+
+
+def check_rest(z, K, T, others):
+    """The rest of row 0 against the (value, count) of all classes that are not
+    taken; the rows are equal."""
+    from tcc_amd import training
+
+    values, ids, rest = training.top_logits(z, K, temperature=T)
+    m = max(v for v, _ in others)
+    s = sum(n * math.exp((v - m) / T) for v, n in others)
+    mean = sum(n * (m - v) / T * math.exp((v - m) / T) for v, n in others) / s
+    want = m + T * math.log(s)
+    assert bool((rest == rest[0]).all())
+    # log2 and its product with T log 2 round to two ulps each of what they give
+    assert abs(float(rest[0]) - want) <= T * (64 + 4 * mean) * U + 4 * U * (abs(m) + T * math.log(s))
+    return values, ids
+
+
+@BY_DTYPE
+def test_rest_of_a_streamed_row(gpu, dtype):
+    """A workgroup's row: each of its waves has one class at the bound."""
+    C, V = 1 << 28, 16 // dtype.itemsize
+    z = torch.full((1, C), -1.25, dtype=dtype, device="cuda")
+    high = [w * 64 * V for w in range(4)]
+    z[0, 1:256 * V:V] = 0.0  # the largest of each lane's rest
+    z[0, high] = 0.5
+    values, ids = check_rest(z, 1, 1.0, [(0.5, 3), (0.0, 256), (-1.25, C - 260)])
+    assert ids.tolist() == [[0]] and values.tolist() == [[0.5]]
+    values, ids = check_rest(z, 4, 2.0, [(0.0, 256), (-1.25, C - 260)])
+    assert ids.tolist() == [high]
+
+
+@BY_DTYPE
+def test_rest_of_rows_streamed_by_waves(gpu, dtype):
+    """A wave a row, where there are many: each of its lanes has a class at the bound."""
+    n = 12 * torch.cuda.get_device_properties(0).multi_processor_count
+    C, V = 1 << 20, 16 // dtype.itemsize
+    z = torch.full((n, C), -1.25, dtype=dtype, device="cuda")
+    z[:, 1:64 * V:V] = 0.0
+    z[:, :64 * V:V] = 0.5
+    values, ids = check_rest(z, 17, 1.0, [(0.5, 64 - 17), (0.0, 64), (-1.25, C - 128)])
+    assert bool((values == 0.5).all()) and bool((ids == torch.arange(0, 17 * V, V, device="cuda")).all())
+
+
+@BY_DTYPE
+def test_rest_of_a_row_of_equal_logits(gpu, dtype):
+    """More classes at the bound than there is room for."""
+    C = 1 << 26
+    z = torch.full((1, C), -1.25, dtype=dtype, device="cuda")
+    z[0, C // 2] = 3.0
+    _, ids = check_rest(z, 3, 1.0, [(-1.25, C - 3)])
+    assert ids.tolist() == [[C // 2, 0, 1]]
+
+
+@pytest.mark.parametrize("ends", [(-9.0, 9.0), (-0.5, 0.25)])
+def test_rest_of_a_sorted_row(gpu, ends):
+    """Every class beats those before it."""
+    from tcc_amd import training
+
+    row = torch.linspace(*ends, 1 << 24, device="cuda")
+    values, ids, rest = training.top_logits(row[None], 5)
+    order = torch.sort(row[-2000:], descending=True, stable=True)
+    assert torch.equal(ids[0].long(), order.indices[:5] + row.numel() - 2000)
+    m, s, mean = share(row, 1.0, ids[0].tolist())
+    assert abs(float(rest) - m - math.log(s)) <= (64 + 4 * mean) * U + 4 * U * (abs(m) + math.log(s))
