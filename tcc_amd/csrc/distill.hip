@@ -39,6 +39,9 @@ constexpr std::uint32_t kMaxEntries = 64;
 constexpr int kThreads = 256;
 constexpr int kBatch = 4;  // vectors that a lane loads before it uses the first
 
+using Share = ShareOf<false>;  // a row with an infinity has no softmax
+using LongShare = LongShareOf<false>;
+
 struct Args {
     const void *z, *values, *ids;
     const float *rest, *weight;

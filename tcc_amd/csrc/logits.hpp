@@ -20,19 +20,24 @@ struct Log2 {
         : whole(static_cast<float>(__builtin_amdgcn_frexp_expf(x))), part(log2_of(__builtin_amdgcn_frexp_mantf(x))) {}
     __device__ __forceinline__ float over(const Log2& o) const { return (whole - o.whole) + (part - o.part); }
 };
-// A maximum as it is subtracted: 0 for that of nothing.
-__device__ __forceinline__ float base_of(float m) { return m == kNone ? 0.0f : m; }
+// A maximum as it is subtracted: 0 for that of nothing.  OPEN: and for +inf, so that
+// a sum with an infinity is infinite, and NaN only with a NaN.
+template <bool OPEN = false>
+__device__ __forceinline__ float base_of(float m) {
+    return (OPEN ? fabsf(m) == -kNone : m == kNone) ? 0.0f : m;
+}
 
 // The maximum m of some logits and s = sum of 2^((z - m) c).
-struct Share {
+template <bool OPEN>
+struct ShareOf {
     float m = kNone, s = 0.0f;
     __device__ __forceinline__ void scale_to(float top, float c) {
-        s *= exp2_of((m - base_of(top)) * c);
+        s *= exp2_of((m - base_of<OPEN>(top)) * c);
         m = top;
     }
-    __device__ __forceinline__ Share with(Share o, float c) const {
+    __device__ __forceinline__ ShareOf with(ShareOf o, float c) const {
         const float top = fmaxf(m, o.m);
-        const float b = base_of(top);
+        const float b = base_of<OPEN>(top);
         return {top, s * exp2_of((m - b) * c) + o.s * exp2_of((o.m - b) * c)};
     }
 };
@@ -41,24 +46,25 @@ struct Share {
 // maximum passes by a factor of 2 at most: batches that are summed in 32 bits are
 // added without a rounding of that size each, and a maximum that rises with every
 // one does not scale (and round) the sum every time.
-struct LongShare {
+template <bool OPEN>
+struct LongShareOf {
     float m = kNone, ref = kNone;
     double s = 0.0;
     // Takes in logits up to `top`; what is subtracted from them.
     __device__ __forceinline__ float raise(float top, float c) {
         m = fmaxf(m, top);
         if ((m - ref) * c > 1.0f) {
-            s *= exp2_of((ref - base_of(m)) * c);
+            s *= exp2_of((ref - base_of<OPEN>(m)) * c);
             ref = m;
         }
-        return base_of(ref);
+        return base_of<OPEN>(ref);
     }
     __device__ __forceinline__ void add(float z, float c) {
         const float b = raise(z, c);
         s += exp2_of((z - b) * c);
     }
-    __device__ __forceinline__ Share share(float c) const {
-        return {m, static_cast<float>(s * exp2_of((ref - base_of(m)) * c))};
+    __device__ __forceinline__ ShareOf<OPEN> share(float c) const {
+        return {m, static_cast<float>(s * exp2_of((ref - base_of<OPEN>(m)) * c))};
     }
 };
 

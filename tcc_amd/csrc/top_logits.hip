@@ -31,6 +31,9 @@ constexpr int kWaves = kThreads / kWave;
 constexpr int kBatch = 4;  // vectors that a lane loads before it uses the first
 constexpr std::uint32_t kWaveClasses = 4096;
 
+using Share = ShareOf<true>;  // a rest with an infinity is infinite
+using LongShare = LongShareOf<true>;
+
 struct Args {
     const void* z;
     void* values;
@@ -212,7 +215,7 @@ __device__ __forceinline__ std::uint32_t kth_lane(float v, std::uint32_t K) {
     return static_cast<std::uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(wave_sort<true>(order_of(v))), K - 1));
 }
 __device__ __forceinline__ float as_logit(const Args& a, Share rest) {
-    return rest.m == -kNone ? rest.m : base_of(rest.m) + a.T * kLn2 * log2_of(rest.s);
+    return base_of<true>(rest.m) + a.T * kLn2 * log2_of(rest.s);
 }
 
 // ---------------------------------------------------------------- streamed rows
@@ -752,7 +755,7 @@ __global__ void __launch_bounds__(kThreads, TEAM > 4 && E * V == 16 ? 5 : 1) reg
             v[i] = v[i] < below ? v[i] : kNone;
             rest.m = fmaxf(rest.m, v[i]);
         }
-        const float b = base_of(rest.m);
+        const float b = base_of<true>(rest.m);
 #pragma unroll
         for (int i = 0; i < N; ++i) rest.s += exp2_of((v[i] - b) * a.c);
         if (all <= room) {
