@@ -4,11 +4,11 @@
     python -m tcc_amd.train_embeddings --norm layer --blocks 2 --distill 4
 
 Every graph is a random subset of the nodes of one table with R-MAT edges
-among them, and its nodes' labels follow hidden classes of the table (two, or
---classes), so that only the embeddings can tell them apart.  Prints the loss and
-the gradient norm of every step.  With --norm layer the model has layer norms and
---blocks residual ones; with --distill K a model of one quarter of its widths then
-learns from its K largest logits of every node.
+among them, and its nodes' labels follow hidden classes of the table (two, 3 K with
+--distill K, or --classes), so that only the embeddings can tell them apart.  Prints
+the loss and the gradient norm of every step.  With --norm layer the model has layer
+norms and --blocks residual ones; with --distill K a model of one quarter of its
+widths then learns from its K largest logits of every node.
 """
 from __future__ import annotations
 
@@ -37,12 +37,31 @@ def batch_of_graphs(num_nodes: int, graphs: int, mean_rows: int, seed: int):
     return torch.cat(rows), torch.cat(cols), ids, first.to(torch.int32), int(sizes.max())
 
 
+def checked(norm: str, blocks: int, classes: int | None, distill: int, temperature: float) -> int:
+    """How many classes there are; ValueError for what the model or the student
+    would refuse when their turn comes."""
+    if blocks < 0 or (blocks > 0 and norm != "layer"):
+        raise ValueError("residual blocks go with layer norms")
+    if distill < 0:
+        raise ValueError(f"a student learns from one logit of a node or more (got {distill})")
+    if classes is None:
+        classes = max(2, 3 * distill)
+    if classes < 1:
+        raise ValueError(f"there is one class at least (got {classes})")
+    if distill > min(classes, 64):
+        raise ValueError(f"the {distill} largest of {classes} logits: at most as many as there are classes, and 64")
+    if distill and not 1e-18 <= temperature <= 1e18:
+        raise ValueError(f"the temperature lies between 1e-18 and 1e18 (got {temperature})")
+    return classes
+
+
 def train(nodes: int = 50_000, graphs: int = 200, mean_rows: int = 60, dim: int = 64, hidden: int = 128, steps: int = 20,
           lr: float = 1e-2, max_norm: float = 1.0, seed: int = 0, log=print, norm: str = "group", blocks: int = 0,
-          classes: int = 2, distill: int = 0, temperature: float = 2.0):
+          classes: int | None = None, distill: int = 0, temperature: float = 2.0):
     """The losses and gradient norms of `steps` steps, and the model; with
     `distill`, those of the student that learns from its `distill` largest logits,
     and the student."""
+    classes = checked(norm, blocks, classes, distill, temperature)
     torch.manual_seed(seed)
     rows, cols, ids, offsets, max_rows = batch_of_graphs(nodes, graphs, mean_rows, seed)
     n = ids.numel()
@@ -83,10 +102,14 @@ def main(argv=None) -> int:
     p.add_argument("--max-norm", type=float, default=1.0)
     p.add_argument("--norm", choices=("group", "layer"), default="group")
     p.add_argument("--blocks", type=int, default=0, help="residual blocks (with --norm layer)")
-    p.add_argument("--classes", type=int, default=2)
+    p.add_argument("--classes", type=int, help="2 by default, 3 K with --distill K")
     p.add_argument("--distill", type=int, default=0, metavar="K", help="train a student from the K largest logits")
     p.add_argument("--temperature", type=float, default=2.0)
     a = p.parse_args(argv)
+    try:
+        checked(a.norm, a.blocks, a.classes, a.distill, a.temperature)
+    except ValueError as e:
+        p.error(str(e))
     train(a.nodes, a.graphs, a.mean_rows, a.dim, a.hidden, a.steps, a.lr, a.max_norm,
           log=lambda s: print(s, flush=True), norm=a.norm, blocks=a.blocks, classes=a.classes, distill=a.distill,
           temperature=a.temperature)
