@@ -16,9 +16,11 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <memory>
 #include <numeric>
 #include <optional>
 #include <string>
+#include <unordered_set>
 #include <utility>
 #include <vector>
 
@@ -322,16 +324,25 @@ std::tuple<Tensor, MaybeTensor, MaybeTensor> group_norm_grad(const Tensor& dy, c
 
 // ---------------------------------------------------------------- capture
 
-// Whether one of these is a leaf whose gradient a living graph accumulates on the
-// default stream: a captured backward pass would have to wait for that stream,
-// which a capture does not allow.
+// Whether a gradient of one of these would run through a node of a living graph
+// that was made on the default stream, or be accumulated in a leaf that such a graph
+// holds, however far behind the tensor: a captured backward pass would have to wait
+// for that stream, which a capture does not allow.
 bool held_by_default_stream(const std::vector<MaybeTensor>& tensors) {
-    for (const MaybeTensor& t : tensors) {
-        if (!t || !t->requires_grad() || !t->is_leaf()) continue;
-        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-        if (node == nullptr) continue;
+    using torch::autograd::Node;
+    std::vector<std::shared_ptr<Node>> next;
+    std::unordered_set<const Node*> seen;
+    const auto take = [&](std::shared_ptr<Node> node) {
+        if (node != nullptr && seen.insert(node.get()).second) next.push_back(std::move(node));
+    };
+    for (const MaybeTensor& t : tensors)
+        if (t && t->requires_grad()) take(t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t) : t->grad_fn());
+    while (!next.empty()) {
+        const std::shared_ptr<Node> node = std::move(next.back());
+        next.pop_back();
         const std::optional<c10::Stream> stream = node->stream();
         if (stream && stream->id() == 0) return true;
+        for (const torch::autograd::Edge& e : node->next_edges()) take(e.function);
     }
     return false;
 }

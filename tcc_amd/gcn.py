@@ -324,15 +324,16 @@ class GroupNormFunction(torch.autograd.Function):
         return dx, dw, db, None, None, None, None, None
 
 
-def _capturable(*leaves) -> None:
+def _capturable(*inputs) -> None:
     """Refuses what would end the process: a backward pass, captured into a graph,
-    of leaves that an eager graph made on the default stream still holds."""
+    through nodes or to leaves that an eager graph made on the default stream still
+    holds, behind these inputs."""
     if torch.is_grad_enabled() and torch.cuda.is_current_stream_capturing():
         from . import training
 
-        if training.held_by_default_stream(leaves):
+        if training.held_by_default_stream(inputs):
             raise RuntimeError("an output of an earlier eager pass over these parameters is alive, whose gradients belong "
-                               "to the default stream: drop it before the capture, or make it on a side stream")
+                               "to the default stream: drop it before the capture, detach it, or make it on a side stream")
 
 
 class LayerNormFunction(torch.autograd.Function):

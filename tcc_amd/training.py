@@ -107,8 +107,9 @@ def group_norm_grad(d_y: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd
 
 
 def held_by_default_stream(tensors) -> bool:
-    """Whether one of these (None is none) is a leaf whose gradient a living
-    autograd graph accumulates on the default stream."""
+    """Whether a gradient of one of these (None is none) would run through a node
+    that an eager pass made on the default stream, or to a leaf whose gradient a
+    living graph accumulates there, however far behind the tensor."""
     return _ext.held_by_default_stream(list(tensors))
 
 
