@@ -6,7 +6,7 @@
 //
 // A row is read once from memory.  From what the lanes have at first comes a bound
 // that K elements reach; those that reach it, hardly more than K of a short row and
-// a few hundred of a long one, go to LDS as 64-bit keys (the value's order, then the
+// a few hundred of a long one in random order, go to LDS as 64-bit keys (the value's order, then the
 // index's), and each counts the larger ones, which is its place.  What does not
 // reach the bound, and what K others beat, is summed for the rest, a long row's
 // batches in 64 bits: nothing is subtracted from a sum of all.  Rows of up to 1,024
@@ -226,12 +226,14 @@ static_assert(kMostTop <= kWave);
 
 // A row is read once by a wave, or by the four of a workgroup.  K elements at least
 // reach the K-th largest of the lanes' maxima so far (of four waves: the least of
-// their K/4-th); one wave raises that bound as it goes, four agree on one after the
-// first batch and on another at the end.  The classes that reach it, a few hundred
-// of 50,000, go to LDS; of these, those that reach the last bound each count the
-// larger ones among them, which is their place.  4,096 rows of 50,000 bf16 logits
-// with K = 32 take 101 us, with the kernel after it (5 us) that finds no row left to
-// sort: 410 MB at 4.1 TB/s, three instructions an element beside them.
+// their K/4-th); one wave raises that bound as it goes, four agree on one anew after
+// half as many batches again as there were, and at the end.  The classes that reach
+// it go to LDS: of rows in random order with K = 64 about 110 of 50,000 for a wave,
+// 200 of a million, 370 of 2^27 (where one takes the row, with K = 32, 190, 340 and,
+// of 2^24, 460).  Those that reach the last bound each count the larger ones among
+// them, which is their place.  4,096 rows of 50,000 bf16 logits with K = 32 take 101
+// us, with the kernel after it (5 us) that finds no row left to sort: 410 MB at 4.1
+// TB/s, three instructions an element beside them.
 template <typename T, int V, int WAVES>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 6 : 5) stream_kernel(Args a) {
     static_assert(WAVES == 1 || WAVES == kWaves);
@@ -241,19 +243,24 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 6 : 5) stream_kerne
     __shared__ float bounds[2][kWaves];
     __shared__ float2 rests[kWaves];
     const std::uint32_t w = uniform(threadIdx.x / kWave), first = WAVES == 1 ? 0 : w * kWave;
-    // the least of the waves' bounds; the whole workgroup
-    const auto agreed = [&](int turn, float bound) {
+    // the least of the waves' bounds; the whole workgroup, and the places alternate,
+    // so that one barrier a call is enough
+    std::uint32_t turn = 0;
+    const auto agreed = [&](float bound) {
         if (lane_id() == 0) bounds[turn][w] = bound;
         __syncthreads();
-        return wave_join<WAVES>(bounds[turn][lane_id() % WAVES], Smaller());
+        const float mine = bounds[turn][lane_id() % WAVES];
+        turn ^= 1;
+        return wave_join<WAVES>(mine, Smaller());
     };
     const std::uint64_t rows = static_cast<std::uint64_t>(gridDim.x) * teams;
     for (std::uint64_t r = static_cast<std::uint64_t>(blockIdx.x) * teams + (WAVES == 1 ? w : 0); r < a.n; r += rows) {
         const T* z = static_cast<const T*>(a.z) + r * a.ldz;
         const std::uint32_t K = (a.K + WAVES - 1) / WAVES;
         LongShare rest;
-        std::uint32_t count = 0, batch = 0;
-        float bound = 0.0f, own = kNone;
+        std::uint32_t count = 0;
+        float bound = kNone, own = kNone;
+        std::uint32_t batch = 0, next = 0;  // the batch before which they agree again
         Ahead<T, V> ahead;
         Range<V> range{first, step, a.C};
         ahead.load(z, range);
@@ -262,7 +269,11 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 6 : 5) stream_kerne
             ahead.load(z, {range.first + step * kBatch, step, a.C});
             own = e.largest(own);
             if constexpr (WAVES > 1) {
-                if (batch == 0) bound = agreed(0, value_of(kth_lane(own, K)));
+                // (every wave has this batch, or none agrees)
+                if (batch == next && (range.first - first + step - kWave) * V < a.C) {
+                    bound = fmaxf(bound, agreed(value_of(kth_lane(own, K))));
+                    next = batch + 2 + batch / 2;
+                }
             } else {
                 if (K > 32) {  // the lanes' maxima are few for it: 2.5 times as many would reach the least of 64
                     if (batch == 0) bound = e.halved(value_of(kth_lane(own, K)), K);
@@ -287,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 6 : 5) stream_kerne
         bool fits = count <= kFound;
         if constexpr (WAVES > 1) {
             if (lane_id() == 0) counts[w] = count;
-            bound = agreed(1, bound);
+            bound = agreed(bound);
 #pragma unroll
             for (int o = 0; o < WAVES; ++o) fits &= counts[o] <= kFound;
         }
