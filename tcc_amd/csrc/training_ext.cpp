@@ -413,7 +413,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> layer_norm(const Tensor& x, const May
 std::tuple<Tensor, MaybeTensor, MaybeTensor> layer_norm_grad(const Tensor& dy, const Tensor& h, const Tensor& mean,
                                                              const Tensor& rstd, const MaybeTensor& weight,
                                                              const MaybeTensor& bias, const MaybeTensor& dSum,
-                                                             std::uint32_t activation) {
+                                                             std::uint32_t activation, bool parameters) {
     const LayerNorm k(h, weight, bias, 0.0, activation);
     const Rows rows = rows_like(dy, h, "d_y");
     std::optional<Rows> add;
@@ -427,9 +427,9 @@ std::tuple<Tensor, MaybeTensor, MaybeTensor> layer_norm_grad(const Tensor& dy, c
     const Tensor dx = empty(h.sizes(), h.options());
     const auto f32 = h.options().dtype(at::kFloat);
     MaybeTensor dw, db, ws;
-    if (weight) dw = empty({h.size(-1)}, f32);
-    if (bias) db = empty({h.size(-1)}, f32);
-    const std::size_t need = weight || bias ? tcc_layer_norm_grad_workspace_bytes(&k.s) : 0;
+    if (weight && parameters) dw = empty({h.size(-1)}, f32);
+    if (bias && parameters) db = empty({h.size(-1)}, f32);
+    const std::size_t need = dw || db ? tcc_layer_norm_grad_workspace_bytes(&k.s) : 0;
     if (need > 0) ws = workspace(need, h);
     check(tcc_layer_norm_grad(&k.s, rows.t.data_ptr(), rows.ld, k.rows.t.data_ptr(), k.rows.ld, mean.data_ptr<float>(),
                               rstd.data_ptr<float>(), ptr(k.weight), ptr(k.bias), add ? add->t.data_ptr() : nullptr,

@@ -358,7 +358,8 @@ class LayerNormFunction(torch.autograd.Function):
         if d_y is None:  # only the sum was used
             return d_sum, d_sum, None, None, None, None
         h, weight, bias, mean, rstd = ctx.saved_tensors
-        dx, dw, db = training.layer_norm_grad(d_y, h, mean, rstd, weight, bias, d_sum=d_sum, activation=ctx.activation)
+        dx, dw, db = training.layer_norm_grad(d_y, h, mean, rstd, weight, bias, d_sum=d_sum, activation=ctx.activation,
+                                              parameters=any(ctx.needs_input_grad[2:4]))
         dw = None if dw is None else dw.to(weight.dtype)
         db = None if db is None else db.to(bias.dtype)
         return dx, dx if ctx.summed else None, dw, db, None, None

@@ -125,14 +125,14 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
 
 def layer_norm_grad(d_y: torch.Tensor, h: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
                     weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
-                    d_sum: torch.Tensor | None = None, activation: str = "none",
-                    stream=None) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
+                    d_sum: torch.Tensor | None = None, activation: str = "none", stream=None,
+                    parameters: bool = True) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
     """(dx, dweight, dbias) of layer_norm (tcc_layer_norm_grad), from d_y of
     h's shape and type, the forward's h, mean and rstd, and `d_sum`, the
     gradient that h has from its other uses: dx of h's type is the gradient of
     x and of residual alike, dweight and dbias [C] are fp32 (None where there
-    is no weight or bias)."""
-    return _call(stream, _ext.layer_norm_grad, d_y, h, mean, rstd, weight, bias, d_sum, _activation(activation))
+    is no weight or bias, and without `parameters`, which spares their sums)."""
+    return _call(stream, _ext.layer_norm_grad, d_y, h, mean, rstd, weight, bias, d_sum, _activation(activation), parameters)
 
 
 def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0,
