@@ -552,6 +552,7 @@ __global__ void __launch_bounds__(kThreads) grad_kernel(Args a) {
                 }
                 store_any<T, V>(dz + at.at, d);
             }
+            team_sync<TEAM>();  // the next row's logits go there
         } else {
             for (std::uint32_t base = 0; base < a.C; base += B::stride) {
                 const std::uint32_t first = base & ~(kWindow<TEAM> - 1);
