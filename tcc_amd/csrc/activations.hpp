@@ -8,8 +8,8 @@
 namespace tcc {
 
 // Channels c .. c + N of a weight or bias: one branch and one load for all of
-// them (a branch for each put every load behind the one before).  c is a
-// multiple of N, but the caller's array need only be aligned to its elements.
+// them (a branch for each put every load behind the one before).  The caller's
+// array need only be aligned to its elements, and c is any channel.
 template <int N>
 __device__ __forceinline__ vec_t<float, N> load_params(const void* p, std::uint32_t type, std::uint32_t c, float none) {
     vec_t<float, N> v(none);

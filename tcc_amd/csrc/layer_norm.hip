@@ -348,10 +348,12 @@ __global__ void __launch_bounds__(kParamCols* kParamRows) params_kernel(const fl
 // ---------------------------------------------------------------- launches
 
 // The smallest team that holds rows of C elements; f is called with its <V, E,
-// TEAM>.  Sixteen elements a lane at most.  Where vectors of 16 bytes would leave
-// a third of a wave's lanes without elements, 16-bit rows take 8 bytes a lane:
-// the gradient of 169,000 x 301 bf16 rows with gelu, half of whose time is vector
-// instructions, takes 92 us instead of 104.
+// TEAM>.  Sixteen elements a lane at most.  Rows of 257 to 384 and of 513 to 768
+// 16-bit elements, of which vectors of 16 bytes would leave up to half of a team's
+// lanes without any, take 8 bytes a lane: the gradient of 169,000 x 301 bf16 rows with
+// gelu, half of whose time is vector instructions, takes 92 us instead of 104.
+// (Others whose last vectors are few keep 16 bytes: 6.25M x 16 rows take 146 us,
+// 66,666 x 1,500 ones 115, where a copy takes 98 and 87.)
 template <typename T, typename F>
 void with_team(std::uint32_t C, F f) {
     constexpr int V = kVec<T>;

@@ -24,12 +24,6 @@ __device__ __forceinline__ void store_row(T* p, vec_t<float, N> v) {
     *reinterpret_cast<vec_t<T, N>*>(p) = __builtin_convertvector(v, vec_t<T, N>);
 }
 
-// The same at any address of an element: CDNA4 reads and writes 16 bytes a lane
-// at any of them, and a copy of 2 GiB runs as fast (4.6 TB/s at odd 16-bit
-// elements as at aligned ones; with 2 bytes a lane 2.7).
-template <typename T, int N>
-using any_vec_t = T __attribute__((ext_vector_type(N), aligned(sizeof(T))));
-
 // Bytes that the last level of cache holds: larger outputs are written past
 // its order (ONCE).  A constant, as the compiler makes one plain store of two
 // that a value at run time chooses between.
@@ -41,7 +35,7 @@ __device__ __forceinline__ void write_out(T* p, vec_t<float, N> v) {
     else store_row<T, N>(p, v);
 }
 
-// The same at any address of an element: CDNA4 reads and writes 16 bytes a lane
+// N elements at any address of an element: CDNA4 reads and writes 16 bytes a lane
 // at any of them, and a copy of 2 GiB runs as fast (4.6 TB/s at odd 16-bit
 // elements as at aligned ones; with 2 bytes a lane 2.7).
 template <typename T, int N>

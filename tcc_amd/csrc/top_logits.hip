@@ -6,15 +6,15 @@
 //
 // A row is read once from memory.  From what the lanes have at first comes a bound
 // that K elements reach; those that reach it, hardly more than K of a short row and
-// a few hundred of a long one in random order, go to LDS as 64-bit keys (the value's order, then the
-// index's), and each counts the larger ones, which is its place.  What does not
-// reach the bound, and what K others beat, is summed for the rest, a long row's
-// batches in 64 bits: nothing is subtracted from a sum of all.  Rows of up to 1,024
-// classes are held in registers by 4, 16 or 64 lanes; longer ones are streamed, by a
-// wave up to 4,096 classes, by a workgroup above.  Rows with more at the bound than
-// there is room for (sorted upwards, or many equal) go another way: the short ones
-// take their K one after the other, the long ones by a second kernel that keeps
-// sorted lists.
+// a few hundred of a long one in random order, go to LDS as 64-bit keys (the value's
+// order, then the index's), and each counts the larger ones, which is its place.
+// What does not reach the bound, and what K others beat, is summed for the rest, a
+// long row's batches in 64 bits: nothing is subtracted from a sum of all.  Rows of up
+// to 1,024 classes are held in registers by 4, 16 or 64 lanes; longer ones are
+// streamed, by a wave up to 4,096 classes and where there are many, by a workgroup
+// else.  Rows with more at the bound than there is room for (that rise, or with many
+// equal) go another way: the short ones take their K one after the other, the long
+// ones are read again by a second kernel that keeps sorted lists.
 #include <algorithm>
 
 #include "../../include/tcc_swtcf.h"
