@@ -185,7 +185,9 @@ size_t tcc_distill_loss_workspace_bytes(const tcc_distill_shape* s);
  * of -1 is no entry, and so is any other that is no class: that sets
  * TCC_DEVERR_FEATURE_INDEX in *deviceError, if it is not NULL.  A class may
  * occur in several entries.  A row whose weight is 0 is not read, and it and a
- * row without an entry or rest above -inf have no loss.
+ * row without an entry or rest above -inf have no loss.  The logarithms are
+ * differences of fp32 numbers, whose roundings T^2 multiplies: the mean over
+ * 20,000 rows of 300 classes is off by 2e-8 at T = 2, 2e-6 at 10, 2e-4 at 100.
  *
  * *loss is the sum of the rows' losses (TCC_REDUCE_SUM) or that divided by the
  * sum of the weights (TCC_REDUCE_MEAN; by n without weights; 0 where that is 0),

@@ -337,7 +337,7 @@ struct Front {
 };
 
 // Bound by the reading of the logits: 4,096 rows of 50,000 bf16 logits with 32
-// entries and a rest take 88 us with the kernel that joins the sums (410 MB: 4.7 TB/s).
+// entries and a rest take 89 us with the kernel that joins the sums (410 MB: 4.6 TB/s).
 template <typename T, int V, int TEAM, int E, bool WHOLE, bool REST>
 __global__ void __launch_bounds__(kThreads, WHOLE ? 1 : 4) loss_kernel(Args a) {
     using F = vec_t<float, V>;

@@ -140,7 +140,7 @@ template <typename T, int V, int E, int TEAM>
 constexpr bool kAhead = E * V * sizeof(T) <= 32 && TEAM <= 256;
 
 // Bound by memory: x and residual in, y and h out, once.  2.45M x 256 fp32 rows with
-// a residual take 1,825 us (10.05 GB: 5.5 TB/s, where a copy of 4 GiB has 4.6),
+// a residual take 1,822 us (10.05 GB: 5.5 TB/s, where a copy of 4 GiB has 4.6),
 // 16,384 x 4,096 bf16 rows with one 101 (537 MB: 5.3 TB/s).
 template <typename T, int V, int E, int TEAM, bool ONCE>
 __global__ void __launch_bounds__(kThreads<TEAM>) forward_kernel(Args a) {
@@ -212,9 +212,9 @@ __global__ void __launch_bounds__(kThreads<TEAM>) forward_kernel(Args a) {
 }
 
 // Bound by memory, and by vector instructions where 16-bit rows have an activation:
-// 2.45M x 256 fp32 rows with d_sum and relu take 1,829 us (10.04 GB: 5.5 TB/s),
-// 169,000 x 301 bf16 rows with gelu 93 (305 MB: 3.3 TB/s, the vector units busy for
-// three quarters of it), both with the parameters' kernel.
+// 2.45M x 256 fp32 rows with d_sum and relu take 1,822 us (10.04 GB: 5.5 TB/s),
+// 169,000 x 301 bf16 rows with gelu 94 (305 MB: 3.2 TB/s, the vector units active in
+// 0.9 of the units' busy cycles), both with the parameters' kernel.
 template <typename T, int V, int E, int TEAM, bool ONCE>
 __global__ void __launch_bounds__(kThreads<TEAM>) grad_kernel(Args a) {
     using F = vec_t<float, V>;
@@ -352,8 +352,8 @@ __global__ void __launch_bounds__(kParamCols* kParamRows) params_kernel(const fl
 // 16-bit elements, of which vectors of 16 bytes would leave up to half of a team's
 // lanes without any, take 8 bytes a lane: the gradient of 169,000 x 301 bf16 rows with
 // gelu, half of whose time is vector instructions, takes 92 us instead of 104.
-// (Others whose last vectors are few keep 16 bytes: 6.25M x 16 rows take 146 us,
-// 66,666 x 1,500 ones 115, where a copy takes 98 and 87.)
+// (Others whose last vectors are few keep 16 bytes: 6.25M x 16 rows take 116 us,
+// 66,666 x 1,500 ones 113, where a copy takes 98 and 87.)
 template <typename T, typename F>
 void with_team(std::uint32_t C, F f) {
     constexpr int V = kVec<T>;
@@ -403,7 +403,7 @@ struct Forward {
 };
 
 // The gradient's workgroups are as many as run at once, with equal shares of the
-// rows: 1,829 us for 2.45M x 256 fp32 rows (10.0 GB), 40 less than with three or
+// rows: 1,822 us for 2.45M x 256 fp32 rows (10.0 GB), 40 less than with three or
 // four times as many.  A team sums a run of its rows in 32 bits, a workgroup its
 // teams' in 64, and the parameters' kernel the runs': with one run of 200 rows
 // dWeight's error was twice that of four of 50, at 35 us less.

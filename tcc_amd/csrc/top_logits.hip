@@ -231,8 +231,8 @@ static_assert(kMostTop <= kWave);
 // it go to LDS: of rows in random order with K = 64 about 110 of 50,000 for a wave,
 // 200 of a million, 370 of 2^27 (where one takes the row, with K = 32, 190, 340 and,
 // of 2^24, 460).  Those that reach the last bound each count the larger ones among
-// them, which is their place.  4,096 rows of 50,000 bf16 logits with K = 32 take 101
-// us, with the kernel after it (5 us) that finds no row left to sort: 410 MB at 4.1
+// them, which is their place.  4,096 rows of 50,000 bf16 logits with K = 32 take 102
+// us, with the kernel after it (5 us) that finds no row left to sort: 410 MB at 4.0
 // TB/s, three instructions an element beside them.
 template <typename T, int V, int WAVES>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 6 : 5) stream_kernel(Args a) {
@@ -645,8 +645,9 @@ constexpr bool kNear = N * sizeof(T) <= 64 && (TEAM != 16 || sizeof(T) == 2);
 // the row, goes to LDS, and each of those counts the larger ones among them, which
 // is its place.  Rows with more of them than there is room for (equal ones, or
 // mostly -inf) have their K taken one after the other.  Vector instructions bound it
-// as much as memory: 2.45M x 100 fp32 rows take 425 us with K = 8 (1.15 GB: 250 at a
-// copy's rate, and 285 of vector instructions), 1,840 if all their elements are equal.
+// as much as memory: 2.45M x 100 fp32 rows take 420 us with K = 8 (1.15 GB: 250 at a
+// copy's rate, and 176M vector instructions, 286 at 2.4 GHz), 1,850 if all their
+// elements are equal.
 template <typename T, int V, int E, int TEAM>
 __global__ void __launch_bounds__(kThreads, TEAM > 4 && E * V == 16 ? 5 : 1) registers_kernel(Args a) {
     constexpr int teams = kThreads / TEAM, N = E * V;
