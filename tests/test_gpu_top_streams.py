@@ -85,6 +85,18 @@ def test_a_workgroup_a_row(gpu, dtype, kind, n, C, K):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("batches", [2, 5])
+@pytest.mark.parametrize("waves", [1, 2, 3, 4])
+def test_ends_where_some_waves_have_no_batch(gpu, dtype, batches, waves):
+    """Rows that end inside the batch before which four waves agree anew."""
+    V = 16 // dtype.itemsize
+    C = batches * 4 * 256 * V + (waves - 1) * 64 * V + 3
+    gen = torch.Generator(device="cuda").manual_seed(C)
+    for K in (3, 64):
+        check(rows_of("random", 5, C, dtype, gen), K, 1.0, range(5))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_the_largest_in_one_waves_part(gpu, dtype):
     """A bound from one wave alone would leave out what the others' lack."""
     V = 16 // dtype.itemsize
