@@ -21,8 +21,10 @@
 // far from zero have lost.
 //
 // The gradient's teams walk the rows in equal steps and keep the sums of dz and
-// dz xh of their channels in registers, in up to four runs; a workgroup adds its
-// teams' in LDS in 64 bits and writes a row a run, and a second kernel adds those.
+// dz xh of their channels in registers, of a dozen rows at a time; a workgroup adds
+// them in LDS in 64 bits, where rows of up to 8,192 channels have room for that (longer
+// ones: up to four runs of rows, each written), and a second kernel adds what the
+// workgroups wrote.
 #include <algorithm>
 
 #include "../../include/tcc_swtcf.h"
@@ -35,6 +37,7 @@ namespace tcc {
 namespace {
 
 constexpr std::uint32_t kMaxChannels = 16384;
+constexpr int kTotalChannels = 8192;  // whose parameters' sums have room in LDS, 128 KB
 
 struct Args {
     const void *x, *residual, *dy, *dSum, *weight, *bias;
@@ -135,7 +138,7 @@ struct Raw {
     __device__ __forceinline__ vec_t<float, V> operator[](int e) const { return __builtin_convertvector(v[e], vec_t<float, V>); }
 };
 // Whether there are registers for the next row's elements beside this one's: the
-// gradient of 169,000 x 301 bf16 rows takes 92 us with and 145 without.
+// gradient of 169,000 x 301 bf16 rows took 92 us with and 145 without.
 template <typename T, int V, int E, int TEAM>
 constexpr bool kAhead = E * V * sizeof(T) <= 32 && TEAM <= 256;
 
@@ -211,15 +214,109 @@ __global__ void __launch_bounds__(kThreads<TEAM>) forward_kernel(Args a) {
     }
 }
 
+// The parameters' sums of a workgroup, in 64 bits: those of a wave's teams are added
+// over its lanes, and each wave (or larger team) has a place of its own where these
+// take 32 KB at most, else two waves have one.  A place has a pair, dBias and dWeight,
+// for each element of the lanes' vectors (not for each channel).
+template <int V, int E, int TEAM>
+struct Totals {
+    static constexpr bool used = TEAM * E * V <= kTotalChannels;
+    static constexpr int group = TEAM < kWave ? kWave : TEAM, groups = kThreads<TEAM> / group;
+    static constexpr int sums = used ? 2 * TEAM * E * V : 1;
+    static constexpr int places = groups == 1 || groups * sums * sizeof(double) <= 32768 ? groups : groups / 2;
+    struct Shared {
+        double sum[places][sums] __attribute__((aligned(16)));
+    };
+    Shared& s;
+    __device__ __forceinline__ explicit Totals(Shared& shared) : s(shared) {}
+
+    // a and b of the lanes at distance D (16 or 32) and this one added: of a where bit D
+    // of the lane is 0, of b where it is 1.
+    template <int D>
+    static __device__ __forceinline__ double halves(double a, double b) {
+        const auto x = static_cast<std::uint64_t>(__double_as_longlong(a)), y = static_cast<std::uint64_t>(__double_as_longlong(b));
+        std::uint32_t first[2], second[2];
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            const auto xs = static_cast<std::uint32_t>(x >> (32 * w)), ys = static_cast<std::uint32_t>(y >> (32 * w));
+            if constexpr (D == 16) {
+                const auto r = __builtin_amdgcn_permlane16_swap(xs, ys, false, false);
+                first[w] = r[0], second[w] = r[1];
+            } else {
+                const auto r = __builtin_amdgcn_permlane32_swap(xs, ys, false, false);
+                first[w] = r[0], second[w] = r[1];
+            }
+        }
+        const auto whole = [](const std::uint32_t (&w)[2]) {
+            return __longlong_as_double(static_cast<long long>(static_cast<std::uint64_t>(w[1]) << 32 | w[0]));
+        };
+        return whole(first) + whole(second);
+    }
+    template <int D>
+    static __device__ __forceinline__ double with_other(double v) {
+        return v + __longlong_as_double(static_cast<long long>(other<D>(static_cast<std::uint64_t>(__double_as_longlong(v)))));
+    }
+
+    // Takes in a lane's sums; the whole workgroup.
+    __device__ __forceinline__ void add(bool first, const vec_t<float, V> (&db)[E], const vec_t<float, V> (&dw)[E]) {
+        const int mine = threadIdx.x / group;
+        const std::uint32_t lane = __lane_id();
+        double* to = s.sum[mine % places] + threadIdx.x % TEAM * V * 2;
+#pragma unroll 1
+        for (int phase = 0; phase < groups / places; ++phase) {
+            const auto put = [&](auto* p, auto v) { *p = first && phase == 0 ? v : v + *p; };
+            if (mine / places == phase) {
+                // pairs of elements, two at a time for their registers
+#pragma unroll
+                for (int i = 0; i < E * V; i += 2) {
+                    constexpr int apart = V == 1 ? TEAM : 1;  // of the second element from the first
+                    const int e0 = i / V, e1 = (i + 1) / V;
+                    double* at = to + (e0 * TEAM * V + i % V) * 2;
+                    const double b0 = db[e0][i % V], w0 = dw[e0][i % V], b1 = db[e1][(i + 1) % V], w1 = dw[e1][(i + 1) % V];
+                    if constexpr (TEAM >= kWave) {
+                        static_assert(V > 1);
+                        put(reinterpret_cast<vec_t<double, 2>*>(at), vec_t<double, 2>{b0, w0});
+                        put(reinterpret_cast<vec_t<double, 2>*>(at + 2), vec_t<double, 2>{b1, w1});
+                    } else if constexpr (TEAM == 32) {
+                        put(at + lane / 32, halves<32>(b0, w0));
+                        put(at + lane / 32 + 2 * apart, halves<32>(b1, w1));
+                    } else {  // each row of 16 lanes has one of the four
+                        double v = halves<16>(halves<32>(b0, w0), halves<32>(b1, w1));
+                        if constexpr (TEAM <= 4) v = with_other<4>(v);
+                        if constexpr (TEAM <= 8) v = with_other<8>(v);
+                        if (lane % 16 < TEAM) put(at + lane / 32 + (lane / 16 % 2) * 2 * apart, v);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            if constexpr (places < groups) __syncthreads();
+        }
+    }
+    // Writes dBias and dWeight of all C channels; the whole workgroup.
+    __device__ __forceinline__ void write(float* to, std::uint32_t C) const {
+        __syncthreads();
+        const std::uint32_t body = C / V * V;
+        for (std::uint32_t i = threadIdx.x; i < 2 * C; i += kThreads<TEAM>) {
+            const std::uint32_t k = i < C ? 0 : 1, c = i - k * C, element = c < body ? c : c - C + V + body;
+            double v = 0.0;
+#pragma unroll
+            for (int p = 0; p < places; ++p) v += s.sum[p][2 * element + k];
+            to[i] = static_cast<float>(v);
+        }
+    }
+};
+
 // Bound by memory, and by vector instructions where 16-bit rows have an activation:
-// 2.45M x 256 fp32 rows with d_sum and relu take 1,822 us (10.04 GB: 5.5 TB/s),
-// 169,000 x 301 bf16 rows with gelu 94 (305 MB: 3.2 TB/s, the vector units active in
-// 0.9 of the units' busy cycles), both with the parameters' kernel.
+// 2.45M x 256 fp32 rows with d_sum and relu take 1,781 us (10.04 GB: 5.6 TB/s),
+// 169,000 x 301 bf16 rows with gelu 84 (305 MB: 3.6 TB/s), both with the parameters'
+// kernel.
 template <typename T, int V, int E, int TEAM, bool ONCE>
 __global__ void __launch_bounds__(kThreads<TEAM>) grad_kernel(Args a) {
     using F = vec_t<float, V>;
     __shared__ typename TeamSum<TEAM>::Shared shared;
     TeamSum<TEAM> sum(shared);
+    __shared__ typename Totals<V, E, TEAM>::Shared sums;
+    Totals<V, E, TEAM> totals(sums);
     const Columns<V, E, TEAM> cols(a.C);
     F w[E], b[E], dw[E], db[E];
 #pragma unroll
@@ -289,9 +386,8 @@ __global__ void __launch_bounds__(kThreads<TEAM>) grad_kernel(Args a) {
             }
         }
         if (a.part == nullptr) continue;
-        // the workgroup's sums of the run: its teams', one after the other
-        float* to = a.part + (static_cast<std::uint64_t>(run) * gridDim.x + blockIdx.x) * 2 * a.C;
-        if constexpr (kTeams<TEAM> == 1) {
+        if constexpr (!Totals<V, E, TEAM>::used) {
+            float* to = a.part + (static_cast<std::uint64_t>(run) * gridDim.x + blockIdx.x) * 2 * a.C;
 #pragma unroll
             for (int e = 0; e < E; ++e)
 #pragma unroll
@@ -301,27 +397,13 @@ __global__ void __launch_bounds__(kThreads<TEAM>) grad_kernel(Args a) {
                         to[a.C + cols.c[e] + q] = dw[e][q];
                     }
         } else {
-            __shared__ double total[2][TEAM * E * V];
-            for (int k = 0; k < kTeams<TEAM>; ++k) {
-                if (threadIdx.x / TEAM == k) {
-#pragma unroll
-                    for (int e = 0; e < E; ++e)
-#pragma unroll
-                        for (int q = 0; q < V; ++q)
-                            if (static_cast<std::uint32_t>(q) >= cols.skip[e]) {
-                                const std::uint32_t c = cols.c[e] + q;
-                                total[0][c] = db[e][q] + (k == 0 ? 0.0 : total[0][c]);
-                                total[1][c] = dw[e][q] + (k == 0 ? 0.0 : total[1][c]);
-                            }
-                }
-                __syncthreads();
-            }
-            for (std::uint32_t i = threadIdx.x; i < 2 * a.C; i += kThreads<TEAM>)
-                to[i] = static_cast<float>(i < a.C ? total[0][i] : total[1][i - a.C]);
-            __syncthreads();
+            totals.add(run == 0, db, dw);
         }
 #pragma unroll
         for (int e = 0; e < E; ++e) dw[e] = db[e] = F(0.0f);
+    }
+    if constexpr (Totals<V, E, TEAM>::used) {
+        if (a.part != nullptr) totals.write(a.part + static_cast<std::uint64_t>(blockIdx.x) * 2 * a.C, a.C);
     }
 }
 
@@ -351,7 +433,7 @@ __global__ void __launch_bounds__(kParamCols* kParamRows) params_kernel(const fl
 // TEAM>.  Sixteen elements a lane at most.  Rows of 257 to 384 and of 513 to 768
 // 16-bit elements, of which vectors of 16 bytes would leave up to half of a team's
 // lanes without any, take 8 bytes a lane: the gradient of 169,000 x 301 bf16 rows with
-// gelu, half of whose time is vector instructions, takes 92 us instead of 104.
+// gelu, half of whose time is vector instructions, took 92 us instead of 104.
 // (Others whose last vectors are few keep 16 bytes: 6.25M x 16 rows take 116 us,
 // 66,666 x 1,500 ones 113, where a copy takes 98 and 87.)
 template <typename T, typename F>
@@ -403,13 +485,15 @@ struct Forward {
 };
 
 // The gradient's workgroups are as many as run at once, with equal shares of the
-// rows: 1,822 us for 2.45M x 256 fp32 rows (10.0 GB), 40 less than with three or
-// four times as many.  A team sums a run of its rows in 32 bits, a workgroup its
-// teams' in 64, and the parameters' kernel the runs': with one run of 200 rows
-// dWeight's error was twice that of four of 50, at 35 us less.
+// rows (three or four times as many took 40 us more for 2.45M x 256 fp32 rows).  A
+// team sums a run of its rows in 32 bits, which loses digits by the root of the run's
+// length: dWeight of these is off by 0.8e-7 with runs of 8 rows, 1.0e-7 with 12 and
+// 1.5e-7 with 50 (64-bit sums: 0.5e-7).  16-bit rows are read in half the time, of
+// which runs of 8 take 1 to 4% more than those of 12.
 constexpr std::uint64_t kMostRuns = 4;
-template <int TEAM>
-constexpr std::uint64_t kRun = kTeams<TEAM> == 1 ? 96 : 48;
+template <typename T>
+constexpr std::uint64_t kRun = sizeof(T) == 4 ? 8 : 12;
+constexpr std::uint64_t kLongRun = 96;
 
 // The most of them, for which the workspace is: no compute unit runs more of their
 // size and registers at once.
@@ -428,9 +512,11 @@ struct Backward {
             {(a.N + kTeams<TEAM> - 1) / kTeams<TEAM>, resident_blocks(kernel, kThreads<TEAM>, perCu), most_blocks(a.C)});
         Args k = a;
         const std::uint64_t rows = (a.N + blocks * kTeams<TEAM> - 1) / (blocks * kTeams<TEAM>);
-        k.runs = a.part == nullptr ? 1u : static_cast<std::uint32_t>(std::clamp<std::uint64_t>(rows / kRun<TEAM>, 1, kMostRuns));
+        constexpr bool totals = Totals<V, E, TEAM>::used;
+        const std::uint64_t runs = totals ? rows / kRun<T> : std::min(rows / kLongRun, kMostRuns);
+        k.runs = a.part == nullptr || runs == 0 ? 1u : static_cast<std::uint32_t>(runs);
         k.runRows = (rows + k.runs - 1) / k.runs;
-        parts = blocks * k.runs;
+        parts = totals ? blocks : blocks * k.runs;
         hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kThreads<TEAM>), 0, st, k);
     }
     template <int V, int E, int TEAM>
@@ -505,7 +591,8 @@ extern "C" size_t tcc_layer_norm_grad_workspace_bytes(const tcc_layer_norm_shape
     using namespace tcc;
     if (check_shape(s) != TCC_OK) return 0;
     // the most workgroups of any team, which has one row or more
-    return std::min<std::uint64_t>(s->N, most_blocks(s->C)) * kMostRuns * 2 * s->C * sizeof(float);
+    const std::uint64_t runs = s->C <= kTotalChannels ? 1 : kMostRuns;
+    return std::min<std::uint64_t>(s->N, most_blocks(s->C)) * runs * 2 * s->C * sizeof(float);
 }
 
 extern "C" int tcc_layer_norm_grad(const tcc_layer_norm_shape* s, const void* dY, uint64_t lddy, const void* h,
